@@ -1,0 +1,56 @@
+// What the layer operators' kernels share: element types, reductions inside a warp or CTA.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "hipress/capi.h"
+#include "hipress/layers.h"
+
+namespace hipress {
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+
+// element i of an array whose type is known at run time (uniform over the launch)
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int type) {
+  return type == HP_F32 ? ((const float*)p)[i]
+                        : type == HP_BF16 ? to_f(((const __nv_bfloat16*)p)[i]) : to_f(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, float v, int type) {
+  if (type == HP_F32) ((float*)p)[i] = v;
+  else if (type == HP_BF16) ((__nv_bfloat16*)p)[i] = from_f<__nv_bfloat16>(v);
+  else ((__half*)p)[i] = from_f<__half>(v);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// sum over the CTA, the same value in every thread; `part` holds 32 floats
+__device__ __forceinline__ float cta_sum(float v, float* part) {
+  v = warp_sum(v);
+  __syncthreads();   // part may still be read from the sum before
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < (int)(blockDim.x + 31) / 32; ++i) s += part[i];
+  return s;
+}
+
+inline bool type_ok(int64_t t) { return t >= HP_F32 && t <= HP_F16; }
+
+}  // namespace hipress

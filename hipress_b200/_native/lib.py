@@ -21,7 +21,8 @@ TOPO_RING = 0
 TOPO_PS = 1
 STATUS_TIMEOUT = 0x80000000
 
-ERR_NAMES = {-1: "bad argument", -2: "bucket too large", -3: "emulated ranks would not be co-resident"}
+ERR_NAMES = {-1: "bad argument", -2: "bucket too large", -3: "emulated ranks would not be co-resident",
+             -4: "an earlier kernel gave up waiting, its results are invalid"}
 
 
 class NativeLibraryError(RuntimeError):
