@@ -1,0 +1,82 @@
+// Host side shared by the layer operators: tensor maps, the status word, device facts.
+#include <mutex>
+
+#include "tcgen05.cuh"
+
+namespace hipress {
+namespace {
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {   // looked up in the driver, so that nothing links against it
+  static const Encode f = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (Encode)p;
+  }();
+  return f;
+}
+
+constexpr int kDevices = 64;
+
+}  // namespace
+
+bool tensor_map(CUtensorMap* m, const void* base, int type, int rank, const uint64_t* sizes, const uint64_t* strides_bytes,
+                const uint32_t* box) {
+  const Encode f = encoder();
+  if (!f) return false;
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  cuuint64_t size[5], stride[5];
+  for (int i = 0; i < rank; ++i) {
+    size[i] = sizes[i] ? sizes[i] : 1;
+    if (i) stride[i - 1] = strides_bytes[i - 1];
+  }
+  return f(m, type == HP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
+           (void*)base, size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint32_t* layer_status(int* rc) {
+  static uint32_t* words[kDevices] = {};
+  static std::mutex lock;
+  int dev = 0;
+  *rc = cudaGetDevice(&dev);
+  if (*rc) return nullptr;
+  if (dev >= kDevices) {
+    *rc = HP_ERR_BAD_ARG;
+    return nullptr;
+  }
+  std::lock_guard<std::mutex> hold(lock);
+  if (!words[dev]) {   // pinned for good, 64 bytes
+    void* p = nullptr;
+    *rc = cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+    if (*rc) return nullptr;
+    *(volatile uint32_t*)p = 0;
+    words[dev] = (uint32_t*)p;
+  }
+  volatile uint32_t* w = words[dev];
+  if (*w) {
+    *w = 0;
+    *rc = HP_ERR_TIMEOUT;
+    return nullptr;
+  }
+  return words[dev];
+}
+
+int layer_sms() {
+  static int sms[kDevices] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kDevices) return 1;
+  if (!sms[dev]) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+    sms[dev] = n;
+  }
+  return sms[dev];
+}
+
+}  // namespace hipress

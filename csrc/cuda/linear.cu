@@ -1,47 +1,518 @@
 // The matrix product with bias, activation and residual in its epilogue, and what its
 // backward pass needs besides two more products.
 #include "activation.cuh"
+#include "tcgen05.cuh"
 
 namespace hipress {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16;
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ HpProduct a) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < a.k; k0 += kDepth) {
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      const int ka = a.a_kmajor ? i % kDepth : i / kTile, ra = a.a_kmajor ? i / kDepth : i % kTile;
-      const int64_t m = m0 + ra, k = k0 + ka;
-      sa[ka][ra] = m < a.m && k < a.k ? to_f(((const T*)a.a)[a.a_kmajor ? m * a.lda + k : k * a.lda + m]) : 0.f;
-      const int kb = a.b_kmajor ? i % kDepth : i / kTile, rb = a.b_kmajor ? i / kDepth : i % kTile;
-      const int64_t n = n0 + rb, l = k0 + kb;
-      sb[kb][rb] = n < a.n && l < a.k ? to_f(((const T*)a.b)[a.b_kmajor ? n * a.ldb + l : l * a.ldb + n]) : 0.f;
+// ------------------------------------------------------------------- the product
+// A persistent kernel of specialised warps: one thread fetches tiles (TMA), one issues the
+// matrix products, eight warps empty the accumulators.  Two accumulators in tensor memory: the
+// next tile's products run while the last one's results are written.
+//   CG  CTAs that share a tile: 1, or 2 (each holds half of both operands and 128 rows of results)
+//   BN  columns of a tile; it has 128 CG rows
+constexpr int kBK = 64;            // k of a stage: one line of the swizzle
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kStaging = 4096;     // of a warp: 32 rows of 128 bytes
+
+template <int CG, int BN>
+struct Shape {
+  static constexpr int kRowsB = BN / CG;
+  static constexpr int kBytesA = 128 * 128, kBytesB = kRowsB * 128, kStage = kBytesA + kBytesB;
+  static constexpr int kStages = (kStage <= 24576 ? 6 : kStage <= 32768 ? 5 : 3);
+  static constexpr int kSmem = kStages * kStage + kEpiWarps * (kStaging + 256) + 1024 + 256;
+  static constexpr int kTmem = 2 * BN;
+};
+
+struct Launch {
+  CUtensorMap a, b;
+  HpProduct p;
+  int64_t ldp;               // pitch of the partial sums
+  int tiles_m, tiles_n, kblocks, splits;
+  int vec_y, vec_r;          // elements of an aligned access of y and pre, of residual
+  uint32_t* status;
+};
+
+struct Bars {
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  Guard guard;
+};
+
+struct Unit {
+  int m0, n0, k0, k1, split;
+};
+// Tiles in groups of 16 rows of tiles, so that those at work together share their operands in L2.
+__device__ __forceinline__ Unit unit_of(const Launch& l, int u, int bm, int bn) {
+  Unit w;
+  w.split = u % l.splits;
+  const int t = u / l.splits, group = 16 * l.tiles_n, g = t / group, first = 16 * g;
+  const int rows = min(16, l.tiles_m - first), in = t - g * group;
+  w.m0 = (first + in % rows) * bm;
+  w.n0 = (in / rows) * bn;
+  w.k0 = (int)((int64_t)l.kblocks * w.split / l.splits);
+  w.k1 = (int)((int64_t)l.kblocks * (w.split + 1) / l.splits);
+  return w;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *(const uint32_t*)&v;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *(const uint32_t*)&v;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*(const __nv_bfloat162*)&v);
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*(const __half2*)&v);
+}
+
+// byte `b` of row `r` of a warp's staging rows of 128 bytes: 16-byte pieces change places
+// from row to row, so that a column of rows lies in different banks
+__device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r * 128 + (b ^ ((r & 7) << 4))); }
+
+// The warp's 32 rows of 128 bytes between shared and global memory, along the rows: V bytes to
+// an access.  Rows below `rows` and bytes below `width` only.
+template <int V, bool STORE>
+__device__ __forceinline__ void move_rows(uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
+  constexpr int kLanes = 128 / V >= 32 ? 32 : 128 / V, kAtOnce = 32 / kLanes, kCols = 128 / (V * kLanes);
+#pragma unroll V == 16 ? 8 : 1
+  for (int i = 0; i < 32 / kAtOnce; ++i) {
+    const int r = i * kAtOnce + lane / kLanes;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int b = (c * kLanes + lane % kLanes) * V;
+      uint8_t* at = s + staged(r, b);
+      uint8_t* to = g + r * pitch + b;
+      if (r < rows && b + V <= width) {
+        if (V == 16) {
+          if (STORE) *(uint4*)to = *(uint4*)at;
+          else *(uint4*)at = *(const uint4*)to;
+        } else if (V == 4) {
+          if (STORE) *(uint32_t*)to = *(uint32_t*)at;
+          else *(uint32_t*)at = *(const uint32_t*)to;
+        } else {
+          if (STORE) *(uint16_t*)to = *(uint16_t*)at;
+          else *(uint16_t*)at = *(const uint16_t*)to;
+        }
+      } else if (V > 2 && r < rows) {   // the row ends inside the access
+#pragma unroll
+        for (int e = 0; e < V; e += 2)
+          if (b + e < width) {
+            if (STORE) *(uint16_t*)(to + e) = *(uint16_t*)(at + e);
+            else *(uint16_t*)(at + e) = *(const uint16_t*)(to + e);
+          }
+      }
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= a.m || n >= a.n) continue;
-      float p = acc[i][j];
-      if (a.bias) p += load_any(a.bias, n, (int)a.btype);
-      if (a.pre) ((T*)a.pre)[m * a.ldy + n] = from_f<T>(p);
-      p = activate<ACT>(p);
-      if (a.residual) p += to_f(((const T*)a.residual)[m * a.ldr + n]);
-      store_any(a.y, m * a.ldy + n, p, (int)a.ytype);
+}
+template <bool STORE>   // rows that are not on 16-byte boundaries: kept out of the way of the others
+__device__ __noinline__ void move_ragged_rows(int vec, uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
+  if (vec == 4) move_rows<4, STORE>(s, g, pitch, rows, width, lane);
+  else move_rows<2, STORE>(s, g, pitch, rows, width, lane);
+}
+template <bool STORE>
+__device__ __forceinline__ void move_rows(int vec, uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
+  if (vec == 16) move_rows<16, STORE>(s, g, pitch, rows, width, lane);
+  else move_ragged_rows<STORE>(vec, s, g, pitch, rows, width, lane);
+}
+
+template <int ACT, int N>
+__device__ __forceinline__ void activate_all(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = activate<ACT>(v[i]);
+}
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
+  if (act == HP_ACT_RELU) activate_all<HP_ACT_RELU>(v);
+  else if (act == HP_ACT_GELU) activate_all<HP_ACT_GELU>(v);
+  else if (act == HP_ACT_GELU_TANH) activate_all<HP_ACT_GELU_TANH>(v);
+}
+
+// 32 columns of 32 rows as they are, in 32 bits: partial sums, or a result of that type
+__device__ __forceinline__ void emit32(const Launch& l, uint8_t* stage, uint32_t acc, int row0, int col0, int split,
+                                       int lane, bool last, uint64_t* release, uint32_t remote) {
+  const HpProduct& p = l.p;
+  const int rows = (int)min((int64_t)32, p.m - row0), cols = (int)min((int64_t)32, p.n - col0);
+  uint32_t r[32];
+  tmem_ld32(acc, r);
+  tmem_wait_ld();
+  if (last) {
+    tmem_fence_before();
+    if (lane == 0) {
+      if (release) mbar_arrive(release);
+      else mbar_arrive_cluster(remote);
     }
+  }
+  if (rows <= 0 || cols <= 0) return;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) *(uint4*)(stage + staged(lane, 4 * i)) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+  __syncwarp();
+  float* out = l.splits == 1 ? (float*)p.y + row0 * p.ldy + col0
+                             : (float*)p.workspace + ((int64_t)split * p.m + row0) * l.ldp + col0;
+  const int64_t pitch = 4 * (l.splits == 1 ? p.ldy : l.ldp);
+  move_rows<true>(l.splits == 1 ? l.vec_y : 16, stage, (uint8_t*)out, pitch, rows, 4 * cols, lane);
+  __syncwarp();
+}
+
+// 64 columns of 32 rows in the operands' type
+template <typename T, int COLS>
+__device__ __forceinline__ void emit16(const Launch& l, uint8_t* stage, const float* bias, uint32_t acc, int row0,
+                                       int col0, int lane, bool last, uint64_t* release, uint32_t remote) {
+  const HpProduct& p = l.p;
+  const int rows = (int)min((int64_t)32, p.m - row0), cols = (int)min((int64_t)COLS, p.n - col0);
+  const bool some = rows > 0 && cols > 0;
+  if (some && p.residual) {
+    move_rows<false>(l.vec_r, stage, (uint8_t*)((T*)p.residual + row0 * p.ldr + col0), 2 * p.ldr, rows, 2 * cols, lane);
+    __syncwarp();
+  }
+  uint32_t y[COLS / 2];
+#pragma unroll
+  for (int h = 0; h < COLS; h += 32) {
+    uint32_t r[32];
+    tmem_ld32(acc + h, r);
+    uint32_t res[16];
+    if (some && p.residual)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const uint4 q = *(const uint4*)(stage + staged(lane, 2 * h + 4 * i));
+        res[i] = q.x, res[i + 1] = q.y, res[i + 2] = q.z, res[i + 3] = q.w;
+      }
+    tmem_wait_ld();
+    if (last && h + 32 == COLS) {
+      tmem_fence_before();
+      if (lane == 0) {
+        if (release) mbar_arrive(release);
+        else mbar_arrive_cluster(remote);
+      }
+    }
+    if (!some) continue;
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 b = *(const float4*)(bias + h + i);
+      v[i] = __uint_as_float(r[i]) + b.x;
+      v[i + 1] = __uint_as_float(r[i + 1]) + b.y;
+      v[i + 2] = __uint_as_float(r[i + 2]) + b.z;
+      v[i + 3] = __uint_as_float(r[i + 3]) + b.w;
+    }
+    if (p.pre) {   // this thread has read its residuals of these columns
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        *(uint4*)(stage + staged(lane, 2 * (h + i))) = make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]),
+                                                                  pack2<T>(v[i + 4], v[i + 5]), pack2<T>(v[i + 6], v[i + 7]));
+    }
+    activate_all(p.act, v);
+    if (p.residual)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 q = unpack2<T>(res[i]);
+        v[2 * i] += q.x;
+        v[2 * i + 1] += q.y;
+      }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[h / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+  }
+  if (!some) return;
+  if (p.pre) {
+    __syncwarp();
+    move_rows<true>(l.vec_y, stage, (uint8_t*)((T*)p.pre + row0 * p.ldy + col0), 2 * p.ldy, rows, 2 * cols, lane);
+    __syncwarp();
+  }
+#pragma unroll
+  for (int i = 0; i < COLS / 2; i += 4)
+    *(uint4*)(stage + staged(lane, 4 * i)) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+  __syncwarp();
+  move_rows<true>(l.vec_y, stage, (uint8_t*)((T*)p.y + row0 * p.ldy + col0), 2 * p.ldy, rows, 2 * cols, lane);
+  __syncwarp();
+}
+
+template <typename T, int CG, int BN>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Launch l) {
+  using S = Shape<CG, BN>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* staging = smem + S::kStages * S::kStage;
+  float* biases = (float*)(staging + kEpiWarps * kStaging);
+  Bars& bar = *(Bars*)(biases + kEpiWarps * 64);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const HpProduct& p = l.p;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], CG * kEpiWarps);
+    mbar_init(&bar.drain, 1);
+    mbar_init_fence();
+    bar.guard.gave_up = 0;
+    bar.guard.status = l.status;
+    tma_prefetch(&l.a);
+    tma_prefetch(&l.b);
+  }
+  if (warp == 1) tmem_alloc<CG>(&bar.tmem, S::kTmem);
+  tmem_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();   // the other CTA's barriers are there
+  tmem_fence_after();
+  const uint32_t tmem = bar.tmem;
+  Guard& g = bar.guard;
+  const int units = l.tiles_m * l.tiles_n * l.splits, step = gridDim.x / CG, first = blockIdx.x / CG;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int s = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full0 = CG == 2 ? cluster_addr(&bar.full[0], 0) : 0;
+      for (int u = first; u < units && ok; u += step) {
+        const Unit w = unit_of(l, u, 128 * CG, BN);
+        const int ma = w.m0 + 128 * (int)rank, nb = w.n0 + S::kRowsB * (int)rank;
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          if (!guard_wait(&bar.empty[s], phase ^ 1, g, 0x10000)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a = smem + s * S::kStage;
+          uint8_t* b = a + S::kBytesA;
+          if (rank == 0) mbar_expect_tx(&bar.full[s], CG * S::kStage);
+          auto load = [&](uint8_t* to, const CUtensorMap* map, int x, int y) {
+            if (CG == 2) tma_load_2d_pair(to, map, x, y, full0 + 8 * s);
+            else tma_load_2d(to, map, x, y, &bar.full[s]);
+          };
+          const int k = kb * kBK;
+          if (p.a_kmajor) load(a, &l.a, k, ma);
+          else
+            for (int i = 0; i < 2; ++i) load(a + 8192 * i, &l.a, ma + 64 * i, k);
+          if (p.b_kmajor) load(b, &l.b, k, nb);
+          else
+            for (int i = 0; i < S::kRowsB / 64; ++i) load(b + 8192 * i, &l.b, nb + 64 * i, k);
+          ++issued;
+          if (++s == S::kStages) s = 0, phase ^= 1;
+        }
+      }
+      // every copy has landed before the CTA may end (the products wait for them too, unless they gave up)
+      if (!ok && rank == 0) {
+        g.gave_up = 0;   // these waits are for copies alone
+        for (int i = 0; i < S::kStages && i < issued; ++i) {
+          const int q = (s + S::kStages - 1 - i) % S::kStages, lap = (issued - 1 - i) / S::kStages;
+          guard_wait(&bar.full[q], lap & 1, g, 0x40000);
+        }
+        g.gave_up = 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = mma_idesc(128 * CG, BN, p.type == HP_BF16, p.a_kmajor, p.b_kmajor);
+      const uint32_t lead_a = p.a_kmajor ? 16 : 8192, lead_b = p.b_kmajor ? 16 : 8192;
+      const uint32_t step_a = p.a_kmajor ? 32 : 2048, step_b = p.b_kmajor ? 32 : 2048;
+      int s = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = first; u < units && ok; u += step, ++it) {
+        const Unit w = unit_of(l, u, 128 * CG, BN);
+        const int acc = it & 1;
+        if (!guard_wait(&bar.acc_empty[acc], ((it >> 1) & 1) ^ 1, g, 0x20000)) break;
+        tmem_fence_after();
+        for (int kb = w.k0; kb < w.k1; ++kb) {
+          if (!guard_wait(&bar.full[s], phase, g, 0x30000)) {
+            ok = false;
+            break;
+          }
+          tmem_fence_after();
+          const uint32_t a = smem_u32(smem + s * S::kStage), b = a + S::kBytesA;
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            mma_ss<CG>(tmem + acc * BN, mma_desc(a + k * step_a, lead_a, 1024), mma_desc(b + k * step_b, lead_b, 1024),
+                       idesc, kb > w.k0 || k > 0);
+          mma_commit<CG>(&bar.empty[s]);
+          if (++s == S::kStages) s = 0, phase ^= 1;
+        }
+        if (ok) mma_commit<CG>(&bar.acc_full[acc]);
+      }
+      mma_commit<CG>(&bar.drain);
+    }
+  } else {
+    const int e = warp - 2, quad = warp & 3, half = e >> 2;
+    uint8_t* stage = staging + e * kStaging;
+    float* bias = biases + e * 64;
+    constexpr int kCols = BN / 2, kChunk = kCols >= 64 ? 64 : 32;
+    int it = 0;
+    for (int u = first; u < units; u += step, ++it) {
+      const Unit w = unit_of(l, u, 128 * CG, BN);
+      const int acc = it & 1;
+      if (!guard_wait(&bar.acc_full[acc], (it >> 1) & 1, g, 0x50000)) break;
+      tmem_fence_after();
+      const int row0 = w.m0 + 128 * (int)rank + 32 * quad;
+      uint64_t* release = CG == 2 ? nullptr : &bar.acc_empty[acc];
+      const uint32_t remote = CG == 2 ? cluster_addr(&bar.acc_empty[acc], 0) : 0;
+      const bool wide = l.splits > 1 || p.ytype == HP_F32;
+      for (int c = 0; c < kCols; c += kChunk) {
+        const int col0 = w.n0 + half * kCols + c;
+        const uint32_t at = tmem + acc * BN + half * kCols + c + ((uint32_t)(32 * quad) << 16);
+        const bool last = c + kChunk == kCols;
+        for (int i = lane; i < kChunk; i += 32)
+          bias[i] = p.bias && col0 + i < p.n ? load_any(p.bias, col0 + i, (int)p.btype) : 0.f;
+        __syncwarp();
+        if (wide) {
+          for (int h = 0; h < kChunk; h += 32)
+            emit32(l, stage, at + h, row0, col0 + h, w.split, lane, last && h + 32 == kChunk, release, remote);
+        } else {
+          emit16<T, kChunk>(l, stage, bias, at, row0, col0, lane, last, release, remote);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0) {   // the products have ended, also those nobody waits for
+      g.gave_up = 0;
+      guard_wait(&bar.drain, 0, g, 0x60000);
+    }
+    __syncwarp();
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();   // neither CTA's memory goes while the other's products read it
+  tmem_fence_after();
+  if (warp == 1) tmem_free<CG>(tmem, S::kTmem);
+}
+
+// y from the partial sums of the splits (none: of a product without k), added in their order
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Launch l) {
+  const HpProduct& p = l.p;
+  const int64_t quads = l.ldp / 4, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.m * quads) return;
+  const int64_t m = at / quads, n = at % quads * 4;
+  float v[4] = {};
+  const float* part = (const float*)p.workspace + m * l.ldp + n;
+  for (int s = 0; s < l.splits; ++s) {
+    const float4 q = *(const float4*)(part + (int64_t)s * p.m * l.ldp);
+    v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+  }
+  const int cols = (int)min((int64_t)4, p.n - n);
+  for (int i = 0; i < cols; ++i) {
+    if (p.bias) v[i] += load_any(p.bias, n + i, (int)p.btype);
+    if (p.pre) ((T*)p.pre)[m * p.ldy + n + i] = from_f<T>(v[i]);
+  }
+  activate_all(p.act, v);
+  for (int i = 0; i < cols; ++i) {
+    if (p.residual) v[i] += to_f(((const T*)p.residual)[m * p.ldr + n + i]);
+    store_any(p.y, m * p.ldy + n + i, v[i], (int)p.ytype);
+  }
+}
+
+struct Choice {
+  int cg, bn, splits;
+};
+
+// Which kernel, and into how many parts k is split: the least of an estimate in SM cycles.
+Choice choose(int64_t m, int64_t n, int64_t kblocks, int sms) {
+  const struct {
+    int cg, bn;
+    double stage;   // cycles of 64 k
+  } kinds[] = {{2, 256, 540}, {2, 128, 290}, {1, 128, 300}, {1, 64, 215}};
+  Choice best = {1, 128, 1};
+  double least = 1e30;
+  for (const auto& c : kinds) {
+    const int64_t tiles = ((m + 128 * c.cg - 1) / (128 * c.cg)) * ((n + c.bn - 1) / c.bn), slots = sms / c.cg;
+    for (int64_t s = 1; s <= 64 && s <= kblocks; s = s < 4 ? s + 1 : s + s / 2) {
+      const int64_t rounds = (tiles * s + slots - 1) / slots;
+      const int64_t per = (kblocks + s - 1) / s;
+      double t = rounds * (per * c.stage + 300.0) + 3000.0 + c.bn * 10.0;
+      if (s > 1) t += 5000.0 + (double)m * n * (2 * s) * 4 / 3000.0;   // the partial sums, and one more launch
+      if (t < least) least = t, best = {c.cg, c.bn, (int)s};
+    }
+  }
+  return best;
+}
+
+int64_t pitch4(int64_t n) { return (n + 3) / 4 * 4; }
+
+template <typename T, int CG, int BN>
+int run_product(Launch& l, int sms, cudaStream_t s) {
+  using S = Shape<CG, BN>;
+  const HpProduct& p = l.p;
+  const uint32_t box_k[2] = {kBK, 128}, box_m[2] = {64, kBK};
+  const uint32_t box_kb[2] = {kBK, (uint32_t)S::kRowsB};
+  auto map = [&](CUtensorMap* t, const void* base, int64_t rows, int64_t ld, bool kmajor, const uint32_t* box) {
+    const uint64_t size[2] = {(uint64_t)(kmajor ? p.k : rows), (uint64_t)(kmajor ? rows : p.k)};
+    const uint64_t pitch[1] = {size[1] > 1 ? 2 * (uint64_t)ld : 16};   // of one line there is no next
+    return tensor_map(t, base, (int)p.type, 2, size, pitch, box);
+  };
+  if (!map(&l.a, p.a, p.m, p.lda, p.a_kmajor, p.a_kmajor ? box_k : box_m) ||
+      !map(&l.b, p.b, p.n, p.ldb, p.b_kmajor, p.b_kmajor ? box_kb : box_m))
+    return HP_ERR_BAD_ARG;
+  static const cudaError_t allowed =
+      cudaFuncSetAttribute(product_kernel<T, CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (allowed != cudaSuccess) return allowed;
+  l.tiles_m = (int)((p.m + 128 * CG - 1) / (128 * CG));
+  l.tiles_n = (int)((p.n + BN - 1) / BN);
+  const int64_t units = (int64_t)l.tiles_m * l.tiles_n * l.splits;
+  if (units > INT32_MAX / 2) return HP_ERR_TOO_LARGE;
+  const int64_t slots = sms / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CG * (units < slots ? units : slots)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, product_kernel<T, CG, BN>, l);
+}
+
+int alignment(const void* p, int64_t pitch_bytes) {
+  const uint64_t v = (uint64_t)(uintptr_t)p | (uint64_t)pitch_bytes;
+  return v % 16 == 0 ? 16 : v % 4 == 0 ? 4 : 2;
+}
+
+template <typename T>
+int product(const HpProduct& a, cudaStream_t s) {
+  Launch l;
+  int rc;
+  l.status = layer_status(&rc);
+  if (rc) return rc;
+  const int sms = layer_sms();
+  l.p = a;
+  l.ldp = pitch4(a.n);
+  l.kblocks = (int)((a.k + kBK - 1) / kBK);
+  const int e = a.ytype == HP_F32 ? 4 : 2;
+  l.vec_y = alignment(a.y, a.ldy * e);
+  if (a.pre && alignment(a.pre, a.ldy * 2) < l.vec_y) l.vec_y = alignment(a.pre, a.ldy * 2);
+  l.vec_r = alignment(a.residual, a.ldr * 2);
+  l.splits = 0;
+  if (a.k) {
+    const Choice c = choose(a.m, a.n, l.kblocks, sms);
+    l.splits = c.splits;
+    rc = c.cg == 2 ? (c.bn == 256 ? run_product<T, 2, 256>(l, sms, s) : run_product<T, 2, 128>(l, sms, s))
+                   : (c.bn == 128 ? run_product<T, 1, 128>(l, sms, s) : run_product<T, 1, 64>(l, sms, s));
+    if (rc) return rc;
+    if (l.splits == 1) return 0;
+  }
+  const int64_t quads = a.m * (l.ldp / 4);
+  if (quads > (int64_t)INT32_MAX * 128) return HP_ERR_TOO_LARGE;
+  finish_kernel<T><<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(l);
+  return cudaGetLastError();
 }
 
 template <typename T, int ACT>
@@ -65,18 +536,6 @@ __global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ HpSl
 }
 
 template <typename T>
-int product(const HpProduct& a, cudaStream_t s) {
-  const dim3 grid((unsigned)((a.n + kTile - 1) / kTile), (unsigned)((a.m + kTile - 1) / kTile));
-  switch (a.act) {
-    case HP_ACT_NONE: product_kernel<T, HP_ACT_NONE><<<grid, 256, 0, s>>>(a); break;
-    case HP_ACT_RELU: product_kernel<T, HP_ACT_RELU><<<grid, 256, 0, s>>>(a); break;
-    case HP_ACT_GELU: product_kernel<T, HP_ACT_GELU><<<grid, 256, 0, s>>>(a); break;
-    default: product_kernel<T, HP_ACT_GELU_TANH><<<grid, 256, 0, s>>>(a); break;
-  }
-  return cudaGetLastError();
-}
-
-template <typename T>
 int slopes(const HpSlope& a, cudaStream_t s) {
   const unsigned grid = (unsigned)((a.cols + 31) / 32);
   const dim3 block(32, 8);
@@ -96,15 +555,20 @@ using namespace hipress;
 
 extern "C" int hp_cuda_product(const HpProduct* a, void* stream) {
   if (!a || a->m < 0 || a->n < 0 || a->k < 0 || a->m > INT32_MAX / 2 || a->n > INT32_MAX / 2 || a->k > INT32_MAX / 2 ||
-      (a->type != HP_BF16 && a->type != HP_F16) || !type_ok(a->ytype) || !type_ok(a->btype) || a->act < 0 ||
-      a->act > HP_ACT_GELU_TANH)
+      (a->type != HP_BF16 && a->type != HP_F16) || (a->ytype != a->type && a->ytype != HP_F32) || !type_ok(a->btype) ||
+      a->act < 0 || a->act > HP_ACT_GELU_TANH ||
+      (a->ytype == HP_F32 && (a->bias || a->act || a->residual || a->pre)))
     return HP_ERR_BAD_ARG;
   if (!a->m || !a->n) return 0;
   cudaStream_t s = (cudaStream_t)stream;
   return a->type == HP_BF16 ? product<__nv_bfloat16>(*a, s) : product<__half>(*a, s);
 }
 
-extern "C" uint64_t hp_cuda_product_workspace(int64_t, int64_t, int64_t) { return 0; }
+extern "C" uint64_t hp_cuda_product_workspace(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const Choice c = choose(m, n, (k + kBK - 1) / kBK, layer_sms());
+  return c.splits > 1 ? (uint64_t)c.splits * m * pitch4(n) * 4 : 0;
+}
 
 extern "C" int hp_cuda_slope(const HpSlope* a, void* stream) {
   if (!a || a->rows < 0 || a->cols < 0 || (a->type != HP_BF16 && a->type != HP_F16) || !type_ok(a->btype) ||

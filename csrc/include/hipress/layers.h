@@ -62,7 +62,8 @@ uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols, int64_t unused);
 
 // One product out[m, n] = sum_k a(m, k) b(n, k) with its epilogue: p = out + bias;
 // y = act(p) + residual.  An operand is stored along k (kmajor 1: row m, pitch lda) or along
-// its own index (kmajor 0: row k, pitch lda).
+// its own index (kmajor 0: row k, pitch lda); both bases and pitches on 16-byte boundaries.  y
+// has the operands' type, or is in 32 bits, without an epilogue.
 typedef struct {
   const void* a;
   const void* b;
