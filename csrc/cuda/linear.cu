@@ -1,6 +1,7 @@
 // The matrix product with bias, activation and residual in its epilogue, and what its
 // backward pass needs besides two more products.
 #include "activation.cuh"
+#include "column_sums.cuh"
 #include "tcgen05.cuh"
 
 namespace hipress {
@@ -515,37 +516,115 @@ int product(const HpProduct& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) slope_kernel(const __grid_constant__ HpSlope a) {
-  __shared__ float sums[8][33];
-  const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (col < a.cols)
-    for (int64_t r = threadIdx.y; r < a.rows; r += 8) {
-      float g = to_f(((const T*)a.dy)[r * a.lddy + col]);
-      if (ACT != HP_ACT_NONE) g *= slope<ACT>(to_f(((const T*)a.pre)[r * a.ldpre + col]));
-      if (a.g) ((T*)a.g)[r * a.ldg + col] = from_f<T>(g);
-      s += g;
+// --------------------------------------------------- the gradient before the activation
+// g = dy act'(pre) and the sums of its columns, in one pass over dy and pre: traffic bound.  A
+// thread has V columns (16 bytes where all rows lie on that boundary, else 4 or 2) and the rows
+// of its warp; the CTA's eight warps add up their sums, and leave one row of partial sums.
+constexpr int kSlopeWarps = 8;
+
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { using type = uint4; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<2> { using type = uint16_t; };
+
+template <typename T, int ACT, int V>
+__global__ void __launch_bounds__(32 * kSlopeWarps) slope_kernel(const __grid_constant__ HpSlope a) {
+  using Raw = typename Word<2 * V>::type;
+  __shared__ float sums[kSlopeWarps][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V, step = (int64_t)gridDim.y * kSlopeWarps;
+  float s[V] = {};
+  dependents_may_start();
+  auto put = [&](int64_t row, Raw dy, Raw pre) {
+    T* d = (T*)&dy;
+    const T* q = (const T*)&pre;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float g = to_f(d[j]);
+      if (ACT != HP_ACT_NONE) g *= slope<ACT>(to_f(q[j]));
+      s[j] += g;
+      d[j] = from_f<T>(g);
     }
-  sums[threadIdx.y][threadIdx.x] = s;
+    if (a.g) *(Raw*)((T*)a.g + row * a.ldg + col) = dy;
+  };
+  if (col + V <= a.cols) {
+    int64_t row = (int64_t)blockIdx.y * kSlopeWarps + warp;
+    const T* dy = (const T*)a.dy + col;
+    const T* pre = (const T*)a.pre + col;
+    constexpr int kAhead = 4;
+    for (; row + (kAhead - 1) * step < a.rows; row += kAhead * step) {
+      Raw d[kAhead], q[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        d[i] = *(const Raw*)(dy + (row + i * step) * a.lddy);
+        if (ACT != HP_ACT_NONE) q[i] = *(const Raw*)(pre + (row + i * step) * a.ldpre);
+        else q[i] = d[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) put(row + i * step, d[i], q[i]);
+    }
+    for (; row < a.rows; row += step) {
+      const Raw d = *(const Raw*)(dy + row * a.lddy);
+      put(row, d, ACT != HP_ACT_NONE ? *(const Raw*)(pre + row * a.ldpre) : d);
+    }
+  } else if (V > 1 && col < a.cols) {   // the row ends inside this thread's columns
+    for (int64_t row = (int64_t)blockIdx.y * kSlopeWarps + warp; row < a.rows; row += step)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (col + j < a.cols) {
+          float g = to_f(((const T*)a.dy)[row * a.lddy + col + j]);
+          if (ACT != HP_ACT_NONE) g *= slope<ACT>(to_f(((const T*)a.pre)[row * a.ldpre + col + j]));
+          s[j] += g;
+          if (a.g) ((T*)a.g)[row * a.ldg + col + j] = from_f<T>(g);
+        }
+  }
+  if (!a.dbias) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[warp][j * 32 + lane] = s[j];
   __syncthreads();
-  if (threadIdx.y == 0 && col < a.cols && a.dbias) {
-    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-    store_any(a.dbias, col, s, (int)a.btype);
+  for (int i = threadIdx.x; i < 32 * V; i += 32 * kSlopeWarps) {
+    const int64_t c = (int64_t)blockIdx.x * 32 * V + (i % 32) * V + i / 32;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSlopeWarps; ++w) t += sums[w][i];
+    if (c < a.cols) ((float*)a.workspace)[(int64_t)blockIdx.y * a.cols + c] = t;
   }
 }
 
+constexpr int kSlopeParts = 256;   // rows of partial sums at most
+
+template <typename T, int ACT, int V>
+int slopes(const HpSlope& a, cudaStream_t s) {
+  const int64_t wide = (a.cols + 32 * V - 1) / (32 * V);
+  // four CTAs to an SM; at least four rows to a warp, so that the sums stay few
+  int64_t high = ((int64_t)layer_sms() * 4 + wide - 1) / wide, most = (a.rows + 4 * kSlopeWarps - 1) / (4 * kSlopeWarps);
+  if (high > most) high = most;
+  if (high > kSlopeParts) high = kSlopeParts;
+  if (high < 1) high = 1;
+  slope_kernel<T, ACT, V><<<dim3((unsigned)wide, (unsigned)high), 32 * kSlopeWarps, 0, s>>>(a);
+  int rc = cudaGetLastError();
+  if (rc || !a.dbias) return rc;
+  return column_sums((const float*)a.workspace, (int)high, a.cols, a.cols, a.dbias, nullptr, (int)a.btype, s);
+}
+template <typename T, int ACT>
+int slopes(const HpSlope& a, cudaStream_t s) {
+  int v = alignment(a.dy, 2 * a.lddy);
+  if (ACT != HP_ACT_NONE && alignment(a.pre, 2 * a.ldpre) < v) v = alignment(a.pre, 2 * a.ldpre);
+  if (a.g && alignment(a.g, 2 * a.ldg) < v) v = alignment(a.g, 2 * a.ldg);
+  return v == 16 ? slopes<T, ACT, 8>(a, s) : v == 4 ? slopes<T, ACT, 2>(a, s) : slopes<T, ACT, 1>(a, s);
+}
 template <typename T>
 int slopes(const HpSlope& a, cudaStream_t s) {
-  const unsigned grid = (unsigned)((a.cols + 31) / 32);
-  const dim3 block(32, 8);
   switch (a.act) {
-    case HP_ACT_NONE: slope_kernel<T, HP_ACT_NONE><<<grid, block, 0, s>>>(a); break;
-    case HP_ACT_RELU: slope_kernel<T, HP_ACT_RELU><<<grid, block, 0, s>>>(a); break;
-    case HP_ACT_GELU: slope_kernel<T, HP_ACT_GELU><<<grid, block, 0, s>>>(a); break;
-    default: slope_kernel<T, HP_ACT_GELU_TANH><<<grid, block, 0, s>>>(a); break;
+    case HP_ACT_NONE: return slopes<T, HP_ACT_NONE>(a, s);
+    case HP_ACT_RELU: return slopes<T, HP_ACT_RELU>(a, s);
+    case HP_ACT_GELU: return slopes<T, HP_ACT_GELU>(a, s);
+    default: return slopes<T, HP_ACT_GELU_TANH>(a, s);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace
@@ -579,4 +658,4 @@ extern "C" int hp_cuda_slope(const HpSlope* a, void* stream) {
   return a->type == HP_BF16 ? slopes<__nv_bfloat16>(*a, s) : slopes<__half>(*a, s);
 }
 
-extern "C" uint64_t hp_cuda_slope_workspace(int64_t, int64_t, int64_t) { return 0; }
+extern "C" uint64_t hp_cuda_slope_workspace(int64_t, int64_t cols, int64_t) { return (uint64_t)kSlopeParts * cols * 4; }
