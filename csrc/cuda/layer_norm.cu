@@ -95,239 +95,274 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const __grid_constant__ Hp
 // same: the pieces start `phase` elements ahead of the row, and what is outside the row is left
 // out.  The phase goes by the row modulo the elements of a piece, and the rows of one group
 // of warps are that far apart, so that its columns stay the same.
-template <typename T>
-constexpr int kPiece = 16 / sizeof(T);
-
-template <typename T>
-struct Piece {   // which columns a thread's piece covers
+// The columns that a thread's piece covers.  Unless RAGGED a piece is in the row or behind it.
+template <typename T, bool RAGGED>
+struct Piece {
+  static constexpr int V = kPiece<T>, kBits = 8 * sizeof(T);
   int first;
-  __device__ __forceinline__ bool whole(int cols) const { return first >= 0 && first + kPiece<T> <= cols; }
-  __device__ __forceinline__ bool has(int j, int cols) const { return first + j >= 0 && first + j < cols; }
-};
-
-// A piece at an end of the row goes element by element, shifted through its 128 bits: few
-// registers for what few threads do.
-template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* row, Piece<T> c, int cols) {
-  if (c.whole(cols)) return __ldg((const uint4*)(row + c.first));
-  uint64_t lo = 0, hi = 0;
-  constexpr int kBits = 8 * sizeof(T);
-  if (c.first < cols)
+  __device__ __forceinline__ bool whole(int cols) const {
+    return RAGGED ? first >= 0 && first + V <= cols : first < cols;
+  }
+  __device__ __forceinline__ bool has(int j, int cols) const {
+    return RAGGED ? first + j >= 0 && first + j < cols : first < cols;
+  }
+  __device__ __forceinline__ void load_weights(const void* p, int type, int cols, float none, float (&v)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = p && has(j, cols) ? load_any(p, first + j, type) : none;
+  }
+  // Zeros outside the row.  A piece at an end of it: where the rows next to this one are there
+  // (`inner`; and no row is shorter than a piece) it is loaded whole and what is not the row's
+  // is cleared; else it goes element by element, shifted through its 128 bits: few registers
+  // for what few threads do.
+  __device__ __forceinline__ uint4 load(const T* row, int cols, bool there, bool inner) const {
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (!there) return raw;
+    if (whole(cols)) return __ldg((const uint4*)(row + first));
+    if (!RAGGED || first >= cols) return raw;
+    T* v = (T*)&raw;
+    if (inner && cols >= V) {
+      raw = __ldg((const uint4*)(row + first));
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (!has(j, cols)) v[j] = from_f<T>(0.f);
+      return raw;
+    }
+    uint64_t lo = 0, hi = 0;
 #pragma unroll 1
-    for (int j = 0; j < kPiece<T>; ++j) {
-      T v = from_f<T>(0.f);
-      if (c.has(j, cols)) v = row[c.first + j];
-      uint64_t bits = 0;
-      if (sizeof(T) == 4) bits = *(const uint32_t*)&v;
-      else bits = *(const uint16_t*)&v;
+    for (int j = 0; j < V; ++j) {
+      T e = from_f<T>(0.f);
+      if (has(j, cols)) e = row[first + j];
+      const uint64_t bits = sizeof(T) == 4 ? *(const uint32_t*)&e : *(const uint16_t*)&e;
       lo = lo >> kBits | hi << (64 - kBits);
       hi = hi >> kBits | bits << (64 - kBits);
     }
-  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
-}
-template <typename T>
-__device__ __forceinline__ void store_piece(T* row, Piece<T> c, int cols, const float (&v)[kPiece<T>]) {
-  uint4 raw;
-  T* t = (T*)&raw;
-#pragma unroll
-  for (int j = 0; j < kPiece<T>; ++j) t[j] = from_f<T>(v[j]);
-  if (c.whole(cols)) {
-    *(uint4*)(row + c.first) = raw;
-    return;
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
-  uint64_t lo = raw.x | (uint64_t)raw.y << 32, hi = raw.z | (uint64_t)raw.w << 32;
-  constexpr int kBits = 8 * sizeof(T);
-  if (c.first < cols)
+  __device__ __forceinline__ void store(T* row, int cols, bool there, uint4 raw) const {
+    if (!there) return;
+    if (whole(cols)) {
+      *(uint4*)(row + first) = raw;
+      return;
+    }
+    if (!RAGGED || first >= cols) return;
+    uint64_t lo = raw.x | (uint64_t)raw.y << 32, hi = raw.z | (uint64_t)raw.w << 32;
 #pragma unroll 1
-    for (int j = 0; j < kPiece<T>; ++j) {
-      if (c.has(j, cols)) {
-        if (sizeof(T) == 4) ((uint32_t*)row)[c.first + j] = (uint32_t)lo;
-        else ((uint16_t*)row)[c.first + j] = (uint16_t)lo;
+    for (int j = 0; j < V; ++j) {
+      if (has(j, cols)) {
+        if (sizeof(T) == 4) ((uint32_t*)row)[first + j] = (uint32_t)lo;
+        else ((uint16_t*)row)[first + j] = (uint16_t)lo;
       }
       lo = lo >> kBits | hi << (64 - kBits);
       hi >>= kBits;
     }
-}
-template <typename T>
-__device__ __forceinline__ void unpack(uint4 raw, float (&v)[kPiece<T>]) {
-  const T* t = (const T*)&raw;
+  }
+};
+
+// Sums over the NW warps that share a row, of N values together behind one barrier; `part` is
+// theirs until the barrier after the next.
+template <int NW, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (&part)[N][16], int warp) {
 #pragma unroll
-  for (int j = 0; j < kPiece<T>; ++j) v[j] = to_f(t[j]);
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if (NW == 1) return;
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i][warp] = v[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v[i] += part[i][w];
+  }
 }
 
-// sums over the NW warps that share a row; `part` [2][16] floats, used in turn
-template <int NW>
-__device__ __forceinline__ float row_sum(float v, float* part, int warp) {
-  v = warp_sum(v);
-  if (NW == 1) return v;
-  if ((threadIdx.x & 31) == 0) part[warp] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) s += part[i];
-  return s;
+// From here on `raw` is taken apart anew: the compiler would keep the 32-bit values instead,
+// twice the registers.
+__device__ __forceinline__ void forget(uint4& raw) {
+  asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w));
 }
 
 template <int NW>
 constexpr int kThreadsOf = 32 * (NW < 4 ? 4 : NW);
 
-template <typename T, typename W, int NW, int CH>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? 4 : NW == 8 ? 2 : 1) norm_forward_rows(const __grid_constant__ HpNormForward a, int ragged) {
-  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW);
-  __shared__ float part[2][16];
+// Rows that a group of warps takes at once: their loads are in flight together and their sums
+// share the shuffles' and barriers' latency.
+template <int CH>
+constexpr int kAtOnce = CH == 1 ? 4 : CH == 2 ? 2 : 1;
+
+template <typename T, int NW, int CH, bool RAGGED>
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 7 : 4) : NW == 8 ? (CH == 2 ? 3 : 2) : 1)
+norm_forward_rows(const __grid_constant__ HpNormForward a) {
+  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW), R = kAtOnce<CH>;
+  __shared__ float part[2][R][16];
   const int cols = (int)a.cols, t = threadIdx.x % (32 * NW), warp = t >> 5;
   const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / (32 * NW), step = (int64_t)gridDim.x * kGroups;
   if (first >= a.rows) return;   // the whole CTA where it shares a row
-  const int phase = ragged ? (int)(((uintptr_t)((const T*)a.x + first * a.ldx) / sizeof(T)) % V) : 0;
-  Piece<T> c[CH];
+  const int phase = RAGGED ? (int)(((uintptr_t)((const T*)a.x + first * a.ldx) / sizeof(T)) % V) : 0;
+  Piece<T, RAGGED> c[CH];
   float w[CH][V], b[CH][V];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     c[i].first = (t + i * 32 * NW) * V - phase;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[i][j] = a.weight && c[i].has(j, cols) ? to_f(((const W*)a.weight)[c[i].first + j]) : 1.f;
-      b[i][j] = a.bias && c[i].has(j, cols) ? to_f(((const W*)a.bias)[c[i].first + j]) : 0.f;
-    }
+    c[i].load_weights(a.weight, (int)a.wtype, cols, 1.f, w[i]);
+    c[i].load_weights(a.bias, (int)a.wtype, cols, 0.f, b[i]);
   }
   const float inv = 1.f / (float)cols;
-  uint4 raw[CH], res[CH];
-  auto fetch = [&](int64_t row) {
+  for (int64_t row0 = first; row0 < a.rows; row0 += R * step) {
+    uint4 raw[R][CH], res[R][CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      raw[i] = load_piece((const T*)a.x + row * a.ldx, c[i], cols);
-      if (a.residual) res[i] = load_piece((const T*)a.residual + row * a.ldr, c[i], cols);
-    }
-  };
-  constexpr bool kAhead = CH <= 2;   // with more pieces the registers do not suffice
-  if (kAhead) fetch(first);
-  for (int64_t row = first; row < a.rows; row += step) {
-    if (!kAhead) fetch(row);
-    float v[CH][V], s = 0.f;
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = row0 + k * step;
+      const bool there = row < a.rows, inner = row > 0 && row + 1 < a.rows;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      unpack<T>(raw[i], v[i]);
-      if (a.residual) {
-        float r[V];
-        unpack<T>(res[i], r);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = to_f(from_f<T>(v[i][j] + r[j]));
-        store_piece((T*)a.z + row * a.cols, c[i], cols, v[i]);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) s += v[i][j];
-    }
-    if (kAhead && row + step < a.rows) fetch(row + step);   // on its way while this row is summed
-    const float mean = row_sum<NW>(s, part[0], warp) * inv;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const bool whole = c[i].whole(cols);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[i][j] - mean;
-        v[i][j] = d;
-        if (whole || c[i].has(j, cols)) s = fmaf(d, d, s);
+      for (int i = 0; i < CH; ++i) {
+        raw[k][i] = c[i].load((const T*)a.x + row * a.ldx, cols, there, inner);
+        if (a.residual) res[k][i] = c[i].load((const T*)a.residual + row * a.ldr, cols, there, inner);
       }
     }
-    const float rstd = 1.f / sqrtf(row_sum<NW>(s, part[1], warp) * inv + (float)a.eps);
-    T* y = (T*)a.y + row * a.cols;
+    // a row stays packed as it came; to take it apart costs an instruction for an element, and half
+    // the registers are half the warps
+    float s[R];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
+    for (int k = 0; k < R; ++k) {
+      s[k] = 0.f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
-      store_piece(y, c[i], cols, v[i]);
+      for (int i = 0; i < CH; ++i) {
+        float v[V];
+        unpack<T>(raw[k][i], v);
+        if (a.residual) {
+          float r[V];
+          unpack<T>(res[k][i], r);
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] += r[j];
+          raw[k][i] = pack<T>(v);   // the sum as it is stored is what is normalised
+          unpack<T>(raw[k][i], v);
+          c[i].store((T*)a.z + (row0 + k * step) * a.cols, cols, row0 + k * step < a.rows, raw[k][i]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[k] += v[j];
+      }
     }
-    if (t == 0) {
-      a.mean[row] = mean;
-      a.rstd[row] = rstd;
+    row_sums<NW>(s, part[0], warp);
+    float mean[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      mean[k] = s[k] * inv;
+      s[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        float v[V];
+        forget(raw[k][i]);
+        unpack<T>(raw[k][i], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = v[j] - mean[k];
+          if (c[i].has(j, cols)) s[k] = fmaf(d, d, s[k]);
+        }
+      }
+    }
+    row_sums<NW>(s, part[1], warp);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = row0 + k * step;
+      const float rstd = 1.f / sqrtf(s[k] * inv + (float)a.eps);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        float v[V];
+        forget(raw[k][i]);
+        unpack<T>(raw[k][i], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean[k]) * rstd, w[i][j], b[i][j]);
+        c[i].store((T*)a.y + row * a.cols, cols, row < a.rows, pack<T>(v));
+      }
+      if (t == 0 && row < a.rows) {
+        a.mean[row] = mean[k];
+        a.rstd[row] = rstd;
+      }
     }
   }
 }
 
-template <typename T, typename W, int NW, int CH>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? 4 : NW == 8 ? 2 : 1) norm_backward_rows(const __grid_constant__ HpNormBackward a, int ragged) {
-  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW);
-  __shared__ float part[4][16];
+template <typename T, int NW, int CH, bool RAGGED>
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 5 : 3) : NW == 8 ? (CH == 2 ? 2 : 1) : 1)
+norm_backward_rows(const __grid_constant__ HpNormBackward a) {
+  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW), R = CH >= 3 || NW == 16 ? 1 : 2;
+  __shared__ float part[2][2 * R][16];
   extern __shared__ float joint[];   // [2 cols], where several rows are at work in a CTA
   const int cols = (int)a.cols, t = threadIdx.x % (32 * NW), warp = t >> 5, group = threadIdx.x / (32 * NW);
   const int64_t first = (int64_t)blockIdx.x * kGroups + group, step = (int64_t)gridDim.x * kGroups;
-  const int phase =
-      ragged ? (int)(((uintptr_t)((const T*)a.z + first * a.ldz) / sizeof(T)) % V) : 0;
-  Piece<T> c[CH];
+  const int phase = RAGGED ? (int)(((uintptr_t)((const T*)a.z + first * a.ldz) / sizeof(T)) % V) : 0;
+  Piece<T, RAGGED> c[CH];
   float w[CH][V], dw[CH][V], db[CH][V];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     c[i].first = (t + i * 32 * NW) * V - phase;
+    c[i].load_weights(a.weight, (int)a.wtype, cols, 1.f, w[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      w[i][j] = a.weight && c[i].has(j, cols) ? to_f(((const W*)a.weight)[c[i].first + j]) : 1.f;
-      dw[i][j] = db[i][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
   }
   dependents_may_start();
   const float inv = 1.f / (float)cols;
   int turn = 0;
-  uint4 zn[CH], gn[CH];
-  float mean_next = 0.f, rstd_next = 0.f;
-  auto fetch = [&](int64_t row) {
+  for (int64_t row0 = first; row0 < a.rows; row0 += R * step, turn ^= 1) {
+    uint4 zr[R][CH], gr[R][CH], ur[R][CH];
+    float mean[R], rstd[R], s[2 * R];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      zn[i] = load_piece((const T*)a.z + row * a.ldz, c[i], cols);
-      gn[i] = load_piece((const T*)a.dy + row * a.lddy, c[i], cols);
-    }
-    mean_next = a.mean[row], rstd_next = a.rstd[row];
-  };
-  constexpr bool kAhead = CH <= 2;   // with more pieces the registers do not suffice
-  if (kAhead && first < a.rows) fetch(first);
-  for (int64_t row = first; row < a.rows; row += step, turn ^= 2) {
-    if (!kAhead) fetch(row);
-    uint4 zr[CH], gr[CH];
-    const float mean = mean_next, rstd = rstd_next;
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = row0 + k * step;
+      const bool there = row < a.rows, inner = row > 0 && row + 1 < a.rows;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) zr[i] = zn[i], gr[i] = gn[i];
-    if (row + step < a.rows) fetch(row + step);   // on its way while this row is summed
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      float z[V], g[V];
-      unpack<T>(zr[i], z);
-      unpack<T>(gr[i], g);   // zeros outside the row
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (z[j] - mean) * rstd, gw = g[j] * w[i][j];
-        dw[i][j] = fmaf(g[j], h, dw[i][j]);
-        db[i][j] += g[j];
-        s1 += gw;
-        s2 = fmaf(gw, h, s2);
+      for (int i = 0; i < CH; ++i) {
+        zr[k][i] = c[i].load((const T*)a.z + row * a.ldz, cols, there, inner);
+        gr[k][i] = c[i].load((const T*)a.dy + row * a.lddy, cols, there, inner);
+        if (a.dz) ur[k][i] = c[i].load((const T*)a.dz + row * a.lddz, cols, there, inner);
       }
+      mean[k] = there ? a.mean[row] : 0.f, rstd[k] = there ? a.rstd[row] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        float z[V], g[V];
+        unpack<T>(zr[k][i], z);
+        unpack<T>(gr[k][i], g);   // zeros outside the row
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float h = (z[j] - mean[k]) * rstd[k], gw = g[j] * w[i][j];
+          dw[i][j] = fmaf(g[j], h, dw[i][j]);
+          db[i][j] += g[j];
+          s1 += gw;
+          s2 = fmaf(gw, h, s2);
+        }
+      }
+      s[2 * k] = s1, s[2 * k + 1] = s2;
     }
     if (!a.dx) continue;
-    if (NW == 1) {
-      s1 = warp_sum(s1), s2 = warp_sum(s2);
-    } else {   // both sums behind one barrier; the next row's go to the other half
-      s1 = warp_sum(s1), s2 = warp_sum(s2);
-      if ((threadIdx.x & 31) == 0) part[turn][warp] = s1, part[turn + 1][warp] = s2;
-      __syncthreads();
-      s1 = s2 = 0.f;
+    row_sums<NW>(s, part[turn], warp);   // one barrier a turn: the halves take turns
 #pragma unroll
-      for (int i = 0; i < NW; ++i) s1 += part[turn][i], s2 += part[turn + 1][i];
-    }
-    s1 *= inv, s2 *= inv;
-    T* dx = (T*)a.dx + row * a.cols;
+    for (int k = 0; k < R; ++k) {
+      const int64_t row = row0 + k * step;
+      // rstd (g w - mean(g w) - h mean(g w h)), with h = (z - mean) rstd
+      const float s1 = -s[2 * k] * inv * rstd[k], s2 = s[2 * k + 1] * inv * rstd[k] * rstd[k];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      float z[V], g[V], d[V], up[V];
-      unpack<T>(zr[i], z);
-      unpack<T>(gr[i], g);
-      if (a.dz) unpack<T>(load_piece((const T*)a.dz + row * a.lddz, c[i], cols), up);
+      for (int i = 0; i < CH; ++i) {
+        float z[V], g[V], d[V], up[V];
+        forget(zr[k][i]);
+        forget(gr[k][i]);
+        unpack<T>(zr[k][i], z);
+        unpack<T>(gr[k][i], g);
+        if (a.dz) unpack<T>(ur[k][i], up);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (z[j] - mean) * rstd;
-        d[j] = rstd * (fmaf(g[j], w[i][j], -s1) - h * s2);
-        if (a.dz) d[j] += up[j];
+        for (int j = 0; j < V; ++j) {
+          d[j] = fmaf(mean[k] - z[j], s2, fmaf(g[j], w[i][j] * rstd[k], s1));
+          if (a.dz) d[j] += up[j];
+        }
+        c[i].store((T*)a.dx + row * a.cols, cols, row < a.rows, pack<T>(d));
       }
-      store_piece(dx, c[i], cols, d);
     }
   }
   if (!a.dweight && !a.dbias) return;
@@ -369,6 +404,7 @@ Split split_of(int64_t cols, bool ragged) {
   if (n <= 128) return {4, 1};
   if (n <= 256) return {4, 2};
   if (n <= 512) return {8, 2};
+  if (n <= 768) return {8, 3};
   if (n <= 1024) return {16, 2};
   if (n <= 2048) return {16, 4};
   return {0, 0};
@@ -410,23 +446,23 @@ unsigned ctas_for(int64_t rows, int groups, int per_sm, bool ragged) {
   return (unsigned)(n < most ? n : most);
 }
 
-template <typename T, typename W, int NW, int CH>
-int forward_rows(const HpNormForward& a, bool ragged, cudaStream_t s) {
+template <typename T, int NW, int CH, bool RAGGED>
+int forward_rows(const HpNormForward& a, cudaStream_t s) {
   constexpr int kThreads = kThreadsOf<NW>, kGroups = kThreads / (32 * NW);
-  static const int per_sm = resident(norm_forward_rows<T, W, NW, CH>, kThreads, 0);
-  norm_forward_rows<T, W, NW, CH><<<ctas_for(a.rows, kGroups, per_sm, ragged), kThreads, 0, s>>>(a, ragged);
+  static const int per_sm = resident(norm_forward_rows<T, NW, CH, RAGGED>, kThreads, 0);
+  norm_forward_rows<T, NW, CH, RAGGED><<<ctas_for(a.rows, kGroups, per_sm, RAGGED), kThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
-template <typename T, typename W, int NW, int CH>
-int backward_rows(const HpNormBackward& a, bool ragged, cudaStream_t s) {
+template <typename T, int NW, int CH, bool RAGGED>
+int backward_rows(const HpNormBackward& a, cudaStream_t s) {
   constexpr int kThreads = kThreadsOf<NW>, kGroups = kThreads / (32 * NW);
   const int smem = kGroups > 1 ? (int)(8 * a.cols) : 0;
-  static const int per_sm = resident(norm_backward_rows<T, W, NW, CH>, kThreads, kGroups > 1 ? 8 * 32 * CH * kPiece<T> : 0);
-  const unsigned grid = ctas_for(a.rows, kGroups, per_sm, ragged);
-  norm_backward_rows<T, W, NW, CH><<<grid, kThreads, smem, s>>>(a, ragged);
-  if (!a.dweight && !a.dbias) return cudaGetLastError();
+  static const int per_sm = resident(norm_backward_rows<T, NW, CH, RAGGED>, kThreads, kGroups > 1 ? 8 * 32 * CH * kPiece<T> : 0);
+  const unsigned grid = ctas_for(a.rows, kGroups, per_sm, RAGGED);
+  norm_backward_rows<T, NW, CH, RAGGED><<<grid, kThreads, smem, s>>>(a);
   const int rc = cudaGetLastError();
-  return rc ? rc : column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);
+  if (rc || (!a.dweight && !a.dbias)) return rc;
+  return column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);
 }
 
 #define BY_SPLIT(call)                          \
@@ -436,12 +472,13 @@ int backward_rows(const HpNormBackward& a, bool ragged, cudaStream_t s) {
     case 4 * 8 + 1: return call(4, 1);          \
     case 4 * 8 + 2: return call(4, 2);          \
     case 8 * 8 + 2: return call(8, 2);          \
+    case 8 * 8 + 3: return call(8, 3);          \
     case 16 * 8 + 2: return call(16, 2);        \
     case 16 * 8 + 4: return call(16, 4);        \
     default: break;                             \
   }
 
-template <typename T, typename W>
+template <typename T>
 int forward(const HpNormForward& a, cudaStream_t s) {
   Rows r(sizeof(T));
   r.add(a.x, a.ldx);
@@ -450,14 +487,14 @@ int forward(const HpNormForward& a, cudaStream_t s) {
   r.add(a.z, a.cols);
   if (r.alike) {
     const Split p = split_of<T>(a.cols, r.ragged());
-#define CALL(nw, ch) forward_rows<T, W, nw, ch>(a, r.ragged(), s)
+#define CALL(nw, ch) r.ragged() ? forward_rows<T, nw, ch, true>(a, s) : forward_rows<T, nw, ch, false>(a, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
   norm_forward_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
-template <typename T, typename W>
+template <typename T>
 int backward(const HpNormBackward& a, cudaStream_t s) {
   Rows r(sizeof(T));
   r.add(a.z, a.ldz);
@@ -466,7 +503,7 @@ int backward(const HpNormBackward& a, cudaStream_t s) {
   r.add(a.dx, a.cols);
   if (r.alike && a.rows) {
     const Split p = split_of<T>(a.cols, r.ragged());
-#define CALL(nw, ch) backward_rows<T, W, nw, ch>(a, r.ragged(), s)
+#define CALL(nw, ch) r.ragged() ? backward_rows<T, nw, ch, true>(a, s) : backward_rows<T, nw, ch, false>(a, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
@@ -485,11 +522,7 @@ bool types_ok(const A& a) {
 
 using namespace hipress;
 
-#define BY_TYPE(fn)                                                                              \
-  a->type == HP_F32    ? fn<float, float>(*a, s)                                                 \
-  : a->type == HP_BF16 ? (a->wtype == HP_F32 ? fn<__nv_bfloat16, float>(*a, s)                   \
-                                             : fn<__nv_bfloat16, __nv_bfloat16>(*a, s))          \
-                       : (a->wtype == HP_F32 ? fn<__half, float>(*a, s) : fn<__half, __half>(*a, s))
+#define BY_TYPE(fn) a->type == HP_F32 ? fn<float>(*a, s) : a->type == HP_BF16 ? fn<__nv_bfloat16>(*a, s) : fn<__half>(*a, s)
 
 extern "C" int hp_cuda_norm_forward(const HpNormForward* a, void* stream) {
   if (!a || a->rows < 0 || a->cols < 1 || a->rows > INT32_MAX || !types_ok(*a) || (a->residual && !a->z))

@@ -23,6 +23,55 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
+// two values in one register
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *(const uint32_t*)&v;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *(const uint32_t*)&v;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {   // the upper half of a float
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*(const __half2*)&v);
+}
+
+// 16 bytes of elements, in 32 bits
+template <typename T>
+constexpr int kPiece = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 raw, float (&v)[kPiece<T>]) {
+  const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(r[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void unpack<float>(uint4 raw, float (&v)[4]) {
+  v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y), v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&v)[kPiece<T>]) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+template <>
+__device__ __forceinline__ uint4 pack<float>(const float (&v)[4]) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+
 // element i of an array whose type is known at run time (uniform over the launch)
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int type) {
   return type == HP_F32 ? ((const float*)p)[i]

@@ -8,6 +8,15 @@ namespace hipress {
 namespace {
 
 
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { using type = uint4; };
+template <>
+struct Word<4> { using type = uint32_t; };
+template <>
+struct Word<2> { using type = uint16_t; };
+
 // ------------------------------------------------------------------- the product
 // A persistent kernel of specialised warps: one thread fetches tiles (TMA), one issues the
 // matrix products, eight warps empty the accumulators.  Two accumulators in tensor memory: the
@@ -15,25 +24,26 @@ namespace {
 //   CG  CTAs that share a tile: 1, or 2 (each holds half of both operands and 128 rows of results)
 //   BN  columns of a tile; it has 128 CG rows
 constexpr int kBK = 64;            // k of a stage: one line of the swizzle
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps);
-constexpr int kStaging = 4096;     // of a warp: 32 rows of 128 bytes
+constexpr int kStaging = 4096;     // a warp has two of 32 rows of 128 bytes
 
 template <int CG, int BN>
 struct Shape {
   static constexpr int kRowsB = BN / CG;
   static constexpr int kBytesA = 128 * 128, kBytesB = kRowsB * 128, kStage = kBytesA + kBytesB;
-  static constexpr int kStages = (kStage <= 24576 ? 6 : kStage <= 32768 ? 5 : 3);
-  static constexpr int kSmem = kStages * kStage + kEpiWarps * (kStaging + 256) + 1024 + 256;
+  static constexpr int kStages = kStage <= 24576 ? 6 : 4;
+  // warps that empty an accumulator: each 32 rows of all columns, or of one half of them
+  static constexpr int kEpiWarps = BN >= 128 ? 8 : 4, kCols = BN * 4 / kEpiWarps;
+  static constexpr int kThreads = 32 * (2 + kEpiWarps);
+  static constexpr int kSmem = kStages * kStage + kEpiWarps * (2 * kStaging + kCols * 4) + 512 + 1024;
   static constexpr int kTmem = 2 * BN;
 };
 
 struct Launch {
-  CUtensorMap a, b;
+  CUtensorMap a, b, y, pre;  // y: the partial sums where k is split
   HpProduct p;
   int64_t ldp;               // pitch of the partial sums
   int tiles_m, tiles_n, kblocks, splits;
-  int vec_y, vec_r;          // elements of an aligned access of y and pre, of residual
+  int vec_y, vec_r;          // bytes of an aligned access to y and pre, to the residual
   uint32_t* status;
 };
 
@@ -59,78 +69,61 @@ __device__ __forceinline__ Unit unit_of(const Launch& l, int u, int bm, int bn) 
   return w;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-  return *(const uint32_t*)&v;
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-  const __half2 v = __floats2half2_rn(x, y);
-  return *(const uint32_t*)&v;
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-  return __bfloat1622float2(*(const __nv_bfloat162*)&v);
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-  return __half22float2(*(const __half2*)&v);
-}
-
-// byte `b` of row `r` of a warp's staging rows of 128 bytes: 16-byte pieces change places
-// from row to row, so that a column of rows lies in different banks
+// byte `b` of row `r` of a warp's staging rows, as the 128-byte swizzle of a TMA store has it
 __device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r * 128 + (b ^ ((r & 7) << 4))); }
 
-// The warp's 32 rows of 128 bytes between shared and global memory, along the rows: V bytes to
-// an access.  Rows below `rows` and bytes below `width` only.
-template <int V, bool STORE>
-__device__ __forceinline__ void move_rows(uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
-  constexpr int kLanes = 128 / V >= 32 ? 32 : 128 / V, kAtOnce = 32 / kLanes, kCols = 128 / (V * kLanes);
-#pragma unroll V == 16 ? 8 : 1
-  for (int i = 0; i < 32 / kAtOnce; ++i) {
-    const int r = i * kAtOnce + lane / kLanes;
+// A warp's 32 staged rows of 128 bytes to rows that TMA cannot address: V bytes an access.
+// Rows below `rows` and bytes below `width` only.
+template <int V>
+__device__ __forceinline__ void store_rows(const uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
+  using Raw = typename Word<V>::type;
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r)
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      const int b = (c * kLanes + lane % kLanes) * V;
-      uint8_t* at = s + staged(r, b);
+    for (int b = lane * V; b < 128; b += 32 * V) {
+      const uint8_t* at = s + staged(r, b);
       uint8_t* to = g + r * pitch + b;
-      if (r < rows && b + V <= width) {
-        if (V == 16) {
-          if (STORE) *(uint4*)to = *(uint4*)at;
-          else *(uint4*)at = *(const uint4*)to;
-        } else if (V == 4) {
-          if (STORE) *(uint32_t*)to = *(uint32_t*)at;
-          else *(uint32_t*)at = *(const uint32_t*)to;
-        } else {
-          if (STORE) *(uint16_t*)to = *(uint16_t*)at;
-          else *(uint16_t*)at = *(const uint16_t*)to;
-        }
-      } else if (V > 2 && r < rows) {   // the row ends inside the access
-#pragma unroll
-        for (int e = 0; e < V; e += 2)
-          if (b + e < width) {
-            if (STORE) *(uint16_t*)(to + e) = *(uint16_t*)(at + e);
-            else *(uint16_t*)(at + e) = *(const uint16_t*)(to + e);
-          }
-      }
+      if (b + V <= width) *(Raw*)to = *(const Raw*)at;
+      else if (V == 4 && b + 2 <= width) *(uint16_t*)to = *(const uint16_t*)at;
     }
+}
+__device__ __noinline__ void store_ragged(int vec, const uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
+  if (vec >= 4) store_rows<4>(s, g, pitch, rows, width, lane);
+  else store_rows<2>(s, g, pitch, rows, width, lane);
+}
+
+// Emptied staging rows leave through a tensor map, or by plain stores where y has no 16-byte
+// rows.  Two buffers take turns.
+struct Out {
+  uint8_t* base;
+  int turn;
+  __device__ __forceinline__ uint8_t* buffer() const { return base + turn * kStaging; }
+  // before the buffer is filled: what was stored from it has been read
+  __device__ __forceinline__ void ready(int lane) const {
+    if (lane == 0) tma_store_wait_read<1>();
+    __syncwarp();
   }
-}
-template <bool STORE>   // rows that are not on 16-byte boundaries: kept out of the way of the others
-__device__ __noinline__ void move_ragged_rows(int vec, uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
-  if (vec == 4) move_rows<4, STORE>(s, g, pitch, rows, width, lane);
-  else move_rows<2, STORE>(s, g, pitch, rows, width, lane);
-}
-template <bool STORE>
-__device__ __forceinline__ void move_rows(int vec, uint8_t* s, uint8_t* g, int64_t pitch, int rows, int width, int lane) {
-  if (vec == 16) move_rows<16, STORE>(s, g, pitch, rows, width, lane);
-  else move_ragged_rows<STORE>(vec, s, g, pitch, rows, width, lane);
-}
+  __device__ __forceinline__ void send(const Launch& l, const CUtensorMap& map, void* plain, int64_t pitch, int bytes,
+                                       int row0, int col0, int split, int lane) {
+    const HpProduct& p = l.p;
+    if (l.vec_y == 16) {
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        if (row0 < p.m && col0 < p.n) tma_store_3d(&map, buffer(), col0, row0, split);
+        tma_store_commit();
+      }
+    } else {
+      __syncwarp();
+      const int64_t rows = p.m - row0, width = (p.n - col0) * bytes;
+      if (rows > 0 && width > 0)
+        store_ragged(l.vec_y, buffer(), (uint8_t*)plain + (row0 * pitch + col0) * bytes, pitch * bytes,
+                     rows < 32 ? (int)rows : 32, width < 128 ? (int)width : 128, lane);
+      __syncwarp();
+    }
+    turn ^= 1;
+  }
+};
 
 template <int ACT, int N>
 __device__ __forceinline__ void activate_all(float (&v)[N]) {
@@ -144,125 +137,52 @@ __device__ __forceinline__ void activate_all(int act, float (&v)[N]) {
   else if (act == HP_ACT_GELU_TANH) activate_all<HP_ACT_GELU_TANH>(v);
 }
 
-// 32 columns of 32 rows as they are, in 32 bits: partial sums, or a result of that type
-__device__ __forceinline__ void emit32(const Launch& l, uint8_t* stage, uint32_t acc, int row0, int col0, int split,
-                                       int lane, bool last, uint64_t* release, uint32_t remote) {
+// Sixteen pairs of residuals of one row, zeros where there are none.
+template <typename T>
+__device__ __forceinline__ void load_residual(const Launch& l, int row, int col, uint32_t (&r)[16]) {
   const HpProduct& p = l.p;
-  const int rows = (int)min((int64_t)32, p.m - row0), cols = (int)min((int64_t)32, p.n - col0);
-  uint32_t r[32];
-  tmem_ld32(acc, r);
-  tmem_wait_ld();
-  if (last) {
-    tmem_fence_before();
-    if (lane == 0) {
-      if (release) mbar_arrive(release);
-      else mbar_arrive_cluster(remote);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = 0;
+  if (!p.residual || row >= p.m) return;
+  const T* from = (const T*)p.residual + row * p.ldr + col;
+  if (l.vec_r == 16 && col + 32 <= p.n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 q = *(const uint4*)(from + 8 * i);
+      r[4 * i] = q.x, r[4 * i + 1] = q.y, r[4 * i + 2] = q.z, r[4 * i + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t lo = col + 2 * i < p.n ? *(const uint16_t*)(from + 2 * i) : 0;
+      const uint32_t hi = col + 2 * i + 1 < p.n ? *(const uint16_t*)(from + 2 * i + 1) : 0;
+      r[i] = lo | hi << 16;
     }
   }
-  if (rows <= 0 || cols <= 0) return;
-#pragma unroll
-  for (int i = 0; i < 32; i += 4) *(uint4*)(stage + staged(lane, 4 * i)) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-  __syncwarp();
-  float* out = l.splits == 1 ? (float*)p.y + row0 * p.ldy + col0
-                             : (float*)p.workspace + ((int64_t)split * p.m + row0) * l.ldp + col0;
-  const int64_t pitch = 4 * (l.splits == 1 ? p.ldy : l.ldp);
-  move_rows<true>(l.splits == 1 ? l.vec_y : 16, stage, (uint8_t*)out, pitch, rows, 4 * cols, lane);
-  __syncwarp();
-}
-
-// 64 columns of 32 rows in the operands' type
-template <typename T, int COLS>
-__device__ __forceinline__ void emit16(const Launch& l, uint8_t* stage, const float* bias, uint32_t acc, int row0,
-                                       int col0, int lane, bool last, uint64_t* release, uint32_t remote) {
-  const HpProduct& p = l.p;
-  const int rows = (int)min((int64_t)32, p.m - row0), cols = (int)min((int64_t)COLS, p.n - col0);
-  const bool some = rows > 0 && cols > 0;
-  if (some && p.residual) {
-    move_rows<false>(l.vec_r, stage, (uint8_t*)((T*)p.residual + row0 * p.ldr + col0), 2 * p.ldr, rows, 2 * cols, lane);
-    __syncwarp();
-  }
-  uint32_t y[COLS / 2];
-#pragma unroll
-  for (int h = 0; h < COLS; h += 32) {
-    uint32_t r[32];
-    tmem_ld32(acc + h, r);
-    uint32_t res[16];
-    if (some && p.residual)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const uint4 q = *(const uint4*)(stage + staged(lane, 2 * h + 4 * i));
-        res[i] = q.x, res[i + 1] = q.y, res[i + 2] = q.z, res[i + 3] = q.w;
-      }
-    tmem_wait_ld();
-    if (last && h + 32 == COLS) {
-      tmem_fence_before();
-      if (lane == 0) {
-        if (release) mbar_arrive(release);
-        else mbar_arrive_cluster(remote);
-      }
-    }
-    if (!some) continue;
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 b = *(const float4*)(bias + h + i);
-      v[i] = __uint_as_float(r[i]) + b.x;
-      v[i + 1] = __uint_as_float(r[i + 1]) + b.y;
-      v[i + 2] = __uint_as_float(r[i + 2]) + b.z;
-      v[i + 3] = __uint_as_float(r[i + 3]) + b.w;
-    }
-    if (p.pre) {   // this thread has read its residuals of these columns
-#pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        *(uint4*)(stage + staged(lane, 2 * (h + i))) = make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]),
-                                                                  pack2<T>(v[i + 4], v[i + 5]), pack2<T>(v[i + 6], v[i + 7]));
-    }
-    activate_all(p.act, v);
-    if (p.residual)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 q = unpack2<T>(res[i]);
-        v[2 * i] += q.x;
-        v[2 * i + 1] += q.y;
-      }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[h / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-  }
-  if (!some) return;
-  if (p.pre) {
-    __syncwarp();
-    move_rows<true>(l.vec_y, stage, (uint8_t*)((T*)p.pre + row0 * p.ldy + col0), 2 * p.ldy, rows, 2 * cols, lane);
-    __syncwarp();
-  }
-#pragma unroll
-  for (int i = 0; i < COLS / 2; i += 4)
-    *(uint4*)(stage + staged(lane, 4 * i)) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-  __syncwarp();
-  move_rows<true>(l.vec_y, stage, (uint8_t*)((T*)p.y + row0 * p.ldy + col0), 2 * p.ldy, rows, 2 * cols, lane);
-  __syncwarp();
 }
 
 template <typename T, int CG, int BN>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Launch l) {
+__global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(const __grid_constant__ Launch l) {
   using S = Shape<CG, BN>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + S::kStages * S::kStage;
-  float* biases = (float*)(staging + kEpiWarps * kStaging);
-  Bars& bar = *(Bars*)(biases + kEpiWarps * 64);
+  float* biases = (float*)(staging + S::kEpiWarps * 2 * kStaging);   // [kEpiWarps][kCols]
+  Bars& bar = *(Bars*)(biases + S::kEpiWarps * S::kCols);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const HpProduct& p = l.p;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(&bar.full[i], 1), mbar_init(&bar.empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], CG * kEpiWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.acc_full[i], 1), mbar_init(&bar.acc_empty[i], CG * S::kEpiWarps);
     mbar_init(&bar.drain, 1);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
     tma_prefetch(&l.a);
     tma_prefetch(&l.b);
+    if (l.vec_y == 16) tma_prefetch(&l.y);
   }
   if (warp == 1) tmem_alloc<CG>(&bar.tmem, S::kTmem);
   tmem_fence_before();
@@ -348,35 +268,101 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     }
   } else {
     const int e = warp - 2, quad = warp & 3, half = e >> 2;
-    uint8_t* stage = staging + e * kStaging;
-    float* bias = biases + e * 64;
-    constexpr int kCols = BN / 2, kChunk = kCols >= 64 ? 64 : 32;
+    const int base = half * S::kCols;          // this warp's columns of a tile
+    const bool raw = l.splits > 1 || p.ytype == HP_F32;   // the sums as they are, in 32 bits
+    Out out = {staging + e * 2 * kStaging, 0};
     int it = 0;
     for (int u = first; u < units; u += step, ++it) {
       const Unit w = unit_of(l, u, 128 * CG, BN);
-      const int acc = it & 1;
+      const int acc = it & 1, row0 = w.m0 + 128 * (int)rank + 32 * quad, col = w.n0 + base;
+      const uint32_t from = tmem + acc * BN + base + ((uint32_t)(32 * quad) << 16);
+      auto release = [&] {   // the accumulator has been read
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 2) mbar_arrive_cluster(cluster_addr(&bar.acc_empty[acc], 0));
+          else mbar_arrive(&bar.acc_empty[acc]);
+        }
+      };
+      if (raw) {
+        if (!guard_wait(&bar.acc_full[acc], (it >> 1) & 1, g, 0x50000)) break;
+        tmem_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < S::kCols; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(from + c, r);
+          out.ready(lane);
+          tmem_wait_ld();
+          if (c + 32 == S::kCols) release();
+          uint8_t* to = out.buffer();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *(uint4*)(to + staged(lane, 4 * i)) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          out.send(l, l.y, p.y, p.ldy, 4, row0, col + c, w.split, lane);
+        }
+        continue;
+      }
+      // bias and the first residuals come while the products still run
+      float* bias = biases + e * S::kCols;
+      if (p.bias)
+        for (int i = lane; i < S::kCols; i += 32) bias[i] = col + i < p.n ? load_any(p.bias, col + i, (int)p.btype) : 0.f;
+      uint32_t next[16];
+      load_residual<T>(l, row0 + lane, col, next);
       if (!guard_wait(&bar.acc_full[acc], (it >> 1) & 1, g, 0x50000)) break;
       tmem_fence_after();
-      const int row0 = w.m0 + 128 * (int)rank + 32 * quad;
-      uint64_t* release = CG == 2 ? nullptr : &bar.acc_empty[acc];
-      const uint32_t remote = CG == 2 ? cluster_addr(&bar.acc_empty[acc], 0) : 0;
-      const bool wide = l.splits > 1 || p.ytype == HP_F32;
-      for (int c = 0; c < kCols; c += kChunk) {
-        const int col0 = w.n0 + half * kCols + c;
-        const uint32_t at = tmem + acc * BN + half * kCols + c + ((uint32_t)(32 * quad) << 16);
-        const bool last = c + kChunk == kCols;
-        for (int i = lane; i < kChunk; i += 32)
-          bias[i] = p.bias && col0 + i < p.n ? load_any(p.bias, col0 + i, (int)p.btype) : 0.f;
-        __syncwarp();
-        if (wide) {
-          for (int h = 0; h < kChunk; h += 32)
-            emit32(l, stage, at + h, row0, col0 + h, w.split, lane, last && h + 32 == kChunk, release, remote);
-        } else {
-          emit16<T, kChunk>(l, stage, bias, at, row0, col0, lane, last, release, remote);
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; c < S::kCols; c += 64) {
+        uint32_t y[32];
+#pragma unroll
+        for (int h = 0; h < 64; h += 32) {
+          uint32_t r[32], res[16];
+          tmem_ld32(from + c + h, r);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) res[i] = next[i];
+          if (c + h + 32 < S::kCols) load_residual<T>(l, row0 + lane, col + c + h + 32, next);
+          if (h == 0) out.ready(lane);
+          tmem_wait_ld();
+          if (c + h + 32 == S::kCols) release();
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          if (p.bias)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 b = *(const float4*)(bias + c + h + i);
+              v[i] += b.x, v[i + 1] += b.y, v[i + 2] += b.z, v[i + 3] += b.w;
+            }
+          if (p.pre) {
+            uint8_t* to = out.buffer();
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              *(uint4*)(to + staged(lane, 2 * (h + i))) =
+                  make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
+                             pack2<T>(v[i + 6], v[i + 7]));
+          }
+          activate_all(p.act, v);
+          if (p.residual)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 q = unpack2<T>(res[i]);
+              v[2 * i] += q.x, v[2 * i + 1] += q.y;
+            }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[h / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
         }
-        __syncwarp();
+        if (p.pre) {
+          out.send(l, l.pre, p.pre, p.ldy, 2, row0, col + c, 0, lane);
+          out.ready(lane);
+        }
+        uint8_t* to = out.buffer();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *(uint4*)(to + staged(lane, 4 * i)) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        out.send(l, l.y, p.y, p.ldy, 2, row0, col + c, 0, lane);
       }
     }
+    if (lane == 0) tma_store_wait_read<0>();   // before the shared memory goes
   }
   __syncwarp();
   __syncthreads();
@@ -460,6 +446,16 @@ int run_product(Launch& l, int sms, cudaStream_t s) {
   if (!map(&l.a, p.a, p.m, p.lda, p.a_kmajor, p.a_kmajor ? box_k : box_m) ||
       !map(&l.b, p.b, p.n, p.ldb, p.b_kmajor, p.b_kmajor ? box_kb : box_m))
     return HP_ERR_BAD_ARG;
+  if (l.vec_y == 16) {
+    const bool split = l.splits > 1, wide = split || p.ytype == HP_F32;
+    const uint64_t e = wide ? 4 : 2, row = e * (uint64_t)(split ? l.ldp : p.ldy);
+    const uint64_t size[3] = {(uint64_t)p.n, (uint64_t)p.m, (uint64_t)l.splits};
+    const uint64_t pitch[2] = {p.m > 1 ? row : 16, p.m > 1 ? row * (uint64_t)p.m : split ? row : 16};
+    const uint32_t box[3] = {(uint32_t)(128 / e), 32, 1};
+    if (!tensor_map(&l.y, split ? p.workspace : p.y, wide ? HP_F32 : (int)p.type, 3, size, pitch, box) ||
+        (p.pre && !split && !tensor_map(&l.pre, p.pre, (int)p.type, 3, size, pitch, box)))
+      return HP_ERR_BAD_ARG;
+  }
   static const cudaError_t allowed =
       cudaFuncSetAttribute(product_kernel<T, CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (allowed != cudaSuccess) return allowed;
@@ -470,7 +466,7 @@ int run_product(Launch& l, int sms, cudaStream_t s) {
   const int64_t slots = sms / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * (units < slots ? units : slots)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -505,6 +501,7 @@ int product(const HpProduct& a, cudaStream_t s) {
   if (a.k) {
     const Choice c = choose(a.m, a.n, l.kblocks, sms);
     l.splits = c.splits;
+    if (l.splits > 1) l.vec_y = 16;   // the partial sums' rows
     rc = c.cg == 2 ? (c.bn == 256 ? run_product<T, 2, 256>(l, sms, s) : run_product<T, 2, 128>(l, sms, s))
                    : (c.bn == 128 ? run_product<T, 1, 128>(l, sms, s) : run_product<T, 1, 64>(l, sms, s));
     if (rc) return rc;
@@ -521,15 +518,6 @@ int product(const HpProduct& a, cudaStream_t s) {
 // thread has V columns (16 bytes where all rows lie on that boundary, else 4 or 2) and the rows
 // of its warp; the CTA's eight warps add up their sums, and leave one row of partial sums.
 constexpr int kSlopeWarps = 8;
-
-template <int BYTES>
-struct Word;
-template <>
-struct Word<16> { using type = uint4; };
-template <>
-struct Word<4> { using type = uint32_t; };
-template <>
-struct Word<2> { using type = uint16_t; };
 
 template <typename T, int ACT, int V>
 __global__ void __launch_bounds__(32 * kSlopeWarps) slope_kernel(const __grid_constant__ HpSlope a) {

@@ -89,6 +89,18 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+// shared -> global; outside the tensor nothing is written
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(m), "r"(x),
+               "r"(y), "r"(z), "r"(smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>   // all but the last N groups have read what they store
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
 // ------------------------------------------------------------- tensor memory
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {   // one whole warp
@@ -167,8 +179,8 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 }
 
 // ------------------------------------------------------------------- host side
-// A tensor of `rank` axes (the first one dense) in boxes, swizzled by 128 bytes; elements of
-// 16 bits, outside the tensor zeros.  False where the driver refuses it.
+// A tensor of `rank` axes (the first one dense) in boxes of 128 bytes by rows, swizzled;
+// loads read zeros outside it.  False where the driver refuses it.
 bool tensor_map(CUtensorMap* m, const void* base, int type, int rank, const uint64_t* sizes, const uint64_t* strides_bytes,
                 const uint32_t* box);
 
