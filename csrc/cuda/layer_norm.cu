@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256) norm_forward_kernel(const __grid_constant
     const float d = value(i) - mean;
     s = fmaf(d, d, s);
   }
-  const float rstd = 1.f / sqrtf(cta_sum(s, part) / (float)a.cols + (float)a.eps);
+  const float rstd = rsqrtf(cta_sum(s, part) / (float)a.cols + (float)a.eps);
   for (int64_t i = threadIdx.x; i < a.cols; i += blockDim.x) {
     const float v = value(i);
     float o = (v - mean) * rstd;
@@ -88,58 +88,56 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const __grid_constant__ Hp
   }
 }
 
-// ------------------------------------------------------------- rows in registers
-// NW warps share a row, each thread CH pieces of 16 bytes of it.  A thread keeps its columns
-// from row to row, and with them the weights and (backward) the sums of the weights' gradients.
-// Rows whose first element is not on a 16-byte boundary are cut at the boundaries all the
-// same: the pieces start `phase` elements ahead of the row, and what is outside the row is left
-// out.  The phase goes by the row modulo the elements of a piece, and the rows of one group
-// of warps are that far apart, so that its columns stay the same.
-// The columns that a thread's piece covers.  Unless RAGGED a piece is in the row or behind it.
+// ------------------------------------------------------------- rows through shared memory
+// NW warps share a row, each thread CH pieces of 16 bytes of it.  Whole rows are fetched ahead by
+// bulk copies into a ring of `depth` slots, so that what is in flight does not cost registers;
+// a thread keeps its columns from row to row, and with them the weights and (backward) the sums
+// of the weights' gradients.  With plain loads into registers the forward pass of 65536 x 1024
+// bf16 took 69 to 86 us, however many rows were loaded ahead.
+//
+// Rows whose first element is not on a 16-byte boundary (RAGGED) are cut at the boundaries all
+// the same: the pieces start `phase` elements ahead of the row, and what is outside the row is
+// cleared.  The phase goes by the row modulo the elements of a piece, and the rows of one group
+// of warps are a multiple of eight apart, so that its columns stay the same.  The first and the
+// last row have no neighbour to be read along with them and are loaded element by element.
 template <typename T, bool RAGGED>
 struct Piece {
   static constexpr int V = kPiece<T>, kBits = 8 * sizeof(T);
-  int first;
+  int first;   // column of its first element
   __device__ __forceinline__ bool whole(int cols) const {
     return RAGGED ? first >= 0 && first + V <= cols : first < cols;
   }
   __device__ __forceinline__ bool has(int j, int cols) const {
     return RAGGED ? first + j >= 0 && first + j < cols : first < cols;
   }
-  __device__ __forceinline__ void load_weights(const void* p, int type, int cols, float none, float (&v)[V]) const {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = p && has(j, cols) ? load_any(p, first + j, type) : none;
-  }
-  // Zeros outside the row.  A piece at an end of it: where the rows next to this one are there
-  // (`inner`; and no row is shorter than a piece) it is loaded whole and what is not the row's
-  // is cleared; else it goes element by element, shifted through its 128 bits: few registers
-  // for what few threads do.
-  __device__ __forceinline__ uint4 load(const T* row, int cols, bool there, bool inner) const {
+  // from a slot whose first 16 bytes hold the row's first element; zeros outside the row
+  __device__ __forceinline__ uint4 take(const uint8_t* slot, int cols, int phase) const {
     uint4 raw = make_uint4(0, 0, 0, 0);
-    if (!there) return raw;
-    if (whole(cols)) return __ldg((const uint4*)(row + first));
-    if (!RAGGED || first >= cols) return raw;
-    T* v = (T*)&raw;
-    if (inner && cols >= V) {
-      raw = __ldg((const uint4*)(row + first));
+    if (first >= cols) return raw;
+    raw = *(const uint4*)(slot + (first + phase) * (int)sizeof(T));
+    if (RAGGED && !whole(cols)) {
+      T* v = (T*)&raw;
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (!has(j, cols)) v[j] = from_f<T>(0.f);
-      return raw;
     }
+    return raw;
+  }
+  // the same element by element, shifted through 128 bits: few registers for what is rare
+  __device__ __forceinline__ uint4 take_from(const T* row, int cols) const {
     uint64_t lo = 0, hi = 0;
+    if (first < cols)
 #pragma unroll 1
-    for (int j = 0; j < V; ++j) {
-      T e = from_f<T>(0.f);
-      if (has(j, cols)) e = row[first + j];
-      const uint64_t bits = sizeof(T) == 4 ? *(const uint32_t*)&e : *(const uint16_t*)&e;
-      lo = lo >> kBits | hi << (64 - kBits);
-      hi = hi >> kBits | bits << (64 - kBits);
-    }
+      for (int j = 0; j < V; ++j) {
+        T e = from_f<T>(0.f);
+        if (has(j, cols)) e = row[first + j];
+        const uint64_t bits = sizeof(T) == 4 ? *(const uint32_t*)&e : *(const uint16_t*)&e;
+        lo = lo >> kBits | hi << (64 - kBits);
+        hi = hi >> kBits | bits << (64 - kBits);
+      }
     return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
-  __device__ __forceinline__ void store(T* row, int cols, bool there, uint4 raw) const {
-    if (!there) return;
+  __device__ __forceinline__ void store(T* row, int cols, uint4 raw) const {
     if (whole(cols)) {
       *(uint4*)(row + first) = raw;
       return;
@@ -158,8 +156,52 @@ struct Piece {
   }
 };
 
-// Sums over the NW warps that share a row, of N values together behind one barrier; `part` is
-// theirs until the barrier after the next.
+constexpr int kMostSlots = 8;
+template <int NW>
+constexpr int kThreadsOf = 32 * (NW < 4 ? 4 : NW);
+template <int NW>
+constexpr int kGroupsOf = kThreadsOf<NW> / (32 * NW);
+
+// A row of weights in 32 bits, in shared memory: pieces of four, so that lanes read next to
+// each other (a piece's first half here, its second half `half` further on).  Threads whose rows start at
+// different phases (groups of one warp, RAGGED) each need other columns and read global memory.
+template <typename T, bool RAGGED, int NW>
+struct Weights {
+  static constexpr int V = kPiece<T>;
+  static constexpr bool kShared = !RAGGED || kGroupsOf<NW> == 1;
+  const void* global;
+  int type, half;
+  float none;
+  float4* shared;
+  __device__ __forceinline__ void place(const void* p, int t, float otherwise, int cols, int phase, float4* space) {
+    global = p, type = t, none = otherwise, shared = space;
+    half = (cols + phase + V - 1) / V;
+    if (!kShared || !p) return;
+    for (int i = threadIdx.x; i < half * V; i += blockDim.x) {
+      const int c = i - phase;
+      const float v = c >= 0 && c < cols ? load_any(p, c, type) : 0.f;
+      ((float*)(shared + (i % V / 4) * half + i / V))[i % 4] = v;
+    }
+  }
+  __device__ __forceinline__ void get(Piece<T, RAGGED> c, int cols, int phase, float (&v)[V]) const {
+    if (!global) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = none;
+    } else if (kShared) {
+      const int piece = c.first < cols ? (c.first + phase) / V : 0;
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        const float4 f = shared[q * half + piece];
+        v[4 * q] = f.x, v[4 * q + 1] = f.y, v[4 * q + 2] = f.z, v[4 * q + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = c.has(j, cols) ? load_any(global, c.first + j, type) : 0.f;
+    }
+  }
+};
+
+// Sums over the NW warps that share a row, of N values together behind one barrier.
 template <int NW, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (&part)[N][16], int warp) {
 #pragma unroll
@@ -185,186 +227,263 @@ __device__ __forceinline__ void forget(uint4& raw) {
   asm volatile("" : "+r"(raw.x), "+r"(raw.y), "+r"(raw.z), "+r"(raw.w));
 }
 
-template <int NW>
-constexpr int kThreadsOf = 32 * (NW < 4 ? 4 : NW);
-
-// Rows that a group of warps takes at once: their loads are in flight together and their sums
-// share the shuffles' and barriers' latency.
-template <int CH>
-constexpr int kAtOnce = CH == 1 ? 4 : CH == 2 ? 2 : 1;
-
-template <typename T, int NW, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 7 : 4) : NW == 8 ? (CH == 2 ? 3 : 2) : 1)
-norm_forward_rows(const __grid_constant__ HpNormForward a) {
-  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW), R = kAtOnce<CH>;
-  __shared__ float part[2][R][16];
-  const int cols = (int)a.cols, t = threadIdx.x % (32 * NW), warp = t >> 5;
-  const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / (32 * NW), step = (int64_t)gridDim.x * kGroups;
-  if (first >= a.rows) return;   // the whole CTA where it shares a row
-  const int phase = RAGGED ? (int)(((uintptr_t)((const T*)a.x + first * a.ldx) / sizeof(T)) % V) : 0;
-  Piece<T, RAGGED> c[CH];
-  float w[CH][V], b[CH][V];
+// The ring of one group of warps: in a slot one row of each of the tensors that are read together.
+template <typename T, int N, bool RAGGED>
+struct Ring {
+  const T* base[N];
+  int64_t pitch[N];
+  int n;                    // tensors there are; a slot has their rows one behind the other
+  int64_t rows;
+  uint8_t* slots;
+  uint64_t* full;
+  int cols, depth, bytes;   // bytes of one row in a slot
+  bool leader;
+  uint32_t waited, pending; // a bit for each slot: the phase its barrier is in; a copy is on its way
+  __device__ __forceinline__ bool alone(int64_t row) const { return RAGGED && (row == 0 || row + 1 >= rows); }
+  __device__ __forceinline__ const uint8_t* slot(int s, int i) const { return slots + (s * n + i) * bytes; }
+  // once nobody reads slot s any more
+  __device__ __forceinline__ void fetch(int64_t row, int s) {
+    if (!leader || row >= rows || alone(row)) return;
+    uint32_t total = 0, size[N];
+    uintptr_t from[N];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    c[i].first = (t + i * 32 * NW) * V - phase;
-    c[i].load_weights(a.weight, (int)a.wtype, cols, 1.f, w[i]);
-    c[i].load_weights(a.bias, (int)a.wtype, cols, 0.f, b[i]);
+    for (int i = 0; i < N; ++i) {
+      if (i >= n) continue;
+      const uintptr_t p = (uintptr_t)(base[i] + row * pitch[i]), end = p + cols * sizeof(T);
+      from[i] = p & ~(uintptr_t)15;
+      size[i] = (uint32_t)(((end + 15) & ~(uintptr_t)15) - from[i]);
+      total += size[i];
+    }
+    mbar_expect_tx(&full[s], total);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) bulk_load((void*)slot(s, i), (const void*)from[i], size[i], &full[s]);
+    pending |= 1u << s;
   }
-  const float inv = 1.f / (float)cols;
-  for (int64_t row0 = first; row0 < a.rows; row0 += R * step) {
-    uint4 raw[R][CH], res[R][CH];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int64_t row = row0 + k * step;
-      const bool there = row < a.rows, inner = row > 0 && row + 1 < a.rows;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        raw[k][i] = c[i].load((const T*)a.x + row * a.ldx, cols, there, inner);
-        if (a.residual) res[k][i] = c[i].load((const T*)a.residual + row * a.ldr, cols, there, inner);
-      }
-    }
-    // a row stays packed as it came; to take it apart costs an instruction for an element, and half
-    // the registers are half the warps
-    float s[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      s[k] = 0.f;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float v[V];
-        unpack<T>(raw[k][i], v);
-        if (a.residual) {
-          float r[V];
-          unpack<T>(res[k][i], r);
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[j] += r[j];
-          raw[k][i] = pack<T>(v);   // the sum as it is stored is what is normalised
-          unpack<T>(raw[k][i], v);
-          c[i].store((T*)a.z + (row0 + k * step) * a.cols, cols, row0 + k * step < a.rows, raw[k][i]);
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[k] += v[j];
-      }
-    }
-    row_sums<NW>(s, part[0], warp);
-    float mean[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      mean[k] = s[k] * inv;
-      s[k] = 0.f;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float v[V];
-        forget(raw[k][i]);
-        unpack<T>(raw[k][i], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[j] - mean[k];
-          if (c[i].has(j, cols)) s[k] = fmaf(d, d, s[k]);
-        }
-      }
-    }
-    row_sums<NW>(s, part[1], warp);
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int64_t row = row0 + k * step;
-      const float rstd = 1.f / sqrtf(s[k] * inv + (float)a.eps);
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float v[V];
-        forget(raw[k][i]);
-        unpack<T>(raw[k][i], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean[k]) * rstd, w[i][j], b[i][j]);
-        c[i].store((T*)a.y + row * a.cols, cols, row < a.rows, pack<T>(v));
-      }
-      if (t == 0 && row < a.rows) {
-        a.mean[row] = mean[k];
-        a.rstd[row] = rstd;
-      }
-    }
+  __device__ __forceinline__ void wait(int s, Guard& g) {
+    if (!guard_wait(&full[s], waited >> s & 1, g, 0x70000)) return;
+    waited ^= 1u << s;
+    pending &= ~(1u << s);
   }
+  // before the CTA ends after a wait that ran out: the copies that are still on their way
+  __device__ __forceinline__ void drain(Guard& g) {
+    if (!leader) return;
+    for (int s = 0; s < depth; ++s)
+      if (pending >> s & 1) mbar_wait_bounded(&full[s], waited >> s & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x80000);
+  }
+};
+
+// What a kernel of rows starts with: barriers, the ring, the first rows on their way.
+template <typename T, int NW, int N, bool RAGGED>
+__device__ __forceinline__ void start_ring(Ring<T, N, RAGGED>& ring, uint8_t* space, uint64_t (*full)[kMostSlots], Guard& guard,
+                                           uint32_t* status, int64_t first, int64_t step) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kGroupsOf<NW> * kMostSlots; ++i) mbar_init(&full[0][0] + i, 1);
+    mbar_init_fence();
+    guard.gave_up = 0;
+    guard.status = status;
+  }
+  __syncthreads();
+  const int group = threadIdx.x / (32 * NW);
+  ring.slots = space + group * ring.depth * ring.n * ring.bytes;
+  ring.full = full[group];
+  ring.leader = threadIdx.x % (32 * NW) == 0;
+  ring.waited = ring.pending = 0;
+  for (int s = 0; s < ring.depth; ++s) ring.fetch(first + s * step, s);
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 5 : 3) : NW == 8 ? (CH == 2 ? 2 : 1) : 1)
-norm_backward_rows(const __grid_constant__ HpNormBackward a) {
-  constexpr int V = kPiece<T>, kGroups = kThreadsOf<NW> / (32 * NW), R = CH >= 3 || NW == 16 ? 1 : 2;
-  __shared__ float part[2][2 * R][16];
-  extern __shared__ float joint[];   // [2 cols], where several rows are at work in a CTA
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH <= 2 ? 4 : 3) : NW == 8 ? 2 : 1)
+norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
+  constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
+  extern __shared__ __align__(128) uint8_t space[];
+  __shared__ float part[2][1][16];
+  __shared__ uint64_t full[kGroups][kMostSlots];
+  __shared__ Guard guard;
+  const int cols = (int)a.cols, t = threadIdx.x % (32 * NW), warp = t >> 5;
+  const int64_t first = (int64_t)blockIdx.x * kGroups + threadIdx.x / (32 * NW), step = (int64_t)gridDim.x * kGroups;
+  const bool sum_in_front = a.residual != nullptr;
+  Ring<T, 2, RAGGED> ring;
+  ring.base[0] = (const T*)a.x, ring.base[1] = (const T*)a.residual;
+  ring.pitch[0] = a.ldx, ring.pitch[1] = a.ldr;
+  ring.n = sum_in_front ? 2 : 1;
+  ring.rows = a.rows, ring.cols = cols, ring.depth = depth, ring.bytes = slot_bytes;
+  start_ring<T, NW>(ring, space, full, guard, status, first, step);
+  const int phase = RAGGED ? (int)(((uintptr_t)((const T*)a.x + first * a.ldx) / sizeof(T)) % V) : 0;
+  Piece<T, RAGGED> c[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) c[i].first = (t + i * 32 * NW) * V - phase;
+  Weights<T, RAGGED, NW> weight, bias;
+  weight.place(a.weight, (int)a.wtype, 1.f, cols, phase, (float4*)(space + ring_bytes));
+  bias.place(a.bias, (int)a.wtype, 0.f, cols, phase, (float4*)(space + ring_bytes) + weight.half * (V / 4));
+  __syncthreads();
+  float w[CH][V], b[CH][V];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    weight.get(c[i], cols, phase, w[i]);
+    bias.get(c[i], cols, phase, b[i]);
+  }
+  const float inv = 1.f / (float)cols;
+  int s = 0;
+  for (int64_t row = first; row < a.rows; row += step) {
+    uint4 raw[CH];
+    float sum[1] = {0.f};
+    const bool alone = ring.alone(row);
+    if (!alone) ring.wait(s, guard);
+    auto piece = [&](int i, int k) {
+      return alone ? c[i].take_from(ring.base[k] + row * ring.pitch[k], cols) : c[i].take(ring.slot(s, k), cols, phase);
+    };
+    // a row stays packed as it came; to take it apart costs an instruction for an element
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      raw[i] = piece(i, 0);
+      float v[V];
+      unpack<T>(raw[i], v);
+      if (sum_in_front) {
+        float r[V];
+        unpack<T>(piece(i, 1), r);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += r[j];
+        raw[i] = pack<T>(v);   // the sum as it is stored is what is normalised
+        unpack<T>(raw[i], v);
+        c[i].store((T*)a.z + row * a.cols, cols, raw[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[0] += v[j];
+    }
+    row_sums<NW>(sum, part[0], warp);   // everybody has read the slot
+    if (!guard.gave_up) ring.fetch(row + depth * step, s);
+    if (++s == depth) s = 0;
+    const float mean = sum[0] * inv;
+    sum[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      float v[V];
+      forget(raw[i]);
+      unpack<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = v[j] - mean;
+        if (c[i].has(j, cols)) sum[0] = fmaf(d, d, sum[0]);
+      }
+    }
+    row_sums<NW>(sum, part[1], warp);
+    const float rstd = rsqrtf(sum[0] * inv + (float)a.eps);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      float v[V];
+      forget(raw[i]);
+      unpack<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * rstd, w[i][j], b[i][j]);
+      c[i].store((T*)a.y + row * a.cols, cols, pack<T>(v));
+    }
+    if (t == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
+    }
+  }
+  if (guard.gave_up) ring.drain(guard);
+}
+
+template <typename T, int NW, int CH, bool RAGGED>
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 4 : CH == 2 ? 3 : 2) : NW == 8 ? 2 : 1)
+norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
+  constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
+  extern __shared__ __align__(128) uint8_t space[];
+  __shared__ float part[2][2][16];
+  __shared__ uint64_t full[kGroups][kMostSlots];
+  __shared__ Guard guard;
   const int cols = (int)a.cols, t = threadIdx.x % (32 * NW), warp = t >> 5, group = threadIdx.x / (32 * NW);
   const int64_t first = (int64_t)blockIdx.x * kGroups + group, step = (int64_t)gridDim.x * kGroups;
+  const bool more = a.dz != nullptr;
+  Ring<T, 3, RAGGED> ring;
+  ring.base[0] = (const T*)a.z, ring.base[1] = (const T*)a.dy, ring.base[2] = (const T*)a.dz;
+  ring.pitch[0] = a.ldz, ring.pitch[1] = a.lddy, ring.pitch[2] = a.lddz;
+  ring.n = more ? 3 : 2;
+  ring.rows = a.rows, ring.cols = cols, ring.depth = depth, ring.bytes = slot_bytes;
+  start_ring<T, NW>(ring, space, full, guard, status, first, step);
   const int phase = RAGGED ? (int)(((uintptr_t)((const T*)a.z + first * a.ldz) / sizeof(T)) % V) : 0;
   Piece<T, RAGGED> c[CH];
-  float w[CH][V], dw[CH][V], db[CH][V];
+  float dw[CH][V], db[CH][V];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     c[i].first = (t + i * 32 * NW) * V - phase;
-    c[i].load_weights(a.weight, (int)a.wtype, cols, 1.f, w[i]);
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
   }
+  Weights<T, RAGGED, NW> weight;
+  weight.place(a.weight, (int)a.wtype, 1.f, cols, phase, (float4*)(space + ring_bytes));
+  __syncthreads();
+  // the sums take the registers; what is left holds the weights of short rows
+  constexpr bool kHold = NW <= 4;
+  float held[CH][V];
+  if (kHold)
+#pragma unroll
+    for (int i = 0; i < CH; ++i) weight.get(c[i], cols, phase, held[i]);
+  auto weights = [&](int i, float (&w)[V]) {
+    if (!kHold) {
+      weight.get(c[i], cols, phase, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] = held[i][j];
+    }
+  };
   dependents_may_start();
   const float inv = 1.f / (float)cols;
-  int turn = 0;
-  for (int64_t row0 = first; row0 < a.rows; row0 += R * step, turn ^= 1) {
-    uint4 zr[R][CH], gr[R][CH], ur[R][CH];
-    float mean[R], rstd[R], s[2 * R];
+  int s = 0, turn = 0;
+  float mean_next = first < a.rows ? a.mean[first] : 0.f, rstd_next = first < a.rows ? a.rstd[first] : 0.f;
+  for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
+    uint4 zr[CH], gr[CH], ur[CH];
+    const float mean = mean_next, rstd = rstd_next;
+    if (row + step < a.rows) mean_next = a.mean[row + step], rstd_next = a.rstd[row + step];
+    const bool alone = ring.alone(row);
+    if (!alone) ring.wait(s, guard);
+    auto piece = [&](int i, int k) {
+      return alone ? c[i].take_from(ring.base[k] + row * ring.pitch[k], cols) : c[i].take(ring.slot(s, k), cols, phase);
+    };
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int64_t row = row0 + k * step;
-      const bool there = row < a.rows, inner = row > 0 && row + 1 < a.rows;
+    for (int i = 0; i < CH; ++i) {
+      float z[V], g[V], w[V];
+      weights(i, w);
+      zr[i] = piece(i, 0), gr[i] = piece(i, 1);
+      if (more) ur[i] = piece(i, 2);
+      unpack<T>(zr[i], z);
+      unpack<T>(gr[i], g);   // zeros outside the row
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        zr[k][i] = c[i].load((const T*)a.z + row * a.ldz, cols, there, inner);
-        gr[k][i] = c[i].load((const T*)a.dy + row * a.lddy, cols, there, inner);
-        if (a.dz) ur[k][i] = c[i].load((const T*)a.dz + row * a.lddz, cols, there, inner);
+      for (int j = 0; j < V; ++j) {
+        const float h = (z[j] - mean) * rstd, gw = g[j] * w[j];
+        dw[i][j] = fmaf(g[j], h, dw[i][j]);
+        db[i][j] += g[j];
+        sum[0] += gw;
+        sum[1] = fmaf(gw, h, sum[1]);
       }
-      mean[k] = there ? a.mean[row] : 0.f, rstd[k] = there ? a.rstd[row] : 0.f;
     }
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float z[V], g[V];
-        unpack<T>(zr[k][i], z);
-        unpack<T>(gr[k][i], g);   // zeros outside the row
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float h = (z[j] - mean[k]) * rstd[k], gw = g[j] * w[i][j];
-          dw[i][j] = fmaf(g[j], h, dw[i][j]);
-          db[i][j] += g[j];
-          s1 += gw;
-          s2 = fmaf(gw, h, s2);
-        }
-      }
-      s[2 * k] = s1, s[2 * k + 1] = s2;
-    }
+    row_sums<NW>(sum, part[turn], warp);   // everybody has read the slot
+    if (!guard.gave_up) ring.fetch(row + depth * step, s);
+    if (++s == depth) s = 0;
     if (!a.dx) continue;
-    row_sums<NW>(s, part[turn], warp);   // one barrier a turn: the halves take turns
+    // rstd (g w - mean(g w) - h mean(g w h)), with h = (z - mean) rstd
+    const float s1 = -sum[0] * inv * rstd, s2 = sum[1] * inv * rstd * rstd;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int64_t row = row0 + k * step;
-      // rstd (g w - mean(g w) - h mean(g w h)), with h = (z - mean) rstd
-      const float s1 = -s[2 * k] * inv * rstd[k], s2 = s[2 * k + 1] * inv * rstd[k] * rstd[k];
+    for (int i = 0; i < CH; ++i) {
+      float z[V], g[V], d[V], up[V], w[V];
+      weights(i, w);
+      forget(zr[i]);
+      forget(gr[i]);
+      unpack<T>(zr[i], z);
+      unpack<T>(gr[i], g);
+      if (more) unpack<T>(ur[i], up);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        float z[V], g[V], d[V], up[V];
-        forget(zr[k][i]);
-        forget(gr[k][i]);
-        unpack<T>(zr[k][i], z);
-        unpack<T>(gr[k][i], g);
-        if (a.dz) unpack<T>(ur[k][i], up);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          d[j] = fmaf(mean[k] - z[j], s2, fmaf(g[j], w[i][j] * rstd[k], s1));
-          if (a.dz) d[j] += up[j];
-        }
-        c[i].store((T*)a.dx + row * a.cols, cols, row < a.rows, pack<T>(d));
+      for (int j = 0; j < V; ++j) {
+        d[j] = fmaf(mean - z[j], s2, fmaf(g[j], w[j] * rstd, s1));
+        if (more) d[j] += up[j];
       }
+      c[i].store((T*)a.dx + row * a.cols, cols, pack<T>(d));
     }
   }
+  if (guard.gave_up) ring.drain(guard);
   if (!a.dweight && !a.dbias) return;
   float* out = (float*)a.workspace + (int64_t)blockIdx.x * 2 * cols;
   if constexpr (kGroups == 1) {
@@ -374,20 +493,29 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a) {
       for (int j = 0; j < V; ++j)
         if (c[i].has(j, cols)) out[c[i].first + j] = dw[i][j], out[cols + c[i].first + j] = db[i][j];
   } else {
-    for (int k = 0; k < kGroups; ++k) {   // one row's warps after the other
-      if (group == k)
+    // every group its own sums, a thread's next to its neighbours'; then by columns
+    float* joint = (float*)space;   // the ring is done with
+    const int pieces = 32 * NW * CH, most = kGroups * V * pieces;
+    __syncthreads();
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (c[i].has(j, cols)) {
-              float* at = joint + c[i].first + j;
-              at[0] = k ? at[0] + dw[i][j] : dw[i][j];
-              at[cols] = k ? at[cols] + db[i][j] : db[i][j];
-            }
-      __syncthreads();
+      for (int j = 0; j < V; ++j) {
+        const int at = (group * V + j) * pieces + t + i * 32 * NW;
+        joint[at] = dw[i][j], joint[most + at] = db[i][j];
+      }
+    __syncthreads();
+    for (int e = threadIdx.x; e < cols; e += blockDim.x) {
+      float sw = 0.f, sb = 0.f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const int64_t row = (int64_t)blockIdx.x * kGroups + k;
+        const int at = e + (RAGGED ? (int)(((uintptr_t)((const T*)a.z + row * a.ldz) / sizeof(T)) % V) : 0);
+        const int q = (k * V + at % V) * pieces + at / V;
+        sw += joint[q], sb += joint[most + q];
+      }
+      out[e] = sw, out[cols + e] = sb;
     }
-    for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) out[i] = joint[i];
   }
 }
 
@@ -398,10 +526,11 @@ struct Split {
 };
 template <typename T>
 Split split_of(int64_t cols, bool ragged) {
+  if (ragged && cols < kPiece<T>) return {0, 0};   // a row's boundaries would reach beyond its neighbours
   const int64_t n = (cols + kPiece<T> - 1) / kPiece<T> + (ragged ? 1 : 0);
   if (n <= 32) return {1, 1};
   if (n <= 64) return {1, 2};
-  if (n <= 128) return {4, 1};
+  if (n <= 128) return {1, 4};
   if (n <= 256) return {4, 2};
   if (n <= 512) return {8, 2};
   if (n <= 768) return {8, 3};
@@ -430,13 +559,6 @@ struct Rows {
 
 constexpr int kMostCtas = 1024;   // rows of partial sums
 
-template <typename K>
-int resident(K kernel, int threads, int smem) {
-  int n = 1;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
-  return n;
-}
-
 // CTAs for `rows` rows, `groups` at once in each: at most `per_sm` to an SM and kMostCtas; where
 // rows start anywhere a multiple of eight, which keeps a group's rows alike
 unsigned ctas_for(int64_t rows, int groups, int per_sm, bool ragged) {
@@ -446,20 +568,53 @@ unsigned ctas_for(int64_t rows, int groups, int per_sm, bool ragged) {
   return (unsigned)(n < most ? n : most);
 }
 
+// Shared memory of a CTA at most: what an SM has, divided by the CTAs it is meant to hold.  The
+// weights take their part of it, the ring the rest; when the ring is done with, its space holds
+// the groups' sums.
+template <int NW>
+constexpr int kSpace = NW <= 4 ? 54 * 1024 : NW == 8 ? 100 * 1024 : 216 * 1024;
+
+struct RingSize {
+  int slot, depth, ring, bytes;
+};
 template <typename T, int NW, int CH, bool RAGGED>
-int forward_rows(const HpNormForward& a, cudaStream_t s) {
-  constexpr int kThreads = kThreadsOf<NW>, kGroups = kThreads / (32 * NW);
-  static const int per_sm = resident(norm_forward_rows<T, NW, CH, RAGGED>, kThreads, 0);
-  norm_forward_rows<T, NW, CH, RAGGED><<<ctas_for(a.rows, kGroups, per_sm, RAGGED), kThreads, 0, s>>>(a);
+RingSize ring_size(int64_t cols, int tensors, int weights, bool sums) {
+  RingSize r;
+  r.slot = (int)((cols * sizeof(T) + (RAGGED ? 30 : 0) + 15) / 16 * 16);
+  const int set = kGroupsOf<NW> * tensors * r.slot;
+  const int w = Weights<T, RAGGED, NW>::kShared ? weights * (int)((cols + 2 * kPiece<T>) * 4) : 0;
+  r.depth = (kSpace<NW> - w) / set;
+  if (r.depth > kMostSlots) r.depth = kMostSlots;
+  r.ring = (r.depth * set + 127) / 128 * 128;
+  r.bytes = r.ring + w;
+  const int joint = sums && kGroupsOf<NW> > 1 ? kGroupsOf<NW> * 2 * kPiece<T> * 32 * NW * CH * 4 : 0;
+  if (r.bytes < joint) r.bytes = joint;
+  return r;
+}
+
+// CTAs of the kernel that an SM holds, with the largest ring
+template <typename K>
+int prepared(K kernel, int threads, int smem) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
+  int n = 1;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
+  return n;
+}
+
+template <typename T, int NW, int CH, bool RAGGED>
+int forward_rows(const HpNormForward& a, uint32_t* status, cudaStream_t s) {
+  static const int per_sm = prepared(norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
+  const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.residual ? 2 : 1, 2, false);
+  norm_forward_rows<T, NW, CH, RAGGED><<<ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>, r.bytes, s>>>(
+      a, r.depth, r.slot, r.ring, status);
   return cudaGetLastError();
 }
 template <typename T, int NW, int CH, bool RAGGED>
-int backward_rows(const HpNormBackward& a, cudaStream_t s) {
-  constexpr int kThreads = kThreadsOf<NW>, kGroups = kThreads / (32 * NW);
-  const int smem = kGroups > 1 ? (int)(8 * a.cols) : 0;
-  static const int per_sm = resident(norm_backward_rows<T, NW, CH, RAGGED>, kThreads, kGroups > 1 ? 8 * 32 * CH * kPiece<T> : 0);
-  const unsigned grid = ctas_for(a.rows, kGroups, per_sm, RAGGED);
-  norm_backward_rows<T, NW, CH, RAGGED><<<grid, kThreads, smem, s>>>(a);
+int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
+  static const int per_sm = prepared(norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
+  const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.dz ? 3 : 2, 1, true);
+  const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
+  norm_backward_rows<T, NW, CH, RAGGED><<<grid, kThreadsOf<NW>, r.bytes, s>>>(a, r.depth, r.slot, r.ring, status);
   const int rc = cudaGetLastError();
   if (rc || (!a.dweight && !a.dbias)) return rc;
   return column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);
@@ -469,7 +624,7 @@ int backward_rows(const HpNormBackward& a, cudaStream_t s) {
   switch (p.warps * 8 + p.pieces) {             \
     case 1 * 8 + 1: return call(1, 1);          \
     case 1 * 8 + 2: return call(1, 2);          \
-    case 4 * 8 + 1: return call(4, 1);          \
+    case 1 * 8 + 4: return call(1, 4);          \
     case 4 * 8 + 2: return call(4, 2);          \
     case 8 * 8 + 2: return call(8, 2);          \
     case 8 * 8 + 3: return call(8, 3);          \
@@ -487,7 +642,10 @@ int forward(const HpNormForward& a, cudaStream_t s) {
   r.add(a.z, a.cols);
   if (r.alike) {
     const Split p = split_of<T>(a.cols, r.ragged());
-#define CALL(nw, ch) r.ragged() ? forward_rows<T, nw, ch, true>(a, s) : forward_rows<T, nw, ch, false>(a, s)
+    int rc;
+    uint32_t* status = layer_status(&rc);
+    if (rc) return rc;
+#define CALL(nw, ch) r.ragged() ? forward_rows<T, nw, ch, true>(a, status, s) : forward_rows<T, nw, ch, false>(a, status, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
@@ -503,7 +661,10 @@ int backward(const HpNormBackward& a, cudaStream_t s) {
   r.add(a.dx, a.cols);
   if (r.alike && a.rows) {
     const Split p = split_of<T>(a.cols, r.ragged());
-#define CALL(nw, ch) r.ragged() ? backward_rows<T, nw, ch, true>(a, s) : backward_rows<T, nw, ch, false>(a, s)
+    int rc;
+    uint32_t* status = layer_status(&rc);
+    if (rc) return rc;
+#define CALL(nw, ch) r.ragged() ? backward_rows<T, nw, ch, true>(a, status, s) : backward_rows<T, nw, ch, false>(a, status, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
