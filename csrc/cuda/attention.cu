@@ -342,109 +342,365 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
   if (warp == 1) tmem_free<1>(tmem, F::kTmem);
 }
 
-constexpr int kWarps = 4, kMaxDim = 128;
+constexpr int kMaxDim = 128;
 
-__device__ __forceinline__ bool sees(const HpAttention& a, int64_t b, int64_t i, int64_t j) {
-  return j < a.sk && (!a.causal || j <= i + a.sk - a.sq) && (!a.key_mask || a.key_mask[b * a.mask_b + j]);
-}
+// --------------------------------------------------------------------- backward
+// Rows of d_o against rows of o (delta), and the logarithm of the softmax sums to base 2; both
+// in tiles of 128 rows, [batch, heads, rows rounded up].  Behind the last row, and where a row
+// saw nothing: infinity, so that every probability comes out as zero.
+__host__ __device__ __forceinline__ int64_t padded(int64_t rows) { return (rows + kB - 1) / kB * kB; }
 
-template <typename T>
-__device__ __forceinline__ float dot(const float* x, const T* y, int d) {
-  float s = 0.f;
-  for (int i = 0; i < d; ++i) s = fmaf(x[i], to_f(y[i]), s);
-  return s;
-}
-
-// rows of d_o against rows of o: [batch, heads, sq]
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) attention_delta_kernel(const __grid_constant__ HpAttention a) {
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * kWarps + w, h = blockIdx.y, b = blockIdx.z;
-  if (i >= a.sq) return;
-  const T* o = (const T*)a.o + b * a.o_b + i * a.o_s + h * a.o_h;
-  const T* g = (const T*)a.d_o + b * a.do_b + i * a.do_s + h * a.do_h;
-  float s = 0.f;
-  for (int c = lane; c < a.dim; c += 32) s = fmaf(to_f(o[c]), to_f(g[c]), s);
-  s = warp_sum(s);
-  if (lane == 0) a.delta[(b * a.heads + h) * a.sq + i] = s;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) attention_dq_kernel(const __grid_constant__ HpAttention a) {
-  __shared__ float sq[kWarps][kMaxDim], sg[kWarps][kMaxDim];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, d = (int)a.dim;
-  const int64_t i = (int64_t)blockIdx.x * kWarps + w, h = blockIdx.y, b = blockIdx.z, hk = h / (a.heads / a.kv_heads);
-  if (i >= a.sq) return;
-  const T* q = (const T*)a.q + b * a.q_b + i * a.q_s + h * a.q_h;
-  const T* g = (const T*)a.d_o + b * a.do_b + i * a.do_s + h * a.do_h;
-  const T* k = (const T*)a.k + b * a.k_b + hk * a.k_h;
-  const T* v = (const T*)a.v + b * a.v_b + hk * a.v_h;
-  for (int c = lane; c < d; c += 32) sq[w][c] = to_f(q[c]), sg[w][c] = to_f(g[c]);
-  __syncwarp();
-  const int64_t at = (b * a.heads + h) * a.sq + i;
-  const float lse = a.lse[at], delta = a.delta[at];
-  float acc[kMaxDim / 32] = {};
-  for (int64_t j0 = 0; j0 < a.sk; j0 += 32) {
-    const int64_t j = j0 + lane;
-    float ds = 0.f;
-    const bool see = sees(a, b, i, j);
-    if (see) {
-      const float p = expf(dot(sq[w], k + j * a.k_s, d) * (float)a.scale - lse);
-      ds = p * (dot(sg[w], v + j * a.v_s, d) - delta);
+template <typename T, int LANES>   // that share a row, 16 bytes each
+__global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ HpAttention a) {
+  const int lane = threadIdx.x % LANES;
+  const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, h = blockIdx.y, b = blockIdx.z;
+  const int64_t rows = padded(a.sq);
+  if (i >= rows) return;
+  float s = 0.f, lse = INFINITY;
+  if (i < a.sq) {
+    if (8 * lane < a.dim) {
+      float o[8], g[8];
+      unpack<T>(*(const uint4*)((const T*)a.o + b * a.o_b + i * a.o_s + h * a.o_h + 8 * lane), o);
+      unpack<T>(*(const uint4*)((const T*)a.d_o + b * a.do_b + i * a.do_s + h * a.do_h + 8 * lane), g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s = fmaf(o[k], g[k], s);
     }
-    for (unsigned left = __ballot_sync(0xffffffffu, see); left; left &= left - 1) {
-      const int l = __ffs(left) - 1;
-      const float dl = __shfl_sync(0xffffffffu, ds, l);
-      for (int c = 0; c < kMaxDim / 32; ++c)
-        if (32 * c + lane < d) acc[c] = fmaf(dl, to_f(k[(j0 + l) * a.k_s + 32 * c + lane]), acc[c]);
-    }
+    if (lane == 0) lse = a.lse[(b * a.heads + h) * a.sq + i] * kLog2e;
   }
-  T* o = (T*)a.dq + b * a.dq_b + i * a.dq_s + h * a.dq_h;
-  for (int c = 0; c < kMaxDim / 32; ++c)
-    if (32 * c + lane < d) o[32 * c + lane] = from_f<T>(acc[c] * (float)a.scale);
+#pragma unroll
+  for (int k = LANES / 2; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+  if (lane == 0) {
+    float* out = a.delta + (b * a.heads + h) * 2 * rows + i;
+    out[0] = lse == -INFINITY ? INFINITY : lse;
+    out[rows] = s;
+  }
 }
 
-// One warp for each key row: the lanes share the queries of a chunk, of every head that reads it.
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) attention_dkv_kernel(const __grid_constant__ HpAttention a) {
-  __shared__ float sk[kWarps][kMaxDim], sv[kWarps][kMaxDim];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, d = (int)a.dim;
-  const int64_t j = (int64_t)blockIdx.x * kWarps + w, hk = blockIdx.y, b = blockIdx.z, group = a.heads / a.kv_heads;
-  if (j >= a.sk) return;
-  const T* k = (const T*)a.k + b * a.k_b + j * a.k_s + hk * a.k_h;
-  const T* v = (const T*)a.v + b * a.v_b + j * a.v_s + hk * a.v_h;
-  for (int c = lane; c < d; c += 32) sk[w][c] = to_f(k[c]), sv[w][c] = to_f(v[c]);
-  __syncwarp();
-  float dk[kMaxDim / 32] = {}, dv[kMaxDim / 32] = {};
-  for (int64_t h = hk * group; h < (hk + 1) * group; ++h) {
-    const T* q = (const T*)a.q + b * a.q_b + h * a.q_h;
-    const T* g = (const T*)a.d_o + b * a.do_b + h * a.do_h;
-    for (int64_t i0 = 0; i0 < a.sq; i0 += 32) {
-      const int64_t i = i0 + lane, at = (b * a.heads + h) * a.sq + i;
-      float p = 0.f, ds = 0.f;
-      const bool see = i < a.sq && sees(a, b, i, j);
-      if (see) {
-        p = expf(dot(sk[w], q + i * a.q_s, d) * (float)a.scale - a.lse[at]);
-        ds = p * (dot(sv[w], g + i * a.do_s, d) - a.delta[at]);
+// Two kinds of CTA, each with a tile of 128 rows that stays and tiles that pass by:
+//   keys     k, v stay; q, d_o pass.  S^T = k q^T, dP^T = v d_o^T; dv += P^T d_o, dk += dS^T q
+//   queries  q, d_o stay; k, v pass.  S = q k^T, dP = d_o v^T; dq += dS k
+// with P = 2^(c S - lse) and dS = P (dP - delta).  Computing S and dP for each kind costs two
+// products of seven more than one kernel that adds its parts of dq up in memory, and saves
+// those additions, their 32-bit buffer and their order, which would differ from run to run.
+// P and dS go back to tensor memory over S, as the left operands; eight warps share the rows, one
+// thread half a row.  The next tile's S is computed meanwhile (a second buffer), except for keys
+// with more than 64 dimensions, whose two results leave no room for it.
+template <int DP>
+struct Backward {
+  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = DP == 64 ? 4 : 2;
+  static constexpr int kThreads = 64 + 256;
+  static constexpr int kSmem = 2 * kTile + kStages * (2 * kTile + 1024) + 1024 + 1024;
+  // columns: S (buffers kS apart), dP, the results
+  static constexpr uint32_t kS = 256, kDP = 128, kAcc1 = DP == 64 ? 384 : 256, kAcc2 = DP == 64 ? 448 : 384;
+};
+struct BackwardBars {
+  uint64_t stay_full, in_full[4], in_empty[4], mask_full[4], s_full[2], dp_full, p_full, acc_full;
+  Seen seen[4];
+  uint32_t tmem;
+  int keys;
+  Guard guard;
+};
+
+// By the whole CTA: one more than the last key that a sequence's mask lets see.
+__device__ __forceinline__ int visible_keys(const uint8_t* mask, int sk, int* shared) {
+  if (threadIdx.x == 0) *shared = 0;
+  __syncthreads();
+  int last = 0;
+  for (int k = threadIdx.x; k < sk; k += blockDim.x)
+    if (mask[k]) last = k + 1;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+  if ((threadIdx.x & 31) == 0) atomicMax(shared, last);
+  __syncthreads();
+  return *shared;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_constant__ Launch l) {
+  using F = Backward<DP>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* stay = smem;
+  uint8_t* pass = smem + 2 * F::kTile;
+  float* rows_of = (float*)(pass + F::kStages * 2 * F::kTile);   // a stage's lse and delta
+  BackwardBars& bar = *(BackwardBars*)(rows_of + F::kStages * 2 * kB);
+  const HpAttention& p = l.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nq = (int)((p.sq + kB - 1) / kB), nk = (int)((p.sk + kB - 1) / kB), group = (int)(p.heads / p.kv_heads);
+  const int sk = (int)p.sk, shift = (int)(p.sk - p.sq);
+  // keys first: with shared heads they have more to do
+  const int b = blockIdx.y;
+  int id = blockIdx.x, head, tile;
+  const bool keys = id < nk * (int)p.kv_heads;
+  if (keys) {
+    head = id / nk, tile = id % nk;   // under a causal mask the first keys are seen by most
+  } else {
+    id -= nk * (int)p.kv_heads;
+    head = id / nq, tile = nq - 1 - id % nq;
+  }
+  const int r0 = tile * kB;           // first row that stays
+  const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
+  const bool masked = mask != nullptr;
+  // tiles that pass: queries from `first` on, of each head of the group in turn; or keys up to the last seen
+  int first = 0, count;
+  if (keys) {
+    if (p.causal) first = max(0, r0 - shift) / kB;
+    count = max(0, nq - first);
+    if (masked) {
+      const Seen m = mask_bits(mask, r0, sk);
+      if (!(m.w[0] | m.w[1] | m.w[2] | m.w[3])) count = 0;
+    }
+  } else {
+    int see = masked && sk > kB ? visible_keys(mask, sk, &bar.keys) : sk;
+    if (p.causal) see = min(see, max(0, min(r0 + kB, (int)p.sq) + shift));
+    count = (see + kB - 1) / kB;
+  }
+  const int n = keys ? count * group : count;
+  const int buffers = DP == 64 || !keys ? 2 : 1;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar.stay_full, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&bar.in_full[i], 1), mbar_init(&bar.in_empty[i], 1), mbar_init(&bar.mask_full[i], 1);
+    mbar_init(&bar.s_full[0], 1), mbar_init(&bar.s_full[1], 1), mbar_init(&bar.dp_full, 1);
+    mbar_init(&bar.p_full, 256), mbar_init(&bar.acc_full, 1);
+    mbar_init_fence();
+    bar.guard.gave_up = 0;
+    bar.guard.status = l.status;
+  }
+  if (warp == 1) tmem_alloc<1>(&bar.tmem, 512);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = bar.tmem;
+  Guard& g = bar.guard;
+
+  if (warp == 0) {
+    const uint32_t bytes = 2 * F::kTile + (keys ? 8 * kB : 0);
+    const int64_t rows = padded(p.sq);
+    int waits = 0;
+    if (lane == 0 && n) {
+      mbar_expect_tx(&bar.stay_full, 2 * F::kTile);
+      for (int i = 0; i < F::kPanels; ++i) {
+        tma_load_4d(stay + i * kPanel, keys ? &l.map.k : &l.map.q, 64 * i, head, r0, b, &bar.stay_full);
+        tma_load_4d(stay + F::kTile + i * kPanel, keys ? &l.map.v : &l.map.d_o, 64 * i, head, r0, b, &bar.stay_full);
       }
-      for (unsigned left = __ballot_sync(0xffffffffu, see); left; left &= left - 1) {
-        const int l = __ffs(left) - 1;
-        const float pl = __shfl_sync(0xffffffffu, p, l), dl = __shfl_sync(0xffffffffu, ds, l);
-        for (int c = 0; c < kMaxDim / 32; ++c)
-          if (32 * c + lane < d) {
-            dv[c] = fmaf(pl, to_f(g[(i0 + l) * a.do_s + 32 * c + lane]), dv[c]);
-            dk[c] = fmaf(dl, to_f(q[(i0 + l) * a.q_s + 32 * c + lane]), dk[c]);
+    }
+    for (int j = 0; j < n; ++j) {
+      const int s = j % F::kStages;
+      if (!guard_wait(&bar.in_empty[s], ((j / F::kStages) & 1) ^ 1, g, 0x11001)) break;
+      if (lane == 0) {
+        uint8_t* to = pass + s * 2 * F::kTile;
+        const int h = keys ? head * group + j / count : head / group, at = keys ? (first + j % count) * kB : j * kB;
+        mbar_expect_tx(&bar.in_full[s], bytes);
+        for (int i = 0; i < F::kPanels; ++i) {
+          tma_load_4d(to + i * kPanel, keys ? &l.map.q : &l.map.k, 64 * i, h, at, b, &bar.in_full[s]);
+          tma_load_4d(to + F::kTile + i * kPanel, keys ? &l.map.d_o : &l.map.v, 64 * i, h, at, b, &bar.in_full[s]);
+        }
+        if (keys) {
+          const float* from = p.delta + (b * p.heads + h) * 2 * rows + at;
+          bulk_load(rows_of + s * 2 * kB, from, 4 * kB, &bar.in_full[s]);
+          bulk_load(rows_of + s * 2 * kB + kB, from + rows, 4 * kB, &bar.in_full[s]);
+        }
+      }
+      if (!keys && masked) {
+        const Seen m = mask_bits(mask, (int64_t)j * kB, sk);
+        if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
+      }
+      waits = j + 1;
+    }
+    __syncwarp();
+    if (g.gave_up && lane == 0 && n) {   // nothing may land once the CTA is gone
+      mbar_wait_bounded(&bar.stay_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11002);
+      for (int j = max(0, waits - F::kStages); j < waits; ++j)
+        mbar_wait_bounded(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11003);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n) {
+      const bool bf = p.type == HP_BF16;
+      const uint32_t id_s = mma_idesc(128, 128, bf, true, true) | (l.negative ? kNegateA : 0);
+      const uint32_t id_dp = mma_idesc(128, 128, bf, true, true), id_acc = mma_idesc(128, DP, bf, true, false);
+      const uint32_t a = smem_u32(stay);
+      auto in = [&](int j) { return smem_u32(pass + (j % F::kStages) * 2 * F::kTile); };
+      auto wide = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t id) {   // rows by rows, over the dimensions
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t at = (i / 4) * kPanel + (i % 4) * 32;
+          mma_ss<1>(d, mma_desc(x + at, 16, 1024), mma_desc(y + at, 16, 1024), id, i > 0);
+        }
+      };
+      auto deep = [&](uint32_t d, uint32_t x, uint32_t y, bool add) {      // P or dS, over the tile's columns
+#pragma unroll
+        for (int i = 0; i < kB / 16; ++i)
+          mma_ts(d, x + (i / 2) * 32 + (i % 2) * 8, mma_desc(y + i * 2048, kPanel, 1024), id_acc, add || i > 0);
+      };
+      auto scores = [&](int j) {
+        const int q = buffers == 2 ? j & 1 : 0;
+        wide(tmem + F::kS * q, a, in(j), id_s);
+        mma_commit<1>(&bar.s_full[q]);
+      };
+      auto dprobs = [&](int j) {
+        wide(tmem + F::kDP, a + F::kTile, in(j) + F::kTile, id_dp);
+        mma_commit<1>(&bar.dp_full);
+      };
+      auto there = [&](int j) { return guard_wait(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, g, 0x21001); };
+      bool ok = guard_wait(&bar.stay_full, 0, g, 0x21002) && there(0);
+      if (ok) {
+        tmem_fence_after();
+        scores(0);
+        dprobs(0);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) {
+          ok = there(j + 1);
+          if (!ok) break;
+          if (buffers == 2) scores(j + 1);
+        }
+        ok = guard_wait(&bar.p_full, j & 1, g, 0x21003);
+        if (!ok) break;
+        tmem_fence_after();
+        if (j + 1 < n) dprobs(j + 1);
+        const uint32_t s = tmem + F::kS * (buffers == 2 ? j & 1 : 0);
+        if (keys) deep(tmem + F::kAcc1, s, in(j) + F::kTile, j > 0);
+        deep(tmem + F::kAcc2, s + 16, in(j), j > 0);
+        mma_commit<1>(&bar.in_empty[j % F::kStages]);
+        if (buffers == 1 && j + 1 < n) scores(j + 1);
+      }
+      mma_commit<1>(&bar.acc_full);
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2, r = 32 * quad + lane, row = r0 + r;
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+    float lse = INFINITY, delta = 0.f;   // of a query that stays
+    bool mine = true;                    // a key that stays is seen at all
+    if (keys) {
+      mine = row < sk && (!masked || mask[row]);
+    } else {
+      const float* from = p.delta + (b * p.heads + head) * 2 * padded(p.sq) + row;
+      lse = from[0], delta = from[padded(p.sq)];
+    }
+    const int sees = p.causal ? min(sk, row + shift + 1) : sk;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      const int s = j % F::kStages, q = buffers == 2 ? j & 1 : 0;
+      Seen seen;
+      bool whole;
+      if (keys) {
+        const int from = p.causal ? row - shift - (first + j % count) * kB : 0;   // its first query in this tile
+        whole = mine && from <= 0;
+        if (!__all_sync(0xffffffffu, whole)) {
+          seen = seen_between(mine ? from : kB, kB);
+          whole = false;
+        }
+      } else {
+        whole = sees >= (j + 1) * kB;
+        if (masked) {
+          if (!guard_wait(&bar.mask_full[s], (j / F::kStages) & 1, g, 0x31001)) { ok = false; break; }
+          seen = bar.seen[s];
+          const bool all = (seen.w[0] & seen.w[1] & seen.w[2] & seen.w[3]) == 0xffffffffu;
+          if (!all) {   // what a masked key holds is left out of dq: its k counts as zero
+            if (!guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31002)) { ok = false; break; }
+            if (half == 0 && !(seen.w[quad] >> lane & 1)) {
+              uint4* k = (uint4*)(pass + s * 2 * F::kTile + r * 128);
+#pragma unroll
+              for (int i = 0; i < F::kPanels; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) k[i * (kPanel / 16) + e] = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_shared();
           }
+          whole = whole && all;
+        }
+        if (!__all_sync(0xffffffffu, whole)) {
+          const Seen up_to = seen_between(0, sees - j * kB);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) seen.w[i] = masked ? seen.w[i] & up_to.w[i] : up_to.w[i];
+          whole = false;
+        }
       }
+      const bool here = guard_wait(&bar.s_full[q], (buffers == 2 ? j >> 1 : j) & 1, g, 0x31003) &&
+                        guard_wait(&bar.dp_full, j & 1, g, 0x31004);
+      if (!here) { ok = false; break; }
+      if (keys && !guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31005)) { ok = false; break; }
+      tmem_fence_after();
+      const float* cols = rows_of + s * 2 * kB + 64 * half;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        const uint32_t at = tmem + lanes + 64 * half + c;
+        uint32_t x[32], y[32], e[16], d[16];
+        tmem_ld32(at + F::kS * q, x);
+        tmem_ld32(at + F::kDP, y);
+        tmem_wait_ld();
+        const uint32_t bits = whole ? 0xffffffffu : seen.w[2 * half + c / 32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4 ls = make_float4(lse, lse, lse, lse), de = make_float4(delta, delta, delta, delta);
+          if (keys) ls = *(const float4*)(cols + c + i), de = *(const float4*)(cols + kB + c + i);
+          float pr[4], ds[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float w = k == 0 ? ls.x : k == 1 ? ls.y : k == 2 ? ls.z : ls.w;
+            const float v = k == 0 ? de.x : k == 1 ? de.y : k == 2 ? de.z : de.w;
+            pr[k] = exp2_fast(fmaf(__uint_as_float(x[i + k]), l.c, -w));
+            ds[k] = pr[k] * (__uint_as_float(y[i + k]) - v);
+            if (!whole && !(bits >> (i + k) & 1)) pr[k] = ds[k] = 0.f;
+          }
+          e[i / 2] = pack2<T>(pr[0], pr[1]), e[i / 2 + 1] = pack2<T>(pr[2], pr[3]);
+          d[i / 2] = pack2<T>(ds[0], ds[1]), d[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
+        }
+        if (keys) tmem_st16(at + F::kS * q, e);
+        tmem_st16(at + F::kS * q + 16, d);
+      }
+      tmem_wait_st();
+      tmem_fence_before();
+      mbar_arrive(&bar.p_full);
     }
+    if (ok && n) ok = guard_wait(&bar.acc_full, 0, g, 0x31006);
+    tmem_fence_after();
+    // results leave through the space of what stayed: panels of 64 columns, by turns of the two halves
+    const int64_t length = keys ? p.sk : p.sq;
+    if (ok && r0 < length)
+      for (int job = half; job < (keys ? 2 : 1) * F::kPanels; job += 2) {
+        const bool is_v = keys && job < F::kPanels;   // dv first, then dk; or dq alone
+        const int panel = job % F::kPanels;
+        const uint32_t from = tmem + lanes + (is_v ? F::kAcc1 : F::kAcc2) + 64 * panel;
+        const float scale = is_v ? 1.f : (float)p.scale;
+        uint8_t* to = stay + job * kPanel + 32 * quad * 128;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t o[32];
+          if (n) {
+            tmem_ld32(from + c, o);
+            tmem_wait_ld();
+          }
+          float v[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] = n ? __uint_as_float(o[k]) * scale : 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            *(uint4*)(to + staged(lane, 2 * (c + k))) =
+                make_uint4(pack2<T>(v[k], v[k + 1]), pack2<T>(v[k + 2], v[k + 3]), pack2<T>(v[k + 4], v[k + 5]),
+                           pack2<T>(v[k + 6], v[k + 7]));
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(keys ? (is_v ? &l.map.dv : &l.map.dk) : &l.map.dq, to, 64 * panel, head, r0 + 32 * quad, b);
+          tma_store_commit();
+        }
+      }
+    if (lane == 0) tma_store_wait_read<0>();
+    tmem_fence_before();
   }
-  T* ok = (T*)a.dk + b * a.dk_b + j * a.dk_s + hk * a.dk_h;
-  T* ov = (T*)a.dv + b * a.dv_b + j * a.dv_s + hk * a.dv_h;
-  for (int c = 0; c < kMaxDim / 32; ++c)
-    if (32 * c + lane < d) {
-      ok[32 * c + lane] = from_f<T>(dk[c] * (float)a.scale);
-      ov[32 * c + lane] = from_f<T>(dv[c]);
+  __syncwarp();
+  __syncthreads();
+  if (warp == 1 && n) {
+    if (lane == 0) {
+      g.gave_up = 0;
+      guard_wait(&bar.acc_full, 0, g, 0x60002);
     }
+    __syncwarp();
+  }
+  tmem_fence_after();
+  if (warp == 1) tmem_free<1>(tmem, 512);
 }
 
 bool args_ok(const HpAttention* a) {
@@ -497,16 +753,40 @@ int forward(const HpAttention& a, cudaStream_t s) {
   if (a.dim <= 64) return two ? forward_tiles<T, 64, 2>(l, s) : forward_tiles<T, 64, 1>(l, s);
   return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
 }
+template <typename T, int DP>
+int backward_tiles(const Launch& l, cudaStream_t s) {
+  using F = Backward<DP>;
+  static const cudaError_t allowed =
+      cudaFuncSetAttribute(attention_backward_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  if (allowed != cudaSuccess) return allowed;
+  const HpAttention& a = l.p;
+  const int64_t nq = (a.sq + kB - 1) / kB, nk = (a.sk + kB - 1) / kB, tiles = nk * a.kv_heads + nq * a.heads;
+  if (tiles > INT32_MAX) return HP_ERR_TOO_LARGE;
+  if (a.sq) {
+    constexpr int kLanes = DP / 8;
+    attention_rows<T, kLanes><<<dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch), 256, 0, s>>>(a);
+    if (const cudaError_t e = cudaGetLastError()) return e;
+  }
+  attention_backward_tiles<T, DP><<<dim3((unsigned)tiles, (unsigned)a.batch), F::kThreads, F::kSmem, s>>>(l);
+  return cudaGetLastError();
+}
+
 template <typename T>
 int backward(const HpAttention& a, cudaStream_t s) {
-  const dim3 grid((unsigned)((a.sq + kWarps - 1) / kWarps), (unsigned)a.heads, (unsigned)a.batch);
-  const dim3 keys((unsigned)((a.sk + kWarps - 1) / kWarps), (unsigned)a.kv_heads, (unsigned)a.batch);
-  if (a.sq) {
-    attention_delta_kernel<T><<<grid, 32 * kWarps, 0, s>>>(a);
-    attention_dq_kernel<T><<<grid, 32 * kWarps, 0, s>>>(a);
-  }
-  if (a.sk) attention_dkv_kernel<T><<<keys, 32 * kWarps, 0, s>>>(a);
-  return cudaGetLastError();
+  if (!a.sq && !a.sk) return 0;
+  Launch l;
+  if (const int rc = prepare(l, a)) return rc;
+  const void* some = a.sq ? a.q : a.k;   // an address for tensors without elements, of which nothing is read
+  auto map = [&](CUtensorMap* m, const void* base, bool key, int64_t sb, int64_t ss, int64_t sh, uint32_t rows) {
+    const int64_t length = key ? a.sk : a.sq;
+    return head_map(m, length ? base : some, a, length, key ? a.kv_heads : a.heads, sb, ss, sh, rows);
+  };
+  if (!map(&l.map.q, a.q, false, a.q_b, a.q_s, a.q_h, kB) || !map(&l.map.k, a.k, true, a.k_b, a.k_s, a.k_h, kB) ||
+      !map(&l.map.v, a.v, true, a.v_b, a.v_s, a.v_h, kB) || !map(&l.map.d_o, a.d_o, false, a.do_b, a.do_s, a.do_h, kB) ||
+      !map(&l.map.dq, a.dq, false, a.dq_b, a.dq_s, a.dq_h, 32) || !map(&l.map.dk, a.dk, true, a.dk_b, a.dk_s, a.dk_h, 32) ||
+      !map(&l.map.dv, a.dv, true, a.dv_b, a.dv_s, a.dv_h, 32))
+    return HP_ERR_BAD_ARG;
+  return a.dim <= 64 ? backward_tiles<T, 64>(l, s) : backward_tiles<T, 128>(l, s);
 }
 
 }  // namespace

@@ -36,9 +36,18 @@ bool tensor_map(CUtensorMap* m, const void* base, int type, int rank, const uint
     size[i] = sizes[i] ? sizes[i] : 1;
     if (i) stride[i - 1] = strides_bytes[i - 1];
   }
-  return f(m, type == HP_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : type == HP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank,
-           (void*)base, size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const CUtensorMapDataType t = type == HP_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : type == HP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto encode = [&] {
+    return f(m, t, (cuuint32_t)rank, (void*)base, size, stride, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  if (encode() == CUDA_SUCCESS) return true;
+  // a thread that has not used the device yet (autograd's, in its first backward pass) has no context
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+  return encode() == CUDA_SUCCESS;
 }
 
 uint32_t* layer_status(int* rc) {

@@ -458,7 +458,7 @@ def _attention_backward(q, k, v, o, lse, do, mask, causal, scale, dq, dk, dv):
         dv.copy_(group(p.transpose(2, 3) @ g))
         return
     q, k, v, do, mask = _tileable(q), _tileable(k), _tileable(v), _tileable(do), _mask(mask)
-    delta = torch.empty(b, h, sq, dtype=torch.float32, device=q.device)
+    delta = torch.empty(b, h, 2, (sq + 127) // 128 * 128, dtype=torch.float32, device=q.device)
     _call("attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(mask),
           do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), b, sq, sk, h, hk, d,
           *_strides(q), *_strides(k), *_strides(v), *_strides(o), *_strides(do), *_strides(dq), *_strides(dk),

@@ -330,6 +330,20 @@ def test_layers_on_a_stream_of_their_own():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_layers_in_a_thread_that_has_not_used_the_gpu():
+    import threading
+    from hipress_b200.ops import attention, linear
+    torch.manual_seed(11)
+    x, w = rand(40, 64, dtype=BF16), rand(64, 64, dtype=BF16)
+    want = linear(x, w), attention(*(x.view(1, 40, 1, 64),) * 3)
+    got = []
+    for call in (lambda: linear(x, w), lambda: attention(*(x.view(1, 40, 1, 64),) * 3)):
+        t = threading.Thread(target=lambda: got.append(call()))
+        t.start()
+        t.join()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_layers_in_a_graph():
     from hipress_b200.ops import attention, layer_norm, linear
     torch.manual_seed(10)
