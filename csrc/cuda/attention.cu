@@ -13,6 +13,13 @@ __device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r *
 // 2^x for the softmax is exp2_fast(); what a masked score becomes
 constexpr float kNone = -INFINITY;
 
+struct Yes {
+  __device__ constexpr operator bool() const { return true; }
+};
+struct No {
+  __device__ constexpr operator bool() const { return false; }
+};
+
 // Which of a tile's 128 columns a row may see, a bit each.
 struct Seen {
   uint32_t w[4];
@@ -41,6 +48,20 @@ __device__ __forceinline__ Seen mask_bits(const uint8_t* mask, int64_t k0, int64
   return s;
 }
 
+// By the whole CTA: one more than the last key that a sequence's mask lets see.
+__device__ __forceinline__ int visible_keys(const uint8_t* mask, int sk, int* shared) {
+  if (threadIdx.x == 0) *shared = 0;
+  __syncthreads();
+  int last = 0;
+  for (int k = threadIdx.x; k < sk; k += blockDim.x)
+    if (mask[k]) last = k + 1;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+  if ((threadIdx.x & 31) == 0) atomicMax(shared, last);
+  __syncthreads();
+  return *shared;
+}
+
 struct Maps {
   CUtensorMap q, k, v, o, d_o, dq, dk, dv;
 };
@@ -58,23 +79,35 @@ struct Launch {
 // scores, O += P v.  While one tile's rows are at work the other's products run.  The sums keep a
 // running maximum; the results so far are scaled anew only when it rises by more than 2^8 (the
 // factor that 32-bit sums and 16-bit probabilities bear easily).  Bound: 2^x, 16 a cycle and SM.
-template <int DP, int QT>
+// SHORT is for up to 128 queries and keys: one tile each, nothing to walk over.  Its results take
+// the half of the scores' columns that the probabilities leave, so that four CTAs fit an SM and
+// hide one another's latency.
+template <int DP, int QT, bool SHORT>
 struct Forward {
-  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = DP == 64 && QT == 2 ? 4 : 2;
-  static constexpr int kThreads = 64 + 128 * QT;
+  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = SHORT ? 1 : DP == 64 && QT == 2 ? 4 : 2;
+  // four warps that fetch and issue, four for each tile's rows; the former give registers to the latter
+  static constexpr int kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
+  static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : 168, kFew = SHORT ? 64 : 72, kMany = SHORT ? 64 : QT == 1 ? 184 : 216;
+  static_assert(kFew + QT * kMany <= (1 + QT) * kAtStart, "more registers than the CTA has");
   static constexpr int kSmem = QT * kTile + kStages * 2 * kTile + 1024 + 1024;
-  static constexpr int kTmem = QT == 2 ? 512 : 256;
+  static constexpr int kTmem = SHORT ? 128 : QT == 2 ? 512 : 256;
+  // columns: scores of each tile, results, probabilities.  With 64 dimensions these have columns of
+  // their own, and the next scores need not wait for the product that reads them
+  static constexpr bool kApart = !SHORT && DP == 64;
+  static constexpr uint32_t kO = SHORT ? 64 : QT * 128, kP = kApart ? QT * (128 + 64) : 0, kPStep = kApart ? 64 : 128;
 };
 struct ForwardBars {
-  uint64_t q_full, k_full[4], v_full[4], k_empty[4], v_empty[4], mask_full[4], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t q_full, k_full[4], v_full[4], k_empty[4], v_empty[4], mask_full[4], s_full[2], s_free[2], p_full[2], o_full[2], drain;
   Seen seen[4];
   uint32_t tmem;
+  int keys;
   Guard guard;
 };
 
-template <typename T, int DP, int QT>
-__global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forward_tiles(const __grid_constant__ Launch l) {
-  using F = Forward<DP, QT>;
+template <typename T, int DP, int QT, bool SHORT>
+__global__ void __launch_bounds__(128 + 128 * QT, (Forward<DP, QT, SHORT>::kPerSm))
+attention_forward_tiles(const __grid_constant__ Launch l) {
+  using F = Forward<DP, QT, SHORT>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = smem;
@@ -84,7 +117,10 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the tiles with the most keys first, where the mask is causal
   const int qt = (int)gridDim.x - 1 - (int)blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(p.heads / p.kv_heads);
-  const int q0 = qt * kB * QT, sk = (int)p.sk, shift = (int)(p.sk - p.sq);
+  const int q0 = qt * kB * QT, shift = (int)(p.sk - p.sq);
+  const bool masked = p.key_mask != nullptr;
+  const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
+  const int sk = !SHORT && masked && p.sk > kB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
   // key tiles of each query tile
   int n[QT], most = 0;
 #pragma unroll
@@ -100,7 +136,10 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
       mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.k_empty[i], 1), mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.mask_full[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1), mbar_init(&bar.p_full[i], 128), mbar_init(&bar.o_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.s_full[i], 1), mbar_init(&bar.s_free[i], 128);
+      mbar_init(&bar.p_full[i], 128), mbar_init(&bar.o_full[i], 1);
+    }
     mbar_init(&bar.drain, 1);
     mbar_init_fence();
     bar.guard.gave_up = 0;
@@ -110,10 +149,11 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = bar.tmem, tmem_o = tmem + QT * 128;   // scores, then results
+  const uint32_t tmem = bar.tmem, tmem_o = tmem + F::kO;
   Guard& g = bar.guard;
-  const bool masked = p.key_mask != nullptr;
 
+  if (warp < 4) {
+  if (F::kFew < F::kMany) fewer_registers<F::kFew>();
   if (warp == 0) {
     // k and v of key tile j into stage j; the mask's bits beside them
     int waits = 0;   // copies to wait for should the CTA give up
@@ -137,7 +177,7 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
       // whoever reads the bits gives probabilities before the product that frees v
       if (!guard_wait(&bar.v_empty[s], ph ^ 1, g, 0x10003)) break;
       if (masked) {
-        const Seen m = mask_bits(p.key_mask + b * p.mask_b, (int64_t)j * kB, sk);
+        const Seen m = mask_bits(mask, (int64_t)j * kB, sk);
         if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
       }
       if (lane == 0) {
@@ -165,42 +205,56 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
       bool ok = guard_wait(&bar.q_full, 0, g, 0x20001);
       auto scores = [&](int t, int j) {   // S_t = q_t k_j^T
         const int s = j % F::kStages;
-        const uint32_t a = smem_u32(sq + t * F::kTile), k = smem_u32(skv + s * 2 * F::kTile);
+        const uint64_t a = mma_desc(smem_u32(sq + t * F::kTile), 16, 1024), k = mma_desc(smem_u32(skv + s * 2 * F::kTile), 16, 1024);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t at = (i / 4) * kPanel + (i % 4) * 32;
-          mma_ss<1>(tmem + t * 128, mma_desc(a + at, 16, 1024), mma_desc(k + at, 16, 1024), id_s, i > 0);
+          const uint32_t at = ((i / 4) * kPanel + (i % 4) * 32) >> 4;
+          mma_ss<1>(tmem + t * 128, a + at, k + at, id_s, i > 0);
         }
         mma_commit<1>(&bar.s_full[t]);
       };
+      auto results = [&](int t, int j) {   // O_t += P_t v_j
+        const uint64_t v = mma_desc(smem_u32(skv + (j % F::kStages) * 2 * F::kTile + F::kTile), kPanel, 1024);
+#pragma unroll
+        for (int i = 0; i < kB / 16; ++i)
+          mma_ts(tmem_o + t * DP, tmem + F::kP + t * F::kPStep + i * 8, v + i * 128, id_o, j > 0 || i > 0);
+        mma_commit<1>(&bar.o_full[t]);
+      };
       for (int j = 0; j <= most && ok; ++j) {   // scores of tile j, results of tile j - 1
         if (j < most) ok = guard_wait(&bar.k_full[j % F::kStages], (j / F::kStages) & 1, g, 0x20002);
+        if (F::kApart && ok) {   // scores as soon as the last ones have been read
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            if (j >= n[t] || !ok) continue;
+            if (j > 0) ok = guard_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
+            tmem_fence_after();
+            if (ok) scores(t, j);
+          }
+          if (ok && j < most) mma_commit<1>(&bar.k_empty[j % F::kStages]);
+        }
         if (j > 0 && ok) ok = guard_wait(&bar.v_full[(j - 1) % F::kStages], ((j - 1) / F::kStages) & 1, g, 0x20003);
         tmem_fence_after();
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          if (!ok) break;
-          if (j > 0 && j - 1 < n[t]) {
+          if (j > 0 && j - 1 < n[t] && ok) {
             ok = guard_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
-            if (!ok) break;
             tmem_fence_after();
-            const uint32_t v = smem_u32(skv + ((j - 1) % F::kStages) * 2 * F::kTile + F::kTile);
-#pragma unroll
-            for (int i = 0; i < kB / 16; ++i)
-              mma_ts(tmem_o + t * DP, tmem + t * 128 + i * 8, mma_desc(v + i * 2048, kPanel, 1024), id_o, j > 1 || i > 0);
-            mma_commit<1>(&bar.o_full[t]);
+            if (ok) results(t, j - 1);
           }
-          if (j < n[t]) scores(t, j);
+          if (!F::kApart && j < n[t] && ok) scores(t, j);   // over the probabilities just used
         }
         if (j > 0) mma_commit<1>(&bar.v_empty[(j - 1) % F::kStages]);
-        if (j < most) mma_commit<1>(&bar.k_empty[j % F::kStages]);
+        if (!F::kApart && j < most) mma_commit<1>(&bar.k_empty[j % F::kStages]);
       }
       mma_commit<1>(&bar.drain);
     }
+  }
   } else {
-    const int t = (warp - 2) >> 2, quad = warp & 3, r = 32 * quad + lane;   // one row to a thread
+    if (F::kFew < F::kMany) more_registers<F::kMany>();
+    const int t = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane;   // one row to a thread
     const int row = q0 + t * kB + r, nt = QT == 1 ? n[0] : (t ? n[QT - 1] : n[0]);
     const uint32_t lanes = (uint32_t)(32 * quad) << 16, ts = tmem + t * 128 + lanes, to = tmem_o + t * DP + lanes;
+    const uint32_t tp = tmem + F::kP + t * F::kPStep + lanes;
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;   // keys this row sees but for the mask
     float m = kNone, sum = 0.f;
     bool ok = true;
@@ -238,20 +292,40 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
       // the product before these scores is done too; every phase is waited for, so that none is mistaken
       if (j > 0 && !guard_wait(&bar.o_full[t], (j - 1) & 1, g, 0x30004)) { ok = false; break; }
       tmem_fence_after();
-      float top = kNone;
+      // a row of scores stays in registers where those suffice, else it is read twice, in steps
+      constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : kB;
+      uint32_t x[kHeld];
+      auto read = [&](int c, uint32_t* to) {
+        if constexpr (SHORT) tmem_ld16(ts + c, *(uint32_t(*)[16])to);
+        else tmem_ld32(ts + c, *(uint32_t(*)[32])to);
+      };
+      float part[4] = {kNone, kNone, kNone, kNone};
+      if (kHeld == kB) {
 #pragma unroll
-      for (int c = 0; c < kB; c += 32) {
-        uint32_t x[32];
-        tmem_ld32(ts + c, x);
+        for (int c = 0; c < kB; c += kStep) read(c, x + c % kHeld);
         tmem_wait_ld();
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, seen.w[c / 32] >> i & 1 ? __uint_as_float(x[i]) : kNone);
+        if (F::kApart) {
+          tmem_fence_before();
+          mbar_arrive(&bar.s_free[t]);
         }
       }
+      auto highest = [&](auto all) {   // tiles that are seen whole test no bits
+#pragma unroll
+        for (int c = 0; c < kB; c += kStep) {
+          if (kHeld != kB) {
+            read(c, x);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int i = 0; i < kStep; ++i) {
+            const float v = __uint_as_float(x[(c + i) % kHeld]);
+            part[i & 3] = fmaxf(part[i & 3], all || (seen.w[c / 32] >> (c % 32 + i) & 1) ? v : kNone);
+          }
+        }
+      };
+      if (whole) highest(Yes());
+      else highest(No());
+      float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       top = top == kNone ? kNone : top * l.c;   // 0 times infinity otherwise
       if (__any_sync(0xffffffffu, top > m + 8.f || (m == kNone && top != kNone))) {
         const float now = fmaxf(m, top), keep = now == kNone ? 1.f : exp2_fast(m - now);
@@ -272,24 +346,33 @@ __global__ void __launch_bounds__(64 + 128 * QT, QT == 1 ? 2 : 1) attention_forw
       }
       const float base = m == kNone ? 0.f : -m;
 #pragma unroll
-      for (int c = 0; c < kB; c += 32) {
-        uint32_t x[32], y[16];
-        tmem_ld32(ts + c, x);
-        tmem_wait_ld();
-        float e[32];
+      for (int k = 0; k < 4; ++k) part[k] = 0.f;
+      auto probabilities = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          e[i] = exp2_fast(fmaf(__uint_as_float(x[i]), l.c, base));
-          if (!whole) e[i] = seen.w[c / 32] >> i & 1 ? e[i] : 0.f;
+        for (int c = 0; c < kB; c += kStep) {
+          uint32_t y[kStep / 2];
+          if (kHeld != kB) {
+            read(c, x);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int i = 0; i < kStep; i += 2) {
+            float e[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              e[k] = exp2_fast(fmaf(__uint_as_float(x[(c + i + k) % kHeld]), l.c, base));
+              if (!all) e[k] = seen.w[c / 32] >> (c % 32 + i + k) & 1 ? e[k] : 0.f;
+              part[(i + k) & 3] += e[k];
+            }
+            y[i / 2] = pack2<T>(e[0], e[1]);
+          }
+          if constexpr (SHORT) tmem_st8(tp + c / 2, y);
+          else tmem_st16(tp + c / 2, y);
         }
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 32; ++i) part[i & 3] += e[i];
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = pack2<T>(e[2 * i], e[2 * i + 1]);
-        tmem_st16(ts + c / 2, y);
-      }
+      };
+      if (whole) probabilities(Yes());
+      else probabilities(No());
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
       tmem_wait_st();
       tmem_fence_before();
       mbar_arrive(&bar.p_full[t]);
@@ -388,35 +471,23 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
 template <int DP>
 struct Backward {
   static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = DP == 64 ? 4 : 2;
-  static constexpr int kThreads = 64 + 256;
+  // four warps that fetch and issue, eight for the rows; the former give registers to the latter
+  static constexpr int kThreads = 128 + 256, kAtStart = 168, kFew = 72, kMany = 216;
+  static_assert(kFew + 2 * kMany <= 3 * kAtStart, "more registers than the CTA has");
   static constexpr int kSmem = 2 * kTile + kStages * (2 * kTile + 1024) + 1024 + 1024;
   // columns: S (buffers kS apart), dP, the results
   static constexpr uint32_t kS = 256, kDP = 128, kAcc1 = DP == 64 ? 384 : 256, kAcc2 = DP == 64 ? 448 : 384;
 };
 struct BackwardBars {
-  uint64_t stay_full, in_full[4], in_empty[4], mask_full[4], s_full[2], dp_full, p_full, acc_full;
+  uint64_t stay_full, in_full[4], in_empty[4], mask_full[4], s_full[2], dp_full, dp_free, p_full, acc_full;
   Seen seen[4];
   uint32_t tmem;
   int keys;
   Guard guard;
 };
 
-// By the whole CTA: one more than the last key that a sequence's mask lets see.
-__device__ __forceinline__ int visible_keys(const uint8_t* mask, int sk, int* shared) {
-  if (threadIdx.x == 0) *shared = 0;
-  __syncthreads();
-  int last = 0;
-  for (int k = threadIdx.x; k < sk; k += blockDim.x)
-    if (mask[k]) last = k + 1;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-  if ((threadIdx.x & 31) == 0) atomicMax(shared, last);
-  __syncthreads();
-  return *shared;
-}
-
 template <typename T, int DP>
-__global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_constant__ Launch l) {
+__global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_constant__ Launch l) {
   using F = Backward<DP>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -461,7 +532,7 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
     mbar_init(&bar.stay_full, 1);
     for (int i = 0; i < 4; ++i) mbar_init(&bar.in_full[i], 1), mbar_init(&bar.in_empty[i], 1), mbar_init(&bar.mask_full[i], 1);
     mbar_init(&bar.s_full[0], 1), mbar_init(&bar.s_full[1], 1), mbar_init(&bar.dp_full, 1);
-    mbar_init(&bar.p_full, 256), mbar_init(&bar.acc_full, 1);
+    mbar_init(&bar.dp_free, 256), mbar_init(&bar.p_full, 256), mbar_init(&bar.acc_full, 1);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
@@ -473,6 +544,8 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
   const uint32_t tmem = bar.tmem;
   Guard& g = bar.guard;
 
+  if (warp < 4) {
+  fewer_registers<F::kFew>();
   if (warp == 0) {
     const uint32_t bytes = 2 * F::kTile + (keys ? 8 * kB : 0);
     const int64_t rows = padded(p.sq);
@@ -521,16 +594,17 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
       const uint32_t a = smem_u32(stay);
       auto in = [&](int j) { return smem_u32(pass + (j % F::kStages) * 2 * F::kTile); };
       auto wide = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t id) {   // rows by rows, over the dimensions
+        const uint64_t dx = mma_desc(x, 16, 1024), dy = mma_desc(y, 16, 1024);
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t at = (i / 4) * kPanel + (i % 4) * 32;
-          mma_ss<1>(d, mma_desc(x + at, 16, 1024), mma_desc(y + at, 16, 1024), id, i > 0);
+          const uint32_t at = ((i / 4) * kPanel + (i % 4) * 32) >> 4;
+          mma_ss<1>(d, dx + at, dy + at, id, i > 0);
         }
       };
       auto deep = [&](uint32_t d, uint32_t x, uint32_t y, bool add) {      // P or dS, over the tile's columns
+        const uint64_t dy = mma_desc(y, kPanel, 1024);
 #pragma unroll
-        for (int i = 0; i < kB / 16; ++i)
-          mma_ts(d, x + (i / 2) * 32 + (i % 2) * 8, mma_desc(y + i * 2048, kPanel, 1024), id_acc, add || i > 0);
+        for (int i = 0; i < kB / 16; ++i) mma_ts(d, x + (i / 2) * 32 + (i % 2) * 8, dy + i * 128, id_acc, add || i > 0);
       };
       auto scores = [&](int j) {
         const int q = buffers == 2 ? j & 1 : 0;
@@ -553,11 +627,14 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
           ok = there(j + 1);
           if (!ok) break;
           if (buffers == 2) scores(j + 1);
+          ok = guard_wait(&bar.dp_free, j & 1, g, 0x21004);
+          if (!ok) break;
+          tmem_fence_after();
+          dprobs(j + 1);
         }
         ok = guard_wait(&bar.p_full, j & 1, g, 0x21003);
         if (!ok) break;
         tmem_fence_after();
-        if (j + 1 < n) dprobs(j + 1);
         const uint32_t s = tmem + F::kS * (buffers == 2 ? j & 1 : 0);
         if (keys) deep(tmem + F::kAcc1, s, in(j) + F::kTile, j > 0);
         deep(tmem + F::kAcc2, s + 16, in(j), j > 0);
@@ -566,8 +643,10 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
       }
       mma_commit<1>(&bar.acc_full);
     }
+  }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2, r = 32 * quad + lane, row = r0 + r;
+    more_registers<F::kMany>();
+    const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane, row = r0 + r;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
     float lse = INFINITY, delta = 0.f;   // of a query that stays
     bool mine = true;                    // a key that stays is seen at all
@@ -622,32 +701,49 @@ __global__ void __launch_bounds__(320, 1) attention_backward_tiles(const __grid_
       if (keys && !guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31005)) { ok = false; break; }
       tmem_fence_after();
       const float* cols = rows_of + s * 2 * kB + 64 * half;
+      // both of this thread's halves at once: dP's columns are free for the next tile's then
+      uint32_t xs[2][32], ys[2][32];
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
-        const uint32_t at = tmem + lanes + 64 * half + c;
-        uint32_t x[32], y[32], e[16], d[16];
-        tmem_ld32(at + F::kS * q, x);
-        tmem_ld32(at + F::kDP, y);
-        tmem_wait_ld();
-        const uint32_t bits = whole ? 0xffffffffu : seen.w[2 * half + c / 32];
+      for (int c = 0; c < 2; ++c) {
+        tmem_ld32(tmem + lanes + 64 * half + 32 * c + F::kS * q, xs[c]);
+        tmem_ld32(tmem + lanes + 64 * half + 32 * c + F::kDP, ys[c]);
+      }
+      tmem_wait_ld();
+      tmem_fence_before();
+      mbar_arrive(&bar.dp_free);
+      auto gradients = [&](auto all, auto of_keys) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 ls = make_float4(lse, lse, lse, lse), de = make_float4(delta, delta, delta, delta);
-          if (keys) ls = *(const float4*)(cols + c + i), de = *(const float4*)(cols + kB + c + i);
-          float pr[4], ds[4];
+        for (int c = 0; c < 64; c += 32) {
+          const uint32_t at = tmem + lanes + 64 * half + c;
+          const uint32_t(&x)[32] = xs[c / 32], (&y)[32] = ys[c / 32];
+          const uint32_t bits = all ? 0xffffffffu : seen.w[2 * half + c / 32];
+          uint32_t e[16], d[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float w = k == 0 ? ls.x : k == 1 ? ls.y : k == 2 ? ls.z : ls.w;
-            const float v = k == 0 ? de.x : k == 1 ? de.y : k == 2 ? de.z : de.w;
-            pr[k] = exp2_fast(fmaf(__uint_as_float(x[i + k]), l.c, -w));
-            ds[k] = pr[k] * (__uint_as_float(y[i + k]) - v);
-            if (!whole && !(bits >> (i + k) & 1)) pr[k] = ds[k] = 0.f;
+          for (int i = 0; i < 32; i += 4) {
+            float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta}, pr[4], ds[4];
+            if (of_keys) {
+              *(float4*)ls = *(const float4*)(cols + c + i);
+              *(float4*)de = *(const float4*)(cols + kB + c + i);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              pr[k] = exp2_fast(fmaf(__uint_as_float(x[i + k]), l.c, -ls[k]));
+              ds[k] = pr[k] * (__uint_as_float(y[i + k]) - de[k]);
+              if (!all && !(bits >> (i + k) & 1)) pr[k] = ds[k] = 0.f;
+            }
+            if (of_keys) e[i / 2] = pack2<T>(pr[0], pr[1]), e[i / 2 + 1] = pack2<T>(pr[2], pr[3]);
+            d[i / 2] = pack2<T>(ds[0], ds[1]), d[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
           }
-          e[i / 2] = pack2<T>(pr[0], pr[1]), e[i / 2 + 1] = pack2<T>(pr[2], pr[3]);
-          d[i / 2] = pack2<T>(ds[0], ds[1]), d[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
+          if (of_keys) tmem_st16(at + F::kS * q, e);
+          tmem_st16(at + F::kS * q + 16, d);
         }
-        if (keys) tmem_st16(at + F::kS * q, e);
-        tmem_st16(at + F::kS * q + 16, d);
+      };
+      if (keys) {
+        if (whole) gradients(Yes(), Yes());
+        else gradients(No(), Yes());
+      } else {
+        if (whole) gradients(Yes(), No());
+        else gradients(No(), No());
       }
       tmem_wait_st();
       tmem_fence_before();
@@ -729,14 +825,14 @@ int prepare(Launch& l, const HpAttention& a) {
   return rc;
 }
 
-template <typename T, int DP, int QT>
+template <typename T, int DP, int QT, bool SHORT = false>
 int forward_tiles(const Launch& l, cudaStream_t s) {
-  using F = Forward<DP, QT>;
+  using F = Forward<DP, QT, SHORT>;
   static const cudaError_t allowed =
-      cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+      cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (allowed != cudaSuccess) return allowed;
   const dim3 grid((unsigned)((l.p.sq + kB * QT - 1) / (kB * QT)), (unsigned)l.p.heads, (unsigned)l.p.batch);
-  attention_forward_tiles<T, DP, QT><<<grid, F::kThreads, F::kSmem, s>>>(l);
+  attention_forward_tiles<T, DP, QT, SHORT><<<grid, F::kThreads, F::kSmem, s>>>(l);
   return cudaGetLastError();
 }
 
@@ -750,6 +846,7 @@ int forward(const HpAttention& a, cudaStream_t s) {
       !head_map(&l.map.o, a.o, a, a.sq, a.heads, a.o_b, a.o_s, a.o_h, 32))
     return HP_ERR_BAD_ARG;
   const bool two = a.sq > kB;
+  if (a.dim <= 64 && !two && a.sk <= kB) return forward_tiles<T, 64, 1, true>(l, s);
   if (a.dim <= 64) return two ? forward_tiles<T, 64, 2>(l, s) : forward_tiles<T, 64, 1>(l, s);
   return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
 }
