@@ -699,7 +699,7 @@ extern "C" int hp_cuda_norm_backward(const HpNormBackward* a, void* stream) {
   return BY_TYPE(backward);
 }
 
-extern "C" uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols, int64_t) {
+extern "C" uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols) {
   const int64_t ctas = rows + 8 < kMostCtas ? rows + 8 : kMostCtas;
   return (uint64_t)ctas * 2 * cols * 4;
 }

@@ -646,4 +646,4 @@ extern "C" int hp_cuda_slope(const HpSlope* a, void* stream) {
   return a->type == HP_BF16 ? slopes<__nv_bfloat16>(*a, s) : slopes<__half>(*a, s);
 }
 
-extern "C" uint64_t hp_cuda_slope_workspace(int64_t, int64_t cols, int64_t) { return (uint64_t)kSlopeParts * cols * 4; }
+extern "C" uint64_t hp_cuda_slope_workspace(int64_t, int64_t cols) { return (uint64_t)kSlopeParts * cols * 4; }

@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include "hipress/capi.h"
+#include "hipress/layers.h"
 #include "sync.cuh"
 
 namespace hipress {
@@ -54,6 +55,7 @@ const char* hp_cuda_error_string(int code) {
   if (code == HP_ERR_TOO_LARGE)
     return "hipress: input larger than this entry point supports (bucket or element limit)";
   if (code == HP_ERR_RESIDENCY) return "hipress: emulated ranks would not be co-resident";
+  if (code == HP_ERR_TIMEOUT) return "hipress: an earlier kernel gave up waiting, its results are invalid";
   return cudaGetErrorString((cudaError_t)code);
 }
 

@@ -17,7 +17,6 @@
 
 #include "hipress/capi.h"
 #include "hipress/common.h"
-#include "hipress/layers.h"
 
 namespace {
 
@@ -40,23 +39,6 @@ FusedDense f_fused_dense;
 FusedSparse f_fused_sparse_ps, f_fused_sparse_ring;
 StreamOrder f_stream_order;
 
-// the layer operators take a block of 8-byte words
-using Layer = int (*)(const void*, void*);
-constexpr int kLayers = 6, kLayerWords = 64;
-Layer f_layer[kLayers];
-const struct {
-  const char* name;
-  int words;
-} kLayer[kLayers] = {{"norm_forward", sizeof(HpNormForward) / 8},
-                     {"norm_backward", sizeof(HpNormBackward) / 8},
-                     {"product", sizeof(HpProduct) / 8},
-                     {"slope", sizeof(HpSlope) / 8},
-                     {"attention_forward", sizeof(HpAttention) / 8},
-                     {"attention_backward", sizeof(HpAttention) / 8}};
-using LayerWorkspace = uint64_t (*)(int64_t, int64_t, int64_t);
-LayerWorkspace f_layer_workspace[3];
-static_assert(sizeof(HpAttention) <= 8 * kLayerWords, "the block of words is too small");
-
 struct Name {
   const char* name;
   void** slot;
@@ -70,15 +52,6 @@ const Name kNames[] = {
     {"hp_cuda_fused_sparse_ps", (void**)&f_fused_sparse_ps},
     {"hp_cuda_fused_sparse_ring", (void**)&f_fused_sparse_ring},
     {"hp_cuda_stream_order", (void**)&f_stream_order},
-    {"hp_cuda_norm_forward", (void**)&f_layer[0]},
-    {"hp_cuda_norm_backward", (void**)&f_layer[1]},
-    {"hp_cuda_product", (void**)&f_layer[2]},
-    {"hp_cuda_slope", (void**)&f_layer[3]},
-    {"hp_cuda_attention_forward", (void**)&f_layer[4]},
-    {"hp_cuda_attention_backward", (void**)&f_layer[5]},
-    {"hp_cuda_norm_workspace", (void**)&f_layer_workspace[0]},
-    {"hp_cuda_product_workspace", (void**)&f_layer_workspace[1]},
-    {"hp_cuda_slope_workspace", (void**)&f_layer_workspace[2]},
 };
 
 // ------------------------------------------------------------ argument readers
@@ -195,33 +168,6 @@ PyObject* py_stream_order(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!arity(n, 3, "stream_order") || !bound((void*)f_stream_order, "stream_order")) return nullptr;
   void *ev = as_ptr(a[0]), *src = as_ptr(a[1]), *dst = as_ptr(a[2]);
   LAUNCH(f_stream_order(ev, src, dst));
-}
-
-// One call of a layer operator: the fields of its block in order (an address or None, an
-// integer, a float where the block has a double), then the stream.
-template <int I>
-PyObject* py_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!arity(n, kLayer[I].words + 1, kLayer[I].name) || !bound((void*)f_layer[I], kLayer[I].name)) return nullptr;
-  uint64_t w[kLayerWords];
-  for (int i = 0; i < kLayer[I].words; ++i) {
-    if (PyFloat_Check(a[i])) {
-      const double d = PyFloat_AS_DOUBLE(a[i]);
-      memcpy(&w[i], &d, 8);
-    } else {
-      w[i] = a[i] == Py_None ? 0 : as_u64(a[i]);
-    }
-  }
-  void* st = as_ptr(a[n - 1]);
-  LAUNCH(f_layer[I](w, st));
-}
-
-// bytes of scratch an operator wants for these sizes: (rows, cols), or (m, n, k)
-template <int I>
-PyObject* py_layer_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  const int want = I == 1 ? 3 : 2;
-  if (!arity(n, want, "workspace") || !bound((void*)f_layer_workspace[I], "workspace")) return nullptr;
-  const int64_t x = (int64_t)as_u64(a[0]), y = (int64_t)as_u64(a[1]), z = want == 3 ? (int64_t)as_u64(a[2]) : 0;
-  return PyErr_Occurred() ? nullptr : PyLong_FromUnsignedLongLong(f_layer_workspace[I](x, y, z));
 }
 
 // ---------------------------------------------------------------- bucket plans
@@ -353,15 +299,6 @@ PyMethodDef kMethods[] = {
     FAST("sparse_encode", py_sparse_encode, "hp_cuda_sparse_encode"),
     FAST("sparse_decode", py_sparse_decode, "hp_cuda_sparse_decode"),
     FAST("stream_order", py_stream_order, "hp_cuda_stream_order"),
-    FAST("norm_forward", py_layer<0>, "hp_cuda_norm_forward"),
-    FAST("norm_backward", py_layer<1>, "hp_cuda_norm_backward"),
-    FAST("product", py_layer<2>, "hp_cuda_product"),
-    FAST("slope", py_layer<3>, "hp_cuda_slope"),
-    FAST("attention_forward", py_layer<4>, "hp_cuda_attention_forward"),
-    FAST("attention_backward", py_layer<5>, "hp_cuda_attention_backward"),
-    FAST("norm_workspace", py_layer_workspace<0>, "hp_cuda_norm_workspace"),
-    FAST("product_workspace", py_layer_workspace<1>, "hp_cuda_product_workspace"),
-    FAST("slope_workspace", py_layer_workspace<2>, "hp_cuda_slope_workspace"),
     FAST("plan", py_plan, "plan of a fused bucket"),
     FAST("launch", py_launch, "one fused launch of a plan"),
     {nullptr, nullptr, 0, nullptr}};

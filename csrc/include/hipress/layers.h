@@ -1,6 +1,5 @@
 // C ABI of the layer operators: layer norm, the matrix product with an epilogue and
-// attention.  Every function takes one block of 8-byte words (addresses, int64, double),
-// so that the caller can hand them over without a copy per field, and the stream.
+// attention.  Every function takes a structure of its arguments and the stream.
 //
 // Return values as in capi.h.  Kernels that wait (for copies or matrix products of their
 // own CTA) bound every wait; one that expired is reported by the next call on that device
@@ -58,7 +57,7 @@ typedef struct {
   int64_t type, wtype;
 } HpNormBackward;
 int hp_cuda_norm_backward(const HpNormBackward* a, void* stream);
-uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols, int64_t unused);
+uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols);
 
 // One product out[m, n] = sum_k a(m, k) b(n, k) with its epilogue: p = out + bias;
 // y = act(p) + residual.  An operand is stored along k (kmajor 1: row m, pitch lda) or along
@@ -93,7 +92,7 @@ typedef struct {
   int64_t type, btype, act;
 } HpSlope;
 int hp_cuda_slope(const HpSlope* a, void* stream);
-uint64_t hp_cuda_slope_workspace(int64_t rows, int64_t cols, int64_t unused);
+uint64_t hp_cuda_slope_workspace(int64_t rows, int64_t cols);
 
 // Attention, forward (o, lse) and backward (dq, dk, dv from d_o, o and lse).  Tensors are
 // [batch, length, heads, dim] with the last axis dense; strides in elements.

@@ -3,9 +3,10 @@
 ``libhipress_cpu.so``  g++   CPU oracle, planner cost model, host runtime
 ``libhipress_cuda.so`` nvcc  sm_100a kernels (``-gencode arch=compute_100a,code=sm_100a``)
 ``_fastcall.so``       g++   CPython extension for the calls made once per tensor or bucket
+``_layers.so``         g++   PyTorch extension: the layer operators' autograd nodes
 
 The first two expose a plain C ABI that :mod:`hipress_b200._native.lib` binds with
-ctypes; none needs the PyTorch headers and a full rebuild takes well under a minute.
+ctypes; only ``_layers.so`` needs the PyTorch headers.  A full rebuild takes about a minute.
 Run ``python -m hipress_b200._native.build`` (add ``--force`` to rebuild).
 """
 from __future__ import annotations
@@ -96,12 +97,37 @@ def build_debug(force: bool = False, verbose: bool = False):
     return out
 
 
+def _cuda_home(nv: str) -> Path:
+    return Path(nv).resolve().parent.parent
+
+
+def build_layers(force: bool, verbose: bool, log):
+    """The PyTorch binding of the layer operators (needs PyTorch's and CUDA's headers)."""
+    import torch
+    out = HERE / "_layers.so"
+    src = sorted((CSRC / "torch").glob("*.cpp"))
+    stamp = OBJ / "layers.sha"
+    dg = _digest(src) + sys.version + torch.__version__
+    if not force and out.exists() and stamp.exists() and stamp.read_text() == dg:
+        return
+    root = Path(torch.__file__).parent
+    inc = [CSRC / "include", root / "include", root / "include/torch/csrc/api/include", sysconfig.get_path("include"),
+           _cuda_home(nvcc_path()) / "include"]
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_layers",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *[x for i in inc for x in ("-isystem" if i != CSRC / "include" else "-I", str(i))], "-o", str(out),
+          *map(str, src), "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], log)
+    stamp.write_text(dg)
+    if verbose:
+        print("built", out)
+
+
 def build(force: bool = False, verbose: bool = False) -> dict:
     """Compile whatever is out of date; returns the paths of the libraries."""
     cpu_src, cuda_src = _sources()
     OBJ.mkdir(exist_ok=True)
     out = {"cpu": HERE / "libhipress_cpu.so", "fast": HERE / "_fastcall.so",
-           "cuda": HERE / "libhipress_cuda.so"}
+           "cuda": HERE / "libhipress_cuda.so", "layers": HERE / "_layers.so"}
     inc = ["-I", str(CSRC / "include")]
     with open(OBJ / "build.log", "a") as log:
         stamp = OBJ / "cpu.sha"
@@ -122,8 +148,9 @@ def build(force: bool = False, verbose: bool = False) -> dict:
                 print("built", out["fast"])
         nv = nvcc_path()
         if nv is None:
-            if not out["cuda"].exists():
-                out["cuda"] = None
+            for name in ("cuda", "layers"):
+                if not out[name].exists():
+                    out[name] = None
             return out
         stamp = OBJ / "cuda.sha"
         dg = _digest(cuda_src)
@@ -134,12 +161,16 @@ def build(force: bool = False, verbose: bool = False) -> dict:
                 s, o = pair
                 return _run([nv, *NVCC_FLAGS, *inc, "-I", str(CSRC / "cuda"), "-c", str(s), "-o", str(o)], log)
 
-            with ThreadPoolExecutor(max_workers=min(8, len(cuda_src))) as ex:
+            with ThreadPoolExecutor(max_workers=min(8, len(cuda_src) + 1)) as ex:
+                layers = ex.submit(build_layers, force, verbose, log)
                 list(ex.map(one, zip(cuda_src, objs)))
+                layers.result()
             _run([nv, "-shared", "-o", str(out["cuda"]), *map(str, objs), "-lcudart"], log)
             stamp.write_text(dg)
             if verbose:
                 print("built", out["cuda"])
+        else:
+            build_layers(force, verbose, log)
     return out
 
 

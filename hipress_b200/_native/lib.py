@@ -33,6 +33,7 @@ _cpu = None
 _cuda = None
 _fast = None
 _fast_cuda = None
+_layers = None
 
 
 def _ensure_built():
@@ -172,6 +173,24 @@ def fast_cuda():
         F.bind({n: C.cast(getattr(L, n), C.c_void_p).value for n in F.symbols()})
         _fast_cuda = F
     return _fast_cuda
+
+
+def layers():
+    """The extension module ``_layers`` (csrc/torch/layers.cpp): the layer operators on CUDA
+    tensors, calling the library that :func:`cuda` loads."""
+    global _layers
+    if _layers is None:
+        path = HERE / "_layers.so"
+        err = None
+        if not path.exists() or os.environ.get("HIPRESS_REBUILD"):
+            err = _ensure_built()
+        if not path.exists():
+            raise NativeLibraryError(f"{path} missing and could not be built: {err}")
+        from . import _layers as module
+        L = cuda()
+        module.bind({n: C.cast(getattr(L, n), C.c_void_p).value for n in module.symbols()})
+        _layers = module
+    return _layers
 
 
 class OrderEvent(dict):

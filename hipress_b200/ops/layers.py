@@ -27,28 +27,9 @@ from torch.autograd.function import once_differentiable
 
 from .._native import lib as _lib
 
-TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+TYPES = (torch.float32, torch.bfloat16, torch.float16)
 HALF = (torch.bfloat16, torch.float16)
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _call(name, device, *args):
-    F = _lib.fast_cuda()
-    if device.index == _lib.current_device():
-        rc = getattr(F, name)(*args, _lib.stream_ptr())
-    else:
-        with torch.cuda.device(device):
-            rc = getattr(F, name)(*args, _lib.stream_ptr())
-    if rc:
-        _lib.check(rc, name)
-
-
-def _scratch(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _same_device(what, *ts):
@@ -57,10 +38,6 @@ def _same_device(what, *ts):
         if t is not None and t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
     return dev
-
-
-def _differentiable(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 def _autocast(x):
@@ -74,17 +51,6 @@ def _wide(x):
     return x if x.dtype == torch.float64 else x.float()   # CPU: float64 is taken as it is
 
 
-def _rows(x):
-    """``x`` as a matrix whose rows are dense; a copy only where there is no such view."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
-
-
-def _pitch(x):
-    # of one row there is no second to be reached, and its stride may be anything
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-
-
 # ================================================================== layer norm
 def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
     """Normalises the last axis of ``x``: ``(z - mean) / sqrt(var + eps) * weight + bias``.
@@ -95,7 +61,7 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
     for both."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: no columns in a tensor of shape {tuple(x.shape)}")
-    if x.dtype not in TYPE and not (x.dtype == torch.float64 and not x.is_cuda):
+    if x.dtype not in TYPES and not (x.dtype == torch.float64 and not x.is_cuda):
         raise TypeError(f"layer_norm: {x.dtype} is not supported")
     _same_device("layer_norm", x, weight, bias, residual)
     for name, w in (("weight", weight), ("bias", bias)):
@@ -110,50 +76,27 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"layer_norm: a residual of {tuple(residual.shape)} {residual.dtype} for x of "
                          f"{tuple(x.shape)} {x.dtype}")
-    if _differentiable(x, weight, bias, residual):
-        y, z = _LayerNorm.apply(x, weight, bias, residual, eps)
-    else:
-        y, z, _, _, _ = _norm_forward(x, weight, bias, residual, eps)
+    y, z = (_lib.layers().layer_norm if x.is_cuda else _LayerNorm.apply)(x, weight, bias, residual, eps)
     return y if residual is None else (y, z)
 
 
-def _norm_forward(x, weight, bias, residual, eps):
-    """y, z (None without a residual), the rows that were normalised, and their statistics."""
-    x2 = _rows(x)
-    r2 = None if residual is None else _rows(residual)
-    rows, cols = x2.shape
-    if not x.is_cuda:
-        z2 = x2 if r2 is None else (_wide(x2) + _wide(r2)).to(x.dtype)
-        var, mean = torch.var_mean(_wide(z2), 1, unbiased=False)
+class _LayerNorm(torch.autograd.Function):
+    """On CPU tensors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        z = x if residual is None else (_wide(x) + _wide(residual)).to(x.dtype)
+        var, mean = torch.var_mean(_wide(z), -1, unbiased=False, keepdim=True)
         rstd = (var + eps).rsqrt()
-        y = (_wide(z2) - mean[:, None]) * rstd[:, None]
+        y = (_wide(z) - mean) * rstd
         if weight is not None:
             y = y * _wide(weight)
         if bias is not None:
             y = y + _wide(bias)
-        return (y.to(x.dtype).view(x.shape), None if r2 is None else z2.view(x.shape), z2, mean, rstd)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    z = None if r2 is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    w = weight if weight is not None else bias
-    _call("norm_forward", x.device, x2.data_ptr(), _p(r2), _p(_dense(weight)), _p(_dense(bias)), y.data_ptr(), _p(z),
-          stats.data_ptr(), stats.data_ptr() + 4 * rows, rows, cols, _pitch(x2), 0 if r2 is None else _pitch(r2),
-          TYPE[x.dtype], 0 if w is None else TYPE[w.dtype], float(eps))
-    return y, z, (x2 if z is None else z.view(rows, cols)), stats[0], stats[1]
-
-
-def _dense(w):
-    return w if w is None or w.is_contiguous() else w.contiguous()
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, eps):
-        y, z, rows, mean, rstd = _norm_forward(x, weight, bias, residual, eps)
-        ctx.save_for_backward(rows, weight, mean, rstd)
-        ctx.shape, ctx.bias, ctx.set_z = x.shape, None if bias is None else bias.dtype, z is not None
+        ctx.save_for_backward(z, weight, mean, rstd)
+        ctx.bias = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
-        return y, z
+        return y.to(x.dtype), None if residual is None else z
 
     @staticmethod
     @once_differentiable
@@ -162,31 +105,16 @@ class _LayerNorm(torch.autograd.Function):
         if dy is None and dz is None:
             return None, None, None, None, None
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        if dy is None:   # only the sum was used further on
-            zero = lambda need, w: torch.zeros(z.shape[1], dtype=w, device=z.device) if need else None  # noqa: E731
-            return (dz if need_x else None, zero(need_w, weight.dtype if need_w else None), zero(need_b, ctx.bias),
-                    dz if need_r else None, None)
-        dy2, dz2 = _rows(dy), None if dz is None else _rows(dz)
-        rows, cols = z.shape
-        if not z.is_cuda:
-            h, g = (_wide(z) - mean[:, None]) * rstd[:, None], _wide(dy2)
-            dw = (g * h).sum(0).to(weight.dtype) if need_w else None
-            db = g.sum(0).to(ctx.bias) if need_b else None
-            if weight is not None:
-                g = g * _wide(weight)
-            dx = rstd[:, None] * (g - g.mean(1, keepdim=True) - h * (g * h).mean(1, keepdim=True))
-            if dz2 is not None:
-                dx = dx + _wide(dz2)
-            dx = dx.to(z.dtype).view(ctx.shape)
-        else:
-            wtype = weight.dtype if weight is not None else ctx.bias
-            dx = torch.empty(ctx.shape, dtype=z.dtype, device=z.device) if need_x or need_r else None
-            dw = torch.empty(cols, dtype=wtype, device=z.device) if need_w else None
-            db = torch.empty(cols, dtype=wtype, device=z.device) if need_b else None
-            ws = _scratch(_lib.fast_cuda().norm_workspace(rows, cols) if need_w or need_b else 0, z.device)
-            _call("norm_backward", z.device, z.data_ptr(), dy2.data_ptr(), _p(dz2), _p(_dense(weight)), mean.data_ptr(),
-                  rstd.data_ptr(), _p(dx), _p(dw), _p(db), _p(ws), rows, cols, _pitch(z), _pitch(dy2),
-                  0 if dz2 is None else _pitch(dz2), TYPE[z.dtype], 0 if wtype is None else TYPE[wtype])
+        g = torch.zeros_like(mean).expand_as(z) if dy is None else _wide(dy)   # only the sum was used further on
+        h = (_wide(z) - mean) * rstd
+        dw = (g * h).reshape(-1, z.shape[-1]).sum(0).to(weight.dtype) if need_w else None
+        db = g.reshape(-1, z.shape[-1]).sum(0).to(ctx.bias) if need_b else None
+        if weight is not None:
+            g = g * _wide(weight)
+        dx = rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
+        if dz is not None:
+            dx = dx + _wide(dz)
+        dx = dx.to(z.dtype)
         return dx if need_x else None, dw, db, dx if need_r else None, None
 
 
@@ -214,26 +142,7 @@ def linear(x, weight, bias=None, *, activation: str | None = None, residual=None
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError(f"linear: a residual of {tuple(residual.shape)} {residual.dtype} for a result of "
                          f"{tuple(shape)} {x.dtype}")
-    if _differentiable(x, weight, bias, residual):
-        return _Linear.apply(x, weight, bias, residual, activation)
-    return _linear_forward(x, weight, bias, residual, activation, False)[0]
-
-
-def _operand(x, dtype):
-    """A matrix a kernel can fetch by tiles: of that type, rows on 16-byte boundaries."""
-    if x.dtype == dtype and x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (_pitch(x) % 8 == 0 or x.shape[0] == 1):
-        return x
-    rows, cols = x.shape
-    return torch.empty(rows, (cols + 7) // 8 * 8, dtype=dtype, device=x.device)[:, :cols].copy_(x)
-
-
-def _product(a, b, m, n, k, a_k, b_k, out_type, *, bias=None, residual=None, pre=None, act=0):
-    y = torch.empty(m, n, dtype=out_type, device=a.device)
-    ws = _scratch(_lib.fast_cuda().product_workspace(m, n, k), a.device)
-    _call("product", a.device, a.data_ptr(), b.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(pre), _p(ws),
-          m, n, k, _pitch(a), _pitch(b), n, 0 if residual is None else _pitch(residual), a_k, b_k,
-          TYPE[a.dtype], TYPE[out_type], 0 if bias is None else TYPE[bias.dtype], act)
-    return y
+    return (_lib.layers().linear if x.is_cuda else _Linear.apply)(x, weight, bias, residual, ACTIVATIONS[activation])
 
 
 def _act(p, kind):
@@ -256,73 +165,32 @@ def _act_slope(p, kind):
     return 0.5 * (1 + t) + 0.5 * p * (1 - t * t) * c * (1 + 3 * 0.044715 * p * p)
 
 
-def _linear_forward(x, weight, bias, residual, activation, keep):
-    """y and, with ``keep``, what the backward pass reads: x and the weight as the product
-    took them, and the product in front of the activation."""
-    act = ACTIVATIONS[activation]
-    x2 = _rows(x)
-    r2 = None if residual is None else _rows(residual)
-    m, k = x2.shape
-    n = weight.shape[0]
-    shape = x.shape[:-1] + (n,)
-    if not x.is_cuda:
-        w = weight if x.dtype == weight.dtype else weight.to(x.dtype)
-        p = _wide(x2) @ _wide(w).t()
+class _Linear(torch.autograd.Function):
+    """On CPU tensors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        w = weight.to(x.dtype)
+        p = _wide(x) @ _wide(w).t()
         if bias is not None:
             p = p + _wide(bias)
         y = _act(p, act)
-        if r2 is not None:
-            y = y + _wide(r2)
-        return y.to(x.dtype).view(shape), x2, w, (p.to(x.dtype) if act and keep else None)
-    a, w = _operand(x2, x.dtype), _operand(weight.detach(), x.dtype)
-    pre = torch.empty(m, n, dtype=x.dtype, device=x.device) if act and keep else None
-    y = _product(a, w, m, n, k, 1, 1, x.dtype, bias=_dense(bias), residual=r2, pre=pre, act=act)
-    return y.view(shape), a, w, pre
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        y, a, w, pre = _linear_forward(x, weight, bias, residual, activation, True)
-        ctx.save_for_backward(a, w, pre)
-        ctx.act, ctx.shape = ACTIVATIONS[activation], x.shape
-        ctx.types = weight.dtype, None if bias is None else bias.dtype
-        return y
+        if residual is not None:
+            y = y + _wide(residual)
+        ctx.save_for_backward(x, w, p.to(x.dtype) if act else None)
+        ctx.act, ctx.types = act, (weight.dtype, None if bias is None else bias.dtype)
+        return y.to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, w, pre = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        dy2 = _rows(dy)
-        (m, k), n, act = x.shape, w.shape[0], ctx.act
-        wtype, btype = ctx.types
-        dx = dw = db = None
-        if not x.is_cuda:
-            g = _wide(dy2) if pre is None else _wide(dy2) * _act_slope(_wide(pre), act)
-            if need_b:
-                db = g.sum(0).to(btype)
-            g = _wide(g.to(x.dtype))
-            if need_x:
-                dx = (g @ _wide(w)).to(x.dtype).view(ctx.shape)
-            if need_w:
-                dw = (g.t() @ _wide(x)).to(wtype)
-        else:
-            g = dy2
-            # rows that a tile copy cannot start at are laid out anew, as is what an activation changes
-            ragged = dy2.data_ptr() % 16 != 0 or (_pitch(dy2) % 8 != 0 and m > 1)
-            if act or ragged:
-                g = torch.empty(m, (n + 7) // 8 * 8, dtype=x.dtype, device=x.device)[:, :n]
-            if g is not dy2 or need_b:
-                if need_b:
-                    db = torch.empty(n, dtype=btype, device=x.device)
-                ws = _scratch(_lib.fast_cuda().slope_workspace(m, n) if need_b else 0, x.device)
-                _call("slope", x.device, dy2.data_ptr(), _p(pre), None if g is dy2 else g.data_ptr(), _p(db), _p(ws),
-                      m, n, _pitch(dy2), n, _pitch(g), TYPE[x.dtype], 0 if btype is None else TYPE[btype], act)
-            if need_x:
-                dx = _product(g, w, m, k, n, 1, 0, x.dtype).view(ctx.shape)
-            if need_w:
-                dw = _product(g, x, n, k, m, 0, 0, wtype)
+        g = _wide(dy) if pre is None else _wide(dy) * _act_slope(_wide(pre), ctx.act)
+        db = g.reshape(-1, g.shape[-1]).sum(0).to(ctx.types[1]) if need_b else None
+        g = _wide(g.to(x.dtype))
+        dx = (g @ _wide(w)).to(x.dtype) if need_x else None
+        dw = (g.reshape(-1, g.shape[-1]).t() @ _wide(x).reshape(-1, x.shape[-1])).to(ctx.types[0]) if need_w else None
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -342,10 +210,7 @@ def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: float | No
     computes the probabilities again, from that logarithm; there is no dropout."""
     q, k, v = _autocast(q), _autocast(k), _autocast(v)
     scale = _check_attention(q, k, v, key_mask, scale)
-    if _differentiable(q, k, v):
-        o, lse = _Attention.apply(q, k, v, key_mask, causal, scale)
-    else:
-        o, lse = _attention_forward(q, k, v, key_mask, causal, scale)
+    o, lse = (_lib.layers().attention if q.is_cuda else _Attention.apply)(q, k, v, key_mask, causal, scale)
     return (o, lse) if return_lse else o
 
 
@@ -355,11 +220,12 @@ def self_attention(qkv, *, causal: bool = False, key_mask=None, scale: float | N
     qkv = _autocast(qkv)
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError(f"self_attention: [batch, length, 3, heads, dim] is wanted, not {tuple(qkv.shape)}")
-    scale = _check_attention(*qkv.unbind(2), key_mask, scale)
-    if _differentiable(qkv):
-        o, lse = _SelfAttention.apply(qkv, key_mask, causal, scale)
+    q, k, v = qkv.unbind(2)
+    scale = _check_attention(q, k, v, key_mask, scale)
+    if qkv.is_cuda:
+        o, lse = _lib.layers().self_attention(qkv, key_mask, causal, scale)
     else:
-        o, lse = _attention_forward(*qkv.unbind(2), key_mask, causal, scale)
+        o, lse = _Attention.apply(q, k, v, key_mask, causal, scale)
     return (o, lse) if return_lse else o
 
 
@@ -389,26 +255,6 @@ def _check_attention(q, k, v, mask, scale):
     return scale
 
 
-def _tileable(x):
-    """``x`` itself where tiles of it can be fetched (the last axis dense, everything on 16-byte
-    boundaries), else a copy."""
-    if x.stride(3) == 1 and x.data_ptr() % 16 == 0 and not (x.stride(0) | x.stride(1) | x.stride(2)) % 8 and \
-            min(x.stride()) > 0:
-        return x
-    return x.contiguous() if not x.is_contiguous() else x.clone()
-
-
-def _strides(x):
-    return x.stride()[:3]
-
-
-_NO_STRIDES = (0, 0, 0)
-
-
-def _mask(mask):
-    return mask if mask is None or mask.stride(1) == 1 else mask.contiguous()
-
-
 def _hidden(q, k, mask, causal):
     sq, sk = q.shape[1], k.shape[1]
     seen = torch.ones(sq, sk, dtype=torch.bool, device=q.device)
@@ -426,49 +272,17 @@ def _cpu_heads(q, k, v, mask):
     return (_wide(q).transpose(1, 2), *(_wide(x).transpose(1, 2).repeat_interleave(group, 1) for x in (k, v)))
 
 
-def _attention_forward(q, k, v, mask, causal, scale):
-    (b, sq, h, d), sk = q.shape, k.shape[1]
-    if not q.is_cuda:
+class _Attention(torch.autograd.Function):
+    """On CPU tensors."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, causal, scale):
+        (b, sq, h, _), sk = q.shape, k.shape[1]
         qh, kh, vh = _cpu_heads(q, k, v, mask)
         s = (qh @ kh.transpose(2, 3) * scale).masked_fill(~_hidden(q, k, mask, causal), -math.inf)
         lse = torch.logsumexp(s, -1) if sk else s.new_full((b, h, sq), -math.inf)
         p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
-        return (p @ vh).transpose(1, 2).to(q.dtype).contiguous(), lse
-    o = torch.empty(b, sq, h, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(b, h, sq, dtype=torch.float32, device=q.device)
-    q, k, v, mask = _tileable(q), _tileable(k), _tileable(v), _mask(mask)
-    _call("attention_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(mask),
-          None, None, None, None, None, b, sq, sk, h, k.shape[2], d, *_strides(q), *_strides(k), *_strides(v),
-          *_strides(o), *_NO_STRIDES, *_NO_STRIDES, *_NO_STRIDES, *_NO_STRIDES, 0 if mask is None else mask.stride(0),
-          TYPE[q.dtype], 1 if causal else 0, scale)
-    return o, lse
-
-
-def _attention_backward(q, k, v, o, lse, do, mask, causal, scale, dq, dk, dv):
-    (b, sq, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
-    if not q.is_cuda:
-        qh, kh, vh = _cpu_heads(q, k, v, mask)
-        g, oh = _wide(do).transpose(1, 2), _wide(o).transpose(1, 2)
-        s = (qh @ kh.transpose(2, 3) * scale).masked_fill(~_hidden(q, k, mask, causal), -math.inf)
-        p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
-        ds = p * (g @ vh.transpose(2, 3) - (g * oh).sum(-1, keepdim=True)) * scale
-        group = lambda x: x.view(b, hk, h // hk, sk, d).sum(2).transpose(1, 2)  # noqa: E731
-        dq.copy_((ds @ kh).transpose(1, 2))
-        dk.copy_(group(ds.transpose(2, 3) @ qh))
-        dv.copy_(group(p.transpose(2, 3) @ g))
-        return
-    q, k, v, do, mask = _tileable(q), _tileable(k), _tileable(v), _tileable(do), _mask(mask)
-    delta = torch.empty(b, h, 2, (sq + 127) // 128 * 128, dtype=torch.float32, device=q.device)
-    _call("attention_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), _p(mask),
-          do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), b, sq, sk, h, hk, d,
-          *_strides(q), *_strides(k), *_strides(v), *_strides(o), *_strides(do), *_strides(dq), *_strides(dk),
-          *_strides(dv), 0 if mask is None else mask.stride(0), TYPE[q.dtype], 1 if causal else 0, scale)
-
-
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, mask, causal, scale):
-        o, lse = _attention_forward(q, k, v, mask, causal, scale)
+        o = (p @ vh).transpose(1, 2).to(q.dtype).contiguous()
         ctx.save_for_backward(q, k, v, o, lse, mask)
         ctx.causal, ctx.scale = causal, scale
         ctx.mark_non_differentiable(lse)
@@ -481,28 +295,13 @@ class _Attention(torch.autograd.Function):
         if do is None:
             return (None,) * 6
         q, k, v, o, lse, mask = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        _attention_backward(q, k, v, o, lse, do, mask, ctx.causal, ctx.scale, dq, dk, dv)
+        (b, _, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
+        qh, kh, vh = _cpu_heads(q, k, v, mask)
+        g, oh = _wide(do).transpose(1, 2), _wide(o).transpose(1, 2)
+        s = (qh @ kh.transpose(2, 3) * ctx.scale).masked_fill(~_hidden(q, k, mask, ctx.causal), -math.inf)
+        p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
+        ds = p * (g @ vh.transpose(2, 3) - (g * oh).sum(-1, keepdim=True)) * ctx.scale
+        group = lambda x: x.view(b, hk, h // hk, sk, d).sum(2)  # noqa: E731
+        out = ds @ kh, group(ds.transpose(2, 3) @ qh), group(p.transpose(2, 3) @ g)
         need = ctx.needs_input_grad
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
-
-
-class _SelfAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, mask, causal, scale):
-        o, lse = _attention_forward(*qkv.unbind(2), mask, causal, scale)
-        ctx.save_for_backward(qkv, o, lse, mask)
-        ctx.causal, ctx.scale = causal, scale
-        ctx.mark_non_differentiable(lse)
-        ctx.set_materialize_grads(False)
-        return o, lse
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, do, _):
-        if do is None:
-            return (None,) * 4
-        qkv, o, lse, mask = ctx.saved_tensors
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _attention_backward(*qkv.unbind(2), o, lse, do, mask, ctx.causal, ctx.scale, *dqkv.unbind(2))
-        return dqkv, None, None, None
+        return (*(x.transpose(1, 2).to(q.dtype) if n else None for x, n in zip(out, need)), None, None, None)
