@@ -13,6 +13,35 @@ __device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r *
 // 2^x for the softmax is exp2_fast(); what a masked score becomes
 constexpr float kNone = -INFINITY;
 
+// Two values at a time: half the instructions for what is not 2^x.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t bits(F2 v) {
+  return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
+}
+__device__ __forceinline__ F2 f2(uint64_t v) { return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))}; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return f2(d);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return f2(d);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return f2(d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 struct Yes {
   __device__ constexpr operator bool() const { return true; }
 };
@@ -289,8 +318,6 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
         whole = false;
       }
       if (!guard_wait(&bar.s_full[t], j & 1, g, 0x30003)) { ok = false; break; }
-      // the product before these scores is done too; every phase is waited for, so that none is mistaken
-      if (j > 0 && !guard_wait(&bar.o_full[t], (j - 1) & 1, g, 0x30004)) { ok = false; break; }
       tmem_fence_after();
       // a row of scores stays in registers where those suffice, else it is read twice, in steps
       constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : kB;
@@ -317,9 +344,11 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int i = 0; i < kStep; ++i) {
-            const float v = __uint_as_float(x[(c + i) % kHeld]);
-            part[i & 3] = fmaxf(part[i & 3], all || (seen.w[c / 32] >> (c % 32 + i) & 1) ? v : kNone);
+          for (int i = 0; i < kStep; i += 2) {
+            const float v = __uint_as_float(x[(c + i) % kHeld]), w = __uint_as_float(x[(c + i + 1) % kHeld]);
+            const uint32_t two = all ? 3 : seen.w[c / 32] >> (c % 32 + i) & 3;
+            float& top = part[i / 2 & 3];
+            top = max3(top, all || (two & 1) ? v : kNone, all || (two & 2) ? w : kNone);
           }
         }
       };
@@ -327,11 +356,22 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       else highest(No());
       float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
       top = top == kNone ? kNone : top * l.c;   // 0 times infinity otherwise
+      // the product of the last tile's probabilities: awaited before its results are scaled or its
+      // probabilities replaced, and once a tile, so that no phase of the barrier is mistaken
+      bool behind = j > 0;
+      auto settle = [&] {
+        if (!behind) return true;
+        behind = false;
+        const bool done = guard_wait(&bar.o_full[t], (j - 1) & 1, g, 0x30004);
+        tmem_fence_after();
+        return done;
+      };
       if (__any_sync(0xffffffffu, top > m + 8.f || (m == kNone && top != kNone))) {
         const float now = fmaxf(m, top), keep = now == kNone ? 1.f : exp2_fast(m - now);
         sum *= keep;
         m = now;
         if (j > 0) {
+          if (!settle()) { ok = false; break; }
 #pragma unroll
           for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
@@ -345,34 +385,38 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
         }
       }
       const float base = m == kNone ? 0.f : -m;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) part[k] = 0.f;
+      F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
+      uint32_t y[SHORT ? kStep / 2 : kB / 2];   // packed; all of a row before the first is stored, where registers allow
       auto probabilities = [&](auto all) {
 #pragma unroll
         for (int c = 0; c < kB; c += kStep) {
-          uint32_t y[kStep / 2];
+          uint32_t* to_y = SHORT ? y : y + c / 2;
           if (kHeld != kB) {
             read(c, x);
             tmem_wait_ld();
           }
 #pragma unroll
           for (int i = 0; i < kStep; i += 2) {
-            float e[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              e[k] = exp2_fast(fmaf(__uint_as_float(x[(c + i + k) % kHeld]), l.c, base));
-              if (!all) e[k] = seen.w[c / 32] >> (c % 32 + i + k) & 1 ? e[k] : 0.f;
-              part[(i + k) & 3] += e[k];
+            const F2 z = fma2({__uint_as_float(x[(c + i) % kHeld]), __uint_as_float(x[(c + i + 1) % kHeld])}, {l.c, l.c}, {base, base});
+            F2 e = {exp2_fast(z.x), exp2_fast(z.y)};
+            if (!all) {
+              const uint32_t two = seen.w[c / 32] >> (c % 32 + i);
+              e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
             }
-            y[i / 2] = pack2<T>(e[0], e[1]);
+            sums[i / 2 & 1] = add2(sums[i / 2 & 1], e);
+            to_y[i / 2] = pack2<T>(e.x, e.y);
           }
-          if constexpr (SHORT) tmem_st8(tp + c / 2, y);
-          else tmem_st16(tp + c / 2, y);
+          if constexpr (SHORT) tmem_st8(tp + c / 2, *(const uint32_t(*)[8])y);
         }
       };
       if (whole) probabilities(Yes());
       else probabilities(No());
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+      if (!settle()) { ok = false; break; }
+      if constexpr (!SHORT) {
+#pragma unroll
+        for (int c = 0; c < kB; c += 32) tmem_st16(tp + c / 2, *(const uint32_t(*)[16])(y + c / 2));
+      }
       tmem_wait_st();
       tmem_fence_before();
       mbar_arrive(&bar.p_full[t]);
@@ -428,9 +472,9 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
 constexpr int kMaxDim = 128;
 
 // --------------------------------------------------------------------- backward
-// Rows of d_o against rows of o (delta), and the logarithm of the softmax sums to base 2; both
-// in tiles of 128 rows, [batch, heads, rows rounded up].  Behind the last row, and where a row
-// saw nothing: infinity, so that every probability comes out as zero.
+// The logarithm of the softmax sums to base 2, and rows of d_o against rows of o (delta); both
+// negative, in tiles of 128 rows, [batch, heads, 2, rows rounded up].  Behind the last row, and
+// where a row saw nothing: minus infinity, so that every probability comes out as zero.
 __host__ __device__ __forceinline__ int64_t padded(int64_t rows) { return (rows + kB - 1) / kB * kB; }
 
 template <typename T, int LANES>   // that share a row, 16 bytes each
@@ -454,8 +498,8 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
   for (int k = LANES / 2; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0) {
     float* out = a.delta + (b * a.heads + h) * 2 * rows + i;
-    out[0] = lse == -INFINITY ? INFINITY : lse;
-    out[rows] = s;
+    out[0] = lse == -INFINITY ? -INFINITY : -lse;
+    out[rows] = -s;
   }
 }
 
@@ -648,7 +692,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     more_registers<F::kMany>();
     const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane, row = r0 + r;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-    float lse = INFINITY, delta = 0.f;   // of a query that stays
+    float lse = -INFINITY, delta = 0.f;   // of a query that stays, negative
     bool mine = true;                    // a key that stays is seen at all
     if (keys) {
       mine = row < sk && (!masked || mask[row]);
@@ -716,23 +760,28 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         for (int c = 0; c < 64; c += 32) {
           const uint32_t at = tmem + lanes + 64 * half + c;
           const uint32_t(&x)[32] = xs[c / 32], (&y)[32] = ys[c / 32];
-          const uint32_t bits = all ? 0xffffffffu : seen.w[2 * half + c / 32];
+          const uint32_t mine_of = all ? 0xffffffffu : seen.w[2 * half + c / 32];
           uint32_t e[16], d[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta}, pr[4], ds[4];
+            float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta};   // negative both
             if (of_keys) {
               *(float4*)ls = *(const float4*)(cols + c + i);
               *(float4*)de = *(const float4*)(cols + kB + c + i);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              pr[k] = exp2_fast(fmaf(__uint_as_float(x[i + k]), l.c, -ls[k]));
-              ds[k] = pr[k] * (__uint_as_float(y[i + k]) - de[k]);
-              if (!all && !(bits >> (i + k) & 1)) pr[k] = ds[k] = 0.f;
+            for (int k = 0; k < 4; k += 2) {
+              const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {ls[k], ls[k + 1]});
+              F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
+              F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {de[k], de[k + 1]}));
+              if (!all) {
+                const uint32_t two = mine_of >> (i + k);
+                if (!(two & 1)) pr.x = ds.x = 0.f;
+                if (!(two & 2)) pr.y = ds.y = 0.f;
+              }
+              if (of_keys) e[(i + k) / 2] = pack2<T>(pr.x, pr.y);
+              d[(i + k) / 2] = pack2<T>(ds.x, ds.y);
             }
-            if (of_keys) e[i / 2] = pack2<T>(pr[0], pr[1]), e[i / 2 + 1] = pack2<T>(pr[2], pr[3]);
-            d[i / 2] = pack2<T>(ds[0], ds[1]), d[i / 2 + 1] = pack2<T>(ds[2], ds[3]);
           }
           if (of_keys) tmem_st16(at + F::kS * q, e);
           tmem_st16(at + F::kS * q + 16, d);
@@ -831,6 +880,10 @@ int forward_tiles(const Launch& l, cudaStream_t s) {
   static const cudaError_t allowed =
       cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (allowed != cudaSuccess) return allowed;
+  static const cudaError_t shared =   // or the CTAs meant to share an SM find no room
+      cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT, SHORT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                           cudaSharedmemCarveoutMaxShared);
+  if (shared != cudaSuccess) return shared;
   const dim3 grid((unsigned)((l.p.sq + kB * QT - 1) / (kB * QT)), (unsigned)l.p.heads, (unsigned)l.p.batch);
   attention_forward_tiles<T, DP, QT, SHORT><<<grid, F::kThreads, F::kSmem, s>>>(l);
   return cudaGetLastError();

@@ -124,24 +124,24 @@ __device__ __forceinline__ void tma_store_wait_read() {
 }
 
 // ------------------------------------------------------------- tensor memory
+// By one whole warp.  The right to allocate is given up at once: while a CTA holds it, no other
+// one is started on the SM.
 template <int CG>
-__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {   // one whole warp
-  if (CG == 1)
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {
+  if (CG == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(cols)
                  : "memory");
-  else
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(cols)
                  : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
 }
 template <int CG>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {   // the same warp
-  if (CG == 1) {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
-  } else {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
-  }
+  if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
