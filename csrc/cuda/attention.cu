@@ -6,6 +6,7 @@ namespace hipress {
 namespace {
 
 constexpr int kB = 128;                 // queries and keys of a tile
+constexpr int kMaxDim = 128;
 constexpr uint32_t kPanel = kB * 128;   // bytes of 64 columns of a tile
 
 __device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r * 128 + (b ^ ((r & 7) << 4))); }
@@ -42,6 +43,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// 2^x by the multipliers, for a part of the values: 2^x proper is 16 a cycle and SM, and by itself
+// takes longer than all the rest.  x = n + f with |f| <= 1/2; 2^f by the polynomial of the fourth
+// degree whose greatest relative error there is least, 2.6e-6 (a Remez-like fit; 16-bit
+// probabilities are rounded by 2^-9 or 2^-12); n goes into the exponent.  Below 2^-126 it stays there.
+__device__ __forceinline__ float at_least(float x, float low) {   // NaN stays
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(low));
+  return d;
+}
+__device__ __forceinline__ F2 exp2_multiplied(F2 x) {
+  x = {at_least(x.x, -126.f), at_least(x.y, -126.f)};
+  constexpr float kRound = 12582912.f;   // 1.5 2^23: added, the integer is in the lowest bits
+  const F2 r = add2(x, {kRound, kRound}), f = fma2(add2(r, {-kRound, -kRound}), {-1.f, -1.f}, x);
+  F2 p = fma2(f, {0.00957003638f, 0.00957003638f}, {0.0559177165f, 0.0559177165f});
+  p = fma2(f, p, {0.24024745f, 0.24024745f});
+  p = fma2(f, p, {0.693121833f, 0.693121833f});
+  p = fma2(f, p, {0.999999262f, 0.999999262f});
+  return {__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
+          __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23))};
+}
+
+constexpr int kMultiplied = 3;   // of eight pairs
+
 struct Yes {
   __device__ constexpr operator bool() const { return true; }
 };
@@ -49,15 +73,29 @@ struct No {
   __device__ constexpr operator bool() const { return false; }
 };
 
-// Which of a tile's 128 columns a row may see, a bit each.
+// Which of a tile's columns a row may see, a bit each.
+template <int COLS>
 struct Seen {
-  uint32_t w[4];
+  uint32_t w[COLS / 32];
+  __device__ __forceinline__ bool all() const {
+    uint32_t a = w[0];
+#pragma unroll
+    for (int i = 1; i < COLS / 32; ++i) a &= w[i];
+    return a == 0xffffffffu;
+  }
+  __device__ __forceinline__ bool none() const {
+    uint32_t a = w[0];
+#pragma unroll
+    for (int i = 1; i < COLS / 32; ++i) a |= w[i];
+    return a == 0;
+  }
 };
 // columns lo .. hi-1 of the tile
-__device__ __forceinline__ Seen seen_between(int lo, int hi) {
-  Seen s;
+template <int COLS>
+__device__ __forceinline__ Seen<COLS> seen_between(int lo, int hi) {
+  Seen<COLS> s;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < COLS / 32; ++i) {
     const int a = min(max(lo - 32 * i, 0), 32), b = min(max(hi - 32 * i, 0), 32);
     const uint32_t below_b = b == 32 ? 0xffffffffu : (1u << b) - 1, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1;
     s.w[i] = below_b & ~below_a;
@@ -65,12 +103,13 @@ __device__ __forceinline__ Seen seen_between(int lo, int hi) {
   return s;
 }
 
-// By a whole warp: the mask's bits of keys k0 .. k0+127 of one sequence, all in every lane.
-__device__ __forceinline__ Seen mask_bits(const uint8_t* mask, int64_t k0, int64_t sk) {
-  Seen s;
+// By a whole warp: the mask's bits of keys from k0 on of one sequence, all in every lane.
+template <int COLS>
+__device__ __forceinline__ Seen<COLS> mask_bits(const uint8_t* mask, int64_t k0, int64_t sk) {
+  Seen<COLS> s;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < COLS / 32; ++i) {
     const int64_t k = k0 + 32 * i + lane;
     s.w[i] = __ballot_sync(0xffffffffu, k < sk && mask[k]);
   }
@@ -103,69 +142,77 @@ struct Launch {
 };
 
 // ---------------------------------------------------------------------- forward
-// A CTA has QT tiles of 128 queries of one head and walks over the keys, 128 at a time: scores
+// A CTA has QT tiles of 128 queries of one head and walks over the keys, KB at a time: scores
 // S = q k^T into tensor memory, one thread a row for the softmax, probabilities back over the
-// scores, O += P v.  While one tile's rows are at work the other's products run.  The sums keep a
+// scores, O += P v.  While some tiles' rows are at work the others' products run.  The sums keep a
 // running maximum; the results so far are scaled anew only when it rises by more than 2^8 (the
 // factor that 32-bit sums and 16-bit probabilities bear easily).  Bound: 2^x, 16 a cycle and SM.
-// SHORT is for up to 128 queries and keys: one tile each, nothing to walk over.  Its results take
-// the half of the scores' columns that the probabilities leave, so that four CTAs fit an SM and
-// hide one another's latency.
-template <int DP, int QT, bool SHORT>
+//   <64, 4, 64>    up to 64 dimensions, long: what one row does between its 2^x (fetch, maximum,
+//                  store, wait) takes as long as they do; four tiles in flight hide it, two of
+//                  128 keys did everything at the same time
+//   <64, 2, 128>, <128, 2, 128>, <., 1, 128>   fewer queries, or wider heads, whose results fill
+//                  tensor memory
+//   SHORT          up to 128 queries and keys: one tile each, nothing to walk over.  Results take the
+//                  half of the scores' columns that the probabilities leave, so that four CTAs fit
+//                  an SM and hide one another's latency
+template <int DP, int QT, int KB, bool SHORT>
 struct Forward {
-  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = SHORT ? 1 : DP == 64 && QT == 2 ? 4 : 2;
+  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kKeys = kPanels * KB * 128;   // bytes
+  static constexpr int kStages = SHORT ? 1 : KB == 64 ? 6 : DP == 64 && QT == 2 ? 4 : 2;
   // four warps that fetch and issue, four for each tile's rows; the former give registers to the latter
   static constexpr int kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
-  static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : 168, kFew = SHORT ? 64 : 72, kMany = SHORT ? 64 : QT == 1 ? 184 : 216;
+  static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : QT == 2 ? 168 : 96;
+  static constexpr int kFew = SHORT ? 64 : QT == 4 ? 56 : 72, kMany = SHORT ? 64 : QT == 1 ? 184 : QT == 2 ? 216 : 104;
   static_assert(kFew + QT * kMany <= (1 + QT) * kAtStart, "more registers than the CTA has");
-  static constexpr int kSmem = QT * kTile + kStages * 2 * kTile + 1024 + 1024;
-  static constexpr int kTmem = SHORT ? 128 : QT == 2 ? 512 : 256;
-  // columns: scores of each tile, results, probabilities.  With 64 dimensions these have columns of
+  static constexpr int kSmem = QT * kTile + kStages * 2 * kKeys + 1024 + 1024;
+  static constexpr int kTmem = SHORT ? 128 : QT == 1 ? 256 : 512;
+  // columns: scores of each tile, results, probabilities.  Where there is room these have columns of
   // their own, and the next scores need not wait for the product that reads them
-  static constexpr bool kApart = !SHORT && DP == 64;
-  static constexpr uint32_t kO = SHORT ? 64 : QT * 128, kP = kApart ? QT * (128 + 64) : 0, kPStep = kApart ? 64 : 128;
+  static constexpr bool kApart = !SHORT && DP == 64 && KB == 128;
+  static constexpr uint32_t kO = SHORT ? 64 : QT * KB, kP = kApart ? QT * (KB + DP) : 0, kPStep = kApart ? KB / 2 : KB;
 };
+template <int KB>
 struct ForwardBars {
-  uint64_t q_full, k_full[4], v_full[4], k_empty[4], v_empty[4], mask_full[4], s_full[2], s_free[2], p_full[2], o_full[2], drain;
-  Seen seen[4];
+  uint64_t q_full, k_full[6], v_full[6], k_empty[6], v_empty[6], mask_full[6], s_full[4], s_free[4], p_full[4], o_full[4], drain;
+  Seen<KB> seen[6];
   uint32_t tmem;
   int keys;
   Guard guard;
 };
 
-template <typename T, int DP, int QT, bool SHORT>
-__global__ void __launch_bounds__(128 + 128 * QT, (Forward<DP, QT, SHORT>::kPerSm))
+template <typename T, int DP, int QT, int KB, bool SHORT>
+__global__ void __launch_bounds__((Forward<DP, QT, KB, SHORT>::kThreads), (Forward<DP, QT, KB, SHORT>::kPerSm))
 attention_forward_tiles(const __grid_constant__ Launch l) {
-  using F = Forward<DP, QT, SHORT>;
+  using F = Forward<DP, QT, KB, SHORT>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = smem;
   uint8_t* skv = smem + QT * F::kTile;   // stages of k and v
-  ForwardBars& bar = *(ForwardBars*)(skv + F::kStages * 2 * F::kTile);
+  ForwardBars<KB>& bar = *(ForwardBars<KB>*)(skv + F::kStages * 2 * F::kKeys);
   const HpAttention& p = l.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the tiles with the most keys first, where the mask is causal
   const int qt = (int)gridDim.x - 1 - (int)blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(p.heads / p.kv_heads);
   const int q0 = qt * kB * QT, shift = (int)(p.sk - p.sq);
   const bool masked = p.key_mask != nullptr;
   const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
-  const int sk = !SHORT && masked && p.sk > kB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
-  // key tiles of each query tile
+  const int sk = !SHORT && masked && p.sk > KB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
+  // key tiles of a query tile: up to the last that its last query sees
+  auto tiles_of = [&](int t) {
+    const int first = q0 + t * kB, last = min(first + kB, (int)p.sq) - 1;
+    const int keys = first >= p.sq ? 0 : p.causal ? min(sk, max(0, last + shift + 1)) : sk;
+    return (keys + KB - 1) / KB;
+  };
   int n[QT], most = 0;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int last = min(q0 + (t + 1) * kB, (int)p.sq) - 1;   // its last query
-    const int keys = q0 + t * kB >= p.sq ? 0 : p.causal ? min(sk, max(0, last + shift + 1)) : sk;
-    n[t] = (keys + kB - 1) / kB;
-    most = max(most, n[t]);
-  }
+  for (int t = 0; t < QT; ++t) n[t] = tiles_of(t), most = max(most, n[t]);
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < F::kStages; ++i) {
       mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.k_empty[i], 1), mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.mask_full[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < QT; ++i) {
       mbar_init(&bar.s_full[i], 1), mbar_init(&bar.s_free[i], 128);
       mbar_init(&bar.p_full[i], 128), mbar_init(&bar.o_full[i], 1);
     }
@@ -178,158 +225,163 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = bar.tmem, tmem_o = tmem + F::kO;
+  const uint32_t tmem = uniform(bar.tmem), tmem_o = tmem + F::kO;
   Guard& g = bar.guard;
 
   if (warp < 4) {
-  if (F::kFew < F::kMany) fewer_registers<F::kFew>();
-  if (warp == 0) {
-    // k and v of key tile j into stage j; the mask's bits beside them
-    int waits = 0;   // copies to wait for should the CTA give up
-    if (lane == 0 && most) {
-      tma_prefetch(&l.map.k);
-      tma_prefetch(&l.map.v);
-      mbar_expect_tx(&bar.q_full, QT * F::kTile);
-      for (int t = 0; t < QT; ++t)
-        for (int i = 0; i < F::kPanels; ++i)
-          tma_load_4d(sq + t * F::kTile + i * kPanel, &l.map.q, 64 * i, h, q0 + t * kB, b, &bar.q_full);
-    }
-    for (int j = 0; j < most; ++j) {
-      const int s = j % F::kStages;
-      const uint32_t ph = (j / F::kStages) & 1;
-      uint8_t* k = skv + s * 2 * F::kTile;
-      if (!guard_wait(&bar.k_empty[s], ph ^ 1, g, 0x10001)) break;
-      if (lane == 0) {
-        mbar_expect_tx(&bar.k_full[s], F::kTile);
-        for (int i = 0; i < F::kPanels; ++i) tma_load_4d(k + i * kPanel, &l.map.k, 64 * i, hk, j * kB, b, &bar.k_full[s]);
+    if (F::kFew < F::kMany) fewer_registers<F::kFew>();
+    if (warp == 0) {
+      // k and v of key tile j into stage j; the mask's bits beside them
+      int waits = 0;   // copies to wait for should the CTA give up
+      if (lane == 0 && most) {
+        tma_prefetch(&l.map.k);
+        tma_prefetch(&l.map.v);
+        mbar_expect_tx(&bar.q_full, QT * F::kTile);
+#pragma unroll 1
+        for (int i = 0; i < QT * F::kPanels; ++i)
+          tma_load_4d(sq + i * kPanel, &l.map.q, 64 * (i % F::kPanels), h, q0 + i / F::kPanels * kB, b, &bar.q_full);
       }
-      // whoever reads the bits gives probabilities before the product that frees v
-      if (!guard_wait(&bar.v_empty[s], ph ^ 1, g, 0x10003)) break;
-      if (masked) {
-        const Seen m = mask_bits(mask, (int64_t)j * kB, sk);
-        if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
-      }
-      if (lane == 0) {
-        mbar_expect_tx(&bar.v_full[s], F::kTile);
-        for (int i = 0; i < F::kPanels; ++i)
-          tma_load_4d(k + F::kTile + i * kPanel, &l.map.v, 64 * i, hk, j * kB, b, &bar.v_full[s]);
-      }
-      waits = j + 1;
-    }
-    __syncwarp();
-    if (g.gave_up && lane == 0 && most) {   // nothing may land once the CTA is gone
-      mbar_wait_bounded(&bar.q_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10004);
-      for (int j = max(0, waits - F::kStages); j < waits; ++j) {
-        mbar_wait_bounded(&bar.k_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10005);
-        mbar_wait_bounded(&bar.v_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10006);
-      }
-      if (waits < most)   // the k of a tile whose v was not fetched
-        mbar_wait_bounded(&bar.k_full[waits % F::kStages], (waits / F::kStages) & 1, kWaitNs / 64, g.status, HP_STATUS_TIMEOUT | 0x10007);
-    }
-  } else if (warp == 1) {
-    if (lane == 0 && most) {
-      const bool bf = p.type == HP_BF16;
-      const uint32_t id_s = mma_idesc(128, 128, bf, true, true) | (l.negative ? kNegateA : 0);
-      const uint32_t id_o = mma_idesc(128, DP, bf, true, false);
-      bool ok = guard_wait(&bar.q_full, 0, g, 0x20001);
-      auto scores = [&](int t, int j) {   // S_t = q_t k_j^T
-        const int s = j % F::kStages;
-        const uint64_t a = mma_desc(smem_u32(sq + t * F::kTile), 16, 1024), k = mma_desc(smem_u32(skv + s * 2 * F::kTile), 16, 1024);
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t at = ((i / 4) * kPanel + (i % 4) * 32) >> 4;
-          mma_ss<1>(tmem + t * 128, a + at, k + at, id_s, i > 0);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int j = 0; j < most; ++j) {
+        uint8_t* k = skv + s * 2 * F::kKeys;
+        if (!guard_wait(&bar.k_empty[s], ph ^ 1, g, 0x10001)) break;
+        if (lane == 0) {
+          mbar_expect_tx(&bar.k_full[s], F::kKeys);
+          for (int i = 0; i < F::kPanels; ++i) tma_load_4d(k + i * KB * 128, &l.map.k, 64 * i, hk, j * KB, b, &bar.k_full[s]);
         }
-        mma_commit<1>(&bar.s_full[t]);
-      };
-      auto results = [&](int t, int j) {   // O_t += P_t v_j
-        const uint64_t v = mma_desc(smem_u32(skv + (j % F::kStages) * 2 * F::kTile + F::kTile), kPanel, 1024);
+        // whoever reads the bits gives probabilities before the product that frees v
+        if (!guard_wait(&bar.v_empty[s], ph ^ 1, g, 0x10003)) break;
+        if (masked) {
+          const Seen<KB> m = mask_bits<KB>(mask, (int64_t)j * KB, sk);
+          if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
+        }
+        if (lane == 0) {
+          mbar_expect_tx(&bar.v_full[s], F::kKeys);
+          for (int i = 0; i < F::kPanels; ++i)
+            tma_load_4d(k + F::kKeys + i * KB * 128, &l.map.v, 64 * i, hk, j * KB, b, &bar.v_full[s]);
+        }
+        waits = j + 1;
+        if (++s == F::kStages) s = 0, ph ^= 1;
+      }
+      __syncwarp();
+      if (g.gave_up && lane == 0 && most) {   // nothing may land once the CTA is gone
+        mbar_wait_bounded(&bar.q_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10004);
+        for (int j = max(0, waits - F::kStages); j < waits; ++j) {
+          mbar_wait_bounded(&bar.k_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10005);
+          mbar_wait_bounded(&bar.v_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x10006);
+        }
+        if (waits < most)   // the k of a tile whose v was not fetched
+          mbar_wait_bounded(&bar.k_full[waits % F::kStages], (waits / F::kStages) & 1, kWaitNs / 64, g.status, HP_STATUS_TIMEOUT | 0x10007);
+      }
+    } else if (warp == 1) {
+      if (most) {
+        const uint32_t leader = elect_one();
+        const bool bf = p.type == HP_BF16;
+        const uint32_t id_s = mma_idesc(128, KB, bf, true, true) | (l.negative ? kNegateA : 0);
+        const uint32_t id_o = mma_idesc(128, DP, bf, true, false);
+        bool ok = warp_wait(&bar.q_full, 0, g, 0x20001);
+        auto scores = [&](int t, int s) {   // S_t = q_t k^T of the stage
+          const uint64_t a = mma_desc(smem_u32(sq + t * F::kTile), 16, 1024), k = mma_desc(smem_u32(skv + s * 2 * F::kKeys), 16, 1024);
 #pragma unroll
-        for (int i = 0; i < kB / 16; ++i)
-          mma_ts(tmem_o + t * DP, tmem + F::kP + t * F::kPStep + i * 8, v + i * 128, id_o, j > 0 || i > 0);
-        mma_commit<1>(&bar.o_full[t]);
-      };
-      for (int j = 0; j <= most && ok; ++j) {   // scores of tile j, results of tile j - 1
-        if (j < most) ok = guard_wait(&bar.k_full[j % F::kStages], (j / F::kStages) & 1, g, 0x20002);
-        if (F::kApart && ok) {   // scores as soon as the last ones have been read
+          for (int i = 0; i < DP / 16; ++i)
+            mma_ss<1>(leader, tmem + t * KB, a + ((i / 4) * kPanel + (i % 4) * 32) / 16, k + ((i / 4) * KB * 128 + (i % 4) * 32) / 16, id_s, i > 0);
+          mma_commit<1>(leader, &bar.s_full[t]);
+        };
+        auto results = [&](int t, int s, bool add) {   // O_t += P_t v
+          const uint64_t v = mma_desc(smem_u32(skv + s * 2 * F::kKeys + F::kKeys), KB * 128, 1024);
+#pragma unroll
+          for (int i = 0; i < KB / 16; ++i)
+            mma_ts(leader, tmem_o + t * DP, tmem + F::kP + t * F::kPStep + i * 8, v + i * 128, id_o, add || i > 0);
+          mma_commit<1>(leader, &bar.o_full[t]);
+        };
+        int s = 0, s_before = 0;
+        uint32_t ph = 0, ph_before = 0;
+        for (int j = 0; j <= most && ok; ++j) {   // scores of tile j, results of tile j - 1
+          if (j < most) ok = warp_wait(&bar.k_full[s], ph, g, 0x20002);
+          if (F::kApart && ok) {   // scores as soon as the last ones have been read
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              if (j >= n[t] || !ok) continue;
+              if (j > 0) ok = warp_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
+              tmem_fence_after();
+              if (ok) scores(t, s);
+            }
+            if (ok && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
+          }
+          if (j > 0 && ok) ok = warp_wait(&bar.v_full[s_before], ph_before, g, 0x20003);
+          tmem_fence_after();
 #pragma unroll
           for (int t = 0; t < QT; ++t) {
-            if (j >= n[t] || !ok) continue;
-            if (j > 0) ok = guard_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
-            tmem_fence_after();
-            if (ok) scores(t, j);
+            if (j > 0 && j - 1 < n[t] && ok) {
+              ok = warp_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
+              tmem_fence_after();
+              if (ok) results(t, s_before, j > 1);
+            }
+            if (!F::kApart && j < n[t] && ok) scores(t, s);   // over the probabilities just used
           }
-          if (ok && j < most) mma_commit<1>(&bar.k_empty[j % F::kStages]);
+          if (j > 0) mma_commit<1>(leader, &bar.v_empty[s_before]);
+          if (!F::kApart && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
+          s_before = s, ph_before = ph;
+          if (++s == F::kStages) s = 0, ph ^= 1;
         }
-        if (j > 0 && ok) ok = guard_wait(&bar.v_full[(j - 1) % F::kStages], ((j - 1) / F::kStages) & 1, g, 0x20003);
-        tmem_fence_after();
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          if (j > 0 && j - 1 < n[t] && ok) {
-            ok = guard_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
-            tmem_fence_after();
-            if (ok) results(t, j - 1);
-          }
-          if (!F::kApart && j < n[t] && ok) scores(t, j);   // over the probabilities just used
-        }
-        if (j > 0) mma_commit<1>(&bar.v_empty[(j - 1) % F::kStages]);
-        if (!F::kApart && j < most) mma_commit<1>(&bar.k_empty[j % F::kStages]);
+        mma_commit<1>(leader, &bar.drain);
       }
-      mma_commit<1>(&bar.drain);
     }
-  }
   } else {
     if (F::kFew < F::kMany) more_registers<F::kMany>();
     const int t = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane;   // one row to a thread
-    const int row = q0 + t * kB + r, nt = QT == 1 ? n[0] : (t ? n[QT - 1] : n[0]);
-    const uint32_t lanes = (uint32_t)(32 * quad) << 16, ts = tmem + t * 128 + lanes, to = tmem_o + t * DP + lanes;
+    const int row = q0 + t * kB + r, nt = tiles_of(t);
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16, ts = tmem + t * KB + lanes, to = tmem_o + t * DP + lanes;
     const uint32_t tp = tmem + F::kP + t * F::kPStep + lanes;
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;   // keys this row sees but for the mask
     float m = kNone, sum = 0.f;
     bool ok = true;
+    int s = 0;
+    uint32_t ph = 0;
     for (int j = 0; j < nt; ++j) {
-      const int s = j % F::kStages;
-      Seen seen;
-      bool whole = sees >= (j + 1) * kB;
+      Seen<KB> seen;
+      bool whole = sees >= (j + 1) * KB;
       if (masked) {
-        if (!guard_wait(&bar.mask_full[s], (j / F::kStages) & 1, g, 0x30001)) { ok = false; break; }
+        if (!guard_wait(&bar.mask_full[s], ph, g, 0x30001)) { ok = false; break; }
         seen = bar.seen[s];
-        const bool all = (seen.w[0] & seen.w[1] & seen.w[2] & seen.w[3]) == 0xffffffffu;
+        const bool all = seen.all();
         if (!all) {
           // no probability is left where a key is masked, but a product with what it holds would be
           // no number if that is none: its v counts as zero (rows behind the last key already do).
           // Each tile sees to it before it gives its probabilities.
-          if (!guard_wait(&bar.v_full[s], (j / F::kStages) & 1, g, 0x30002)) { ok = false; break; }
-          if (!(seen.w[quad] >> lane & 1)) {
-            uint4* v = (uint4*)(skv + s * 2 * F::kTile + F::kTile + r * 128);
+          if (!guard_wait(&bar.v_full[s], ph, g, 0x30002)) { ok = false; break; }
+          if (r < KB && !(seen.w[quad % (KB / 32)] >> lane & 1)) {
+            uint4* v = (uint4*)(skv + s * 2 * F::kKeys + F::kKeys + r * 128);
 #pragma unroll
             for (int i = 0; i < F::kPanels; ++i)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[i * (kPanel / 16) + k] = make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < 8; ++k) v[i * KB * 8 + k] = make_uint4(0, 0, 0, 0);
           }
           fence_async_shared();
         }
         whole = whole && all;
       }
       if (!__all_sync(0xffffffffu, whole)) {
-        const Seen mine = seen_between(0, sees - j * kB);
+        const Seen<KB> mine = seen_between<KB>(0, sees - j * KB);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) seen.w[i] = masked ? seen.w[i] & mine.w[i] : mine.w[i];
+        for (int i = 0; i < KB / 32; ++i) seen.w[i] = masked ? seen.w[i] & mine.w[i] : mine.w[i];
         whole = false;
       }
+      if (++s == F::kStages) s = 0, ph ^= 1;
       if (!guard_wait(&bar.s_full[t], j & 1, g, 0x30003)) { ok = false; break; }
       tmem_fence_after();
       // a row of scores stays in registers where those suffice, else it is read twice, in steps
-      constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : kB;
+      constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : KB;
       uint32_t x[kHeld];
       auto read = [&](int c, uint32_t* to) {
         if constexpr (SHORT) tmem_ld16(ts + c, *(uint32_t(*)[16])to);
         else tmem_ld32(ts + c, *(uint32_t(*)[32])to);
       };
       float part[4] = {kNone, kNone, kNone, kNone};
-      if (kHeld == kB) {
+      if (!SHORT) {
 #pragma unroll
-        for (int c = 0; c < kB; c += kStep) read(c, x + c % kHeld);
+        for (int c = 0; c < KB; c += kStep) read(c, x + c % kHeld);
         tmem_wait_ld();
         if (F::kApart) {
           tmem_fence_before();
@@ -338,8 +390,8 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       }
       auto highest = [&](auto all) {   // tiles that are seen whole test no bits
 #pragma unroll
-        for (int c = 0; c < kB; c += kStep) {
-          if (kHeld != kB) {
+        for (int c = 0; c < KB; c += kStep) {
+          if (SHORT) {
             read(c, x);
             tmem_wait_ld();
           }
@@ -354,10 +406,11 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       };
       if (whole) highest(Yes());
       else highest(No());
-      float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+      float top = max3(fmaxf(part[0], part[1]), part[2], part[3]);
       top = top == kNone ? kNone : top * l.c;   // 0 times infinity otherwise
       // the product of the last tile's probabilities: awaited before its results are scaled or its
-      // probabilities replaced, and once a tile, so that no phase of the barrier is mistaken
+      // probabilities replaced, and once a tile, so that no phase of the barrier is mistaken.  Where
+      // scores and probabilities share columns these scores have come after it.
       bool behind = j > 0;
       auto settle = [&] {
         if (!behind) return true;
@@ -372,33 +425,33 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
         m = now;
         if (j > 0) {
           if (!settle()) { ok = false; break; }
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + c, o);
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {   // rare, and the scores hold most registers
+            uint32_t o[16];
+            tmem_ld16(to + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-            tmem_st32(to + c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+            tmem_st16(to + c, o);
           }
           tmem_wait_st();
         }
       }
       const float base = m == kNone ? 0.f : -m;
       F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
-      uint32_t y[SHORT ? kStep / 2 : kB / 2];   // packed; all of a row before the first is stored, where registers allow
+      uint32_t y[SHORT ? kStep / 2 : KB / 2];   // packed; all of a row before the first is stored, where registers allow
       auto probabilities = [&](auto all) {
 #pragma unroll
-        for (int c = 0; c < kB; c += kStep) {
+        for (int c = 0; c < KB; c += kStep) {
           uint32_t* to_y = SHORT ? y : y + c / 2;
-          if (kHeld != kB) {
+          if (SHORT) {
             read(c, x);
             tmem_wait_ld();
           }
 #pragma unroll
           for (int i = 0; i < kStep; i += 2) {
             const F2 z = fma2({__uint_as_float(x[(c + i) % kHeld]), __uint_as_float(x[(c + i + 1) % kHeld])}, {l.c, l.c}, {base, base});
-            F2 e = {exp2_fast(z.x), exp2_fast(z.y)};
+            F2 e = all && KB == 64 && i / 2 % 8 < kMultiplied ? exp2_multiplied(z) : F2{exp2_fast(z.x), exp2_fast(z.y)};
             if (!all) {
               const uint32_t two = seen.w[c / 32] >> (c % 32 + i);
               e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
@@ -415,7 +468,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       if (!settle()) { ok = false; break; }
       if constexpr (!SHORT) {
 #pragma unroll
-        for (int c = 0; c < kB; c += 32) tmem_st16(tp + c / 2, *(const uint32_t(*)[16])(y + c / 2));
+        for (int c = 0; c < KB; c += 32) tmem_st16(tp + c / 2, *(const uint32_t(*)[16])(y + c / 2));
       }
       tmem_wait_st();
       tmem_fence_before();
@@ -429,10 +482,10 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     tmem_fence_after();
     // the rows leave through the space of their queries, which all products have read
     if (ok && q0 + t * kB < p.sq) {
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < F::kPanels; ++i) {
         uint8_t* to_smem = sq + t * F::kTile + i * kPanel + 32 * quad * 128;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 64; c += 32) {
           uint32_t o[32];
           if (nt) {
@@ -468,8 +521,6 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   tmem_fence_after();
   if (warp == 1) tmem_free<1>(tmem, F::kTmem);
 }
-
-constexpr int kMaxDim = 128;
 
 // --------------------------------------------------------------------- backward
 // The logarithm of the softmax sums to base 2, and rows of d_o against rows of o (delta); both
@@ -524,7 +575,7 @@ struct Backward {
 };
 struct BackwardBars {
   uint64_t stay_full, in_full[4], in_empty[4], mask_full[4], s_full[2], dp_full, dp_free, p_full, acc_full;
-  Seen seen[4];
+  Seen<kB> seen[4];
   uint32_t tmem;
   int keys;
   Guard guard;
@@ -540,7 +591,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   float* rows_of = (float*)(pass + F::kStages * 2 * F::kTile);   // a stage's lse and delta
   BackwardBars& bar = *(BackwardBars*)(rows_of + F::kStages * 2 * kB);
   const HpAttention& p = l.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int nq = (int)((p.sq + kB - 1) / kB), nk = (int)((p.sk + kB - 1) / kB), group = (int)(p.heads / p.kv_heads);
   const int sk = (int)p.sk, shift = (int)(p.sk - p.sq);
   // keys first: with shared heads they have more to do
@@ -562,8 +613,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     if (p.causal) first = max(0, r0 - shift) / kB;
     count = max(0, nq - first);
     if (masked) {
-      const Seen m = mask_bits(mask, r0, sk);
-      if (!(m.w[0] | m.w[1] | m.w[2] | m.w[3])) count = 0;
+      if (mask_bits<kB>(mask, r0, sk).none()) count = 0;
     }
   } else {
     int see = masked && sk > kB ? visible_keys(mask, sk, &bar.keys) : sk;
@@ -585,7 +635,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  const uint32_t tmem = bar.tmem;
+  const uint32_t tmem = uniform(bar.tmem);
   Guard& g = bar.guard;
 
   if (warp < 4) {
@@ -619,7 +669,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         }
       }
       if (!keys && masked) {
-        const Seen m = mask_bits(mask, (int64_t)j * kB, sk);
+        const Seen<kB> m = mask_bits<kB>(mask, (int64_t)j * kB, sk);
         if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
       }
       waits = j + 1;
@@ -631,7 +681,8 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         mbar_wait_bounded(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11003);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n) {
+    if (n) {
+      const uint32_t leader = elect_one();
       const bool bf = p.type == HP_BF16;
       const uint32_t id_s = mma_idesc(128, 128, bf, true, true) | (l.negative ? kNegateA : 0);
       const uint32_t id_dp = mma_idesc(128, 128, bf, true, true), id_acc = mma_idesc(128, DP, bf, true, false);
@@ -642,25 +693,25 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
           const uint32_t at = ((i / 4) * kPanel + (i % 4) * 32) >> 4;
-          mma_ss<1>(d, dx + at, dy + at, id, i > 0);
+          mma_ss<1>(leader, d, dx + at, dy + at, id, i > 0);
         }
       };
       auto deep = [&](uint32_t d, uint32_t x, uint32_t y, bool add) {      // P or dS, over the tile's columns
         const uint64_t dy = mma_desc(y, kPanel, 1024);
 #pragma unroll
-        for (int i = 0; i < kB / 16; ++i) mma_ts(d, x + (i / 2) * 32 + (i % 2) * 8, dy + i * 128, id_acc, add || i > 0);
+        for (int i = 0; i < kB / 16; ++i) mma_ts(leader, d, x + (i / 2) * 32 + (i % 2) * 8, dy + i * 128, id_acc, add || i > 0);
       };
       auto scores = [&](int j) {
         const int q = buffers == 2 ? j & 1 : 0;
         wide(tmem + F::kS * q, a, in(j), id_s);
-        mma_commit<1>(&bar.s_full[q]);
+        mma_commit<1>(leader, &bar.s_full[q]);
       };
       auto dprobs = [&](int j) {
         wide(tmem + F::kDP, a + F::kTile, in(j) + F::kTile, id_dp);
-        mma_commit<1>(&bar.dp_full);
+        mma_commit<1>(leader, &bar.dp_full);
       };
-      auto there = [&](int j) { return guard_wait(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, g, 0x21001); };
-      bool ok = guard_wait(&bar.stay_full, 0, g, 0x21002) && there(0);
+      auto there = [&](int j) { return warp_wait(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, g, 0x21001); };
+      bool ok = warp_wait(&bar.stay_full, 0, g, 0x21002) && there(0);
       if (ok) {
         tmem_fence_after();
         scores(0);
@@ -671,21 +722,21 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
           ok = there(j + 1);
           if (!ok) break;
           if (buffers == 2) scores(j + 1);
-          ok = guard_wait(&bar.dp_free, j & 1, g, 0x21004);
+          ok = warp_wait(&bar.dp_free, j & 1, g, 0x21004);
           if (!ok) break;
           tmem_fence_after();
           dprobs(j + 1);
         }
-        ok = guard_wait(&bar.p_full, j & 1, g, 0x21003);
+        ok = warp_wait(&bar.p_full, j & 1, g, 0x21003);
         if (!ok) break;
         tmem_fence_after();
         const uint32_t s = tmem + F::kS * (buffers == 2 ? j & 1 : 0);
         if (keys) deep(tmem + F::kAcc1, s, in(j) + F::kTile, j > 0);
         deep(tmem + F::kAcc2, s + 16, in(j), j > 0);
-        mma_commit<1>(&bar.in_empty[j % F::kStages]);
+        mma_commit<1>(leader, &bar.in_empty[j % F::kStages]);
         if (buffers == 1 && j + 1 < n) scores(j + 1);
       }
-      mma_commit<1>(&bar.acc_full);
+      mma_commit<1>(leader, &bar.acc_full);
     }
   }
   } else {
@@ -704,13 +755,13 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int s = j % F::kStages, q = buffers == 2 ? j & 1 : 0;
-      Seen seen;
+      Seen<kB> seen;
       bool whole;
       if (keys) {
         const int from = p.causal ? row - shift - (first + j % count) * kB : 0;   // its first query in this tile
         whole = mine && from <= 0;
         if (!__all_sync(0xffffffffu, whole)) {
-          seen = seen_between(mine ? from : kB, kB);
+          seen = seen_between<kB>(mine ? from : kB, kB);
           whole = false;
         }
       } else {
@@ -718,7 +769,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         if (masked) {
           if (!guard_wait(&bar.mask_full[s], (j / F::kStages) & 1, g, 0x31001)) { ok = false; break; }
           seen = bar.seen[s];
-          const bool all = (seen.w[0] & seen.w[1] & seen.w[2] & seen.w[3]) == 0xffffffffu;
+          const bool all = seen.all();
           if (!all) {   // what a masked key holds is left out of dq: its k counts as zero
             if (!guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31002)) { ok = false; break; }
             if (half == 0 && !(seen.w[quad] >> lane & 1)) {
@@ -733,7 +784,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
           whole = whole && all;
         }
         if (!__all_sync(0xffffffffu, whole)) {
-          const Seen up_to = seen_between(0, sees - j * kB);
+          const Seen<kB> up_to = seen_between<kB>(0, sees - j * kB);
 #pragma unroll
           for (int i = 0; i < 4; ++i) seen.w[i] = masked ? seen.w[i] & up_to.w[i] : up_to.w[i];
           whole = false;
@@ -874,18 +925,20 @@ int prepare(Launch& l, const HpAttention& a) {
   return rc;
 }
 
-template <typename T, int DP, int QT, bool SHORT = false>
-int forward_tiles(const Launch& l, cudaStream_t s) {
-  using F = Forward<DP, QT, SHORT>;
-  static const cudaError_t allowed =
-      cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+template <typename T, int DP, int QT, int KB = kB, bool SHORT = false>
+int forward_tiles(Launch& l, cudaStream_t s) {
+  using F = Forward<DP, QT, KB, SHORT>;
+  const auto kernel = attention_forward_tiles<T, DP, QT, KB, SHORT>;
+  static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (allowed != cudaSuccess) return allowed;
-  static const cudaError_t shared =   // or the CTAs meant to share an SM find no room
-      cudaFuncSetAttribute(attention_forward_tiles<T, DP, QT, SHORT>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                           cudaSharedmemCarveoutMaxShared);
-  if (shared != cudaSuccess) return shared;
-  const dim3 grid((unsigned)((l.p.sq + kB * QT - 1) / (kB * QT)), (unsigned)l.p.heads, (unsigned)l.p.batch);
-  attention_forward_tiles<T, DP, QT, SHORT><<<grid, F::kThreads, F::kSmem, s>>>(l);
+  const HpAttention& a = l.p;
+  if (!head_map(&l.map.q, a.q, a, a.sq, a.heads, a.q_b, a.q_s, a.q_h, kB) ||
+      !head_map(&l.map.k, a.sk ? a.k : a.q, a, a.sk, a.kv_heads, a.k_b, a.k_s, a.k_h, KB) ||
+      !head_map(&l.map.v, a.sk ? a.v : a.q, a, a.sk, a.kv_heads, a.v_b, a.v_s, a.v_h, KB) ||
+      !head_map(&l.map.o, a.o, a, a.sq, a.heads, a.o_b, a.o_s, a.o_h, 32))
+    return HP_ERR_BAD_ARG;
+  const dim3 grid((unsigned)((a.sq + kB * QT - 1) / (kB * QT)), (unsigned)a.heads, (unsigned)a.batch);
+  kernel<<<grid, F::kThreads, F::kSmem, s>>>(l);
   return cudaGetLastError();
 }
 
@@ -893,16 +946,12 @@ template <typename T>
 int forward(const HpAttention& a, cudaStream_t s) {
   Launch l;
   if (const int rc = prepare(l, a)) return rc;
-  if (!head_map(&l.map.q, a.q, a, a.sq, a.heads, a.q_b, a.q_s, a.q_h, kB) ||
-      !head_map(&l.map.k, a.sk ? a.k : a.q, a, a.sk, a.kv_heads, a.k_b, a.k_s, a.k_h, kB) ||
-      !head_map(&l.map.v, a.sk ? a.v : a.q, a, a.sk, a.kv_heads, a.v_b, a.v_s, a.v_h, kB) ||
-      !head_map(&l.map.o, a.o, a, a.sq, a.heads, a.o_b, a.o_s, a.o_h, 32))
-    return HP_ERR_BAD_ARG;
   const bool two = a.sq > kB;
-  if (a.dim <= 64 && !two && a.sk <= kB) return forward_tiles<T, 64, 1, true>(l, s);
-  if (a.dim <= 64) return two ? forward_tiles<T, 64, 2>(l, s) : forward_tiles<T, 64, 1>(l, s);
-  return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
+  if (a.dim > 64) return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
+  if (!two) return a.sk <= kB ? forward_tiles<T, 64, 1, kB, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
+  return a.sq > 2 * kB ? forward_tiles<T, 64, 4, 64>(l, s) : forward_tiles<T, 64, 2>(l, s);
 }
+
 template <typename T, int DP>
 int backward_tiles(const Launch& l, cudaStream_t s) {
   using F = Backward<DP>;

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
   uint8_t* staging = smem + S::kStages * S::kStage;
   float* biases = (float*)(staging + S::kEpiWarps * 2 * kStaging);   // [kEpiWarps][kCols]
   Bars& bar = *(Bars*)(biases + S::kEpiWarps * S::kCols);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const HpProduct& p = l.p;
 
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
   __syncthreads();
   if (CG == 2) cluster_sync();   // the other CTA's barriers are there
   tmem_fence_after();
-  const uint32_t tmem = bar.tmem;
+  const uint32_t tmem = uniform(bar.tmem);
   Guard& g = bar.guard;
   const int units = l.tiles_m * l.tiles_n * l.splits, step = gridDim.x / CG, first = blockIdx.x / CG;
 
@@ -236,35 +236,36 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
       }
     }
   } else if (warp == 1) {
-    if (rank == 0 && elect_one()) {
+    if (rank == 0) {
+      const uint32_t leader = elect_one();
       const uint32_t idesc = mma_idesc(128 * CG, BN, p.type == HP_BF16, p.a_kmajor, p.b_kmajor);
       const uint32_t lead_a = p.a_kmajor ? 16 : 8192, lead_b = p.b_kmajor ? 16 : 8192;
-      const uint32_t step_a = p.a_kmajor ? 32 : 2048, step_b = p.b_kmajor ? 32 : 2048;
+      const uint32_t step_a = p.a_kmajor ? 2 : 128, step_b = p.b_kmajor ? 2 : 128;   // 16 k further on, 16 bytes to a unit
       int s = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int u = first; u < units && ok; u += step, ++it) {
         const Unit w = unit_of(l, u, 128 * CG, BN);
         const int acc = it & 1;
-        if (!guard_wait(&bar.acc_empty[acc], ((it >> 1) & 1) ^ 1, g, 0x20000)) break;
+        if (!warp_wait(&bar.acc_empty[acc], ((it >> 1) & 1) ^ 1, g, 0x20000)) break;
         tmem_fence_after();
         for (int kb = w.k0; kb < w.k1; ++kb) {
-          if (!guard_wait(&bar.full[s], phase, g, 0x30000)) {
+          if (!warp_wait(&bar.full[s], phase, g, 0x30000)) {
             ok = false;
             break;
           }
           tmem_fence_after();
-          const uint32_t a = smem_u32(smem + s * S::kStage), b = a + S::kBytesA;
+          const uint64_t a = mma_desc(smem_u32(smem + s * S::kStage), lead_a, 1024);
+          const uint64_t b = mma_desc(smem_u32(smem + s * S::kStage + S::kBytesA), lead_b, 1024);
 #pragma unroll
           for (int k = 0; k < kBK / 16; ++k)
-            mma_ss<CG>(tmem + acc * BN, mma_desc(a + k * step_a, lead_a, 1024), mma_desc(b + k * step_b, lead_b, 1024),
-                       idesc, kb > w.k0 || k > 0);
-          mma_commit<CG>(&bar.empty[s]);
+            mma_ss<CG>(leader, tmem + acc * BN, a + k * step_a, b + k * step_b, idesc, kb > w.k0 || k > 0);
+          mma_commit<CG>(leader, &bar.empty[s]);
           if (++s == S::kStages) s = 0, phase ^= 1;
         }
-        if (ok) mma_commit<CG>(&bar.acc_full[acc]);
+        if (ok) mma_commit<CG>(leader, &bar.acc_full[acc]);
       }
-      mma_commit<CG>(&bar.drain);
+      mma_commit<CG>(leader, &bar.drain);
     }
   } else {
     const int e = warp - 2, quad = warp & 3, half = e >> 2;

@@ -66,10 +66,16 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void fence_async_shared() {   // plain stores, then TMA or the tensor cores
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ bool elect_one() {
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t p;
   asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(p));
-  return p != 0;
+  return p;
+}
+// a value that is the same in all threads of the warp, so that the compiler knows
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+// a whole warp waits
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Guard& g, uint32_t code) {
+  return __all_sync(0xffffffffu, guard_wait(bar, parity, g, code));
 }
 
 // A warpgroup's registers a thread from here on.  The sum over the CTA's warpgroups is at most
@@ -206,37 +212,47 @@ __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool bf16, bool a
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_kmajor ? 0u : 1u << 15) | (b_kmajor ? 0u : 1u << 16) |
          (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
+// Matrix products are issued by one thread of a warp, but all its threads go through the code, and
+// `leader` (elect_one()) says which of them does it: in a branch of one thread the compiler cannot
+// keep descriptors in uniform registers, and moving them there took 90 cycles for each product.
 template <int CG>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   if (CG == 1)
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
         : "memory");
   else
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
         : "memory");
 }
 // the same with the left operand in tensor memory, two 16-bit values to a column
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
       : "memory");
 }
 // arrives at `bar` once the products issued so far are done (CG 2: at both CTAs' barriers)
 template <int CG>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
   if (CG == 1)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+    asm volatile(
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
   else
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+        "{\n.reg .pred q;\nsetp.ne.b32 q, %2, 0;\n"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}" ::"r"(
             smem_u32(bar)),
-        "h"((uint16_t)3)
+        "h"((uint16_t)3), "r"(leader)
         : "memory");
 }
 
