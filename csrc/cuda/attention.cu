@@ -64,7 +64,7 @@ __device__ __forceinline__ F2 exp2_multiplied(F2 x) {
           __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23))};
 }
 
-constexpr int kMultiplied = 3;   // of eight pairs
+constexpr int kMultiplied = 0;   // of eight pairs
 
 struct Yes {
   __device__ constexpr operator bool() const { return true; }
@@ -132,6 +132,7 @@ __device__ __forceinline__ int visible_keys(const uint8_t* mask, int sk, int* sh
 
 struct Maps {
   CUtensorMap q, k, v, o, d_o, dq, dk, dv;
+  CUtensorMap q64, k64, v64, do64;   // in boxes of 64 rows
 };
 struct Launch {
   Maps map;
@@ -158,6 +159,8 @@ struct Launch {
 template <int DP, int QT, int KB, bool SHORT>
 struct Forward {
   static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kKeys = kPanels * KB * 128;   // bytes
+  // warps that issue products, each for its own tiles: a product of 64 keys takes as long to issue as to run
+  static constexpr int kIssue = QT > 1 ? 2 : 1;
   static constexpr int kStages = SHORT ? 1 : KB == 64 ? 6 : DP == 64 && QT == 2 ? 4 : 2;
   // four warps that fetch and issue, four for each tile's rows; the former give registers to the latter
   static constexpr int kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
@@ -191,8 +194,9 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   ForwardBars<KB>& bar = *(ForwardBars<KB>*)(skv + F::kStages * 2 * F::kKeys);
   const HpAttention& p = l.p;
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  // the tiles with the most keys first, where the mask is causal
-  const int qt = (int)gridDim.x - 1 - (int)blockIdx.x, h = blockIdx.y, b = blockIdx.z, hk = h / (int)(p.heads / p.kv_heads);
+  // of all heads first the tiles with the most keys, where the mask is causal
+  const int qt = (int)gridDim.y - 1 - (int)blockIdx.y, h = blockIdx.x % (int)p.heads, b = blockIdx.x / (int)p.heads;
+  const int hk = h / (int)(p.heads / p.kv_heads);
   const int q0 = qt * kB * QT, shift = (int)(p.sk - p.sq);
   const bool masked = p.key_mask != nullptr;
   const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
@@ -203,20 +207,20 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     const int keys = first >= p.sq ? 0 : p.causal ? min(sk, max(0, last + shift + 1)) : sk;
     return (keys + KB - 1) / KB;
   };
-  int n[QT], most = 0;
+  int most = 0;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) n[t] = tiles_of(t), most = max(most, n[t]);
+  for (int t = 0; t < QT; ++t) most = max(most, tiles_of(t));
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 1);
     for (int i = 0; i < F::kStages; ++i) {
-      mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.k_empty[i], 1), mbar_init(&bar.v_empty[i], 1);
-      mbar_init(&bar.mask_full[i], 1);
+      mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.mask_full[i], 1);
+      mbar_init(&bar.k_empty[i], F::kIssue), mbar_init(&bar.v_empty[i], F::kIssue);
     }
     for (int i = 0; i < QT; ++i) {
       mbar_init(&bar.s_full[i], 1), mbar_init(&bar.s_free[i], 128);
       mbar_init(&bar.p_full[i], 128), mbar_init(&bar.o_full[i], 1);
     }
-    mbar_init(&bar.drain, 1);
+    mbar_init(&bar.drain, F::kIssue);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
@@ -274,8 +278,9 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
         if (waits < most)   // the k of a tile whose v was not fetched
           mbar_wait_bounded(&bar.k_full[waits % F::kStages], (waits / F::kStages) & 1, kWaitNs / 64, g.status, HP_STATUS_TIMEOUT | 0x10007);
       }
-    } else if (warp == 1) {
+    } else if (warp <= F::kIssue) {
       if (most) {
+        const int mine = warp - 1;   // its first tile; every kIssue-th is its own
         const uint32_t leader = elect_one();
         const bool bf = p.type == HP_BF16;
         const uint32_t id_s = mma_idesc(128, KB, bf, true, true) | (l.negative ? kNegateA : 0);
@@ -295,14 +300,18 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
             mma_ts(leader, tmem_o + t * DP, tmem + F::kP + t * F::kPStep + i * 8, v + i * 128, id_o, add || i > 0);
           mma_commit<1>(leader, &bar.o_full[t]);
         };
+        int tiles[QT / F::kIssue];
+#pragma unroll
+        for (int i = 0; i < QT / F::kIssue; ++i) tiles[i] = tiles_of(i * F::kIssue + mine);
         int s = 0, s_before = 0;
         uint32_t ph = 0, ph_before = 0;
         for (int j = 0; j <= most && ok; ++j) {   // scores of tile j, results of tile j - 1
           if (j < most) ok = warp_wait(&bar.k_full[s], ph, g, 0x20002);
           if (F::kApart && ok) {   // scores as soon as the last ones have been read
 #pragma unroll
-            for (int t = 0; t < QT; ++t) {
-              if (j >= n[t] || !ok) continue;
+            for (int i = 0; i < QT / F::kIssue; ++i) {
+              const int t = i * F::kIssue + mine;
+              if (j >= tiles[i] || !ok) continue;
               if (j > 0) ok = warp_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
               tmem_fence_after();
               if (ok) scores(t, s);
@@ -312,13 +321,14 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
           if (j > 0 && ok) ok = warp_wait(&bar.v_full[s_before], ph_before, g, 0x20003);
           tmem_fence_after();
 #pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            if (j > 0 && j - 1 < n[t] && ok) {
+          for (int i = 0; i < QT / F::kIssue; ++i) {
+            const int t = i * F::kIssue + mine;
+            if (j > 0 && j - 1 < tiles[i] && ok) {
               ok = warp_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
               tmem_fence_after();
               if (ok) results(t, s_before, j > 1);
             }
-            if (!F::kApart && j < n[t] && ok) scores(t, s);   // over the probabilities just used
+            if (!F::kApart && j < tiles[i] && ok) scores(t, s);   // over the probabilities just used
           }
           if (j > 0) mma_commit<1>(leader, &bar.v_empty[s_before]);
           if (!F::kApart && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
@@ -554,28 +564,32 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
   }
 }
 
-// Two kinds of CTA, each with a tile of 128 rows that stays and tiles that pass by:
+// Two kinds of CTA, each with a tile of 128 rows that stays and tiles of 64 that pass by:
 //   keys     k, v stay; q, d_o pass.  S^T = k q^T, dP^T = v d_o^T; dv += P^T d_o, dk += dS^T q
 //   queries  q, d_o stay; k, v pass.  S = q k^T, dP = d_o v^T; dq += dS k
 // with P = 2^(c S - lse) and dS = P (dP - delta).  Computing S and dP for each kind costs two
 // products of seven more than one kernel that adds its parts of dq up in memory, and saves
 // those additions, their 32-bit buffer and their order, which would differ from run to run.
-// P and dS go back to tensor memory over S, as the left operands; eight warps share the rows, one
-// thread half a row.  The next tile's S is computed meanwhile (a second buffer), except for keys
-// with more than 64 dimensions, whose two results leave no room for it.
+// P and dS go back to tensor memory over S, as the left operands.  Two groups of four warps, a row
+// to a thread, take the tiles by turns, so that what one waits for (fetch, store, products) goes on
+// behind the other's 2^x: with tiles of 128 that both groups shared, 2600 cycles passed for each
+// where its products take 1000.  Tensor memory holds S and dP of three tiles, or of two where the
+// results of keys with more than 64 dimensions take half of it.
+constexpr int kPass = 64;
 template <int DP>
 struct Backward {
-  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kStages = DP == 64 ? 4 : 2;
+  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kPassed = kPanels * kPass * 128;   // bytes
+  static constexpr int kStages = DP == 64 ? 8 : 4;   // even: a stage is always the same group's
   // four warps that fetch and issue, eight for the rows; the former give registers to the latter
   static constexpr int kThreads = 128 + 256, kAtStart = 168, kFew = 72, kMany = 216;
   static_assert(kFew + 2 * kMany <= 3 * kAtStart, "more registers than the CTA has");
-  static constexpr int kSmem = 2 * kTile + kStages * (2 * kTile + 1024) + 1024 + 1024;
-  // columns: S (buffers kS apart), dP, the results
-  static constexpr uint32_t kS = 256, kDP = 128, kAcc1 = DP == 64 ? 384 : 256, kAcc2 = DP == 64 ? 448 : 384;
+  static constexpr int kSmem = 2 * kTile + kStages * (2 * kPassed + 8 * kPass) + 1024 + 1024;
+  // columns: tile j's S (later P, dS) at kBuffer times its buffer, dP kPass further on; the results
+  static constexpr uint32_t kBuffer = 2 * kPass, kAcc1 = DP == 64 ? 384 : 256, kAcc2 = DP == 64 ? 448 : 384;
 };
 struct BackwardBars {
-  uint64_t stay_full, in_full[4], in_empty[4], mask_full[4], s_full[2], dp_full, dp_free, p_full, acc_full;
-  Seen<kB> seen[4];
+  uint64_t stay_full, in_full[8], in_empty[8], mask_full[8], s_full[6], s_free[3], p_full[3], acc_full;
+  Seen<kPass> seen[8];
   uint32_t tmem;
   int keys;
   Guard guard;
@@ -588,45 +602,52 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* stay = smem;
   uint8_t* pass = smem + 2 * F::kTile;
-  float* rows_of = (float*)(pass + F::kStages * 2 * F::kTile);   // a stage's lse and delta
-  BackwardBars& bar = *(BackwardBars*)(rows_of + F::kStages * 2 * kB);
+  float* rows_of = (float*)(pass + F::kStages * 2 * F::kPassed);   // a stage's lse and delta
+  BackwardBars& bar = *(BackwardBars*)(rows_of + F::kStages * 2 * kPass);
   const HpAttention& p = l.p;
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int nq = (int)((p.sq + kB - 1) / kB), nk = (int)((p.sk + kB - 1) / kB), group = (int)(p.heads / p.kv_heads);
   const int sk = (int)p.sk, shift = (int)(p.sk - p.sq);
-  // keys first: with shared heads they have more to do
-  const int b = blockIdx.y;
+  // Of all heads first the tiles with the most to do: under a causal mask the first keys and the
+  // last queries, side by side where there are as many of both; else keys first, which with shared
+  // heads have more to do.
+  const int hk = (int)(p.kv_heads * p.batch), hq = (int)(p.heads * p.batch);
   int id = blockIdx.x, head, tile;
-  const bool keys = id < nk * (int)p.kv_heads;
-  if (keys) {
-    head = id / nk, tile = id % nk;   // under a causal mask the first keys are seen by most
+  bool keys;
+  if (nq == nk) {
+    tile = id / (hk + hq), id %= hk + hq;
+    keys = id < hk;
+    if (!keys) id -= hk, tile = nq - 1 - tile;
   } else {
-    id -= nk * (int)p.kv_heads;
-    head = id / nq, tile = nq - 1 - id % nq;
+    keys = id < nk * hk;
+    if (!keys) id -= nk * hk;
+    tile = keys ? id / hk : nq - 1 - id / hq;
+    id %= keys ? hk : hq;
   }
+  const int heads = keys ? (int)p.kv_heads : (int)p.heads, b = id / heads;
+  head = id % heads;
   const int r0 = tile * kB;           // first row that stays
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const bool masked = mask != nullptr;
   // tiles that pass: queries from `first` on, of each head of the group in turn; or keys up to the last seen
   int first = 0, count;
   if (keys) {
-    if (p.causal) first = max(0, r0 - shift) / kB;
-    count = max(0, nq - first);
-    if (masked) {
-      if (mask_bits<kB>(mask, r0, sk).none()) count = 0;
-    }
+    if (p.causal) first = max(0, r0 - shift) / kPass;
+    count = max(0, (int)((p.sq + kPass - 1) / kPass) - first);
+    if (masked && mask_bits<kB>(mask, r0, sk).none()) count = 0;
   } else {
-    int see = masked && sk > kB ? visible_keys(mask, sk, &bar.keys) : sk;
+    int see = masked && sk > kPass ? visible_keys(mask, sk, &bar.keys) : sk;
     if (p.causal) see = min(see, max(0, min(r0 + kB, (int)p.sq) + shift));
-    count = (see + kB - 1) / kB;
+    count = (see + kPass - 1) / kPass;
   }
   const int n = keys ? count * group : count;
-  const int buffers = DP == 64 || !keys ? 2 : 1;
+  const int buffers = DP == 64 || !keys ? 3 : 2, turns = buffers == 3 ? 6 : 2;   // a turn is one group's, of one buffer
   if (threadIdx.x == 0) {
     mbar_init(&bar.stay_full, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&bar.in_full[i], 1), mbar_init(&bar.in_empty[i], 1), mbar_init(&bar.mask_full[i], 1);
-    mbar_init(&bar.s_full[0], 1), mbar_init(&bar.s_full[1], 1), mbar_init(&bar.dp_full, 1);
-    mbar_init(&bar.dp_free, 256), mbar_init(&bar.p_full, 256), mbar_init(&bar.acc_full, 1);
+    for (int i = 0; i < F::kStages; ++i) mbar_init(&bar.in_full[i], 1), mbar_init(&bar.in_empty[i], 1), mbar_init(&bar.mask_full[i], 1);
+    for (int i = 0; i < 6; ++i) mbar_init(&bar.s_full[i], 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&bar.s_free[i], 1), mbar_init(&bar.p_full[i], 128);
+    mbar_init(&bar.acc_full, 2);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
@@ -639,112 +660,108 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   Guard& g = bar.guard;
 
   if (warp < 4) {
-  fewer_registers<F::kFew>();
-  if (warp == 0) {
-    const uint32_t bytes = 2 * F::kTile + (keys ? 8 * kB : 0);
-    const int64_t rows = padded(p.sq);
-    int waits = 0;
-    if (lane == 0 && n) {
-      mbar_expect_tx(&bar.stay_full, 2 * F::kTile);
-      for (int i = 0; i < F::kPanels; ++i) {
-        tma_load_4d(stay + i * kPanel, keys ? &l.map.k : &l.map.q, 64 * i, head, r0, b, &bar.stay_full);
-        tma_load_4d(stay + F::kTile + i * kPanel, keys ? &l.map.v : &l.map.d_o, 64 * i, head, r0, b, &bar.stay_full);
-      }
-    }
-    for (int j = 0; j < n; ++j) {
-      const int s = j % F::kStages;
-      if (!guard_wait(&bar.in_empty[s], ((j / F::kStages) & 1) ^ 1, g, 0x11001)) break;
-      if (lane == 0) {
-        uint8_t* to = pass + s * 2 * F::kTile;
-        const int h = keys ? head * group + j / count : head / group, at = keys ? (first + j % count) * kB : j * kB;
-        mbar_expect_tx(&bar.in_full[s], bytes);
+    fewer_registers<F::kFew>();
+    if (warp == 0) {
+      const uint32_t bytes = 2 * F::kPassed + (keys ? 8 * kPass : 0);
+      const int64_t rows = padded(p.sq);
+      int waits = 0;
+      if (lane == 0 && n) {
+        mbar_expect_tx(&bar.stay_full, 2 * F::kTile);
         for (int i = 0; i < F::kPanels; ++i) {
-          tma_load_4d(to + i * kPanel, keys ? &l.map.q : &l.map.k, 64 * i, h, at, b, &bar.in_full[s]);
-          tma_load_4d(to + F::kTile + i * kPanel, keys ? &l.map.d_o : &l.map.v, 64 * i, h, at, b, &bar.in_full[s]);
-        }
-        if (keys) {
-          const float* from = p.delta + (b * p.heads + h) * 2 * rows + at;
-          bulk_load(rows_of + s * 2 * kB, from, 4 * kB, &bar.in_full[s]);
-          bulk_load(rows_of + s * 2 * kB + kB, from + rows, 4 * kB, &bar.in_full[s]);
+          tma_load_4d(stay + i * kPanel, keys ? &l.map.k : &l.map.q, 64 * i, head, r0, b, &bar.stay_full);
+          tma_load_4d(stay + F::kTile + i * kPanel, keys ? &l.map.v : &l.map.d_o, 64 * i, head, r0, b, &bar.stay_full);
         }
       }
-      if (!keys && masked) {
-        const Seen<kB> m = mask_bits<kB>(mask, (int64_t)j * kB, sk);
-        if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
+      int s = 0, h = keys ? head * group : head / group, at = first;
+      uint32_t ph = 0;
+      for (int j = 0; j < n; ++j) {
+        if (!guard_wait(&bar.in_empty[s], ph ^ 1, g, 0x11001)) break;
+        if (lane == 0) {
+          uint8_t* to = pass + s * 2 * F::kPassed;
+          mbar_expect_tx(&bar.in_full[s], bytes);
+          for (int i = 0; i < F::kPanels; ++i) {
+            tma_load_4d(to + i * kPass * 128, keys ? &l.map.q64 : &l.map.k64, 64 * i, h, at * kPass, b, &bar.in_full[s]);
+            tma_load_4d(to + F::kPassed + i * kPass * 128, keys ? &l.map.do64 : &l.map.v64, 64 * i, h, at * kPass, b, &bar.in_full[s]);
+          }
+          if (keys) {
+            const float* from = p.delta + (b * p.heads + h) * 2 * rows + at * kPass;
+            bulk_load(rows_of + s * 2 * kPass, from, 4 * kPass, &bar.in_full[s]);
+            bulk_load(rows_of + s * 2 * kPass + kPass, from + rows, 4 * kPass, &bar.in_full[s]);
+          }
+        }
+        if (!keys && masked) {
+          const Seen<kPass> m = mask_bits<kPass>(mask, (int64_t)j * kPass, sk);
+          if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
+        }
+        waits = j + 1;
+        if (++at == first + count) at = first, ++h;   // the next head of the group
+        if (++s == F::kStages) s = 0, ph ^= 1;
       }
-      waits = j + 1;
-    }
-    __syncwarp();
-    if (g.gave_up && lane == 0 && n) {   // nothing may land once the CTA is gone
-      mbar_wait_bounded(&bar.stay_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11002);
-      for (int j = max(0, waits - F::kStages); j < waits; ++j)
-        mbar_wait_bounded(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11003);
-    }
-  } else if (warp == 1) {
-    if (n) {
-      const uint32_t leader = elect_one();
-      const bool bf = p.type == HP_BF16;
-      const uint32_t id_s = mma_idesc(128, 128, bf, true, true) | (l.negative ? kNegateA : 0);
-      const uint32_t id_dp = mma_idesc(128, 128, bf, true, true), id_acc = mma_idesc(128, DP, bf, true, false);
-      const uint32_t a = smem_u32(stay);
-      auto in = [&](int j) { return smem_u32(pass + (j % F::kStages) * 2 * F::kTile); };
-      auto wide = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t id) {   // rows by rows, over the dimensions
-        const uint64_t dx = mma_desc(x, 16, 1024), dy = mma_desc(y, 16, 1024);
+      __syncwarp();
+      if (g.gave_up && lane == 0 && n) {   // nothing may land once the CTA is gone
+        mbar_wait_bounded(&bar.stay_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11002);
+        for (int j = max(0, waits - F::kStages); j < waits; ++j)
+          mbar_wait_bounded(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11003);
+      }
+    } else if (warp <= 2) {
+      // one warp issues S and dP, the other the results: each product takes as long to issue as to run
+      if (n) {
+        const uint32_t leader = elect_one();
+        const bool bf = p.type == HP_BF16;
+        const uint32_t id_s = mma_idesc(128, kPass, bf, true, true) | (l.negative ? kNegateA : 0);
+        const uint32_t id_dp = mma_idesc(128, kPass, bf, true, true), id_acc = mma_idesc(128, DP, bf, true, false);
+        auto in = [&](int s) { return smem_u32(pass + s * 2 * F::kPassed); };
+        auto wide = [&](uint32_t d, uint32_t x, uint32_t y, uint32_t id) {   // rows by rows, over the dimensions
+          const uint64_t dx = mma_desc(x, 16, 1024), dy = mma_desc(y, 16, 1024);
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t at = ((i / 4) * kPanel + (i % 4) * 32) >> 4;
-          mma_ss<1>(leader, d, dx + at, dy + at, id, i > 0);
-        }
-      };
-      auto deep = [&](uint32_t d, uint32_t x, uint32_t y, bool add) {      // P or dS, over the tile's columns
-        const uint64_t dy = mma_desc(y, kPanel, 1024);
+          for (int i = 0; i < DP / 16; ++i)
+            mma_ss<1>(leader, d, dx + ((i / 4) * kPanel + (i % 4) * 32) / 16, dy + ((i / 4) * kPass * 128 + (i % 4) * 32) / 16, id, i > 0);
+        };
+        auto deep = [&](uint32_t d, uint32_t x, uint32_t y, bool add) {      // P or dS, over the tile's columns
+          const uint64_t dy = mma_desc(y, kPass * 128, 1024);
 #pragma unroll
-        for (int i = 0; i < kB / 16; ++i) mma_ts(leader, d, x + (i / 2) * 32 + (i % 2) * 8, dy + i * 128, id_acc, add || i > 0);
-      };
-      auto scores = [&](int j) {
-        const int q = buffers == 2 ? j & 1 : 0;
-        wide(tmem + F::kS * q, a, in(j), id_s);
-        mma_commit<1>(leader, &bar.s_full[q]);
-      };
-      auto dprobs = [&](int j) {
-        wide(tmem + F::kDP, a + F::kTile, in(j) + F::kTile, id_dp);
-        mma_commit<1>(leader, &bar.dp_full);
-      };
-      auto there = [&](int j) { return warp_wait(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, g, 0x21001); };
-      bool ok = warp_wait(&bar.stay_full, 0, g, 0x21002) && there(0);
-      if (ok) {
-        tmem_fence_after();
-        scores(0);
-        dprobs(0);
-      }
-      for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) {
-          ok = there(j + 1);
-          if (!ok) break;
-          if (buffers == 2) scores(j + 1);
-          ok = warp_wait(&bar.dp_free, j & 1, g, 0x21004);
-          if (!ok) break;
-          tmem_fence_after();
-          dprobs(j + 1);
+          for (int i = 0; i < kPass / 16; ++i) mma_ts(leader, d, x + i * 8, dy + i * 128, id_acc, add || i > 0);
+        };
+        int s = 0, q = 0, turn = 0;
+        uint32_t ph = 0, round = 0;   // of the stages, of the buffers
+        bool ok = true;
+        if (warp == 1) {
+          const uint32_t a = smem_u32(stay);
+          ok = warp_wait(&bar.stay_full, 0, g, 0x21002);
+          for (int j = 0; j < n && ok; ++j) {
+            ok = warp_wait(&bar.in_full[s], ph, g, 0x21001) && warp_wait(&bar.s_free[q], round ^ 1, g, 0x21005);
+            if (!ok) break;
+            tmem_fence_after();
+            const uint32_t d = tmem + F::kBuffer * q;
+            wide(d, a, in(s), id_s);
+            wide(d + kPass, a + F::kTile, in(s) + F::kPassed, id_dp);
+            mma_commit<1>(leader, &bar.s_full[turn]);
+            if (++s == F::kStages) s = 0, ph ^= 1;
+            if (++q == buffers) q = 0, round ^= 1;
+            if (++turn == turns) turn = 0;
+          }
+        } else {
+          for (int j = 0; j < n; ++j) {
+            if (!warp_wait(&bar.p_full[q], round, g, 0x21003)) break;
+            tmem_fence_after();
+            const uint32_t x = tmem + F::kBuffer * q;
+            if (keys) deep(tmem + F::kAcc1, x, in(s) + F::kPassed, j > 0);
+            deep(tmem + F::kAcc2, x + kPass / 2, in(s), j > 0);
+            mma_commit<1>(leader, &bar.s_free[q]);
+            mma_commit<1>(leader, &bar.in_empty[s]);   // S and dP of this tile are behind p_full
+            if (++s == F::kStages) s = 0;
+            if (++q == buffers) q = 0, round ^= 1;
+          }
         }
-        ok = warp_wait(&bar.p_full, j & 1, g, 0x21003);
-        if (!ok) break;
-        tmem_fence_after();
-        const uint32_t s = tmem + F::kS * (buffers == 2 ? j & 1 : 0);
-        if (keys) deep(tmem + F::kAcc1, s, in(j) + F::kTile, j > 0);
-        deep(tmem + F::kAcc2, s + 16, in(j), j > 0);
-        mma_commit<1>(leader, &bar.in_empty[j % F::kStages]);
-        if (buffers == 1 && j + 1 < n) scores(j + 1);
+        mma_commit<1>(leader, &bar.acc_full);
       }
-      mma_commit<1>(leader, &bar.acc_full);
     }
-  }
   } else {
     more_registers<F::kMany>();
     const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane, row = r0 + r;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
     float lse = -INFINITY, delta = 0.f;   // of a query that stays, negative
-    bool mine = true;                    // a key that stays is seen at all
+    bool mine = true;                     // a key that stays is seen at all
     if (keys) {
       mine = row < sk && (!masked || mask[row]);
     } else {
@@ -753,105 +770,97 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     }
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int s = j % F::kStages, q = buffers == 2 ? j & 1 : 0;
-      Seen<kB> seen;
+    for (int j = half; j < n; j += 2) {
+      const int s = j % F::kStages, q = j % buffers, turn = j % turns;
+      const uint32_t ph = (j / F::kStages) & 1;
+      Seen<kPass> seen;
       bool whole;
       if (keys) {
-        const int from = p.causal ? row - shift - (first + j % count) * kB : 0;   // its first query in this tile
+        const int from = p.causal ? row - shift - (first + j % count) * kPass : 0;   // its first query in this tile
         whole = mine && from <= 0;
         if (!__all_sync(0xffffffffu, whole)) {
-          seen = seen_between<kB>(mine ? from : kB, kB);
+          seen = seen_between<kPass>(mine ? from : kPass, kPass);
           whole = false;
         }
       } else {
-        whole = sees >= (j + 1) * kB;
+        whole = sees >= (j + 1) * kPass;
         if (masked) {
-          if (!guard_wait(&bar.mask_full[s], (j / F::kStages) & 1, g, 0x31001)) { ok = false; break; }
+          if (!guard_wait(&bar.mask_full[s], ph, g, 0x31001)) { ok = false; break; }
           seen = bar.seen[s];
           const bool all = seen.all();
           if (!all) {   // what a masked key holds is left out of dq: its k counts as zero
-            if (!guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31002)) { ok = false; break; }
-            if (half == 0 && !(seen.w[quad] >> lane & 1)) {
-              uint4* k = (uint4*)(pass + s * 2 * F::kTile + r * 128);
+            if (!guard_wait(&bar.in_full[s], ph, g, 0x31002)) { ok = false; break; }
+            if (r < kPass && !(seen.w[quad & 1] >> lane & 1)) {
+              uint4* k = (uint4*)(pass + s * 2 * F::kPassed + r * 128);
 #pragma unroll
               for (int i = 0; i < F::kPanels; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) k[i * (kPanel / 16) + e] = make_uint4(0, 0, 0, 0);
+                for (int e = 0; e < 8; ++e) k[i * kPass * 8 + e] = make_uint4(0, 0, 0, 0);
             }
             fence_async_shared();
           }
           whole = whole && all;
         }
         if (!__all_sync(0xffffffffu, whole)) {
-          const Seen<kB> up_to = seen_between<kB>(0, sees - j * kB);
+          const Seen<kPass> up_to = seen_between<kPass>(0, sees - j * kPass);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) seen.w[i] = masked ? seen.w[i] & up_to.w[i] : up_to.w[i];
+          for (int i = 0; i < kPass / 32; ++i) seen.w[i] = masked ? seen.w[i] & up_to.w[i] : up_to.w[i];
           whole = false;
         }
       }
-      const bool here = guard_wait(&bar.s_full[q], (buffers == 2 ? j >> 1 : j) & 1, g, 0x31003) &&
-                        guard_wait(&bar.dp_full, j & 1, g, 0x31004);
-      if (!here) { ok = false; break; }
-      if (keys && !guard_wait(&bar.in_full[s], (j / F::kStages) & 1, g, 0x31005)) { ok = false; break; }
+      if (!guard_wait(&bar.s_full[turn], (j / turns) & 1, g, 0x31003)) { ok = false; break; }
+      if (keys && !guard_wait(&bar.in_full[s], ph, g, 0x31005)) { ok = false; break; }
       tmem_fence_after();
-      const float* cols = rows_of + s * 2 * kB + 64 * half;
-      // both of this thread's halves at once: dP's columns are free for the next tile's then
-      uint32_t xs[2][32], ys[2][32];
+      const float* cols = rows_of + s * 2 * kPass;
+      const uint32_t at = tmem + lanes + F::kBuffer * q;
+      uint32_t x[kPass], y[kPass];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld32(tmem + lanes + 64 * half + 32 * c + F::kS * q, xs[c]);
-        tmem_ld32(tmem + lanes + 64 * half + 32 * c + F::kDP, ys[c]);
+      for (int c = 0; c < kPass; c += 32) {
+        tmem_ld32(at + c, *(uint32_t(*)[32])(x + c));
+        tmem_ld32(at + kPass + c, *(uint32_t(*)[32])(y + c));
       }
       tmem_wait_ld();
-      tmem_fence_before();
-      mbar_arrive(&bar.dp_free);
-      auto gradients = [&](auto all, auto of_keys) {
+      auto gradients = [&](auto all, auto of_keys) {   // packed P into x, dS into y
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
-          const uint32_t at = tmem + lanes + 64 * half + c;
-          const uint32_t(&x)[32] = xs[c / 32], (&y)[32] = ys[c / 32];
-          const uint32_t mine_of = all ? 0xffffffffu : seen.w[2 * half + c / 32];
-          uint32_t e[16], d[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta};   // negative both
-            if (of_keys) {
-              *(float4*)ls = *(const float4*)(cols + c + i);
-              *(float4*)de = *(const float4*)(cols + kB + c + i);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-              const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {ls[k], ls[k + 1]});
-              F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-              F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {de[k], de[k + 1]}));
-              if (!all) {
-                const uint32_t two = mine_of >> (i + k);
-                if (!(two & 1)) pr.x = ds.x = 0.f;
-                if (!(two & 2)) pr.y = ds.y = 0.f;
-              }
-              if (of_keys) e[(i + k) / 2] = pack2<T>(pr.x, pr.y);
-              d[(i + k) / 2] = pack2<T>(ds.x, ds.y);
-            }
+        for (int i = 0; i < kPass; i += 4) {
+          float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta};   // negative both
+          if (of_keys) {
+            *(float4*)ls = *(const float4*)(cols + i);
+            *(float4*)de = *(const float4*)(cols + kPass + i);
           }
-          if (of_keys) tmem_st16(at + F::kS * q, e);
-          tmem_st16(at + F::kS * q + 16, d);
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {ls[k], ls[k + 1]});
+            F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
+            F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {de[k], de[k + 1]}));
+            if (!all) {
+              const uint32_t two = seen.w[i / 32] >> (i % 32 + k);
+              if (!(two & 1)) pr.x = ds.x = 0.f;
+              if (!(two & 2)) pr.y = ds.y = 0.f;
+            }
+            if (of_keys) x[(i + k) / 2] = pack2<T>(pr.x, pr.y);
+            y[(i + k) / 2] = pack2<T>(ds.x, ds.y);
+          }
         }
       };
       if (keys) {
         if (whole) gradients(Yes(), Yes());
         else gradients(No(), Yes());
+#pragma unroll
+        for (int c = 0; c < kPass / 2; c += 16) tmem_st16(at + c, *(const uint32_t(*)[16])(x + c));
       } else {
         if (whole) gradients(Yes(), No());
         else gradients(No(), No());
       }
+#pragma unroll
+      for (int c = 0; c < kPass / 2; c += 16) tmem_st16(at + kPass / 2 + c, *(const uint32_t(*)[16])(y + c));
       tmem_wait_st();
       tmem_fence_before();
-      mbar_arrive(&bar.p_full);
+      mbar_arrive(&bar.p_full[q]);
     }
     if (ok && n) ok = guard_wait(&bar.acc_full, 0, g, 0x31006);
     tmem_fence_after();
-    // results leave through the space of what stayed: panels of 64 columns, by turns of the two halves
+    // results leave through the space of what stayed: panels of 64 columns, by turns of the two groups
     const int64_t length = keys ? p.sk : p.sq;
     if (ok && r0 < length)
       for (int job = half; job < (keys ? 2 : 1) * F::kPanels; job += 2) {
@@ -860,7 +869,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         const uint32_t from = tmem + lanes + (is_v ? F::kAcc1 : F::kAcc2) + 64 * panel;
         const float scale = is_v ? 1.f : (float)p.scale;
         uint8_t* to = stay + job * kPanel + 32 * quad * 128;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 64; c += 32) {
           uint32_t o[32];
           if (n) {
@@ -937,7 +946,9 @@ int forward_tiles(Launch& l, cudaStream_t s) {
       !head_map(&l.map.v, a.sk ? a.v : a.q, a, a.sk, a.kv_heads, a.v_b, a.v_s, a.v_h, KB) ||
       !head_map(&l.map.o, a.o, a, a.sq, a.heads, a.o_b, a.o_s, a.o_h, 32))
     return HP_ERR_BAD_ARG;
-  const dim3 grid((unsigned)((a.sq + kB * QT - 1) / (kB * QT)), (unsigned)a.heads, (unsigned)a.batch);
+  if (a.heads * a.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
+  const dim3 grid((unsigned)(a.heads * a.batch), (unsigned)((a.sq + kB * QT - 1) / (kB * QT)));
+  if (grid.y > 65535) return HP_ERR_TOO_LARGE;
   kernel<<<grid, F::kThreads, F::kSmem, s>>>(l);
   return cudaGetLastError();
 }
@@ -959,14 +970,14 @@ int backward_tiles(const Launch& l, cudaStream_t s) {
       cudaFuncSetAttribute(attention_backward_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (allowed != cudaSuccess) return allowed;
   const HpAttention& a = l.p;
-  const int64_t nq = (a.sq + kB - 1) / kB, nk = (a.sk + kB - 1) / kB, tiles = nk * a.kv_heads + nq * a.heads;
+  const int64_t nq = (a.sq + kB - 1) / kB, nk = (a.sk + kB - 1) / kB, tiles = (nk * a.kv_heads + nq * a.heads) * a.batch;
   if (tiles > INT32_MAX) return HP_ERR_TOO_LARGE;
   if (a.sq) {
     constexpr int kLanes = DP / 8;
     attention_rows<T, kLanes><<<dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch), 256, 0, s>>>(a);
     if (const cudaError_t e = cudaGetLastError()) return e;
   }
-  attention_backward_tiles<T, DP><<<dim3((unsigned)tiles, (unsigned)a.batch), F::kThreads, F::kSmem, s>>>(l);
+  attention_backward_tiles<T, DP><<<(unsigned)tiles, F::kThreads, F::kSmem, s>>>(l);
   return cudaGetLastError();
 }
 
@@ -983,7 +994,9 @@ int backward(const HpAttention& a, cudaStream_t s) {
   if (!map(&l.map.q, a.q, false, a.q_b, a.q_s, a.q_h, kB) || !map(&l.map.k, a.k, true, a.k_b, a.k_s, a.k_h, kB) ||
       !map(&l.map.v, a.v, true, a.v_b, a.v_s, a.v_h, kB) || !map(&l.map.d_o, a.d_o, false, a.do_b, a.do_s, a.do_h, kB) ||
       !map(&l.map.dq, a.dq, false, a.dq_b, a.dq_s, a.dq_h, 32) || !map(&l.map.dk, a.dk, true, a.dk_b, a.dk_s, a.dk_h, 32) ||
-      !map(&l.map.dv, a.dv, true, a.dv_b, a.dv_s, a.dv_h, 32))
+      !map(&l.map.dv, a.dv, true, a.dv_b, a.dv_s, a.dv_h, 32) ||
+      !map(&l.map.q64, a.q, false, a.q_b, a.q_s, a.q_h, kPass) || !map(&l.map.k64, a.k, true, a.k_b, a.k_s, a.k_h, kPass) ||
+      !map(&l.map.v64, a.v, true, a.v_b, a.v_s, a.v_h, kPass) || !map(&l.map.do64, a.d_o, false, a.do_b, a.do_s, a.do_h, kPass))
     return HP_ERR_BAD_ARG;
   return a.dim <= 64 ? backward_tiles<T, 64>(l, s) : backward_tiles<T, 128>(l, s);
 }
