@@ -908,6 +908,206 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   if (warp == 1) tmem_free<1>(tmem, 512);
 }
 
+// Up to 128 queries and keys of up to 64 dimensions: everything of one head in one CTA, S and dP once,
+// and nothing left for another kernel.  Rows are keys: S^T and dP^T as above; P^T goes back to tensor
+// memory, dS^T into shared memory, where it is the left operand of dk (along its rows) and of dq
+// (across them).  dv and dk take dP's columns, dq those of S.  Two CTAs fit an SM.  Bound: the
+// latency of one pass from fetch to store, not the traffic.
+struct ShortBars {
+  uint64_t kq_full, vo_full, s_full, dp_full, rows_full, p_full, acc_full, out_full;
+  float lse[kB], delta[kB];
+  uint32_t tmem;
+  Guard guard;
+};
+constexpr int kShortSmem = 6 * (int)kPanel + 2048 + 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_constant__ Launch l) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *sk_ = smem, *sq_ = smem + kPanel, *sv_ = smem + 2 * kPanel, *sg_ = smem + 3 * kPanel;
+  uint8_t* sds = smem + 4 * kPanel;   // dS^T: two panels of 64 queries; o before that
+  ShortBars& bar = *(ShortBars*)(smem + 6 * kPanel);
+  const HpAttention& p = l.p;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int h = blockIdx.x % (int)p.heads, b = blockIdx.x / (int)p.heads;
+  const int sq = (int)p.sq, sk = (int)p.sk, shift = sk - sq;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar.kq_full, 1), mbar_init(&bar.vo_full, 1), mbar_init(&bar.s_full, 1), mbar_init(&bar.dp_full, 1);
+    mbar_init(&bar.rows_full, 128), mbar_init(&bar.p_full, 256), mbar_init(&bar.acc_full, 1), mbar_init(&bar.out_full, 256);
+    mbar_init_fence();
+    bar.guard.gave_up = 0;
+    bar.guard.status = l.status;
+    mbar_expect_tx(&bar.kq_full, 2 * kPanel);
+    tma_load_4d(sk_, &l.map.k, 0, h, 0, b, &bar.kq_full);
+    tma_load_4d(sq_, &l.map.q, 0, h, 0, b, &bar.kq_full);
+    mbar_expect_tx(&bar.vo_full, 3 * kPanel);
+    tma_load_4d(sv_, &l.map.v, 0, h, 0, b, &bar.vo_full);
+    tma_load_4d(sg_, &l.map.d_o, 0, h, 0, b, &bar.vo_full);
+    tma_load_4d(sds, &l.map.o, 0, h, 0, b, &bar.vo_full);
+  }
+  if (warp == 1) tmem_alloc<1>(&bar.tmem, 256);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = uniform(bar.tmem);
+  Guard& g = bar.guard;
+  if (warp == 1) {
+    const uint32_t leader = elect_one();
+    const bool bf = p.type == HP_BF16;
+    const uint32_t id_s = mma_idesc(128, 128, bf, true, true), id = mma_idesc(128, 64, bf, true, false);
+    auto desc = [&](uint8_t* x) { return mma_desc(smem_u32(x), kPanel, 1024); };
+    bool ok = warp_wait(&bar.kq_full, 0, g, 0x22001);
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mma_ss<1>(leader, tmem, desc(sk_) + i * 2, desc(sq_) + i * 2, id_s | (l.negative ? kNegateA : 0), i > 0);
+      mma_commit<1>(leader, &bar.s_full);
+      ok = warp_wait(&bar.vo_full, 0, g, 0x22002);
+    }
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mma_ss<1>(leader, tmem + 128, desc(sv_) + i * 2, desc(sg_) + i * 2, id_s, i > 0);
+      mma_commit<1>(leader, &bar.dp_full);
+      ok = warp_wait(&bar.p_full, 0, g, 0x22003);
+      tmem_fence_after();
+    }
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mma_ts(leader, tmem + 128, tmem + (i / 2) * 32 + (i % 2) * 8, desc(sg_) + i * 128, id, i > 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mma_ss<1>(leader, tmem + 192, desc(sds) + (i / 4) * (kPanel / 16) + (i % 4) * 2, desc(sq_) + i * 128, id, i > 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mma_ss<1>(leader, tmem, desc(sds) + i * 128, desc(sk_) + i * 128, mma_idesc(128, 64, bf, false, false), i > 0);
+    }
+    mma_commit<1>(leader, &bar.acc_full);
+  } else if (warp >= 2) {
+    const int quad = warp & 3, half = (warp - 2) >> 2, r = 32 * quad + lane;   // a key, half of the queries
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+    const bool there = r < sk, mine = there && (!p.key_mask || p.key_mask[b * p.mask_b + r]);
+    bool ok = true;
+    if (half == 0) {   // lse and delta, negative, of query r
+      const float lse = r < sq ? p.lse[(b * p.heads + h) * p.sq + r] : -INFINITY;
+      ok = guard_wait(&bar.vo_full, 0, g, 0x32001);
+      float d = 0.f;
+#pragma unroll
+      for (int c = 0; c < 128; c += 16) {
+        float x[8], y[8];
+        unpack<T>(*(const uint4*)(sg_ + staged(r, c)), x);
+        unpack<T>(*(const uint4*)(sds + staged(r, c)), y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d = fmaf(x[i], y[i], d);
+      }
+      bar.lse[r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+      bar.delta[r] = -d;
+      mbar_arrive(&bar.rows_full);
+    }
+    const int from = p.causal ? r - shift : 0;   // the first query that sees this key
+    bool whole = mine && from <= 0;
+    Seen<kB> seen;
+    if (!__all_sync(0xffffffffu, whole)) {
+      seen = seen_between<kB>(mine ? from : kB, kB);
+      whole = false;
+    }
+    ok = ok && guard_wait(&bar.rows_full, 0, g, 0x32002) && guard_wait(&bar.s_full, 0, g, 0x32003) &&
+         guard_wait(&bar.dp_full, 0, g, 0x32004);
+    tmem_fence_after();
+    if (ok) {
+      if (there && !mine && half == 0)   // what a masked key holds is left out of dq: it counts as zero
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *((uint4*)(sk_ + r * 128) + c) = make_uint4(0, 0, 0, 0);
+      auto gradients = [&](auto all) {
+#pragma unroll 1
+        for (int c = 64 * half; c < 64 * half + 64; c += 32) {
+          const uint32_t bits_of = all ? 0xffffffffu : c < 64 ? (c < 32 ? seen.w[0] : seen.w[1]) : (c < 96 ? seen.w[2] : seen.w[3]);
+          uint32_t x[32], y[32];
+          tmem_ld32(tmem + lanes + c, x);
+          tmem_ld32(tmem + lanes + 128 + c, y);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 ls = *(const float4*)(bar.lse + c + i), de = *(const float4*)(bar.delta + c + i);
+            const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {lv[k], lv[k + 1]});
+              F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
+              F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {dv[k], dv[k + 1]}));
+              if (!all) {
+                const uint32_t two = bits_of >> (i + k);
+                if (!(two & 1)) pr.x = ds.x = 0.f;
+                if (!(two & 2)) pr.y = ds.y = 0.f;
+              }
+              x[(i + k) / 2] = pack2<T>(pr.x, pr.y);
+              y[(i + k) / 2] = pack2<T>(ds.x, ds.y);
+            }
+          }
+          tmem_st16(tmem + lanes + c, *(const uint32_t(*)[16])x);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *(uint4*)(sds + half * kPanel + staged(r, 2 * (c % 64) + 4 * i)) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        }
+      };
+      if (whole) gradients(Yes());
+      else gradients(No());
+      tmem_wait_st();
+      fence_async_shared();
+      tmem_fence_before();
+      mbar_arrive(&bar.p_full);
+      ok = guard_wait(&bar.acc_full, 0, g, 0x32005);
+      tmem_fence_after();
+    }
+    // dv (first group) or dk, and half of dq's columns; through the space of v, q and d_o
+    auto emit = [&](uint32_t from_col, float scale, uint8_t* to, int col) {
+      uint32_t o[32];
+      tmem_ld32(tmem + lanes + from_col, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 32; k += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack2<T>(__uint_as_float(o[k + 2 * e]) * scale, __uint_as_float(o[k + 2 * e + 1]) * scale);
+        *(uint4*)(to + staged(r, 2 * (col + k))) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    };
+    if (ok) {
+      const float scale = (float)p.scale;
+      uint8_t* to = half ? sq_ : sv_;
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 32) emit(128 + 64 * half + c, half ? scale : 1.f, to, c);
+      emit(32 * half, scale, sg_, 32 * half);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_4d(half ? &l.map.dk : &l.map.dv, to + 32 * quad * 128, 0, h, 32 * quad, b);
+        tma_store_commit();
+      }
+    }
+    mbar_arrive(&bar.out_full);
+    if (ok && half == 0 && guard_wait(&bar.out_full, 0, g, 0x32006) && lane == 0) {
+      tma_store_4d(&l.map.dq, sg_ + 32 * quad * 128, 0, h, 32 * quad, b);
+      tma_store_commit();
+    }
+    if (lane == 0) tma_store_wait_read<0>();
+    tmem_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0) {
+      if (g.gave_up) {   // nothing may land, and no product run, once the CTA is gone
+        mbar_wait_bounded(&bar.kq_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x12001);
+        mbar_wait_bounded(&bar.vo_full, 0, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x12002);
+      }
+      g.gave_up = 0;
+      guard_wait(&bar.acc_full, 0, g, 0x60003);
+    }
+    __syncwarp();
+  }
+  tmem_fence_after();
+  if (warp == 1) tmem_free<1>(tmem, 256);
+}
+
 bool args_ok(const HpAttention* a) {
   return a && a->batch >= 0 && a->batch <= 65535 && a->sq >= 0 && a->sk >= 0 && a->sq <= INT32_MAX / 2 &&
          a->sk <= INT32_MAX / 2 && a->kv_heads >= 1 && a->heads >= 1 && a->heads <= 65535 &&
@@ -963,6 +1163,16 @@ int forward(const HpAttention& a, cudaStream_t s) {
   return a.sq > 2 * kB ? forward_tiles<T, 64, 4, 64>(l, s) : forward_tiles<T, 64, 2>(l, s);
 }
 
+template <typename T>
+int backward_short(const Launch& l, cudaStream_t s) {
+  const auto kernel = attention_backward_short<T>;
+  static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortSmem);
+  if (allowed != cudaSuccess) return allowed;
+  if (l.p.heads * l.p.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
+  kernel<<<(unsigned)(l.p.heads * l.p.batch), 320, kShortSmem, s>>>(l);
+  return cudaGetLastError();
+}
+
 template <typename T, int DP>
 int backward_tiles(const Launch& l, cudaStream_t s) {
   using F = Backward<DP>;
@@ -995,9 +1205,11 @@ int backward(const HpAttention& a, cudaStream_t s) {
       !map(&l.map.v, a.v, true, a.v_b, a.v_s, a.v_h, kB) || !map(&l.map.d_o, a.d_o, false, a.do_b, a.do_s, a.do_h, kB) ||
       !map(&l.map.dq, a.dq, false, a.dq_b, a.dq_s, a.dq_h, 32) || !map(&l.map.dk, a.dk, true, a.dk_b, a.dk_s, a.dk_h, 32) ||
       !map(&l.map.dv, a.dv, true, a.dv_b, a.dv_s, a.dv_h, 32) ||
+      !map(&l.map.o, a.o, false, a.o_b, a.o_s, a.o_h, kB) ||
       !map(&l.map.q64, a.q, false, a.q_b, a.q_s, a.q_h, kPass) || !map(&l.map.k64, a.k, true, a.k_b, a.k_s, a.k_h, kPass) ||
       !map(&l.map.v64, a.v, true, a.v_b, a.v_s, a.v_h, kPass) || !map(&l.map.do64, a.d_o, false, a.do_b, a.do_s, a.do_h, kPass))
     return HP_ERR_BAD_ARG;
+  if (a.dim <= 64 && a.sq <= kB && a.sk <= kB && a.heads == a.kv_heads && a.sq && a.sk) return backward_short<T>(l, s);
   return a.dim <= 64 ? backward_tiles<T, 64>(l, s) : backward_tiles<T, 128>(l, s);
 }
 
