@@ -38,6 +38,8 @@ def main(argv=None):
     ap.add_argument("--seq-len", type=int, default=128)
     ap.add_argument("--lr", type=float, default=0.01)
     ap.add_argument("--fp32", action="store_true", help="no bf16 autocast")
+    ap.add_argument("--fused-layers", action="store_true",
+                    help="BERT models: the package's own layer kernels (no dropout of attention probabilities)")
     ap.add_argument("--checkpoint-dir", default=None)
     ap.add_argument("--resume", action="store_true")
     ap.add_argument("--metrics", default=None, help="JSONL file for per-step metrics")
@@ -57,7 +59,8 @@ def main(argv=None):
     cfg = config_from_args(a)
     job = build_job(a.model, cfg, batch=a.batch_size, seq_len=a.seq_len, lr=a.lr,
                     dtype=torch.float32 if a.fp32 else torch.bfloat16,
-                    model_kwargs={"num_classes": a.num_classes} if a.num_classes else None)
+                    model_kwargs={**({"num_classes": a.num_classes} if a.num_classes else {}),
+                                  **({"fused": True, "attn_dropout": 0.0} if a.fused_layers else {})})
     if a.train_dir and job.kind != "image":
         raise SystemExit("--train-dir is for the image models")
     start_epoch = 0
