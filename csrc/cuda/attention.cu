@@ -200,6 +200,8 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   const int q0 = qt * kB * QT, shift = (int)(p.sk - p.sq);
   const bool masked = p.key_mask != nullptr;
   const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
+  dependents_may_start();
+  wait_for_kernel_before();
   const int sk = !SHORT && masked && p.sk > KB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
   // key tiles of a query tile: up to the last that its last query sees
   auto tiles_of = [&](int t) {
@@ -543,7 +545,9 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
   const int lane = threadIdx.x % LANES;
   const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, h = blockIdx.y, b = blockIdx.z;
   const int64_t rows = padded(a.sq);
+  dependents_may_start();
   if (i >= rows) return;
+  wait_for_kernel_before();
   float s = 0.f, lse = INFINITY;
   if (i < a.sq) {
     if (8 * lane < a.dim) {
@@ -629,6 +633,8 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   const int r0 = tile * kB;           // first row that stays
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const bool masked = mask != nullptr;
+  dependents_may_start();
+  wait_for_kernel_before();
   // tiles that pass: queries from `first` on, of each head of the group in turn; or keys up to the last seen
   int first = 0, count;
   if (keys) {
@@ -938,6 +944,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
+    wait_for_kernel_before();
     mbar_expect_tx(&bar.kq_full, 2 * kPanel);
     tma_load_4d(sk_, &l.map.k, 0, h, 0, b, &bar.kq_full);
     tma_load_4d(sq_, &l.map.q, 0, h, 0, b, &bar.kq_full);
@@ -947,6 +954,8 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     tma_load_4d(sds, &l.map.o, 0, h, 0, b, &bar.vo_full);
   }
   if (warp == 1) tmem_alloc<1>(&bar.tmem, 256);
+  dependents_may_start();
+  wait_for_kernel_before();
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -1149,8 +1158,7 @@ int forward_tiles(Launch& l, cudaStream_t s) {
   if (a.heads * a.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
   const dim3 grid((unsigned)(a.heads * a.batch), (unsigned)((a.sq + kB * QT - 1) / (kB * QT)));
   if (grid.y > 65535) return HP_ERR_TOO_LARGE;
-  kernel<<<grid, F::kThreads, F::kSmem, s>>>(l);
-  return cudaGetLastError();
+  return launch_behind(kernel, grid, F::kThreads, F::kSmem, s, l);
 }
 
 template <typename T>
@@ -1169,8 +1177,7 @@ int backward_short(const Launch& l, cudaStream_t s) {
   static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortSmem);
   if (allowed != cudaSuccess) return allowed;
   if (l.p.heads * l.p.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
-  kernel<<<(unsigned)(l.p.heads * l.p.batch), 320, kShortSmem, s>>>(l);
-  return cudaGetLastError();
+  return launch_behind(kernel, (unsigned)(l.p.heads * l.p.batch), 320, kShortSmem, s, l);
 }
 
 template <typename T, int DP>
@@ -1184,11 +1191,11 @@ int backward_tiles(const Launch& l, cudaStream_t s) {
   if (tiles > INT32_MAX) return HP_ERR_TOO_LARGE;
   if (a.sq) {
     constexpr int kLanes = DP / 8;
-    attention_rows<T, kLanes><<<dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch), 256, 0, s>>>(a);
-    if (const cudaError_t e = cudaGetLastError()) return e;
+    if (const int rc = launch_behind(attention_rows<T, kLanes>, dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch),
+                                     256, 0, s, a))
+      return rc;
   }
-  attention_backward_tiles<T, DP><<<(unsigned)tiles, F::kThreads, F::kSmem, s>>>(l);
-  return cudaGetLastError();
+  return launch_behind(attention_backward_tiles<T, DP>, (unsigned)tiles, F::kThreads, F::kSmem, s, l);
 }
 
 template <typename T>

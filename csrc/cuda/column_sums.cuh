@@ -5,30 +5,13 @@
 
 namespace hipress {
 
-// a launch that may begin before the kernel in front of it has ended (it waits inside)
-__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <typename... Args>
-int launch_behind(void (*kernel)(Args...), dim3 grid, dim3 block, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // part [parts][cols]; the first `split` columns go to `first`, the others to `second` (either
 // may be NULL).  32 columns to a CTA of 32 warps, which share the rows.
 static __global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, int parts, int64_t cols, int64_t split,
                                                                   void* first, void* second, int type) {
   __shared__ float sums[32][33];
   const int64_t col = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  dependents_may_start();
   wait_for_kernel_before();
   float s = 0.f;
   if (col < cols)
@@ -49,7 +32,7 @@ static __global__ void __launch_bounds__(1024) column_sums_kernel(const float* p
 
 inline int column_sums(const float* part, int parts, int64_t cols, int64_t split, void* first, void* second, int type,
                        cudaStream_t s) {
-  return launch_behind(column_sums_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(32, 32), s, part, parts, cols, split,
+  return launch_behind(column_sums_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(32, 32), 0, s, part, parts, cols, split,
                        first, second, type);
 }
 

@@ -284,6 +284,8 @@ __device__ __forceinline__ void start_ring(Ring<T, N, RAGGED>& ring, uint8_t* sp
     guard.status = status;
   }
   __syncthreads();
+  dependents_may_start();
+  wait_for_kernel_before();
   const int group = threadIdx.x / (32 * NW);
   ring.slots = space + group * ring.depth * ring.n * ring.bytes;
   ring.full = full[group];
@@ -429,7 +431,6 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
       for (int j = 0; j < V; ++j) w[j] = held[i][j];
     }
   };
-  dependents_may_start();
   const float inv = 1.f / (float)cols;
   int s = 0, turn = 0;
   float mean_next = first < a.rows ? a.mean[first] : 0.f, rstd_next = first < a.rows ? a.rstd[first] : 0.f;
@@ -605,17 +606,16 @@ template <typename T, int NW, int CH, bool RAGGED>
 int forward_rows(const HpNormForward& a, uint32_t* status, cudaStream_t s) {
   static const int per_sm = prepared(norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
   const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.residual ? 2 : 1, 2, false);
-  norm_forward_rows<T, NW, CH, RAGGED><<<ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>, r.bytes, s>>>(
-      a, r.depth, r.slot, r.ring, status);
-  return cudaGetLastError();
+  return launch_behind(norm_forward_rows<T, NW, CH, RAGGED>, ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>,
+                       r.bytes, s, a, r.depth, r.slot, r.ring, status);
 }
 template <typename T, int NW, int CH, bool RAGGED>
 int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
   static const int per_sm = prepared(norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
   const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.dz ? 3 : 2, 1, true);
   const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
-  norm_backward_rows<T, NW, CH, RAGGED><<<grid, kThreadsOf<NW>, r.bytes, s>>>(a, r.depth, r.slot, r.ring, status);
-  const int rc = cudaGetLastError();
+  const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, r.depth, r.slot,
+                               r.ring, status);
   if (rc || (!a.dweight && !a.dbias)) return rc;
   return column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);
 }

@@ -100,6 +100,27 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
   return s;
 }
 
+// A kernel that may be started while the one in front of it in the stream still runs: its CTAs set
+// up barriers, tensor memory and tensor maps meanwhile, and wait for the end of the one in front
+// (and of what that has waited for) before they touch memory.  Every kernel here calls both.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
 inline bool type_ok(int64_t t) { return t >= HP_F32 && t <= HP_F16; }
 
 }  // namespace hipress

@@ -19,22 +19,24 @@ struct Word<2> { using type = uint16_t; };
 
 // ------------------------------------------------------------------- the product
 // A persistent kernel of specialised warps: one thread fetches tiles (TMA), one issues the
-// matrix products, eight warps empty the accumulators.  Two accumulators in tensor memory: the
+// matrix products, others empty the accumulators.  Two accumulators in tensor memory: the
 // next tile's products run while the last one's results are written.
 //   CG  CTAs that share a tile: 1, or 2 (each holds half of both operands and 128 rows of results)
 //   BN  columns of a tile; it has 128 CG rows
 constexpr int kBK = 64;            // k of a stage: one line of the swizzle
-constexpr int kStaging = 4096;     // a warp has two of 32 rows of 128 bytes
+constexpr int kStaging = 4096;     // a warp's buffer: 32 rows of 128 bytes
 
 template <int CG, int BN>
 struct Shape {
   static constexpr int kRowsB = BN / CG;
   static constexpr int kBytesA = 128 * 128, kBytesB = kRowsB * 128, kStage = kBytesA + kBytesB;
   static constexpr int kStages = kStage <= 24576 ? 6 : 4;
-  // warps that empty an accumulator: each 32 rows of all columns, or of one half of them
-  static constexpr int kEpiWarps = BN >= 128 ? 8 : 4, kCols = BN * 4 / kEpiWarps;
+  // Warps that empty an accumulator, each 32 rows of 64 columns: with 256 columns sixteen, since two
+  // to a scheduler took twice as long over GELU as the products of 1024 k take.  Staging for them:
+  // two buffers each, or one where they are sixteen.
+  static constexpr int kEpiWarps = BN / 16, kCols = 64, kBuffers = kEpiWarps > 8 ? 1 : 2;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
-  static constexpr int kSmem = kStages * kStage + kEpiWarps * (2 * kStaging + kCols * 4) + 512 + 1024;
+  static constexpr int kSmem = kStages * kStage + kEpiWarps * (kBuffers * kStaging + kCols * 4) + 512 + 1024;
   static constexpr int kTmem = 2 * BN;
 };
 
@@ -93,14 +95,15 @@ __device__ __noinline__ void store_ragged(int vec, const uint8_t* s, uint8_t* g,
 }
 
 // Emptied staging rows leave through a tensor map, or by plain stores where y has no 16-byte
-// rows.  Two buffers take turns.
+// rows.  Two buffers take turns, where there are two.
+template <int BUFFERS>
 struct Out {
   uint8_t* base;
   int turn;
   __device__ __forceinline__ uint8_t* buffer() const { return base + turn * kStaging; }
   // before the buffer is filled: what was stored from it has been read
   __device__ __forceinline__ void ready(int lane) const {
-    if (lane == 0) tma_store_wait_read<1>();
+    if (lane == 0) tma_store_wait_read<BUFFERS - 1>();
     __syncwarp();
   }
   __device__ __forceinline__ void send(const Launch& l, const CUtensorMap& map, void* plain, int64_t pitch, int bytes,
@@ -121,7 +124,7 @@ struct Out {
                      rows < 32 ? (int)rows : 32, width < 128 ? (int)width : 128, lane);
       __syncwarp();
     }
-    turn ^= 1;
+    turn = (turn + 1) % BUFFERS;
   }
 };
 
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + S::kStages * S::kStage;
-  float* biases = (float*)(staging + S::kEpiWarps * 2 * kStaging);   // [kEpiWarps][kCols]
+  float* biases = (float*)(staging + S::kEpiWarps * S::kBuffers * kStaging);   // [kEpiWarps][kCols]
   Bars& bar = *(Bars*)(biases + S::kEpiWarps * S::kCols);
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
@@ -190,6 +193,8 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
   if (CG == 2) cluster_sync();   // the other CTA's barriers are there
   tmem_fence_after();
   const uint32_t tmem = uniform(bar.tmem);
+  dependents_may_start();
+  wait_for_kernel_before();
   Guard& g = bar.guard;
   const int units = l.tiles_m * l.tiles_n * l.splits, step = gridDim.x / CG, first = blockIdx.x / CG;
 
@@ -271,7 +276,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::kThreads, 1) product_kernel(con
     const int e = warp - 2, quad = warp & 3, half = e >> 2;
     const int base = half * S::kCols;          // this warp's columns of a tile
     const bool raw = l.splits > 1 || p.ytype == HP_F32;   // the sums as they are, in 32 bits
-    Out out = {staging + e * 2 * kStaging, 0};
+    Out<S::kBuffers> out = {staging + e * S::kBuffers * kStaging, 0};
     int it = 0;
     for (int u = first; u < units; u += step, ++it) {
       const Unit w = unit_of(l, u, 128 * CG, BN);
@@ -386,6 +391,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Launch l) {
   const HpProduct& p = l.p;
   const int64_t quads = l.ldp / 4, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  dependents_may_start();
+  wait_for_kernel_before();
   if (at >= p.m * quads) return;
   const int64_t m = at / quads, n = at % quads * 4;
   float v[4] = {};
@@ -470,12 +477,14 @@ int run_product(Launch& l, int sms, cudaStream_t s) {
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = CG;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, product_kernel<T, CG, BN>, l);
 }
 
@@ -510,8 +519,7 @@ int product(const HpProduct& a, cudaStream_t s) {
   }
   const int64_t quads = a.m * (l.ldp / 4);
   if (quads > (int64_t)INT32_MAX * 128) return HP_ERR_TOO_LARGE;
-  finish_kernel<T><<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(l);
-  return cudaGetLastError();
+  return launch_behind(finish_kernel<T>, (unsigned)((quads + 255) / 256), 256, 0, s, l);
 }
 
 // --------------------------------------------------- the gradient before the activation
@@ -528,6 +536,7 @@ __global__ void __launch_bounds__(32 * kSlopeWarps) slope_kernel(const __grid_co
   const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V, step = (int64_t)gridDim.y * kSlopeWarps;
   float s[V] = {};
   dependents_may_start();
+  wait_for_kernel_before();
   auto put = [&](int64_t row, Raw dy, Raw pre) {
     T* d = (T*)&dy;
     const T* q = (const T*)&pre;
@@ -594,8 +603,7 @@ int slopes(const HpSlope& a, cudaStream_t s) {
   if (high > most) high = most;
   if (high > kSlopeParts) high = kSlopeParts;
   if (high < 1) high = 1;
-  slope_kernel<T, ACT, V><<<dim3((unsigned)wide, (unsigned)high), 32 * kSlopeWarps, 0, s>>>(a);
-  int rc = cudaGetLastError();
+  const int rc = launch_behind(slope_kernel<T, ACT, V>, dim3((unsigned)wide, (unsigned)high), 32 * kSlopeWarps, 0, s, a);
   if (rc || !a.dbias) return rc;
   return column_sums((const float*)a.workspace, (int)high, a.cols, a.cols, a.dbias, nullptr, (int)a.btype, s);
 }
