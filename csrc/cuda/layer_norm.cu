@@ -363,10 +363,18 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
       float v[V];
       forget(raw[i]);
       unpack<T>(raw[i], v);
+      if (c[i].whole(cols)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[j] - mean;
-        if (c[i].has(j, cols)) sum[0] = fmaf(d, d, sum[0]);
+        for (int j = 0; j < V; ++j) {
+          const float d = v[j] - mean;
+          sum[0] = fmaf(d, d, sum[0]);
+        }
+      } else if (RAGGED && c[i].first < cols) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float d = v[j] - mean;
+          if (c[i].has(j, cols)) sum[0] = fmaf(d, d, sum[0]);
+        }
       }
     }
     row_sums<NW>(sum, part[1], warp);

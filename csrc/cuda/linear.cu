@@ -417,12 +417,16 @@ struct Choice {
   int cg, bn, splits;
 };
 
-// Which kernel, and into how many parts k is split: the least of an estimate in SM cycles.
+// Which kernel, and into how many parts k is split: the least of an estimate in SM cycles.  Pairs
+// of CTAs with 256 columns are the fastest where there are tiles enough (4096 x 4096 x 1024: 41 us,
+// against 43, 45 and 66 with 256 x 128, 128 x 128 and 128 x 64); the small tiles where few would
+// leave SMs idle (1024 x 1024 x 4096: 35, 25, 29, 23), and parts of k where even those do (512 x
+// 512 x 32768: 128 x 64 alone 116, in four parts 46; in eight with 256 x 128 40).
 Choice choose(int64_t m, int64_t n, int64_t kblocks, int sms) {
   const struct {
     int cg, bn;
     double stage;   // cycles of 64 k
-  } kinds[] = {{2, 256, 540}, {2, 128, 290}, {1, 128, 300}, {1, 64, 215}};
+  } kinds[] = {{2, 256, 540}, {2, 128, 340}, {1, 128, 350}, {1, 64, 240}};
   Choice best = {1, 128, 1};
   double least = 1e30;
   for (const auto& c : kinds) {
@@ -431,7 +435,7 @@ Choice choose(int64_t m, int64_t n, int64_t kblocks, int sms) {
       const int64_t rounds = (tiles * s + slots - 1) / slots;
       const int64_t per = (kblocks + s - 1) / s;
       double t = rounds * (per * c.stage + 300.0) + 3000.0 + c.bn * 10.0;
-      if (s > 1) t += 5000.0 + (double)m * n * (2 * s) * 4 / 3000.0;   // the partial sums, and one more launch
+      if (s > 1) t += 4000.0 + (double)m * n * (2 * s) * 4 / 3000.0;   // the partial sums, and one more launch
       if (t < least) least = t, best = {c.cg, c.bn, (int)s};
     }
   }
