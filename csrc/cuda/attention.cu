@@ -535,20 +535,31 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
 }
 
 // --------------------------------------------------------------------- backward
-// The logarithm of the softmax sums to base 2, and rows of d_o against rows of o (delta); both
-// negative, in tiles of 128 rows, [batch, heads, 2, rows rounded up].  Behind the last row, and
-// where a row saw nothing: minus infinity, so that every probability comes out as zero.
+// What the backward pass wants of every query: the logarithm of its softmax sum to base 2, and its
+// row of d_o against its row of o (delta); both negative.  [batch, heads] blocks of kRowWords words
+// for each row, rows rounded up to 128: all lse, all delta, then for products (see below) tiles of
+// 64 rows, first -lse / c of each row in three parts that add up to it and have 11 bits each, then
+// -delta likewise.  Behind the last row, and where a row saw nothing, lse is so large that every
+// probability comes out as zero.
+constexpr int kRowWords = 10, kPass = 64;
+constexpr float kNever = 1e35f;
 __host__ __device__ __forceinline__ int64_t padded(int64_t rows) { return (rows + kB - 1) / kB * kB; }
 
+__device__ __forceinline__ float4 three_parts(float v) {
+  auto upper = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); };
+  const float hi = upper(v), mid = upper(v - hi), lo = upper(v - hi - mid);
+  return make_float4(hi, mid, lo, 0.f);
+}
+
 template <typename T, int LANES>   // that share a row, 16 bytes each
-__global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ HpAttention a) {
+__global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ HpAttention a, float c) {
   const int lane = threadIdx.x % LANES;
   const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, h = blockIdx.y, b = blockIdx.z;
   const int64_t rows = padded(a.sq);
   dependents_may_start();
   if (i >= rows) return;
   wait_for_kernel_before();
-  float s = 0.f, lse = INFINITY;
+  float s = 0.f, lse = -INFINITY;
   if (i < a.sq) {
     if (8 * lane < a.dim) {
       float o[8], g[8];
@@ -562,9 +573,13 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
 #pragma unroll
   for (int k = LANES / 2; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
   if (lane == 0) {
-    float* out = a.delta + (b * a.heads + h) * 2 * rows + i;
-    out[0] = lse == -INFINITY ? -INFINITY : -lse;
-    out[rows] = -s;
+    float* out = a.delta + (b * a.heads + h) * kRowWords * rows;
+    float4* parts = (float4*)(out + 2 * rows) + i / kPass * 2 * kPass + i % kPass;
+    const bool none = lse == -INFINITY;
+    out[i] = none ? -kNever : -lse;
+    out[rows + i] = -s;
+    parts[0] = none ? make_float4(-kNever, 0.f, 0.f, 0.f) : three_parts(-lse / c);
+    parts[kPass] = three_parts(-s);
   }
 }
 
@@ -577,9 +592,11 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
 // P and dS go back to tensor memory over S, as the left operands.  Two groups of four warps, a row
 // to a thread, take the tiles by turns, so that what one waits for (fetch, store, products) goes on
 // behind the other's 2^x: with tiles of 128 that both groups shared, 2600 cycles passed for each
-// where its products take 1000.  Tensor memory holds S and dP of three tiles, or of two where the
+// where its products take 1000.  With keys, lse and delta go by the column: read from shared memory,
+// a value for each element, they took half of the rows' time (and of the memory that the products
+// read).  One more product for each of S and dP adds them: ones, three for each row, by the three
+// parts of -lse / c and -delta.  Tensor memory holds S and dP of three tiles, or of two where the
 // results of keys with more than 64 dimensions take half of it.
-constexpr int kPass = 64;
 template <int DP>
 struct Backward {
   static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kPassed = kPanels * kPass * 128;   // bytes
@@ -587,7 +604,8 @@ struct Backward {
   // four warps that fetch and issue, eight for the rows; the former give registers to the latter
   static constexpr int kThreads = 128 + 256, kAtStart = 168, kFew = 72, kMany = 216;
   static_assert(kFew + 2 * kMany <= 3 * kAtStart, "more registers than the CTA has");
-  static constexpr int kSmem = 2 * kTile + kStages * (2 * kPassed + 8 * kPass) + 1024 + 1024;
+  static constexpr int kOnes = 2 * kB * 16, kParts = 2 * kPass * 16;   // bytes: [2][128 rows][4], a stage's [2][64][4]
+  static constexpr int kSmem = 2 * kTile + kStages * (2 * kPassed + kParts) + 2 * kOnes + 1024 + 1024;
   // columns: tile j's S (later P, dS) at kBuffer times its buffer, dP kPass further on; the results
   static constexpr uint32_t kBuffer = 2 * kPass, kAcc1 = DP == 64 ? 384 : 256, kAcc2 = DP == 64 ? 448 : 384;
 };
@@ -606,8 +624,9 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* stay = smem;
   uint8_t* pass = smem + 2 * F::kTile;
-  float* rows_of = (float*)(pass + F::kStages * 2 * F::kPassed);   // a stage's lse and delta
-  BackwardBars& bar = *(BackwardBars*)(rows_of + F::kStages * 2 * kPass);
+  uint8_t* parts = pass + F::kStages * 2 * F::kPassed;   // a stage's -lse / c and -delta
+  uint8_t* ones = parts + F::kStages * F::kParts;        // for the former, for the latter
+  BackwardBars& bar = *(BackwardBars*)(ones + 2 * F::kOnes);
   const HpAttention& p = l.p;
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int nq = (int)((p.sq + kB - 1) / kB), nk = (int)((p.sk + kB - 1) / kB), group = (int)(p.heads / p.kv_heads);
@@ -659,6 +678,12 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     bar.guard.status = l.status;
   }
   if (warp == 1) tmem_alloc<1>(&bar.tmem, 512);
+  if (keys)   // [which][four k][row]: three ones where the parts are that it adds
+    for (int i = threadIdx.x; i < 4 * kB; i += blockDim.x) {
+      const float one = i / (2 * kB) == i / kB % 2 ? 1.f : 0.f;
+      ((float4*)ones)[i] = make_float4(one, one, one, 0.f);
+    }
+  fence_async_shared();
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
@@ -668,7 +693,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   if (warp < 4) {
     fewer_registers<F::kFew>();
     if (warp == 0) {
-      const uint32_t bytes = 2 * F::kPassed + (keys ? 8 * kPass : 0);
+      const uint32_t bytes = 2 * F::kPassed + (keys ? F::kParts : 0);
       const int64_t rows = padded(p.sq);
       int waits = 0;
       if (lane == 0 && n) {
@@ -689,11 +714,9 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
             tma_load_4d(to + i * kPass * 128, keys ? &l.map.q64 : &l.map.k64, 64 * i, h, at * kPass, b, &bar.in_full[s]);
             tma_load_4d(to + F::kPassed + i * kPass * 128, keys ? &l.map.do64 : &l.map.v64, 64 * i, h, at * kPass, b, &bar.in_full[s]);
           }
-          if (keys) {
-            const float* from = p.delta + (b * p.heads + h) * 2 * rows + at * kPass;
-            bulk_load(rows_of + s * 2 * kPass, from, 4 * kPass, &bar.in_full[s]);
-            bulk_load(rows_of + s * 2 * kPass + kPass, from + rows, 4 * kPass, &bar.in_full[s]);
-          }
+          if (keys)
+            bulk_load(parts + s * F::kParts, p.delta + (b * p.heads + h) * kRowWords * rows + 2 * rows + at * (F::kParts / 4), F::kParts,
+                      &bar.in_full[s]);
         }
         if (!keys && masked) {
           const Seen<kPass> m = mask_bits<kPass>(mask, (int64_t)j * kPass, sk);
@@ -741,6 +764,12 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
             const uint32_t d = tmem + F::kBuffer * q;
             wide(d, a, in(s), id_s);
             wide(d + kPass, a + F::kTile, in(s) + F::kPassed, id_dp);
+            if (keys) {
+              const uint64_t rows = mma_desc_plain(smem_u32(parts + s * F::kParts), kPass * 16, 128);
+              const uint64_t one = mma_desc_plain(smem_u32(ones), kB * 16, 128);
+              mma_tf32(leader, d, one, rows, mma_idesc_tf32(128, kPass), true);
+              mma_tf32(leader, d + kPass, one + F::kOnes / 16, rows, mma_idesc_tf32(128, kPass), true);
+            }
             mma_commit<1>(leader, &bar.s_full[turn]);
             if (++s == F::kStages) s = 0, ph ^= 1;
             if (++q == buffers) q = 0, round ^= 1;
@@ -766,12 +795,12 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     more_registers<F::kMany>();
     const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane, row = r0 + r;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-    float lse = -INFINITY, delta = 0.f;   // of a query that stays, negative
-    bool mine = true;                     // a key that stays is seen at all
+    float lse = 0.f, delta = 0.f;   // of a query that stays, negative
+    bool mine = true;               // a key that stays is seen at all
     if (keys) {
       mine = row < sk && (!masked || mask[row]);
     } else {
-      const float* from = p.delta + (b * p.heads + head) * 2 * padded(p.sq) + row;
+      const float* from = p.delta + (b * p.heads + head) * kRowWords * padded(p.sq) + row;
       lse = from[0], delta = from[padded(p.sq)];
     }
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;
@@ -815,9 +844,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         }
       }
       if (!guard_wait(&bar.s_full[turn], (j / turns) & 1, g, 0x31003)) { ok = false; break; }
-      if (keys && !guard_wait(&bar.in_full[s], ph, g, 0x31005)) { ok = false; break; }
       tmem_fence_after();
-      const float* cols = rows_of + s * 2 * kPass;
       const uint32_t at = tmem + lanes + F::kBuffer * q;
       uint32_t x[kPass], y[kPass];
 #pragma unroll
@@ -828,25 +855,18 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
       tmem_wait_ld();
       auto gradients = [&](auto all, auto of_keys) {   // packed P into x, dS into y
 #pragma unroll
-        for (int i = 0; i < kPass; i += 4) {
-          float ls[4] = {lse, lse, lse, lse}, de[4] = {delta, delta, delta, delta};   // negative both
-          if (of_keys) {
-            *(float4*)ls = *(const float4*)(cols + i);
-            *(float4*)de = *(const float4*)(cols + kPass + i);
+        for (int i = 0; i < kPass; i += 2) {
+          const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])}, u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
+          const F2 z = of_keys ? mul2(v, {l.c, l.c}) : fma2(v, {l.c, l.c}, {lse, lse});
+          F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
+          F2 ds = mul2(pr, of_keys ? u : add2(u, {delta, delta}));
+          if (!all) {
+            const uint32_t two = seen.w[i / 32] >> (i % 32);
+            if (!(two & 1)) pr.x = ds.x = 0.f;
+            if (!(two & 2)) pr.y = ds.y = 0.f;
           }
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {ls[k], ls[k + 1]});
-            F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-            F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {de[k], de[k + 1]}));
-            if (!all) {
-              const uint32_t two = seen.w[i / 32] >> (i % 32 + k);
-              if (!(two & 1)) pr.x = ds.x = 0.f;
-              if (!(two & 2)) pr.y = ds.y = 0.f;
-            }
-            if (of_keys) x[(i + k) / 2] = pack2<T>(pr.x, pr.y);
-            y[(i + k) / 2] = pack2<T>(ds.x, ds.y);
-          }
+          if (of_keys) x[i / 2] = pack2<T>(pr.x, pr.y);
+          y[i / 2] = pack2<T>(ds.x, ds.y);
         }
       };
       if (keys) {
@@ -1138,7 +1158,9 @@ int prepare(Launch& l, const HpAttention& a) {
   int rc;
   l.status = layer_status(&rc);
   l.p = a;
+  // Without any scale every score counts as much: a small one does the same, and can be divided by.
   l.c = (float)(a.scale < 0 ? -a.scale : a.scale) * kLog2e;
+  if (l.c < 1e-20f) l.c = 1e-20f;
   l.negative = a.scale < 0;
   return rc;
 }
@@ -1192,7 +1214,7 @@ int backward_tiles(const Launch& l, cudaStream_t s) {
   if (a.sq) {
     constexpr int kLanes = DP / 8;
     if (const int rc = launch_behind(attention_rows<T, kLanes>, dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch),
-                                     256, 0, s, a))
+                                     256, 0, s, a, l.c))
       return rc;
   }
   return launch_behind(attention_backward_tiles<T, DP>, (unsigned)tiles, F::kThreads, F::kSmem, s, l);

@@ -207,6 +207,11 @@ __device__ __forceinline__ uint64_t mma_desc(uint32_t a, uint32_t lead, uint32_t
   return (uint64_t)((a & 0x3FFFF) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 |
          2ull << 61;
 }
+// The same for a tile without swizzle, K-major: blocks of 8 rows by 16 bytes; `lead` is the distance
+// of blocks along k, `stride` along the rows.
+__device__ __forceinline__ uint64_t mma_desc_plain(uint32_t a, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((a & 0x3FFFF) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46;
+}
 // instruction descriptor: fp32 accumulators, both operands of `type`
 __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool bf16, bool a_kmajor, bool b_kmajor) {
   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_kmajor ? 0u : 1u << 15) | (b_kmajor ? 0u : 1u << 16) |
@@ -215,6 +220,17 @@ __host__ __device__ constexpr uint32_t mma_idesc(int m, int n, bool bf16, bool a
 // Matrix products are issued by one thread of a warp, but all its threads go through the code, and
 // `leader` (elect_one()) says which of them does it: in a branch of one thread the compiler cannot
 // keep descriptors in uniform registers, and moving them there took 90 cycles for each product.
+__host__ __device__ constexpr uint32_t mma_idesc_tf32(int m, int n) {
+  return 1u << 4 | 2u << 7 | 2u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+// eight k of 32-bit operands, of which the upper 19 bits count
+__device__ __forceinline__ void mma_tf32(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(leader)
+      : "memory");
+}
 template <int CG>
 __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   if (CG == 1)

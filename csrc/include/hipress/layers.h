@@ -103,7 +103,7 @@ typedef struct {
   const uint8_t* key_mask;  // [batch, sk], nonzero: may be seen; or NULL
   const void* d_o;
   void *dq, *dk, *dv;
-  float* delta;             // backward: workspace, [batch, heads, 2, sq rounded up to 128]
+  float* delta;             // backward: workspace, [batch, heads, 10, sq rounded up to 128]
   int64_t batch, sq, sk, heads, kv_heads, dim;
   int64_t q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, o_b, o_s, o_h, do_b, do_s, do_h;
   int64_t dq_b, dq_s, dq_h, dk_b, dk_s, dk_h, dv_b, dv_s, dv_h;

@@ -277,7 +277,7 @@ std::pair<Tensor, Tensor> attention_forward(const Tensor& q0, const Tensor& k0, 
 void attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& o, const Tensor& lse, const Tensor& do0,
                         const Tensor& mask0, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
   const Tensor q = tileable(q0), k = tileable(k0), v = tileable(v0), d_o = tileable(do0), mask = mask_rows(mask0);
-  const Tensor delta = at::empty({q.size(0), q.size(2), 2, (q.size(1) + 127) / 128 * 128}, q.options().dtype(at::kFloat));
+  const Tensor delta = at::empty({q.size(0), q.size(2), 10, (q.size(1) + 127) / 128 * 128}, q.options().dtype(at::kFloat));
   HpAttention a = block(q, k, v, o, lse, mask, causal, scale);
   a.d_o = ptr(d_o), a.dq = ptr(dq), a.dk = ptr(dk), a.dv = ptr(dv), a.delta = (float*)ptr(delta);
   put(d_o, a.do_b, a.do_s, a.do_h), put(dq, a.dq_b, a.dq_s, a.dq_h), put(dk, a.dk_b, a.dk_s, a.dk_h), put(dv, a.dv_b, a.dv_s, a.dv_h);
