@@ -43,29 +43,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 2^x by the multipliers, for a part of the values: 2^x proper is 16 a cycle and SM, and by itself
-// takes longer than all the rest.  x = n + f with |f| <= 1/2; 2^f by the polynomial of the fourth
-// degree whose greatest relative error there is least, 2.6e-6 (a Remez-like fit; 16-bit
-// probabilities are rounded by 2^-9 or 2^-12); n goes into the exponent.  Below 2^-126 it stays there.
-__device__ __forceinline__ float at_least(float x, float low) {   // NaN stays
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(low));
-  return d;
-}
-__device__ __forceinline__ F2 exp2_multiplied(F2 x) {
-  x = {at_least(x.x, -126.f), at_least(x.y, -126.f)};
-  constexpr float kRound = 12582912.f;   // 1.5 2^23: added, the integer is in the lowest bits
-  const F2 r = add2(x, {kRound, kRound}), f = fma2(add2(r, {-kRound, -kRound}), {-1.f, -1.f}, x);
-  F2 p = fma2(f, {0.00957003638f, 0.00957003638f}, {0.0559177165f, 0.0559177165f});
-  p = fma2(f, p, {0.24024745f, 0.24024745f});
-  p = fma2(f, p, {0.693121833f, 0.693121833f});
-  p = fma2(f, p, {0.999999262f, 0.999999262f});
-  return {__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
-          __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23))};
-}
-
-constexpr int kMultiplied = 0;   // of eight pairs
-
 struct Yes {
   __device__ constexpr operator bool() const { return true; }
 };
@@ -148,11 +125,10 @@ struct Launch {
 // scores, O += P v.  While some tiles' rows are at work the others' products run.  The sums keep a
 // running maximum; the results so far are scaled anew only when it rises by more than 2^8 (the
 // factor that 32-bit sums and 16-bit probabilities bear easily).  Bound: 2^x, 16 a cycle and SM.
-//   <64, 4, 64>    up to 64 dimensions, long: what one row does between its 2^x (fetch, maximum,
-//                  store, wait) takes as long as they do; four tiles in flight hide it, two of
-//                  128 keys did everything at the same time
-//   <64, 2, 128>, <128, 2, 128>, <., 1, 128>   fewer queries, or wider heads, whose results fill
-//                  tensor memory
+//   <., 1, 128>    two CTAs an SM for up to 64 dimensions, one for more
+//   <64, 4, 64>, <128, 2, 128>   many queries: what one row does between its 2^x (fetch, maximum,
+//                  store, wait) takes as long as they do; four tiles, or two of the wider heads whose
+//                  results fill tensor memory, hide it and share the keys they fetch
 //   SHORT          up to 128 queries and keys: one tile each, nothing to walk over.  Results take the
 //                  half of the scores' columns that the probabilities leave, so that four CTAs fit
 //                  an SM and hide one another's latency
@@ -161,7 +137,7 @@ struct Forward {
   static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kKeys = kPanels * KB * 128;   // bytes
   // warps that issue products, each for its own tiles: a product of 64 keys takes as long to issue as to run
   static constexpr int kIssue = QT > 1 ? 2 : 1;
-  static constexpr int kStages = SHORT ? 1 : KB == 64 ? 6 : DP == 64 && QT == 2 ? 4 : 2;
+  static constexpr int kStages = SHORT ? 1 : KB == 64 ? 6 : 2;
   // four warps that fetch and issue, four for each tile's rows; the former give registers to the latter
   static constexpr int kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
   static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : QT == 2 ? 168 : 96;
@@ -463,7 +439,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
 #pragma unroll
           for (int i = 0; i < kStep; i += 2) {
             const F2 z = fma2({__uint_as_float(x[(c + i) % kHeld]), __uint_as_float(x[(c + i + 1) % kHeld])}, {l.c, l.c}, {base, base});
-            F2 e = all && KB == 64 && i / 2 % 8 < kMultiplied ? exp2_multiplied(z) : F2{exp2_fast(z.x), exp2_fast(z.y)};
+            F2 e = {exp2_fast(z.x), exp2_fast(z.y)};
             if (!all) {
               const uint32_t two = seen.w[c / 32] >> (c % 32 + i);
               e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
@@ -670,9 +646,9 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   if (threadIdx.x == 0) {
     mbar_init(&bar.stay_full, 1);
     for (int i = 0; i < F::kStages; ++i) mbar_init(&bar.in_full[i], 1), mbar_init(&bar.in_empty[i], 1), mbar_init(&bar.mask_full[i], 1);
-    for (int i = 0; i < 6; ++i) mbar_init(&bar.s_full[i], 1);
+    for (int i = 0; i < 6; ++i) mbar_init(&bar.s_full[i], 2);
     for (int i = 0; i < 3; ++i) mbar_init(&bar.s_free[i], 1), mbar_init(&bar.p_full[i], 128);
-    mbar_init(&bar.acc_full, 2);
+    mbar_init(&bar.acc_full, 3);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
@@ -732,8 +708,8 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         for (int j = max(0, waits - F::kStages); j < waits; ++j)
           mbar_wait_bounded(&bar.in_full[j % F::kStages], (j / F::kStages) & 1, kWaitNs, g.status, HP_STATUS_TIMEOUT | 0x11003);
       }
-    } else if (warp <= 2) {
-      // one warp issues S and dP, the other the results: each product takes as long to issue as to run
+    } else {
+      // one warp issues S, one dP, one the results: each product takes as long to issue as to run, and more
       if (n) {
         const uint32_t leader = elect_one();
         const bool bf = p.type == HP_BF16;
@@ -754,22 +730,19 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         int s = 0, q = 0, turn = 0;
         uint32_t ph = 0, round = 0;   // of the stages, of the buffers
         bool ok = true;
-        if (warp == 1) {
-          const uint32_t a = smem_u32(stay);
+        if (warp != 2) {
+          const bool of_dp = warp == 3;
+          const uint32_t a = smem_u32(stay) + (of_dp ? F::kTile : 0), id_w = of_dp ? id_dp : id_s;
           ok = warp_wait(&bar.stay_full, 0, g, 0x21002);
           for (int j = 0; j < n && ok; ++j) {
             ok = warp_wait(&bar.in_full[s], ph, g, 0x21001) && warp_wait(&bar.s_free[q], round ^ 1, g, 0x21005);
             if (!ok) break;
             tmem_fence_after();
-            const uint32_t d = tmem + F::kBuffer * q;
-            wide(d, a, in(s), id_s);
-            wide(d + kPass, a + F::kTile, in(s) + F::kPassed, id_dp);
-            if (keys) {
-              const uint64_t rows = mma_desc_plain(smem_u32(parts + s * F::kParts), kPass * 16, 128);
-              const uint64_t one = mma_desc_plain(smem_u32(ones), kB * 16, 128);
-              mma_tf32(leader, d, one, rows, mma_idesc_tf32(128, kPass), true);
-              mma_tf32(leader, d + kPass, one + F::kOnes / 16, rows, mma_idesc_tf32(128, kPass), true);
-            }
+            const uint32_t d = tmem + F::kBuffer * q + (of_dp ? kPass : 0);
+            wide(d, a, in(s) + (of_dp ? F::kPassed : 0), id_w);
+            if (keys)
+              mma_tf32(leader, d, mma_desc_plain(smem_u32(ones) + (of_dp ? F::kOnes : 0), kB * 16, 128),
+                       mma_desc_plain(smem_u32(parts + s * F::kParts), kPass * 16, 128), mma_idesc_tf32(128, kPass), true);
             mma_commit<1>(leader, &bar.s_full[turn]);
             if (++s == F::kStages) s = 0, ph ^= 1;
             if (++q == buffers) q = 0, round ^= 1;
@@ -805,13 +778,22 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     }
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;
     bool ok = true;
-    for (int j = half; j < n; j += 2) {
-      const int s = j % F::kStages, q = j % buffers, turn = j % turns;
-      const uint32_t ph = (j / F::kStages) & 1;
+    // of tile j: stage, buffer, turn, and place among its head's tiles
+    int s = half, q = half, turn = half, place = half;
+    uint32_t ph = 0, round = 0;
+    auto advance = [&] {
+      s += 2, q += 2, turn += 2, place += 2;
+      if (s >= F::kStages) s -= F::kStages, ph ^= 1;
+      if (q >= buffers) q -= buffers;
+      if (turn >= turns) turn -= turns, round ^= 1;
+      while (place >= count) place -= count;
+    };
+    if (n && place >= count) place -= count;   // a head of one tile
+    for (int j = half; j < n; j += 2, advance()) {
       Seen<kPass> seen;
       bool whole;
       if (keys) {
-        const int from = p.causal ? row - shift - (first + j % count) * kPass : 0;   // its first query in this tile
+        const int from = p.causal ? row - shift - (first + place) * kPass : 0;   // its first query in this tile
         whole = mine && from <= 0;
         if (!__all_sync(0xffffffffu, whole)) {
           seen = seen_between<kPass>(mine ? from : kPass, kPass);
@@ -843,7 +825,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
           whole = false;
         }
       }
-      if (!guard_wait(&bar.s_full[turn], (j / turns) & 1, g, 0x31003)) { ok = false; break; }
+      if (!guard_wait(&bar.s_full[turn], round, g, 0x31003)) { ok = false; break; }
       tmem_fence_after();
       const uint32_t at = tmem + lanes + F::kBuffer * q;
       uint32_t x[kPass], y[kPass];
@@ -1187,10 +1169,17 @@ template <typename T>
 int forward(const HpAttention& a, cudaStream_t s) {
   Launch l;
   if (const int rc = prepare(l, a)) return rc;
-  const bool two = a.sq > kB;
-  if (a.dim > 64) return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
-  if (!two) return a.sk <= kB ? forward_tiles<T, 64, 1, kB, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
-  return a.sq > 2 * kB ? forward_tiles<T, 64, 4, 64>(l, s) : forward_tiles<T, 64, 2>(l, s);
+  // Several tiles of queries in a CTA pay once there are more tiles than the SMs hold of them one by
+  // one; before that they leave SMs without work.  One tile a CTA against several, in us, bfloat16:
+  //   64 dimensions    1 x 1024, 8 heads: 16 to 32    1 x 8192, 4 heads, causal: 90 to 205
+  //                    64 x 300, 16 heads: 106 to 95  1 x 4096, 16 heads: 116 to 108   8 x 200, 16 heads: 9.8 to 11
+  //   128 dimensions   1 x 1024, 8 heads: 20 to 26    1 x 4096, 4 heads, causal: 62 to 69
+  //                    4 x 512, 16 heads: 24 to 18    1 x 4096, 16 heads, causal: 120 to 77
+  const int64_t tiles = (a.sq + kB - 1) / kB * a.heads * a.batch;
+  if (a.dim > 64)
+    return a.sq > kB && tiles > layer_sms() ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
+  if (a.sq > 2 * kB && tiles > 2 * layer_sms()) return forward_tiles<T, 64, 4, 64>(l, s);
+  return a.sq <= kB && a.sk <= kB ? forward_tiles<T, 64, 1, kB, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
 }
 
 template <typename T>

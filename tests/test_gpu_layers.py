@@ -260,6 +260,33 @@ def test_attention_masked_keys_hold_anything(dtype, value):
     check_attention(q, k, v, do, mask=mask, causal=True)
 
 
+# more tiles of queries than the SMs hold one by one
+MANY = [(8, 300, 70, 16, 16, 40), (5, 257, 400, 24, 8, 64), (3, 700, 700, 20, 20, 64), (1, 400, 1, 80, 1, 8),
+        (2, 520, 129, 16, 16, 128), (3, 130, 300, 32, 8, 72)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("masked", [None, "lengths", "holes"])
+@pytest.mark.parametrize("shape", MANY)
+def test_attention_many_queries(dtype, causal, masked, shape):
+    test_attention(dtype, causal, masked, shape)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -65504.0])
+def test_attention_many_queries_masked_keys_hold_anything(dim, value):
+    torch.manual_seed(12)
+    b, s, h = 3, 290, 40
+    q, do, k, v = (rand(b, s, h, dim, dtype=BF16) for _ in range(4))
+    mask = torch.rand(b, s, device="cuda") < 0.7
+    mask[1, 64:] = False
+    mask[2] = False
+    k[~mask], v[~mask] = value, value
+    check_attention(q, k, v, do, mask=mask)
+    check_attention(q, k, v, do, mask=mask, causal=True, scale=-0.2)
+
+
 def test_attention_strides():
     torch.manual_seed(6)
     b, s, h, d = 2, 150, 4, 64
