@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const __grid_constant__ Hp
 // the same: the pieces start `phase` elements ahead of the row, and what is outside the row is
 // cleared.  The phase goes by the row modulo the elements of a piece, and the rows of one group
 // of warps are a multiple of eight apart, so that its columns stay the same.  The first and the
-// last row have no neighbour to be read along with them and are loaded element by element.
+// last row have no neighbour to be read along with them: their ends are loaded element by element.
 template <typename T, bool RAGGED>
 struct Piece {
   static constexpr int V = kPiece<T>, kBits = 8 * sizeof(T);
@@ -116,26 +116,20 @@ struct Piece {
     if (first >= cols) return raw;
     raw = *(const uint4*)(slot + (first + phase) * (int)sizeof(T));
     if (RAGGED && !whole(cols)) {
-      T* v = (T*)&raw;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (!has(j, cols)) v[j] = from_f<T>(0.f);
+      // a row is at least a piece long: it either begins or ends in this one
+      const int cut = kBits * (first < 0 ? -first : V + first - cols);   // bits to clear, 0 < cut < 128
+      const uint64_t all = ~(uint64_t)0;
+      uint64_t lo = raw.x | (uint64_t)raw.y << 32, hi = raw.z | (uint64_t)raw.w << 32;
+      if (first < 0) {
+        lo &= cut < 64 ? all << cut : 0;
+        if (cut > 64) hi &= all << (cut - 64);
+      } else {
+        hi &= cut < 64 ? all >> cut : 0;
+        if (cut > 64) lo &= all >> (cut - 64);
+      }
+      raw = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
     }
     return raw;
-  }
-  // the same element by element, shifted through 128 bits: few registers for what is rare
-  __device__ __forceinline__ uint4 take_from(const T* row, int cols) const {
-    uint64_t lo = 0, hi = 0;
-    if (first < cols)
-#pragma unroll 1
-      for (int j = 0; j < V; ++j) {
-        T e = from_f<T>(0.f);
-        if (has(j, cols)) e = row[first + j];
-        const uint64_t bits = sizeof(T) == 4 ? *(const uint32_t*)&e : *(const uint16_t*)&e;
-        lo = lo >> kBits | hi << (64 - kBits);
-        hi = hi >> kBits | bits << (64 - kBits);
-      }
-    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
   __device__ __forceinline__ void store(T* row, int cols, uint4 raw) const {
     if (whole(cols)) {
@@ -143,24 +137,40 @@ struct Piece {
       return;
     }
     if (!RAGGED || first >= cols) return;
-    uint64_t lo = raw.x | (uint64_t)raw.y << 32, hi = raw.z | (uint64_t)raw.w << 32;
-#pragma unroll 1
-    for (int j = 0; j < V; ++j) {
-      if (has(j, cols)) {
-        if (sizeof(T) == 4) ((uint32_t*)row)[first + j] = (uint32_t)lo;
-        else ((uint16_t*)row)[first + j] = (uint16_t)lo;
-      }
-      lo = lo >> kBits | hi << (64 - kBits);
-      hi >>= kBits;
+    // 8, 4 and 2 bytes from the row's side of the boundary on, each on a boundary of its own
+    uint8_t* at = (uint8_t*)(row + first);
+    const int n = (int)sizeof(T) * (first < 0 ? V + first : cols - first);   // bytes, 0 < n < 16
+    if (first < 0) {
+      if (n & 8) *(uint2*)(at + 8) = make_uint2(raw.z, raw.w);
+      if (n & 4) *(uint32_t*)(at + 12 - (n & 8)) = n & 8 ? raw.y : raw.w;
+      const int e = (n & 12) == 12 ? 0 : (n & 12) == 8 ? 1 : (n & 12) == 4 ? 2 : 3;   // the word that is cut
+      if (n & 2) *(uint16_t*)(at + 4 * e + 2) = (uint16_t)((e < 2 ? (e ? raw.y : raw.x) : (e == 2 ? raw.z : raw.w)) >> 16);
+    } else {
+      if (n & 8) *(uint2*)at = make_uint2(raw.x, raw.y);
+      if (n & 4) *(uint32_t*)(at + (n & 8)) = n & 8 ? raw.z : raw.x;
+      const int e = n >> 2;
+      if (n & 2) *(uint16_t*)(at + 4 * e) = (uint16_t)(e < 2 ? (e ? raw.y : raw.x) : (e == 2 ? raw.z : raw.w));
     }
   }
 };
 
 constexpr int kMostSlots = 8;
 template <int NW>
-constexpr int kThreadsOf = 32 * (NW < 4 ? 4 : NW);
+constexpr int kThreadsOf = 32 * (NW == 1 ? 4 : NW);
 template <int NW>
 constexpr int kGroupsOf = kThreadsOf<NW> / (32 * NW);
+
+// CTAs that an SM is to hold: 16 to 20 warps, with the 96 to 128 registers that two pieces take.
+// A CTA goes through its rows one at a time, and what a row takes hardly depends on its length, so
+// more CTAs are better until the ring of each gets too short.
+template <int NW>
+constexpr int kCtasOf = NW == 1 ? 4 : NW == 3 ? 6 : NW <= 5 ? 4 : NW == 6 ? 3 : NW <= 10 ? 2 : 1;
+
+// Backward, where three tensors fill the ring: one CTA of ten warps instead of two took 89 us
+// instead of 97 for 8192 x 5000 fp16, but 134 instead of 110 for the ragged rows of 8191 x 4999
+// (their ends cost latency); of eight warps 74 instead of 64 for 8192 x 4096.
+template <int NW, bool RAGGED>
+constexpr int kCtasBack = NW == 3 ? 4 + RAGGED : NW == 4 ? 3 : NW == 5 || NW == 6 || NW == 10 ? kCtasOf<NW> - !RAGGED : kCtasOf<NW>;
 
 // A row of weights in 32 bits, in shared memory: pieces of four, so that lanes read next to
 // each other (a piece's first half here, its second half `half` further on).  Threads whose rows start at
@@ -240,30 +250,51 @@ struct Ring {
   bool leader;
   uint32_t waited, pending; // a bit for each slot: the phase its barrier is in; a copy is on its way
   __device__ __forceinline__ bool alone(int64_t row) const { return RAGGED && (row == 0 || row + 1 >= rows); }
-  __device__ __forceinline__ const uint8_t* slot(int s, int i) const { return slots + (s * n + i) * bytes; }
+  __device__ __forceinline__ uint8_t* slot(int s, int i) const { return slots + (s * n + i) * bytes; }
   // once nobody reads slot s any more
   __device__ __forceinline__ void fetch(int64_t row, int s) {
-    if (!leader || row >= rows || alone(row)) return;
+    if (!leader || row >= rows) return;
     uint32_t total = 0, size[N];
     uintptr_t from[N];
+    const int in = alone(row) ? 15 : 0;   // only the pieces that lie inside the row
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i >= n) continue;
       const uintptr_t p = (uintptr_t)(base[i] + row * pitch[i]), end = p + cols * sizeof(T);
-      from[i] = p & ~(uintptr_t)15;
-      size[i] = (uint32_t)(((end + 15) & ~(uintptr_t)15) - from[i]);
+      from[i] = (p + in) & ~(uintptr_t)15;
+      size[i] = (uint32_t)(((end + 15 - in) & ~(uintptr_t)15) - from[i]);
       total += size[i];
     }
     mbar_expect_tx(&full[s], total);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < n) bulk_load((void*)slot(s, i), (const void*)from[i], size[i], &full[s]);
+    for (int i = 0; i < N; ++i) {
+      if (i >= n || (RAGGED && !size[i])) continue;
+      const int ahead = RAGGED ? (int)(from[i] - ((uintptr_t)(base[i] + row * pitch[i]) & ~(uintptr_t)15)) : 0;
+      bulk_load(slot(s, i) + ahead, (const void*)from[i], size[i], &full[s]);
+    }
     pending |= 1u << s;
   }
   __device__ __forceinline__ void wait(int s, Guard& g) {
     if (!guard_wait(&full[s], waited >> s & 1, g, 0x70000)) return;
     waited ^= 1u << s;
     pending &= ~(1u << s);
+  }
+  // what fetch() left out of them
+  template <int NW>
+  __device__ __forceinline__ void fill_ends(int64_t row, int s, int phase, int t) {
+    constexpr int V = kPiece<T>;
+    const int head = (V - phase) % V, tail = (phase + cols) % V;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i >= n) continue;
+      const T* from = base[i] + row * pitch[i];
+      T* to = (T*)slot(s, i) + phase;
+      if (t < head) to[t] = from[t];
+      if (t < tail) to[cols - 1 - t] = from[cols - 1 - t];
+    }
+    fence_async_shared();   // a copy will follow into the same slot
+    if (NW == 1) __syncwarp();
+    else __syncthreads();
   }
   // before the CTA ends after a wait that ran out: the copies that are still on their way
   __device__ __forceinline__ void drain(Guard& g) {
@@ -295,7 +326,7 @@ __device__ __forceinline__ void start_ring(Ring<T, N, RAGGED>& ring, uint8_t* sp
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH <= 2 ? 4 : 3) : NW == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 2 ? 3 : kCtasOf<NW>)
 norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
   constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
   extern __shared__ __align__(128) uint8_t space[];
@@ -319,23 +350,19 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
   weight.place(a.weight, (int)a.wtype, 1.f, cols, phase, (float4*)(space + ring_bytes));
   bias.place(a.bias, (int)a.wtype, 0.f, cols, phase, (float4*)(space + ring_bytes) + weight.half * (V / 4));
   __syncthreads();
-  float w[CH][V], b[CH][V];
+  constexpr bool kHold = NW == 1 || CH <= 2;   // in registers
+  float held[kHold ? CH : 1][2][V];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    weight.get(c[i], cols, phase, w[i]);
-    bias.get(c[i], cols, phase, b[i]);
-  }
+  for (int i = 0; kHold && i < CH; ++i) weight.get(c[i], cols, phase, held[i][0]), bias.get(c[i], cols, phase, held[i][1]);
   const float inv = 1.f / (float)cols;
   int s = 0;
   for (int64_t row = first; row < a.rows; row += step) {
     uint4 raw[CH];
-    float sum[1] = {0.f};
-    const bool alone = ring.alone(row);
-    if (!alone) ring.wait(s, guard);
-    auto piece = [&](int i, int k) {
-      return alone ? c[i].take_from(ring.base[k] + row * ring.pitch[k], cols) : c[i].take(ring.slot(s, k), cols, phase);
-    };
+    ring.wait(s, guard);
+    if (ring.alone(row)) ring.template fill_ends<NW>(row, s, phase, t);
+    auto piece = [&](int i, int k) { return c[i].take(ring.slot(s, k), cols, phase); };
     // a row stays packed as it came; to take it apart costs an instruction for an element
+    float sum[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       raw[i] = piece(i, 0);
@@ -348,7 +375,6 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
         for (int j = 0; j < V; ++j) v[j] += r[j];
         raw[i] = pack<T>(v);   // the sum as it is stored is what is normalised
         unpack<T>(raw[i], v);
-        c[i].store((T*)a.z + row * a.cols, cols, raw[i]);
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) sum[0] += v[j];
@@ -357,36 +383,42 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
     if (!guard.gave_up) ring.fetch(row + depth * step, s);
     if (++s == depth) s = 0;
     const float mean = sum[0] * inv;
+    // up to two pieces of a thread stay taken apart from here on, more would not fit the registers
+    constexpr bool kKeep = NW > 1 && CH <= 2;
+    float d[kKeep ? CH : 1][V];
+    auto apart = [&](int i, float (&e)[V]) {
+      forget(raw[i]);
+      unpack<T>(raw[i], e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] -= mean;
+    };
     sum[0] = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      float v[V];
-      forget(raw[i]);
-      unpack<T>(raw[i], v);
+      float(&e)[V] = d[kKeep ? i : 0];
+      apart(i, e);
+      if (sum_in_front) c[i].store((T*)a.z + row * a.cols, cols, raw[i]);
       if (c[i].whole(cols)) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[j] - mean;
-          sum[0] = fmaf(d, d, sum[0]);
-        }
+        for (int j = 0; j < V; ++j) sum[0] = fmaf(e[j], e[j], sum[0]);
       } else if (RAGGED && c[i].first < cols) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[j] - mean;
-          if (c[i].has(j, cols)) sum[0] = fmaf(d, d, sum[0]);
-        }
+        for (int j = 0; j < V; ++j)
+          if (c[i].has(j, cols)) sum[0] = fmaf(e[j], e[j], sum[0]);
       }
     }
     row_sums<NW>(sum, part[1], warp);
     const float rstd = rsqrtf(sum[0] * inv + (float)a.eps);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      float v[V];
-      forget(raw[i]);
-      unpack<T>(raw[i], v);
+      float(&e)[V] = d[kKeep ? i : 0];
+      if (!kKeep) apart(i, e);
+      float(&w)[2][V] = held[kHold ? i : 0];
+      if (!kHold) weight.get(c[i], cols, phase, w[0]), bias.get(c[i], cols, phase, w[1]);
+      float y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = fmaf((v[j] - mean) * rstd, w[i][j], b[i][j]);
-      c[i].store((T*)a.y + row * a.cols, cols, pack<T>(v));
+      for (int j = 0; j < V; ++j) y[j] = fmaf(e[j] * rstd, w[0][j], w[1][j]);
+      c[i].store((T*)a.y + row * a.cols, cols, pack<T>(y));
     }
     if (t == 0) {
       a.mean[row] = mean;
@@ -397,7 +429,7 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW <= 4 ? (CH == 1 ? 4 : CH == 2 ? 3 : 2) : NW == 8 ? 2 : 1)
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 2 ? 2 : NW == 1 && CH == 2 ? 3 : kCtasBack<NW, RAGGED>)
 norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
   constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
   extern __shared__ __align__(128) uint8_t space[];
@@ -446,11 +478,9 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
     uint4 zr[CH], gr[CH], ur[CH];
     const float mean = mean_next, rstd = rstd_next;
     if (row + step < a.rows) mean_next = a.mean[row + step], rstd_next = a.rstd[row + step];
-    const bool alone = ring.alone(row);
-    if (!alone) ring.wait(s, guard);
-    auto piece = [&](int i, int k) {
-      return alone ? c[i].take_from(ring.base[k] + row * ring.pitch[k], cols) : c[i].take(ring.slot(s, k), cols, phase);
-    };
+    ring.wait(s, guard);
+    if (ring.alone(row)) ring.template fill_ends<NW>(row, s, phase, t);
+    auto piece = [&](int i, int k) { return c[i].take(ring.slot(s, k), cols, phase); };
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -529,7 +559,9 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
 }
 
 // How many warps share a row of so many columns, and how many pieces a thread has; 0 where a row
-// does not fit.  One piece more than the row's length takes, where rows start anywhere.
+// does not fit.  Two pieces a thread and as many warps as that takes: three pieces in eight warps
+// needed 242 us for forward and backward of 8191 x 4999 fp16, two in ten 194.  Where rows start
+// anywhere, one piece more than the row's length takes.
 struct Split {
   int warps, pieces;
 };
@@ -540,10 +572,9 @@ Split split_of(int64_t cols, bool ragged) {
   if (n <= 32) return {1, 1};
   if (n <= 64) return {1, 2};
   if (n <= 128) return {1, 4};
-  if (n <= 256) return {4, 2};
-  if (n <= 512) return {8, 2};
-  if (n <= 768) return {8, 3};
-  if (n <= 1024) return {16, 2};
+  for (int warps : {3, 4, 5, 6, 8, 10, 12, 16})
+    if (n <= 64 * warps) return {warps, 2};
+  if (n <= 1536) return {16, 3};
   if (n <= 2048) return {16, 4};
   return {0, 0};
 }
@@ -580,19 +611,18 @@ unsigned ctas_for(int64_t rows, int groups, int per_sm, bool ragged) {
 // Shared memory of a CTA at most: what an SM has, divided by the CTAs it is meant to hold.  The
 // weights take their part of it, the ring the rest; when the ring is done with, its space holds
 // the groups' sums.
-template <int NW>
-constexpr int kSpace = NW <= 4 ? 54 * 1024 : NW == 8 ? 100 * 1024 : 216 * 1024;
+constexpr int space_of(int ctas) { return 216 / ctas * 1024; }
 
 struct RingSize {
   int slot, depth, ring, bytes;
 };
 template <typename T, int NW, int CH, bool RAGGED>
-RingSize ring_size(int64_t cols, int tensors, int weights, bool sums) {
+RingSize ring_size(int space, int64_t cols, int tensors, int weights, bool sums) {
   RingSize r;
   r.slot = (int)((cols * sizeof(T) + (RAGGED ? 30 : 0) + 15) / 16 * 16);
   const int set = kGroupsOf<NW> * tensors * r.slot;
   const int w = Weights<T, RAGGED, NW>::kShared ? weights * (int)((cols + 2 * kPiece<T>) * 4) : 0;
-  r.depth = (kSpace<NW> - w) / set;
+  r.depth = (space - w) / set;
   if (r.depth > kMostSlots) r.depth = kMostSlots;
   r.ring = (r.depth * set + 127) / 128 * 128;
   r.bytes = r.ring + w;
@@ -612,15 +642,15 @@ int prepared(K kernel, int threads, int smem) {
 
 template <typename T, int NW, int CH, bool RAGGED>
 int forward_rows(const HpNormForward& a, uint32_t* status, cudaStream_t s) {
-  static const int per_sm = prepared(norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
-  const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.residual ? 2 : 1, 2, false);
+  static const int per_sm = prepared(norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasOf<NW>));
+  const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasOf<NW>), a.cols, a.residual ? 2 : 1, 2, false);
   return launch_behind(norm_forward_rows<T, NW, CH, RAGGED>, ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>,
                        r.bytes, s, a, r.depth, r.slot, r.ring, status);
 }
 template <typename T, int NW, int CH, bool RAGGED>
 int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
-  static const int per_sm = prepared(norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, kSpace<NW>);
-  const RingSize r = ring_size<T, NW, CH, RAGGED>(a.cols, a.dz ? 3 : 2, 1, true);
+  static const int per_sm = prepared(norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasBack<NW, RAGGED>));
+  const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasBack<NW, RAGGED>), a.cols, a.dz ? 3 : 2, 1, true);
   const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
   const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, r.depth, r.slot,
                                r.ring, status);
@@ -633,10 +663,15 @@ int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
     case 1 * 8 + 1: return call(1, 1);          \
     case 1 * 8 + 2: return call(1, 2);          \
     case 1 * 8 + 4: return call(1, 4);          \
+    case 3 * 8 + 2: return call(3, 2);          \
     case 4 * 8 + 2: return call(4, 2);          \
+    case 5 * 8 + 2: return call(5, 2);          \
+    case 6 * 8 + 2: return call(6, 2);          \
     case 8 * 8 + 2: return call(8, 2);          \
-    case 8 * 8 + 3: return call(8, 3);          \
+    case 10 * 8 + 2: return call(10, 2);        \
+    case 12 * 8 + 2: return call(12, 2);        \
     case 16 * 8 + 2: return call(16, 2);        \
+    case 16 * 8 + 3: return call(16, 3);        \
     case 16 * 8 + 4: return call(16, 4);        \
     default: break;                             \
   }

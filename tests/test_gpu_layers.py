@@ -52,6 +52,17 @@ def test_layer_norm(dtype, wtype, rows, cols, residual):
     check_norm(x, w, b, r, rand(rows, cols, dtype=dtype), rand(rows, cols, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("cols", [8, 9, 33, 200, 257, 513, 769, 1023, 1027, 1600, 2047, 2056, 2561, 3064, 4095, 4096, 4999,
+                                  6143, 6144, 8191, 8192, 12001, 16001, 16384])
+def test_layer_norm_many_rows(dtype, cols):
+    torch.manual_seed(cols)
+    rows = min(4099, 20_000_000 // cols)   # several for every group of warps, and not alike many
+    x, w, b = rand(rows, cols, dtype=dtype, mean=0.5), rand(cols, dtype=FP32, mean=1), rand(cols, dtype=FP32)
+    check_norm(x, w, b, rand(rows, cols, dtype=dtype), rand(rows, cols, dtype=dtype), rand(rows, cols, dtype=dtype))
+    check_norm(x, w, b, None, rand(rows, cols, dtype=dtype), None)
+
+
 @pytest.mark.parametrize("cols", [64, 1000, 1001, 5000])
 def test_layer_norm_strides_and_shapes(cols):
     torch.manual_seed(cols)
