@@ -120,54 +120,53 @@ struct Launch {
 };
 
 // ---------------------------------------------------------------------- forward
-// A CTA has QT tiles of 128 queries of one head and walks over the keys, KB at a time: scores
+// A CTA has QT tiles of 128 queries of one head and walks over the keys, 128 at a time: scores
 // S = q k^T into tensor memory, one thread a row for the softmax, probabilities back over the
-// scores, O += P v.  While some tiles' rows are at work the others' products run.  The sums keep a
-// running maximum; the results so far are scaled anew only when it rises by more than 2^8 (the
-// factor that 32-bit sums and 16-bit probabilities bear easily).  Bound: 2^x, 16 a cycle and SM.
-//   <., 1, 128>    two CTAs an SM for up to 64 dimensions, one for more
-//   <64, 4, 64>, <128, 2, 128>   many queries: what one row does between its 2^x (fetch, maximum,
-//                  store, wait) takes as long as they do; four tiles, or two of the wider heads whose
-//                  results fill tensor memory, hide it and share the keys they fetch
+// scores, O += P v.  While some rows are at work another tile's or another CTA's products run.  The
+// sums keep a running maximum; the results so far are scaled anew only when it rises by more than 2^8
+// (the factor that 32-bit sums and 16-bit probabilities bear easily).  Bound: 2^x, 16 a cycle and SM.
+//   <64, 1>        two CTAs an SM.  Four tiles of queries against 64 keys at a time in one CTA that has
+//                  the SM alone took 0.9 to 1.07 times as long where the SMs were full (64 x 300 tokens
+//                  of 16 heads: 95 against 106 us, 1 x 8192 of 16, causal: both 207) and up to twice as
+//                  long where not (1 x 4096 of 16, causal: 111 against 64)
+//   <128, 1>, <128, 2>   tensor memory holds the results of two CTAs, or of one CTA's two tiles, which
+//                  share the keys they fetch
 //   SHORT          up to 128 queries and keys: one tile each, nothing to walk over.  Results take the
 //                  half of the scores' columns that the probabilities leave, so that four CTAs fit
 //                  an SM and hide one another's latency
-template <int DP, int QT, int KB, bool SHORT>
+template <int DP, int QT, bool SHORT>
 struct Forward {
-  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel, kKeys = kPanels * KB * 128;   // bytes
-  // warps that issue products, each for its own tiles: a product of 64 keys takes as long to issue as to run
-  static constexpr int kIssue = QT > 1 ? 2 : 1;
-  static constexpr int kStages = SHORT ? 1 : KB == 64 ? 6 : 2;
-  // four warps that fetch and issue, four for each tile's rows; the former give registers to the latter
-  static constexpr int kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
-  static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : QT == 2 ? 168 : 96;
-  static constexpr int kFew = SHORT ? 64 : QT == 4 ? 56 : 72, kMany = SHORT ? 64 : QT == 1 ? 184 : QT == 2 ? 216 : 104;
+  static constexpr int kPanels = DP / 64, kTile = kPanels * (int)kPanel;   // bytes
+  // two stages of keys; four warps that fetch and issue, one for each tile, and four for each tile's
+  // rows; the former give registers to the latter
+  static constexpr int kStages = SHORT ? 1 : 2, kThreads = 128 + 128 * QT, kPerSm = SHORT ? 4 : QT == 1 ? 2 : 1;
+  static constexpr int kAtStart = SHORT ? 64 : QT == 1 ? 128 : 168;
+  static constexpr int kFew = SHORT ? 64 : 72, kMany = SHORT ? 64 : QT == 1 ? 184 : 216;
   static_assert(kFew + QT * kMany <= (1 + QT) * kAtStart, "more registers than the CTA has");
-  static constexpr int kSmem = QT * kTile + kStages * 2 * kKeys + 1024 + 1024;
+  static constexpr int kSmem = QT * kTile + kStages * 2 * kTile + 1024 + 1024;
   static constexpr int kTmem = SHORT ? 128 : QT == 1 ? 256 : 512;
   // columns: scores of each tile, results, probabilities.  Where there is room these have columns of
   // their own, and the next scores need not wait for the product that reads them
-  static constexpr bool kApart = !SHORT && DP == 64 && KB == 128;
-  static constexpr uint32_t kO = SHORT ? 64 : QT * KB, kP = kApart ? QT * (KB + DP) : 0, kPStep = kApart ? KB / 2 : KB;
+  static constexpr bool kApart = !SHORT && DP == 64;
+  static constexpr uint32_t kO = SHORT ? 64 : QT * kB, kP = kApart ? kB + DP : 0;
 };
-template <int KB>
 struct ForwardBars {
-  uint64_t q_full, k_full[6], v_full[6], k_empty[6], v_empty[6], mask_full[6], s_full[4], s_free[4], p_full[4], o_full[4], drain;
-  Seen<KB> seen[6];
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], mask_full[2], s_full[2], s_free[2], p_full[2], o_full[2], drain;
+  Seen<kB> seen[2];
   uint32_t tmem;
   int keys;
   Guard guard;
 };
 
-template <typename T, int DP, int QT, int KB, bool SHORT>
-__global__ void __launch_bounds__((Forward<DP, QT, KB, SHORT>::kThreads), (Forward<DP, QT, KB, SHORT>::kPerSm))
+template <typename T, int DP, int QT, bool SHORT>
+__global__ void __launch_bounds__((Forward<DP, QT, SHORT>::kThreads), (Forward<DP, QT, SHORT>::kPerSm))
 attention_forward_tiles(const __grid_constant__ Launch l) {
-  using F = Forward<DP, QT, KB, SHORT>;
+  using F = Forward<DP, QT, SHORT>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = smem;
   uint8_t* skv = smem + QT * F::kTile;   // stages of k and v
-  ForwardBars<KB>& bar = *(ForwardBars<KB>*)(skv + F::kStages * 2 * F::kKeys);
+  ForwardBars& bar = *(ForwardBars*)(skv + F::kStages * 2 * F::kTile);
   const HpAttention& p = l.p;
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // of all heads first the tiles with the most keys, where the mask is causal
@@ -178,12 +177,12 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
   dependents_may_start();
   wait_for_kernel_before();
-  const int sk = !SHORT && masked && p.sk > KB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
+  const int sk = !SHORT && masked && p.sk > kB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
   // key tiles of a query tile: up to the last that its last query sees
   auto tiles_of = [&](int t) {
     const int first = q0 + t * kB, last = min(first + kB, (int)p.sq) - 1;
     const int keys = first >= p.sq ? 0 : p.causal ? min(sk, max(0, last + shift + 1)) : sk;
-    return (keys + KB - 1) / KB;
+    return (keys + kB - 1) / kB;
   };
   int most = 0;
 #pragma unroll
@@ -192,13 +191,13 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     mbar_init(&bar.q_full, 1);
     for (int i = 0; i < F::kStages; ++i) {
       mbar_init(&bar.k_full[i], 1), mbar_init(&bar.v_full[i], 1), mbar_init(&bar.mask_full[i], 1);
-      mbar_init(&bar.k_empty[i], F::kIssue), mbar_init(&bar.v_empty[i], F::kIssue);
+      mbar_init(&bar.k_empty[i], QT), mbar_init(&bar.v_empty[i], QT);
     }
     for (int i = 0; i < QT; ++i) {
       mbar_init(&bar.s_full[i], 1), mbar_init(&bar.s_free[i], 128);
       mbar_init(&bar.p_full[i], 128), mbar_init(&bar.o_full[i], 1);
     }
-    mbar_init(&bar.drain, F::kIssue);
+    mbar_init(&bar.drain, QT);
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
@@ -226,22 +225,22 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       int s = 0;
       uint32_t ph = 0;
       for (int j = 0; j < most; ++j) {
-        uint8_t* k = skv + s * 2 * F::kKeys;
+        uint8_t* k = skv + s * 2 * F::kTile;
         if (!guard_wait(&bar.k_empty[s], ph ^ 1, g, 0x10001)) break;
         if (lane == 0) {
-          mbar_expect_tx(&bar.k_full[s], F::kKeys);
-          for (int i = 0; i < F::kPanels; ++i) tma_load_4d(k + i * KB * 128, &l.map.k, 64 * i, hk, j * KB, b, &bar.k_full[s]);
+          mbar_expect_tx(&bar.k_full[s], F::kTile);
+          for (int i = 0; i < F::kPanels; ++i) tma_load_4d(k + i * kB * 128, &l.map.k, 64 * i, hk, j * kB, b, &bar.k_full[s]);
         }
         // whoever reads the bits gives probabilities before the product that frees v
         if (!guard_wait(&bar.v_empty[s], ph ^ 1, g, 0x10003)) break;
         if (masked) {
-          const Seen<KB> m = mask_bits<KB>(mask, (int64_t)j * KB, sk);
+          const Seen<kB> m = mask_bits<kB>(mask, (int64_t)j * kB, sk);
           if (lane == 0) bar.seen[s] = m, mbar_arrive(&bar.mask_full[s]);
         }
         if (lane == 0) {
-          mbar_expect_tx(&bar.v_full[s], F::kKeys);
+          mbar_expect_tx(&bar.v_full[s], F::kTile);
           for (int i = 0; i < F::kPanels; ++i)
-            tma_load_4d(k + F::kKeys + i * KB * 128, &l.map.v, 64 * i, hk, j * KB, b, &bar.v_full[s]);
+            tma_load_4d(k + F::kTile + i * kB * 128, &l.map.v, 64 * i, hk, j * kB, b, &bar.v_full[s]);
         }
         waits = j + 1;
         if (++s == F::kStages) s = 0, ph ^= 1;
@@ -256,58 +255,46 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
         if (waits < most)   // the k of a tile whose v was not fetched
           mbar_wait_bounded(&bar.k_full[waits % F::kStages], (waits / F::kStages) & 1, kWaitNs / 64, g.status, HP_STATUS_TIMEOUT | 0x10007);
       }
-    } else if (warp <= F::kIssue) {
+    } else if (warp <= QT) {
       if (most) {
-        const int mine = warp - 1;   // its first tile; every kIssue-th is its own
+        const int t = warp - 1, tiles = tiles_of(t);   // each for its own tile
         const uint32_t leader = elect_one();
         const bool bf = p.type == HP_BF16;
-        const uint32_t id_s = mma_idesc(128, KB, bf, true, true) | (l.negative ? kNegateA : 0);
+        const uint32_t id_s = mma_idesc(128, kB, bf, true, true) | (l.negative ? kNegateA : 0);
         const uint32_t id_o = mma_idesc(128, DP, bf, true, false);
         bool ok = warp_wait(&bar.q_full, 0, g, 0x20001);
-        auto scores = [&](int t, int s) {   // S_t = q_t k^T of the stage
-          const uint64_t a = mma_desc(smem_u32(sq + t * F::kTile), 16, 1024), k = mma_desc(smem_u32(skv + s * 2 * F::kKeys), 16, 1024);
+        auto scores = [&](int s) {   // S_t = q_t k^T of the stage
+          const uint64_t a = mma_desc(smem_u32(sq + t * F::kTile), 16, 1024), k = mma_desc(smem_u32(skv + s * 2 * F::kTile), 16, 1024);
 #pragma unroll
           for (int i = 0; i < DP / 16; ++i)
-            mma_ss<1>(leader, tmem + t * KB, a + ((i / 4) * kPanel + (i % 4) * 32) / 16, k + ((i / 4) * KB * 128 + (i % 4) * 32) / 16, id_s, i > 0);
+            mma_ss<1>(leader, tmem + t * kB, a + ((i / 4) * kPanel + (i % 4) * 32) / 16, k + ((i / 4) * kB * 128 + (i % 4) * 32) / 16, id_s, i > 0);
           mma_commit<1>(leader, &bar.s_full[t]);
         };
-        auto results = [&](int t, int s, bool add) {   // O_t += P_t v
-          const uint64_t v = mma_desc(smem_u32(skv + s * 2 * F::kKeys + F::kKeys), KB * 128, 1024);
+        auto results = [&](int s, bool add) {   // O_t += P_t v
+          const uint64_t v = mma_desc(smem_u32(skv + s * 2 * F::kTile + F::kTile), kB * 128, 1024);
 #pragma unroll
-          for (int i = 0; i < KB / 16; ++i)
-            mma_ts(leader, tmem_o + t * DP, tmem + F::kP + t * F::kPStep + i * 8, v + i * 128, id_o, add || i > 0);
+          for (int i = 0; i < kB / 16; ++i)
+            mma_ts(leader, tmem_o + t * DP, tmem + F::kP + t * kB + i * 8, v + i * 128, id_o, add || i > 0);
           mma_commit<1>(leader, &bar.o_full[t]);
         };
-        int tiles[QT / F::kIssue];
-#pragma unroll
-        for (int i = 0; i < QT / F::kIssue; ++i) tiles[i] = tiles_of(i * F::kIssue + mine);
         int s = 0, s_before = 0;
         uint32_t ph = 0, ph_before = 0;
         for (int j = 0; j <= most && ok; ++j) {   // scores of tile j, results of tile j - 1
           if (j < most) ok = warp_wait(&bar.k_full[s], ph, g, 0x20002);
-          if (F::kApart && ok) {   // scores as soon as the last ones have been read
-#pragma unroll
-            for (int i = 0; i < QT / F::kIssue; ++i) {
-              const int t = i * F::kIssue + mine;
-              if (j >= tiles[i] || !ok) continue;
-              if (j > 0) ok = warp_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
-              tmem_fence_after();
-              if (ok) scores(t, s);
-            }
-            if (ok && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
+          if (F::kApart && j < tiles && ok) {   // scores as soon as the last ones have been read
+            if (j > 0) ok = warp_wait(&bar.s_free[t], (j - 1) & 1, g, 0x20005);
+            tmem_fence_after();
+            if (ok) scores(s);
           }
+          if (F::kApart && ok && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
           if (j > 0 && ok) ok = warp_wait(&bar.v_full[s_before], ph_before, g, 0x20003);
           tmem_fence_after();
-#pragma unroll
-          for (int i = 0; i < QT / F::kIssue; ++i) {
-            const int t = i * F::kIssue + mine;
-            if (j > 0 && j - 1 < tiles[i] && ok) {
-              ok = warp_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
-              tmem_fence_after();
-              if (ok) results(t, s_before, j > 1);
-            }
-            if (!F::kApart && j < tiles[i] && ok) scores(t, s);   // over the probabilities just used
+          if (j > 0 && j - 1 < tiles && ok) {
+            ok = warp_wait(&bar.p_full[t], (j - 1) & 1, g, 0x20004);
+            tmem_fence_after();
+            if (ok) results(s_before, j > 1);
           }
+          if (!F::kApart && j < tiles && ok) scores(s);   // over the probabilities just used
           if (j > 0) mma_commit<1>(leader, &bar.v_empty[s_before]);
           if (!F::kApart && j < most) mma_commit<1>(leader, &bar.k_empty[s]);
           s_before = s, ph_before = ph;
@@ -320,16 +307,16 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     if (F::kFew < F::kMany) more_registers<F::kMany>();
     const int t = (warp - 4) >> 2, quad = warp & 3, r = 32 * quad + lane;   // one row to a thread
     const int row = q0 + t * kB + r, nt = tiles_of(t);
-    const uint32_t lanes = (uint32_t)(32 * quad) << 16, ts = tmem + t * KB + lanes, to = tmem_o + t * DP + lanes;
-    const uint32_t tp = tmem + F::kP + t * F::kPStep + lanes;
+    const uint32_t lanes = (uint32_t)(32 * quad) << 16, ts = tmem + t * kB + lanes, to = tmem_o + t * DP + lanes;
+    const uint32_t tp = tmem + F::kP + t * kB + lanes;
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;   // keys this row sees but for the mask
     float m = kNone, sum = 0.f;
     bool ok = true;
     int s = 0;
     uint32_t ph = 0;
     for (int j = 0; j < nt; ++j) {
-      Seen<KB> seen;
-      bool whole = sees >= (j + 1) * KB;
+      Seen<kB> seen;
+      bool whole = sees >= (j + 1) * kB;
       if (masked) {
         if (!guard_wait(&bar.mask_full[s], ph, g, 0x30001)) { ok = false; break; }
         seen = bar.seen[s];
@@ -339,28 +326,28 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
           // no number if that is none: its v counts as zero (rows behind the last key already do).
           // Each tile sees to it before it gives its probabilities.
           if (!guard_wait(&bar.v_full[s], ph, g, 0x30002)) { ok = false; break; }
-          if (r < KB && !(seen.w[quad % (KB / 32)] >> lane & 1)) {
-            uint4* v = (uint4*)(skv + s * 2 * F::kKeys + F::kKeys + r * 128);
+          if (!(seen.w[quad] >> lane & 1)) {
+            uint4* v = (uint4*)(skv + s * 2 * F::kTile + F::kTile + r * 128);
 #pragma unroll
             for (int i = 0; i < F::kPanels; ++i)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[i * KB * 8 + k] = make_uint4(0, 0, 0, 0);
+              for (int k = 0; k < 8; ++k) v[i * kB * 8 + k] = make_uint4(0, 0, 0, 0);
           }
           fence_async_shared();
         }
         whole = whole && all;
       }
       if (!__all_sync(0xffffffffu, whole)) {
-        const Seen<KB> mine = seen_between<KB>(0, sees - j * KB);
+        const Seen<kB> mine = seen_between<kB>(0, sees - j * kB);
 #pragma unroll
-        for (int i = 0; i < KB / 32; ++i) seen.w[i] = masked ? seen.w[i] & mine.w[i] : mine.w[i];
+        for (int i = 0; i < kB / 32; ++i) seen.w[i] = masked ? seen.w[i] & mine.w[i] : mine.w[i];
         whole = false;
       }
       if (++s == F::kStages) s = 0, ph ^= 1;
       if (!guard_wait(&bar.s_full[t], j & 1, g, 0x30003)) { ok = false; break; }
       tmem_fence_after();
       // a row of scores stays in registers where those suffice, else it is read twice, in steps
-      constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : KB;
+      constexpr int kStep = SHORT ? 16 : 32, kHeld = SHORT ? kStep : kB;
       uint32_t x[kHeld];
       auto read = [&](int c, uint32_t* to) {
         if constexpr (SHORT) tmem_ld16(ts + c, *(uint32_t(*)[16])to);
@@ -369,7 +356,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       float part[4] = {kNone, kNone, kNone, kNone};
       if (!SHORT) {
 #pragma unroll
-        for (int c = 0; c < KB; c += kStep) read(c, x + c % kHeld);
+        for (int c = 0; c < kB; c += kStep) read(c, x + c % kHeld);
         tmem_wait_ld();
         if (F::kApart) {
           tmem_fence_before();
@@ -378,7 +365,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       }
       auto highest = [&](auto all) {   // tiles that are seen whole test no bits
 #pragma unroll
-        for (int c = 0; c < KB; c += kStep) {
+        for (int c = 0; c < kB; c += kStep) {
           if (SHORT) {
             read(c, x);
             tmem_wait_ld();
@@ -427,10 +414,10 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       }
       const float base = m == kNone ? 0.f : -m;
       F2 sums[2] = {{0.f, 0.f}, {0.f, 0.f}};
-      uint32_t y[SHORT ? kStep / 2 : KB / 2];   // packed; all of a row before the first is stored, where registers allow
+      uint32_t y[SHORT ? kStep / 2 : kB / 2];   // packed; all of a row before the first is stored, where registers allow
       auto probabilities = [&](auto all) {
 #pragma unroll
-        for (int c = 0; c < KB; c += kStep) {
+        for (int c = 0; c < kB; c += kStep) {
           uint32_t* to_y = SHORT ? y : y + c / 2;
           if (SHORT) {
             read(c, x);
@@ -456,7 +443,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       if (!settle()) { ok = false; break; }
       if constexpr (!SHORT) {
 #pragma unroll
-        for (int c = 0; c < KB; c += 32) tmem_st16(tp + c / 2, *(const uint32_t(*)[16])(y + c / 2));
+        for (int c = 0; c < kB; c += 32) tmem_st16(tp + c / 2, *(const uint32_t(*)[16])(y + c / 2));
       }
       tmem_wait_st();
       tmem_fence_before();
@@ -1147,16 +1134,16 @@ int prepare(Launch& l, const HpAttention& a) {
   return rc;
 }
 
-template <typename T, int DP, int QT, int KB = kB, bool SHORT = false>
+template <typename T, int DP, int QT, bool SHORT = false>
 int forward_tiles(Launch& l, cudaStream_t s) {
-  using F = Forward<DP, QT, KB, SHORT>;
-  const auto kernel = attention_forward_tiles<T, DP, QT, KB, SHORT>;
+  using F = Forward<DP, QT, SHORT>;
+  const auto kernel = attention_forward_tiles<T, DP, QT, SHORT>;
   static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (allowed != cudaSuccess) return allowed;
   const HpAttention& a = l.p;
   if (!head_map(&l.map.q, a.q, a, a.sq, a.heads, a.q_b, a.q_s, a.q_h, kB) ||
-      !head_map(&l.map.k, a.sk ? a.k : a.q, a, a.sk, a.kv_heads, a.k_b, a.k_s, a.k_h, KB) ||
-      !head_map(&l.map.v, a.sk ? a.v : a.q, a, a.sk, a.kv_heads, a.v_b, a.v_s, a.v_h, KB) ||
+      !head_map(&l.map.k, a.sk ? a.k : a.q, a, a.sk, a.kv_heads, a.k_b, a.k_s, a.k_h, kB) ||
+      !head_map(&l.map.v, a.sk ? a.v : a.q, a, a.sk, a.kv_heads, a.v_b, a.v_s, a.v_h, kB) ||
       !head_map(&l.map.o, a.o, a, a.sq, a.heads, a.o_b, a.o_s, a.o_h, 32))
     return HP_ERR_BAD_ARG;
   if (a.heads * a.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
@@ -1169,17 +1156,15 @@ template <typename T>
 int forward(const HpAttention& a, cudaStream_t s) {
   Launch l;
   if (const int rc = prepare(l, a)) return rc;
-  // Several tiles of queries in a CTA pay once there are more tiles than the SMs hold of them one by
-  // one; before that they leave SMs without work.  One tile a CTA against several, in us, bfloat16:
-  //   64 dimensions    1 x 1024, 8 heads: 16 to 32    1 x 8192, 4 heads, causal: 90 to 205
-  //                    64 x 300, 16 heads: 106 to 95  1 x 4096, 16 heads: 116 to 108   8 x 200, 16 heads: 9.8 to 11
-  //   128 dimensions   1 x 1024, 8 heads: 20 to 26    1 x 4096, 4 heads, causal: 62 to 69
-  //                    4 x 512, 16 heads: 24 to 18    1 x 4096, 16 heads, causal: 120 to 77
+  if (a.dim <= 64)
+    return a.sq <= kB && a.sk <= kB ? forward_tiles<T, 64, 1, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
+  // Two tiles of queries in a CTA pay once there are more tiles than SMs, and twice as many where the
+  // mask makes them uneven.  One tile a CTA against two, in us, bfloat16, 148 SMs:
+  //   1 x 1024, 8 heads: 20 to 26           1 x 2048, 16 heads, causal: 38 to 43
+  //   1 x 2048, 12 heads: 66 to 46          1 x 2048, 24 heads, causal: 57 to 44
   const int64_t tiles = (a.sq + kB - 1) / kB * a.heads * a.batch;
-  if (a.dim > 64)
-    return a.sq > kB && tiles > layer_sms() ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
-  if (a.sq > 2 * kB && tiles > 2 * layer_sms()) return forward_tiles<T, 64, 4, 64>(l, s);
-  return a.sq <= kB && a.sk <= kB ? forward_tiles<T, 64, 1, kB, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
+  const bool two = a.sq > kB && tiles > (a.causal ? 2 : 1) * layer_sms();
+  return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
 }
 
 template <typename T>
