@@ -582,13 +582,15 @@ Split split_of(int64_t cols, bool ragged) {
 }
 
 // Rows cut alike: whether every tensor's rows lie alike with regard to 16-byte boundaries, and
-// whether they all begin on one.
+// whether they all begin and end on one.  The length counts for itself: padded rows begin on a
+// boundary whatever it is, and where no dense result is among the tensors it shows nowhere else.
 struct Rows {
   uintptr_t phase;
   int64_t pitch;
   bool alike = true, any = false;
   int size;
-  explicit Rows(int bytes) : size(bytes) {}
+  int64_t end;
+  Rows(int bytes, int64_t cols) : size(bytes), end(cols * bytes % 16) {}
   void add(const void* p, int64_t ld) {
     if (!p) return;
     const uintptr_t f = (uintptr_t)p % 16;
@@ -596,7 +598,7 @@ struct Rows {
     if (any && (f != phase || l != pitch)) alike = false;
     phase = f, pitch = l, any = true;
   }
-  bool ragged() const { return phase != 0 || pitch != 0; }
+  bool ragged() const { return phase != 0 || pitch != 0 || end != 0; }
 };
 
 constexpr int kMostCtas = 1024;   // rows of partial sums
@@ -681,7 +683,7 @@ int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
 
 template <typename T>
 int forward(const HpNormForward& a, cudaStream_t s) {
-  Rows r(sizeof(T));
+  Rows r(sizeof(T), a.cols);
   r.add(a.x, a.ldx);
   r.add(a.residual, a.ldr);
   r.add(a.y, a.cols);
@@ -700,7 +702,7 @@ int forward(const HpNormForward& a, cudaStream_t s) {
 }
 template <typename T>
 int backward(const HpNormBackward& a, cudaStream_t s) {
-  Rows r(sizeof(T));
+  Rows r(sizeof(T), a.cols);
   r.add(a.z, a.ldz);
   r.add(a.dy, a.lddy);
   r.add(a.dz, a.lddz);
