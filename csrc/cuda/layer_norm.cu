@@ -231,6 +231,14 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (&part)[N][16], in
   }
 }
 
+// After row_sums(): all threads of a row have read its slot, which may be filled again.  Where the
+// sums went through a barrier they have; shuffles alone order no memory, least of all reads whose
+// values the sums do not take.
+template <int NW>
+__device__ __forceinline__ void slot_read() {
+  if (NW == 1) __syncwarp();
+}
+
 // From here on `raw` is taken apart anew: the compiler would keep the 32-bit values instead,
 // twice the registers.
 __device__ __forceinline__ void forget(uint4& raw) {
@@ -379,7 +387,8 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
 #pragma unroll
       for (int j = 0; j < V; ++j) sum[0] += v[j];
     }
-    row_sums<NW>(sum, part[0], warp);   // everybody has read the slot
+    row_sums<NW>(sum, part[0], warp);
+    slot_read<NW>();
     if (!guard.gave_up) ring.fetch(row + depth * step, s);
     if (++s == depth) s = 0;
     const float mean = sum[0] * inv;
@@ -499,7 +508,8 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
         sum[1] = fmaf(gw, h, sum[1]);
       }
     }
-    row_sums<NW>(sum, part[turn], warp);   // everybody has read the slot
+    row_sums<NW>(sum, part[turn], warp);
+    slot_read<NW>();
     if (!guard.gave_up) ring.fetch(row + depth * step, s);
     if (++s == depth) s = 0;
     if (!a.dx) continue;

@@ -37,3 +37,19 @@ def test_layer_norm_weights_gradient_alone_of_padded_rows(dtype, rows, cols):
         exact, scale = want[name]
         assert ((got.double() - exact).abs() <= (64 + cols // 32 + rows // 8) * 2.0 ** -23 * scale + 1e-30).all(), name
         close(got, exact, scale, 0, FP32, name, 64 + cols // 32 + rows // 8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("cols", [256, 777, 1024])
+def test_layer_norm_rows_of_one_warp_keep_their_third_tensor(dtype, cols):
+    """The gradient that goes past the norm is read from the ring and in no sum."""
+    from hipress_b200.ops import layer_norm
+    torch.manual_seed(cols)
+    rows = 40000
+    x = rand(rows, cols, dtype=dtype).requires_grad_(True)
+    r = torch.zeros_like(x, requires_grad=False)
+    dz = (torch.arange(rows, device="cuda") % 97)[:, None].to(dtype).expand(rows, cols).contiguous()
+    y, z = layer_norm(x, residual=r)
+    # no gradient of y: what arrives is the third tensor
+    dx, = torch.autograd.grad((y, z), x, (torch.zeros_like(y), dz))
+    assert torch.equal(dx, dz)

@@ -1,0 +1,33 @@
+"""Rules of the layer operators' kernels that no run can show broken: what orders the threads, and
+kernels that overlap, stands in their source."""
+import re
+from pathlib import Path
+
+import pytest
+
+CUDA = Path(__file__).resolve().parent.parent / "csrc" / "cuda"
+
+
+def kernels(name):
+    """Name and body of each kernel of a source file, comments taken out."""
+    text = re.sub(r"//[^\n]*", "", (CUDA / name).read_text())
+    out = {}
+    for m in re.finditer(r"__global__[^{;]*?\b(\w+)\(const __grid_constant__", text):
+        start = text.index("{", text.index(")", m.end()))
+        depth, at = 1, start + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[at], 0)
+            at += 1
+        out[m.group(1)] = text[start:at]
+    return out
+
+
+@pytest.mark.parametrize("kernel", ["norm_forward_rows", "norm_backward_rows"])
+def test_a_slot_is_filled_again_only_behind_its_readers(kernel):
+    body = kernels("layer_norm.cu")[kernel]
+    loop = body[body.index("ring.wait("):]
+    assert loop.count("ring.fetch(") == 1
+    reads = [m.start() for m in re.finditer(r"piece\(i, \d\)", loop)]
+    assert reads and max(reads) < loop.index("row_sums<NW>(") < loop.index("slot_read<NW>()") < loop.index("ring.fetch(")
+    helper = (CUDA / "layer_norm.cu").read_text()
+    assert "if (NW == 1) __syncwarp();" in helper[helper.index("void slot_read()"):][:80]
