@@ -175,7 +175,6 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   const int q0 = qt * kB * QT, shift = (int)(p.sk - p.sq);
   const bool masked = p.key_mask != nullptr;
   const uint8_t* mask = masked ? p.key_mask + b * p.mask_b : nullptr;
-  dependents_may_start();
   wait_for_kernel_before();
   const int sk = !SHORT && masked && p.sk > kB ? visible_keys(mask, (int)p.sk, &bar.keys) : (int)p.sk;
   // key tiles of a query tile: up to the last that its last query sees
@@ -206,6 +205,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
+  dependents_may_start();
   const uint32_t tmem = uniform(bar.tmem), tmem_o = tmem + F::kO;
   Guard& g = bar.guard;
 
@@ -615,7 +615,6 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   const int r0 = tile * kB;           // first row that stays
   const uint8_t* mask = p.key_mask ? p.key_mask + b * p.mask_b : nullptr;
   const bool masked = mask != nullptr;
-  dependents_may_start();
   wait_for_kernel_before();
   // tiles that pass: queries from `first` on, of each head of the group in turn; or keys up to the last seen
   int first = 0, count;
@@ -650,6 +649,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
+  dependents_may_start();
   const uint32_t tmem = uniform(bar.tmem);
   Guard& g = bar.guard;
 
@@ -943,11 +943,11 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     tma_load_4d(sds, &l.map.o, 0, h, 0, b, &bar.vo_full);
   }
   if (warp == 1) tmem_alloc<1>(&bar.tmem, 256);
-  dependents_may_start();
   wait_for_kernel_before();
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
+  dependents_may_start();
   const uint32_t tmem = uniform(bar.tmem);
   Guard& g = bar.guard;
   if (warp == 1) {

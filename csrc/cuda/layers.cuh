@@ -102,7 +102,8 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
 
 // A kernel that may be started while the one in front of it in the stream still runs: its CTAs set
 // up barriers, tensor memory and tensor maps meanwhile, and wait for the end of the one in front
-// (and of what that has waited for) before they touch memory.  Every kernel here calls both.
+// (and of what that has waited for) before they touch memory.  Kernels launched by launch_behind()
+// call both; the plain norm kernels are launched the ordinary way and neither start early nor let others.
 __device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -132,6 +132,11 @@ __device__ __forceinline__ void tma_store_wait_read() {
 // ------------------------------------------------------------- tensor memory
 // By one whole warp.  The right to allocate is given up at once: while a CTA holds it, no other
 // one is started on the SM.
+//
+// An allocation waits until there is room, and that wait has no bound.  What ends it: a CTA lets
+// the kernel behind it start (dependents_may_start()) only once its own allocation is made, behind
+// a barrier of the CTA.  So a CTA that holds tensor memory while it waits for the kernel in front
+// waits for CTAs that all have theirs, whatever fits an SM beside one another.
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t cols) {
   if (CG == 1) {

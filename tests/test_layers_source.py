@@ -31,3 +31,19 @@ def test_a_slot_is_filled_again_only_behind_its_readers(kernel):
     assert reads and max(reads) < loop.index("row_sums<NW>(") < loop.index("slot_read<NW>()") < loop.index("ring.fetch(")
     helper = (CUDA / "layer_norm.cu").read_text()
     assert "if (NW == 1) __syncwarp();" in helper[helper.index("void slot_read()"):][:80]
+
+
+def test_kernels_overlap_only_once_tensor_memory_is_allocated():
+    """A CTA of the kernel behind may hold tensor memory while it waits for the one in front: that
+    one must not be waiting for room."""
+    seen = 0
+    for source in ("linear.cu", "attention.cu"):
+        for name, body in kernels(source).items():
+            if "tmem_alloc<" not in body:
+                continue
+            seen += 1
+            assert body.count("tmem_alloc<") == body.count("dependents_may_start()") == 1, name
+            between = body[body.index("tmem_alloc<"):body.index("dependents_may_start()")] \
+                if body.index("tmem_alloc<") < body.index("dependents_may_start()") else ""
+            assert "__syncthreads();" in between, name
+    assert seen == 4
