@@ -86,7 +86,7 @@ int64_t pitch(const Tensor& m) { return !m.defined() ? 0 : m.size(0) > 1 ? m.str
 
 // ------------------------------------------------------------------ layer norm
 struct Norm {
-  Tensor y, z, rows, stats;
+  Tensor y, z, kept, stats;   // kept: what was normalised, for the backward pass
 };
 
 Norm norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, double eps) {
@@ -101,7 +101,9 @@ Norm norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, con
   a.rows = x2.size(0), a.cols = x2.size(1), a.ldx = pitch(x2), a.ldr = pitch(r2);
   a.type = type_of(x), a.wtype = type_of(w.defined() ? w : b), a.eps = eps;
   check(lib.norm_forward(&a, stream()), "layer_norm");
-  n.rows = n.z.defined() ? n.z.view(x2.sizes()) : x2;
+  // the result itself, of which autograd knows that it is one; a view of it would hold its node, which
+  // holds the view
+  n.kept = n.z.defined() ? n.z : x2;
   return n;
 }
 
@@ -110,7 +112,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Tensor weight = get(w), bias = get(b), residual = get(r);
     ctx->saved_data["present"] = (int64_t)(1 | weight.defined() << 1 | bias.defined() << 2 | residual.defined() << 3);
     Norm n = norm_forward(x, weight, bias, residual, eps);
-    ctx->save_for_backward({n.rows, weight, n.stats});
+    ctx->save_for_backward({n.kept, weight, n.stats});
     ctx->saved_data["sizes"] = x.sizes();
     ctx->saved_data["type"] = (int64_t)(weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : at::kFloat);
     ctx->set_materialize_grads(false);
@@ -119,7 +121,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once(grads, "layer_norm");
     const auto saved = ctx->get_saved_variables();
-    const Tensor z = saved[0], weight = dense(saved[1]), stats = saved[2];
+    const Tensor z = rows_of(saved[0]), weight = dense(saved[1]), stats = saved[2];
     const Tensor dy = grads[0], dz = grads.size() > 1 ? grads[1] : Tensor();
     if (!dy.defined() && !dz.defined()) return variable_list(5);
     c10::cuda::CUDAGuard guard(z.device());

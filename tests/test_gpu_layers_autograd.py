@@ -53,3 +53,36 @@ def test_layer_norm_rows_of_one_warp_keep_their_third_tensor(dtype, cols):
     # no gradient of y: what arrives is the third tensor
     dx, = torch.autograd.grad((y, z), x, (torch.zeros_like(y), dz))
     assert torch.equal(dx, dz)
+
+
+def calls():
+    """Each operator with everything it keeps for its backward pass: name, call, leaves, odd sizes."""
+    from hipress_b200.ops import attention, layer_norm, linear, self_attention
+    torch.manual_seed(4)
+    g = lambda *s, dtype=BF16, std=1.0: rand(*s, dtype=dtype, std=std).requires_grad_(True)  # noqa: E731
+    x, r, nw, nb = g(300, 500), g(300, 500), g(500, dtype=FP32), g(500, dtype=FP32)
+    lx, lw, lb, lr = g(3, 70, 131), g(77, 131, std=0.1), g(77), g(3, 70, 77)
+    q, k, v, qkv = g(2, 150, 4, 40), g(2, 170, 2, 40), g(2, 170, 2, 40), g(2, 100, 3, 2, 64)
+    mask = torch.rand(2, 170, device="cuda") < 0.8
+    return {"layer_norm": (lambda: layer_norm(x, nw, nb), (x, nw, nb)),
+            "layer_norm residual": (lambda: layer_norm(x, nw, nb, residual=r), (x, nw, nb, r)),
+            "linear": (lambda: linear(lx, lw, lb), (lx, lw, lb)),
+            "linear gelu": (lambda: linear(lx, lw, lb, activation="gelu", residual=lr), (lx, lw, lb, lr)),
+            "attention": (lambda: attention(q, k, v, key_mask=mask), (q, k, v)),
+            "attention lse": (lambda: attention(q, k, v, causal=True, return_lse=True)[0], (q, k, v)),
+            "self_attention": (lambda: self_attention(qkv), (qkv,))}
+
+
+NAMES = ["layer_norm", "layer_norm residual", "linear", "linear gelu", "attention", "attention lse", "self_attention"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_graph_that_is_dropped_is_freed(name):
+    call, _ = calls()[name]
+    call()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        call()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
