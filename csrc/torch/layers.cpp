@@ -76,6 +76,14 @@ void once(const variable_list& grads, const char* what) {
     for (const Tensor& g : grads) TORCH_CHECK(!wanted(g), what, ": its gradient cannot be differentiated");
 }
 
+// A saved tensor as it comes back.  Hooks may have kept it elsewhere, and return it in strides of
+// their own, so that whoever takes it lays it out anew; what the kernels read must still be all there.
+Tensor kept(const Tensor& t, const Tensor& grad, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == grad.device() && t.scalar_type() == type && t.sizes() == sizes, what,
+              ": a saved tensor came back as another");
+  return t;
+}
+
 // As a matrix whose rows are dense; a copy only where there is no such view.
 Tensor rows_of(const Tensor& x) {
   Tensor m = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
@@ -103,7 +111,7 @@ Norm norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, con
   check(lib.norm_forward(&a, stream()), "layer_norm");
   // the result itself, of which autograd knows that it is one; a view of it would hold its node, which
   // holds the view
-  n.kept = n.z.defined() ? n.z : x2;
+  n.kept = n.z.defined() ? n.z : x.dim() == 2 ? x2 : x2.view(x.sizes());
   return n;
 }
 
@@ -121,21 +129,24 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once(grads, "layer_norm");
     const auto saved = ctx->get_saved_variables();
-    const Tensor z = rows_of(saved[0]), weight = dense(saved[1]), stats = saved[2];
-    const Tensor dy = grads[0], dz = grads.size() > 1 ? grads[1] : Tensor();
-    if (!dy.defined() && !dz.defined()) return variable_list(5);
-    c10::cuda::CUDAGuard guard(z.device());
+    const Tensor dy = grads[0], dz = grads.size() > 1 ? grads[1] : Tensor(), any = dy.defined() ? dy : dz;
+    if (!any.defined()) return variable_list(5);
+    c10::cuda::CUDAGuard guard(any.device());
     const int64_t present = ctx->saved_data["present"].toInt();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const Tensor z = rows_of(kept(saved[0], any, any.scalar_type(), sizes, "layer_norm"));
     const bool need_x = wants(ctx, present, 0), need_w = wants(ctx, present, 1), need_b = wants(ctx, present, 2),
                need_r = wants(ctx, present, 3);
     const int64_t rows = z.size(0), cols = z.size(1);
     const auto wide = z.options().dtype((at::ScalarType)ctx->saved_data["type"].toInt());
+    const Tensor stats = dense(kept(saved[2], any, at::kFloat, {2, rows}, "layer_norm"));
+    const Tensor weight = present & 2 ? dense(kept(saved[1], any, wide.dtype().toScalarType(), {cols}, "layer_norm")) : Tensor();
     if (!dy.defined())   // only the sum was used further on
       return {need_x ? dz : Tensor(), need_w ? at::zeros({cols}, wide) : Tensor(), need_b ? at::zeros({cols}, wide) : Tensor(),
               need_r ? dz : Tensor(), Tensor()};
     const Tensor g = rows_of(dy), up = dz.defined() ? rows_of(dz) : dz;
     Tensor dx, dw, db, ws;
-    if (need_x || need_r) dx = at::empty(ctx->saved_data["sizes"].toIntVector(), z.options());
+    if (need_x || need_r) dx = at::empty(sizes, z.options());
     if (need_w) dw = at::empty({cols}, wide);
     if (need_b) db = at::empty({cols}, wide);
     if (need_w || need_b) ws = scratch(lib.norm_workspace(rows, cols), z);
@@ -213,9 +224,15 @@ struct Linear : torch::autograd::Function<Linear> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once(grads, "linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor x = saved[0], w = saved[1], pre = saved[2], dy = rows_of(grads[0]);
-    c10::cuda::CUDAGuard guard(x.device());
-    const int64_t m = x.size(0), k = x.size(1), n = w.size(0), act = ctx->saved_data["act"].toInt();
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const Tensor dy = rows_of(grads[0]);
+    const int64_t m = dy.size(0), n = dy.size(1), act = ctx->saved_data["act"].toInt();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t k = sizes.back();
+    const auto type = dy.scalar_type();
+    const Tensor x = operand(kept(saved[0], dy, type, {m, k}, "linear"), type);
+    const Tensor w = operand(kept(saved[1], dy, type, {n, k}, "linear"), type);
+    const Tensor pre = act ? rows_of(kept(saved[2], dy, type, {m, n}, "linear")) : Tensor();
     const int64_t present = ctx->saved_data["present"].toInt();
     const bool need_x = wants(ctx, present, 0), need_w = wants(ctx, present, 1), need_b = wants(ctx, present, 2);
     Tensor g = dy, dx, dw, db;
@@ -223,16 +240,16 @@ struct Linear : torch::autograd::Function<Linear> {
     const bool anew = act || !tiled(dy);
     if (anew) g = at::empty({m, (n + 7) / 8 * 8}, x.options()).narrow(1, 0, n);
     if (anew || need_b) {
-      const auto type = (at::ScalarType)ctx->saved_data["btype"].toInt();
-      if (need_b) db = at::empty({n}, x.options().dtype(type));
+      const auto btype = (at::ScalarType)ctx->saved_data["btype"].toInt();
+      if (need_b) db = at::empty({n}, x.options().dtype(btype));
       const Tensor ws = need_b ? scratch(lib.slope_workspace(m, n), x) : Tensor();
       HpSlope a = {};
       a.dy = ptr(dy), a.pre = ptr(pre), a.g = anew ? ptr(g) : nullptr, a.dbias = ptr(db), a.workspace = ptr(ws);
-      a.rows = m, a.cols = n, a.lddy = pitch(dy), a.ldpre = n, a.ldg = pitch(g);
-      a.type = type_of(x), a.btype = type_of(type), a.act = act;
+      a.rows = m, a.cols = n, a.lddy = pitch(dy), a.ldpre = pitch(pre), a.ldg = pitch(g);
+      a.type = type_of(x), a.btype = type_of(btype), a.act = act;
       check(lib.slope(&a, stream()), "linear backward");
     }
-    if (need_x) dx = product(g, w, m, k, n, true, false, ctx->saved_data["sizes"].toIntVector(), x.scalar_type());
+    if (need_x) dx = product(g, w, m, k, n, true, false, sizes, type);
     if (need_w) dw = product(g, x, n, k, m, false, false, {n, k}, (at::ScalarType)ctx->saved_data["wtype"].toInt());
     return {dx, dw, db, wants(ctx, present, 3) ? grads[0] : Tensor(), Tensor()};
   }
@@ -276,9 +293,10 @@ std::pair<Tensor, Tensor> attention_forward(const Tensor& q0, const Tensor& k0, 
   check(lib.attention_forward(&a, stream()), "attention");
   return {o, lse};
 }
-void attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& o, const Tensor& lse, const Tensor& do0,
+void attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, const Tensor& o0, const Tensor& lse0, const Tensor& do0,
                         const Tensor& mask0, bool causal, double scale, const Tensor& dq, const Tensor& dk, const Tensor& dv) {
-  const Tensor q = tileable(q0), k = tileable(k0), v = tileable(v0), d_o = tileable(do0), mask = mask_rows(mask0);
+  const Tensor q = tileable(q0), k = tileable(k0), v = tileable(v0), o = tileable(o0), d_o = tileable(do0), lse = dense(lse0),
+               mask = mask_rows(mask0);
   const Tensor delta = at::empty({q.size(0), q.size(2), 10, (q.size(1) + 127) / 128 * 128}, q.options().dtype(at::kFloat));
   HpAttention a = block(q, k, v, o, lse, mask, causal, scale);
   a.d_o = ptr(d_o), a.dq = ptr(dq), a.dk = ptr(dk), a.dv = ptr(dv), a.delta = (float*)ptr(delta);
@@ -286,11 +304,21 @@ void attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, co
   check(lib.attention_backward(&a, stream()), "attention backward");
 }
 
-void keep(AutogradContext* ctx, bool causal, double scale, const Tensor& lse) {
+void keep(AutogradContext* ctx, bool causal, double scale, const Tensor& lse, const Tensor& k, const Tensor& mask) {
   ctx->saved_data["causal"] = causal;
   ctx->saved_data["scale"] = scale;
+  ctx->saved_data["keys"] = k.sizes();
+  ctx->saved_data["masked"] = mask.defined();
   ctx->mark_non_differentiable({lse});
   ctx->set_materialize_grads(false);
+}
+
+// o, lse and the mask as they come back
+void kept_results(AutogradContext* ctx, const Tensor& o, const Tensor& lse, const Tensor& mask, const Tensor& d_o, const char* what) {
+  kept(o, d_o, d_o.scalar_type(), d_o.sizes(), what);
+  kept(lse, d_o, at::kFloat, {d_o.size(0), d_o.size(2), d_o.size(1)}, what);
+  const std::vector<int64_t> keys = ctx->saved_data["keys"].toIntVector();
+  if (ctx->saved_data["masked"].toBool()) kept(mask, d_o, at::kBool, {keys[0], keys[1]}, what);
 }
 
 struct Attention : torch::autograd::Function<Attention> {
@@ -299,7 +327,7 @@ struct Attention : torch::autograd::Function<Attention> {
     const Tensor mask = get(m);
     auto [o, lse] = attention_forward(q, k, v, mask, causal, scale);
     ctx->save_for_backward({q, k, v, o, lse, mask});
-    keep(ctx, causal, scale, lse);
+    keep(ctx, causal, scale, lse, k, mask);
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -307,7 +335,10 @@ struct Attention : torch::autograd::Function<Attention> {
     variable_list out(6);
     if (!grads[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    c10::cuda::CUDAGuard guard(s[0].device());
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const std::vector<int64_t> keys = ctx->saved_data["keys"].toIntVector();
+    for (int i = 0; i < 3; ++i) kept(s[i], grads[0], grads[0].scalar_type(), i ? at::IntArrayRef(keys) : grads[0].sizes(), "attention");
+    kept_results(ctx, s[3], s[4], s[5], grads[0], "attention");
     for (int i = 0; i < 3; ++i) out[i] = at::empty(s[i].sizes(), s[i].options());
     attention_backward(s[0], s[1], s[2], s[3], s[4], grads[0], s[5], ctx->saved_data["causal"].toBool(),
                        ctx->saved_data["scale"].toDouble(), out[0], out[1], out[2]);
@@ -322,7 +353,7 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
     const Tensor mask = get(m);
     auto [o, lse] = attention_forward(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2), mask, causal, scale);
     ctx->save_for_backward({qkv, o, lse, mask});
-    keep(ctx, causal, scale, lse);
+    keep(ctx, causal, scale, lse, o, mask);
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -330,8 +361,11 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
     variable_list out(4);
     if (!grads[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
-    c10::cuda::CUDAGuard guard(s[0].device());
-    const Tensor qkv = s[0], d = at::empty(qkv.sizes(), qkv.options());
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const auto size = grads[0].sizes();
+    const Tensor qkv = kept(s[0], grads[0], grads[0].scalar_type(), {size[0], size[1], 3, size[2], size[3]}, "self_attention");
+    kept_results(ctx, s[1], s[2], s[3], grads[0], "self_attention");
+    const Tensor d = at::empty(qkv.sizes(), qkv.options());
     attention_backward(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2), s[1], s[2], grads[0], s[3],
                        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), d.select(2, 0), d.select(2, 1),
                        d.select(2, 2));

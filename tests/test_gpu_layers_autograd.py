@@ -86,3 +86,39 @@ def test_a_graph_that_is_dropped_is_freed(name):
         call()
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() == before
+
+
+def gradients(call, leaves):
+    out = call()
+    out = out if isinstance(out, tuple) else (out,)
+    torch.manual_seed(6)
+    return torch.autograd.grad(out, leaves, [rand(*o.shape, dtype=o.dtype) for o in out])
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_may_be_kept_elsewhere(name):
+    """Offloading brings back what was saved in strides of its own."""
+    call, leaves = calls()[name]
+    want = gradients(call, leaves)
+    with torch.autograd.graph.save_on_cpu():
+        got = gradients(call, leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    def wide(t):   # the same values, a column apart, off every boundary
+        if t.dim() < 2:
+            return t.clone()
+        out = torch.empty(*t.shape[:-1], 2 * t.shape[-1] + 1, dtype=t.dtype, device=t.device)[..., 1::2]
+        return out.copy_(t)
+
+    with torch.autograd.graph.saved_tensors_hooks(wide, lambda t: t):
+        got = gradients(call, leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("change", [lambda t: t.cpu(), lambda t: t.double() if t.is_floating_point() else t.int(), lambda t: t[..., :-1]])
+def test_saved_tensors_that_are_others_are_refused(name, change):
+    """Another device, type or size than what was saved."""
+    call, leaves = calls()[name]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change), pytest.raises(RuntimeError, match="saved tensor"):
+        gradients(call, leaves)
