@@ -60,8 +60,11 @@ Tensor scratch(uint64_t bytes, const Tensor& like) {
 using Maybe = std::optional<Tensor>;
 Tensor get(const Maybe& t) { return t ? *t : Tensor(); }
 bool wanted(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// Whether a node is needed.  Tangents (forward mode) are refused: a tensor may have one without
+// requiring a gradient, and would lose it.
 template <typename... Ts>
-bool differentiable(const Ts&... t) {
+bool differentiable(const char* what, const Ts&... t) {
+  TORCH_CHECK(!((t.defined() && t._fw_grad(0).defined()) || ...), what, ": forward mode differentiation is not supported");
   return at::GradMode::is_enabled() && (wanted(t) || ...);
 }
 // Whether an argument of a node wants its gradient.  A node counts the tensors that are there:
@@ -164,7 +167,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 std::pair<Tensor, Maybe> layer_norm(const Tensor& x, const Maybe& weight, const Maybe& bias, const Maybe& residual, double eps) {
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor w = get(weight), b = get(bias), r = get(residual);
-  if (differentiable(x, w, b, r)) {
+  if (differentiable("layer_norm", x, w, b, r)) {
     variable_list out = LayerNorm::apply(x, weight, bias, residual, eps);
     return {out[0], out.size() > 1 ? Maybe(out[1]) : Maybe()};
   }
@@ -258,7 +261,7 @@ struct Linear : torch::autograd::Function<Linear> {
 Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& residual, int64_t act) {
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor b = get(bias), r = get(residual);
-  if (differentiable(x, weight, b, r)) return Linear::apply(x, weight, bias, residual, act);
+  if (differentiable("linear", x, weight, b, r)) return Linear::apply(x, weight, bias, residual, act);
   return linear_forward(x, weight, b, r, act, false).y;
 }
 
@@ -376,7 +379,7 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
 
 std::pair<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& mask, bool causal, double scale) {
   c10::cuda::CUDAGuard guard(q.device());
-  if (differentiable(q, k, v)) {
+  if (differentiable("attention", q, k, v)) {
     variable_list out = Attention::apply(q, k, v, mask, causal, scale);
     return {out[0], out[1]};
   }
@@ -384,7 +387,7 @@ std::pair<Tensor, Tensor> attention(const Tensor& q, const Tensor& k, const Tens
 }
 std::pair<Tensor, Tensor> self_attention(const Tensor& qkv, const Maybe& mask, bool causal, double scale) {
   c10::cuda::CUDAGuard guard(qkv.device());
-  if (differentiable(qkv)) {
+  if (differentiable("self_attention", qkv)) {
     variable_list out = SelfAttention::apply(qkv, mask, causal, scale);
     return {out[0], out[1]};
   }

@@ -122,3 +122,20 @@ def test_saved_tensors_that_are_others_are_refused(name, change):
     call, leaves = calls()[name]
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change), pytest.raises(RuntimeError, match="saved tensor"):
         gradients(call, leaves)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(name, leaf):
+    import torch.autograd.forward_ad as fwd
+    from hipress_b200.ops import attention, layer_norm, linear, self_attention
+    torch.manual_seed(5)
+    op = {"layer_norm": lambda x: layer_norm(x), "layer_norm residual": lambda x: layer_norm(x.detach(), residual=x),
+          "linear": lambda x: linear(x, x.detach()), "linear gelu": lambda x: linear(x.detach(), x, activation="gelu"),
+          "attention": lambda x: attention(*(x.view(1, 64, 1, 64),) * 3),
+          "attention lse": lambda x: attention(*(x.detach().view(1, 64, 1, 64),) * 2, x.view(1, 64, 1, 64), return_lse=True),
+          "self_attention": lambda x: self_attention(x.view(1, 64, 1, 1, 64).expand(1, 64, 3, 1, 64))}[name]
+    x, t = rand(64, 64, dtype=BF16), rand(64, 64, dtype=BF16)
+    op(x)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+        op(fwd.make_dual(x.requires_grad_(leaf), t))
