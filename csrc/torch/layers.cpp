@@ -89,7 +89,9 @@ Tensor kept(const Tensor& t, const Tensor& grad, at::ScalarType type, at::IntArr
 
 // As a matrix whose rows are dense; a copy only where there is no such view.
 Tensor rows_of(const Tensor& x) {
-  Tensor m = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  int64_t rows = 1;   // counted: of no elements they cannot be divided by the columns
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  Tensor m = x.dim() == 2 ? x : x.reshape({rows, x.size(-1)});
   return m.stride(1) == 1 || m.size(1) == 1 ? m : m.contiguous();
 }
 // of one row there is no second to be reached, and its stride may be anything

@@ -51,6 +51,10 @@ def _wide(x):
     return x if x.dtype == torch.float64 else x.float()   # CPU: float64 is taken as it is
 
 
+def _rows(x):
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])   # also of no elements
+
+
 # ================================================================== layer norm
 def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
     """Normalises the last axis of ``x``: ``(z - mean) / sqrt(var + eps) * weight + bias``.
@@ -107,8 +111,8 @@ class _LayerNorm(torch.autograd.Function):
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         g = torch.zeros_like(mean).expand_as(z) if dy is None else _wide(dy)   # only the sum was used further on
         h = (_wide(z) - mean) * rstd
-        dw = (g * h).reshape(-1, z.shape[-1]).sum(0).to(weight.dtype) if need_w else None
-        db = g.reshape(-1, z.shape[-1]).sum(0).to(ctx.bias) if need_b else None
+        dw = _rows(g * h).sum(0).to(weight.dtype) if need_w else None
+        db = _rows(g).sum(0).to(ctx.bias) if need_b else None
         if weight is not None:
             g = g * _wide(weight)
         dx = rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
@@ -187,10 +191,10 @@ class _Linear(torch.autograd.Function):
         x, w, pre = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         g = _wide(dy) if pre is None else _wide(dy) * _act_slope(_wide(pre), ctx.act)
-        db = g.reshape(-1, g.shape[-1]).sum(0).to(ctx.types[1]) if need_b else None
+        db = _rows(g).sum(0).to(ctx.types[1]) if need_b else None
         g = _wide(g.to(x.dtype))
         dx = (g @ _wide(w)).to(x.dtype) if need_x else None
-        dw = (g.reshape(-1, g.shape[-1]).t() @ _wide(x).reshape(-1, x.shape[-1])).to(ctx.types[0]) if need_w else None
+        dw = (_rows(g).t() @ _rows(_wide(x))).to(ctx.types[0]) if need_w else None
         return dx, dw, db, dy if need_r else None, None
 
 
