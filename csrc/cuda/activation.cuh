@@ -47,17 +47,20 @@ __device__ __forceinline__ float activate(float p) {
   return p;
 }
 
+// p comes back from 16 bits, where a large one may have become an infinity.  Beyond 64 either form is
+// zero or one to the last bit, and every factor below is finite.
 template <int ACT>
 __device__ __forceinline__ float slope(float p) {
   if (ACT == HP_ACT_RELU) return p > 0.f ? 1.f : 0.f;
   if (ACT == HP_ACT_GELU) {
     float e;
-    const float q = normal_tail(p, e);
-    return fmaf(p * 0.3989422804014327f, e, p > 0.f ? 1.f - q : q);
+    const float q = normal_tail(p, e), near = fminf(fmaxf(p, -64.f), 64.f);   // e is no number where p is none
+    return fmaf(near * 0.3989422804014327f, e, p > 0.f ? 1.f - q : q);
   }
   if (ACT == HP_ACT_GELU_TANH) {
-    const float g = tanh_gate(p), du = 2.f * kTanhC * fmaf(3.f * kTanhA, p * p, 1.f);
-    return fmaf(p * g * (1.f - g), du, g);
+    const float g = tanh_gate(p), near = fminf(fmaxf(p, -64.f), 64.f);        // nor is g
+    const float du = 2.f * kTanhC * fmaf(3.f * kTanhA, near * near, 1.f);
+    return fmaf(near * g * (1.f - g), du, g);
   }
   return 1.f;
 }

@@ -162,6 +162,8 @@ def _act(p, kind):
 def _act_slope(p, kind):
     if kind == 1:
         return (p > 0).to(p.dtype)
+    # zero and one to the last bit from here on; p may be an infinity, which its rounding made of a large value
+    p = p.clamp(-64.0, 64.0)
     if kind == 2:
         return 0.5 * (1 + torch.erf(p * math.sqrt(0.5))) + p * torch.exp(-0.5 * p * p) / math.sqrt(2 * math.pi)
     c = math.sqrt(2 / math.pi)

@@ -29,3 +29,32 @@ def test_linear_empty_sizes_of_any_shape():
             dx, dw, db, dr = torch.autograd.grad(y, (x, w, b, r), torch.ones_like(y))
             assert dx.shape == x.shape and not dx.any() and dw.shape == w.shape and not dw.any()
             assert db.shape == b.shape and torch.equal(dr, torch.ones_like(dr))
+
+
+def one_by_one(values, kind):
+    """activation(x) and its derivative of each value, through a product over one k."""
+    from hipress_b200.ops import linear
+    x = values[:, None].detach().requires_grad_(True)
+    y = linear(x, torch.ones(1, 1, device="cuda", dtype=values.dtype), activation=kind)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    return y[:, 0].detach(), dx[:, 0]
+
+
+@pytest.mark.parametrize("kind", ["relu", "gelu", "gelu_tanh"])
+def test_slope_at_an_infinity_that_only_the_rounding_made(kind):
+    """In front of the activation -90000 and 90000 become infinities of fp16."""
+    from hipress_b200.ops import linear
+    x = torch.tensor([[300.0, 0.0], [-300.0, 0.0], [1.0, 1.0]], device="cuda", dtype=FP16).requires_grad_(True)
+    w = torch.tensor([[300.0, 2.0]], device="cuda", dtype=FP16).requires_grad_(True)
+    b = torch.zeros(1, device="cuda", dtype=FP32, requires_grad=True)
+    y = linear(x, w, b, activation=kind)
+    assert y[1].item() == 0
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.tensor([[0.5], [1.0], [0.25]], device="cuda", dtype=FP16))
+    assert torch.equal(dx, torch.tensor([[150.0, 1.0], [0.0, 0.0], [75.0, 0.5]], device="cuda", dtype=FP16))
+    assert torch.equal(dw, torch.tensor([[150.25, 0.25]], device="cuda", dtype=FP16)) and db.item() == 0.75
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh"])
+def test_slope_of_very_large_values(kind):
+    y, dx = one_by_one(torch.tensor([3e38, 1e20, -1e20, -3e38], device="cuda", dtype=BF16), kind)
+    assert dx.tolist() == [1.0, 1.0, 0.0, 0.0] and (y[2:] == 0).all()
