@@ -58,3 +58,22 @@ def test_slope_at_an_infinity_that_only_the_rounding_made(kind):
 def test_slope_of_very_large_values(kind):
     y, dx = one_by_one(torch.tensor([3e38, 1e20, -1e20, -3e38], device="cuda", dtype=BF16), kind)
     assert dx.tolist() == [1.0, 1.0, 0.0, 0.0] and (y[2:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gelu_is_rounded_once(dtype):
+    """All values from -13 to 13.  Besides the result's rounding: the formula's relative error, and
+    that of exp(-p p / 2), whose exponent of up to 122 is rounded to 32 bits (122 2^-24 < 2^-17)."""
+    bits = torch.arange(-32768, 32768, device="cuda", dtype=torch.int32).to(torch.int16)
+    p = bits.view(dtype)
+    p = p[torch.isfinite(p) & (p.abs() <= 13)].contiguous()
+    y, dx = one_by_one(p, "gelu")
+    want, slope = act64(p.double(), "gelu")
+    least = {BF16: 2.0 ** -126, FP16: 2.0 ** -24}[dtype]   # half of the smallest number, or what counts as none
+    off = ((y.double() - want).abs() - least).clamp(min=0) / want.abs().clamp(min=least)
+    assert off.max() <= U[dtype] + 2.0 ** -14, (off.max().item(), p[off.argmax()].item())
+    # the derivative is a sum of two terms, which cancel near -0.75
+    tail = 0.5 * torch.special.erfc(-p.double() / math.sqrt(2))
+    scale = tail + p.double().abs() * torch.exp(-p.double() ** 2 / 2) / math.sqrt(2 * math.pi)
+    off = ((dx.double() - slope).abs() - U[dtype] * slope.abs() - least).clamp(min=0) / scale.clamp(min=least)
+    assert off.max() <= 2.0 ** -14, (off.max().item(), p[off.argmax()].item())
