@@ -1,4 +1,6 @@
 // Attention, forward, and backward from recomputed probabilities.
+#include <type_traits>
+
 #include "activation.cuh"
 #include "tcgen05.cuh"
 
@@ -502,10 +504,32 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
 // row of d_o against its row of o (delta); both negative.  [batch, heads] blocks of kRowWords words
 // for each row, rows rounded up to 128: all lse, all delta, then for products (see below) tiles of
 // 64 rows, first -lse / c of each row in three parts that add up to it and have 11 bits each, then
-// -delta likewise.  Behind the last row, and where a row saw nothing, lse is so large that every
+// -delta likewise.  The fourth word of such a row meets a zero in the product and is used otherwise:
+// in the first tile what dS of this row is multiplied by (2^..), in the second, for the first of the
+// rows that a CTA of attention_rows() has, the exponent of the largest of them.  Behind the last row, and where a row saw nothing, lse is so large that every
 // probability comes out as zero.
 constexpr int kRowWords = 10, kPass = 64;
 constexpr float kNever = 1e35f;
+
+// In fp16 probabilities and dS = P (dP - delta) would leave the type's range downwards where rows are
+// long or d_o is small: P is 1 / keys on average, and below 2^-25 nothing is left.  Both are therefore
+// held times powers of two that the results' scale takes out again.  P, which is 1 at most, times
+// 2^kUpP.  dS times 2^(1 - m), with m the exponent of |d_o|: of the query's own row for dq, of the
+// largest row for dk, whose sum runs over the queries.  It is less than 2 |v| then (P (1 - P) is 1/4
+// at most, and |dP - dP'| at most 2 |d_o| |v|), which fits for |v| up to 32752.  Bfloat16 has the
+// exponents of 32 bits and needs none of this.
+template <typename T>
+constexpr bool kNarrow = std::is_same<T, __half>::value;
+template <typename T>
+constexpr int kUpP = kNarrow<T> ? 14 : 0;
+constexpr int kNoRow = -1000;   // exponent of a row of zeros, or of one that is not finite
+// m from the sum of a row's squares
+__device__ __forceinline__ int row_exponent(float squares) {
+  const uint32_t bits = __float_as_uint(squares);
+  return squares > 0.f && bits < 0x7f800000u ? ((int)(bits >> 23) - 127) >> 1 : kNoRow;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // e normal
+__device__ __forceinline__ int ds_up(int exponent) { return exponent == kNoRow ? 0 : 1 - exponent; }
 __host__ __device__ __forceinline__ int64_t padded(int64_t rows) { return (rows + kB - 1) / kB * kB; }
 
 __device__ __forceinline__ float4 three_parts(float v) {
@@ -520,9 +544,8 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
   const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, h = blockIdx.y, b = blockIdx.z;
   const int64_t rows = padded(a.sq);
   dependents_may_start();
-  if (i >= rows) return;
-  wait_for_kernel_before();
-  float s = 0.f, lse = -INFINITY;
+  wait_for_kernel_before();   // the CTAs' rows add up to `rows`
+  float s = 0.f, lse = -INFINITY, squares = 0.f;
   if (i < a.sq) {
     if (8 * lane < a.dim) {
       float o[8], g[8];
@@ -530,19 +553,36 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
       unpack<T>(*(const uint4*)((const T*)a.d_o + b * a.do_b + i * a.do_s + h * a.do_h + 8 * lane), g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) s = fmaf(o[k], g[k], s);
+      if (kNarrow<T>)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) squares = fmaf(g[k], g[k], squares);
     }
     if (lane == 0) lse = a.lse[(b * a.heads + h) * a.sq + i] * kLog2e;
   }
 #pragma unroll
   for (int k = LANES / 2; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+  int up = 0, largest = kNoRow;
+  if constexpr (kNarrow<T>) {
+    __shared__ int most[8];
+#pragma unroll
+    for (int k = LANES / 2; k; k >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, k);
+    const int e = row_exponent(squares), of_warp = __reduce_max_sync(0xffffffffu, e);
+    up = ds_up(e);
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = of_warp;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) largest = max(largest, most[k]);
+  }
   if (lane == 0) {
     float* out = a.delta + (b * a.heads + h) * kRowWords * rows;
     float4* parts = (float4*)(out + 2 * rows) + i / kPass * 2 * kPass + i % kPass;
     const bool none = lse == -INFINITY;
-    out[i] = none ? -kNever : -lse;
+    out[i] = none ? -kNever : (float)up - lse;
     out[rows + i] = -s;
-    parts[0] = none ? make_float4(-kNever, 0.f, 0.f, 0.f) : three_parts(-lse / c);
-    parts[kPass] = three_parts(-s);
+    float4 first = none ? make_float4(-kNever, 0.f, 0.f, 0.f) : three_parts(((float)kUpP<T> - lse) / c), second = three_parts(-s);
+    if (kNarrow<T>) first.w = power_of_two(up), second.w = (float)largest;
+    parts[0] = first;
+    parts[kPass] = second;
   }
 }
 
@@ -576,9 +616,25 @@ struct BackwardBars {
   uint64_t stay_full, in_full[8], in_empty[8], mask_full[8], s_full[6], s_free[3], p_full[3], acc_full;
   Seen<kPass> seen[8];
   uint32_t tmem;
-  int keys;
+  int keys;       // or the largest row's exponent
   Guard guard;
 };
+
+// By the whole CTA: the exponent of the largest row of d_o among rows from `first` on, of `heads` heads.
+template <int DP>
+__device__ __forceinline__ int largest_row(const float* delta, int heads, int64_t first, int64_t rows, int* shared) {
+  constexpr int kRows = 256 / (DP / 8);   // of a CTA of attention_rows(), which kPass is a multiple of
+  if (threadIdx.x == 0) *shared = kNoRow;
+  __syncthreads();
+  int e = kNoRow;
+  for (int h = 0; h < heads; ++h)
+    for (int64_t i = first + (int64_t)threadIdx.x * kRows; i < rows; i += (int64_t)blockDim.x * kRows)
+      e = max(e, (int)delta[h * kRowWords * rows + 2 * rows + (i / kPass * 2 * kPass + kPass + i % kPass) * 4 + 3]);
+  e = __reduce_max_sync(0xffffffffu, e);
+  if ((threadIdx.x & 31) == 0) atomicMax(shared, e);
+  __syncthreads();
+  return *shared;
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_constant__ Launch l) {
@@ -628,6 +684,10 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     count = (see + kPass - 1) / kPass;
   }
   const int n = keys ? count * group : count;
+  int up = 0;   // dS is held times 2^up, for keys
+  if (kNarrow<T> && keys && n)
+    up = ds_up(largest_row<DP>(p.delta + ((int64_t)b * p.heads + head * group) * kRowWords * padded(p.sq), group, (int64_t)first * kPass,
+                               padded(p.sq), &bar.keys));
   const int buffers = DP == 64 || !keys ? 3 : 2, turns = buffers == 3 ? 6 : 2;   // a turn is one group's, of one buffer
   if (threadIdx.x == 0) {
     mbar_init(&bar.stay_full, 1);
@@ -756,12 +816,15 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     const int quad = warp & 3, half = (warp - 4) >> 2, r = 32 * quad + lane, row = r0 + r;
     const uint32_t lanes = (uint32_t)(32 * quad) << 16;
     float lse = 0.f, delta = 0.f;   // of a query that stays, negative
+    float ds_scale = kNarrow<T> ? power_of_two(keys ? up : 0) : 1.f;   // what dS is held times: a query's own
+    const float of_p = kNarrow<T> ? power_of_two(up - kUpP<T>) : 1.f;  // the same of keys where P is held times 2^kUpP
     bool mine = true;               // a key that stays is seen at all
     if (keys) {
       mine = row < sk && (!masked || mask[row]);
     } else {
       const float* from = p.delta + (b * p.heads + head) * kRowWords * padded(p.sq) + row;
       lse = from[0], delta = from[padded(p.sq)];
+      if (kNarrow<T>) ds_scale = (from - row)[2 * padded(p.sq) + (row / kPass * 2 * kPass + row % kPass) * 4 + 3];
     }
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;
     bool ok = true;
@@ -828,7 +891,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
           const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])}, u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
           const F2 z = of_keys ? mul2(v, {l.c, l.c}) : fma2(v, {l.c, l.c}, {lse, lse});
           F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-          F2 ds = mul2(pr, of_keys ? u : add2(u, {delta, delta}));
+          F2 ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys ? u : add2(u, {delta, delta}));
           if (!all) {
             const uint32_t two = seen.w[i / 32] >> (i % 32);
             if (!(two & 1)) pr.x = ds.x = 0.f;
@@ -862,7 +925,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         const bool is_v = keys && job < F::kPanels;   // dv first, then dk; or dq alone
         const int panel = job % F::kPanels;
         const uint32_t from = tmem + lanes + (is_v ? F::kAcc1 : F::kAcc2) + 64 * panel;
-        const float scale = is_v ? 1.f : (float)p.scale;
+        const float scale = is_v ? 1.f / (float)(1 << kUpP<T>) : (float)p.scale / ds_scale;
         uint8_t* to = stay + job * kPanel + 32 * quad * 128;
 #pragma unroll 1
         for (int c = 0; c < 64; c += 32) {
@@ -912,6 +975,7 @@ struct ShortBars {
   uint64_t kq_full, vo_full, s_full, dp_full, rows_full, p_full, acc_full, out_full;
   float lse[kB], delta[kB];
   uint32_t tmem;
+  int largest;    // exponent of the largest row of d_o
   Guard guard;
 };
 constexpr int kShortSmem = 6 * (int)kPanel + 2048 + 1024;
@@ -933,6 +997,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     mbar_init_fence();
     bar.guard.gave_up = 0;
     bar.guard.status = l.status;
+    bar.largest = kNoRow;
     wait_for_kernel_before();
     mbar_expect_tx(&bar.kq_full, 2 * kPanel);
     tma_load_4d(sk_, &l.map.k, 0, h, 0, b, &bar.kq_full);
@@ -986,7 +1051,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     if (half == 0) {   // lse and delta, negative, of query r
       const float lse = r < sq ? p.lse[(b * p.heads + h) * p.sq + r] : -INFINITY;
       ok = guard_wait(&bar.vo_full, 0, g, 0x32001);
-      float d = 0.f;
+      float d = 0.f, squares = 0.f;
 #pragma unroll
       for (int c = 0; c < 128; c += 16) {
         float x[8], y[8];
@@ -994,9 +1059,16 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
         unpack<T>(*(const uint4*)(sds + staged(r, c)), y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d = fmaf(x[i], y[i], d);
+        if (kNarrow<T>)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) squares = fmaf(x[i], x[i], squares);
       }
-      bar.lse[r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+      bar.lse[r] = lse == -INFINITY ? -INFINITY : (float)kUpP<T> - lse * kLog2e;
       bar.delta[r] = -d;
+      if (kNarrow<T>) {
+        const int e = __reduce_max_sync(0xffffffffu, row_exponent(squares));
+        if (lane == 0) atomicMax(&bar.largest, e);
+      }
       mbar_arrive(&bar.rows_full);
     }
     const int from = p.causal ? r - shift : 0;   // the first query that sees this key
@@ -1009,6 +1081,9 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     ok = ok && guard_wait(&bar.rows_full, 0, g, 0x32002) && guard_wait(&bar.s_full, 0, g, 0x32003) &&
          guard_wait(&bar.dp_full, 0, g, 0x32004);
     tmem_fence_after();
+    // one factor for all of dS, which dk and dq are both made from
+    const int up = kNarrow<T> && ok ? ds_up(bar.largest) : 0;
+    const float of_p = power_of_two(up - kUpP<T>);
     if (ok) {
       if (there && !mine && half == 0)   // what a masked key holds is left out of dq: it counts as zero
 #pragma unroll
@@ -1029,7 +1104,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
             for (int k = 0; k < 4; k += 2) {
               const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {lv[k], lv[k + 1]});
               F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-              F2 ds = mul2(pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {dv[k], dv[k + 1]}));
+              F2 ds = mul2(kNarrow<T> ? mul2(pr, {of_p, of_p}) : pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {dv[k], dv[k + 1]}));
               if (!all) {
                 const uint32_t two = bits_of >> (i + k);
                 if (!(two & 1)) pr.x = ds.x = 0.f;
@@ -1069,10 +1144,10 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
       }
     };
     if (ok) {
-      const float scale = (float)p.scale;
+      const float scale = (float)p.scale * power_of_two(-up);
       uint8_t* to = half ? sq_ : sv_;
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 32) emit(128 + 64 * half + c, half ? scale : 1.f, to, c);
+      for (int c = 0; c < 64; c += 32) emit(128 + 64 * half + c, half ? scale : 1.f / (float)(1 << kUpP<T>), to, c);
       emit(32 * half, scale, sg_, 32 * half);
       fence_async_shared();
       __syncwarp();

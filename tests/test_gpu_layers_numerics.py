@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from _layers import U, act64
+from _layers import U, act64, attention64
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,80 @@ def test_gelu_is_rounded_once(dtype):
     scale = tail + p.double().abs() * torch.exp(-p.double() ** 2 / 2) / math.sqrt(2 * math.pi)
     off = ((dx.double() - slope).abs() - U[dtype] * slope.abs() - least).clamp(min=0) / scale.clamp(min=least)
     assert off.max() <= 2.0 ** -14, (off.max().item(), p[off.argmax()].item())
+
+
+def heads64(q, k, v, do, scale):
+    """dq, dk, dv of one head each in 64 bits, by rows of queries."""
+    q, k, v, do = (t.double().transpose(1, 2) for t in (q, k, v, do))
+    p = torch.softmax(q @ k.transpose(2, 3) * scale, -1)
+    dp = do @ v.transpose(2, 3)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale
+    return tuple(t.transpose(1, 2) for t in (ds @ k, ds.transpose(2, 3) @ q, p.transpose(2, 3) @ do))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sq,sk", [(100, 128), (300, 8000), (3000, 20000), (257, 20000)])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -10, 2.0 ** 9])
+def test_attention_small_gradients_over_long_rows(dim, sq, sk, size):
+    """Probabilities of 1 / 20000 times small gradients are below fp16's smallest number long before
+    the sums over them are; nothing may become zero, or infinite, on the way."""
+    from hipress_b200.ops import attention
+    torch.manual_seed(dim + sk)
+    lean = torch.randn(1, 1, 1, dim, device="cuda")
+    q = rand(1, sq, 1, dim, dtype=FP16, std=0.3)
+    # keys and values lean one way, so that sums over them do not cancel
+    side = torch.sign(torch.randn(1, sk, 1, 1, device="cuda"))
+    k = (rand(1, sk, 1, dim, dtype=FP32, std=0.3) + 2 * side * lean).to(FP16)
+    v = (rand(1, sk, 1, dim, dtype=FP32, std=0.3) + side).to(FP16)
+    do = ((rand(1, sq, 1, dim, dtype=FP32) * 0.1 + 1) * size * 2.0 ** -6).to(FP16)
+    q = (q.float() - (q.float() * lean).sum(-1, keepdim=True) * lean / (lean * lean).sum()).to(FP16)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    got = torch.autograd.grad(attention(*leaves, scale=dim ** -0.5), leaves, do)
+    for name, g, want in zip(("dq", "dk", "dv"), got, heads64(q, k, v, do, dim ** -0.5)):
+        # results down to fp16's smallest numbers: each within a unit of those besides its share of the whole
+        bound = 4 * U[FP16] * want.norm() + math.sqrt(g.numel()) * 2.0 ** -25
+        assert (g.double() - want).norm() <= bound, (name, ((g.double() - want).norm() / want.norm()).item())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sq,sk,causal", [(90, 120, False), (600, 5000, True), (1300, 700, False)])
+def test_attention_rows_of_very_unlike_gradients(dim, sq, sk, causal):
+    """Each query's dq by itself, where rows of d_o lie up to 2^16 apart, and shared key heads."""
+    from hipress_b200.ops import attention
+    torch.manual_seed(sq)
+    q, k, v = rand(1, sq, 4, dim, dtype=FP16, std=0.5), rand(1, sk, 2, dim, dtype=FP16), rand(1, sk, 2, dim, dtype=FP16)
+    power = torch.randint(-12, 5, (1, sq, 1, 1), device="cuda").float()
+    do = (rand(1, sq, 4, dim, dtype=FP32) * 2 ** power).to(FP16)
+    do[0, sq // 2] = 0
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(attention(*leaves, causal=causal), leaves, do)
+    want = attention64(q, k, v, do, causal=causal, mask=None)
+    # a row's share of its own sums of absolute values: dS, delta from the rounded result, dq itself.  The
+    # short kernel has one factor for all rows: 2^-25 of the largest of them, for each key
+    exact, scale = want["dq"]
+    worst = ((dq.double() - exact).norm(dim=-1) - dim ** 0.5 * 2.0 ** -25).clamp(min=0)
+    allowed = (3 * U[FP16] + 2.0 ** -13) * scale.norm(dim=-1)
+    if sq <= 128 and dim <= 64:
+        largest = 2 * do.double().norm(dim=-1).amax()
+        allowed = allowed + 2.0 ** -25 * largest * k.double().norm(dim=-1).amax() * sk ** 0.5 * dim ** -0.5
+    assert (worst <= allowed).all(), (worst / allowed.clamp(min=1e-30)).max().item()
+    assert not dq[0, sq // 2].any()
+    for name, got in (("dk", dk), ("dv", dv)):
+        exact, scale = want[name]
+        assert (got.double() - exact).norm() <= (3 * U[FP16] + 2.0 ** -13) * scale.norm(), name
+
+
+def test_attention_gradients_at_the_end_of_the_range():
+    """Gradients scaled up for fp16's sake, and values near 200: neither result nor dS may become infinite."""
+    from hipress_b200.ops import attention
+    torch.manual_seed(3)
+    for sq, sk, dim in ((100, 100, 64), (500, 700, 64), (300, 400, 128)):
+        q, k = rand(1, sq, 2, dim, dtype=FP16, std=0.2), rand(1, sk, 2, dim, dtype=FP16, std=0.2)
+        v = rand(1, sk, 2, dim, dtype=FP16, std=200)
+        do = rand(1, sq, 2, dim, dtype=FP16, std=0.25)
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        got = torch.autograd.grad(attention(*leaves), leaves, do)
+        want = attention64(q, k, v, do, causal=False, mask=None)
+        for name, g in zip(("dq", "dk", "dv"), got):
+            assert torch.isfinite(g).all()
+            assert (g.double() - want[name][0]).norm() <= (3 * U[FP16] + 2.0 ** -13) * want[name][1].norm(), name
