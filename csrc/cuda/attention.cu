@@ -1213,8 +1213,8 @@ template <typename T, int DP, int QT, bool SHORT = false>
 int forward_tiles(Launch& l, cudaStream_t s) {
   using F = Forward<DP, QT, SHORT>;
   const auto kernel = attention_forward_tiles<T, DP, QT, SHORT>;
-  static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-  if (allowed != cudaSuccess) return allowed;
+  static PerDevice allowed;
+  if (const int rc = allow_shared_memory(allowed, kernel, F::kSmem)) return rc;
   const HpAttention& a = l.p;
   if (!head_map(&l.map.q, a.q, a, a.sq, a.heads, a.q_b, a.q_s, a.q_h, kB) ||
       !head_map(&l.map.k, a.sk ? a.k : a.q, a, a.sk, a.kv_heads, a.k_b, a.k_s, a.k_h, kB) ||
@@ -1245,8 +1245,8 @@ int forward(const HpAttention& a, cudaStream_t s) {
 template <typename T>
 int backward_short(const Launch& l, cudaStream_t s) {
   const auto kernel = attention_backward_short<T>;
-  static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShortSmem);
-  if (allowed != cudaSuccess) return allowed;
+  static PerDevice allowed;
+  if (const int rc = allow_shared_memory(allowed, kernel, kShortSmem)) return rc;
   if (l.p.heads * l.p.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
   return launch_behind(kernel, (unsigned)(l.p.heads * l.p.batch), 320, kShortSmem, s, l);
 }
@@ -1254,9 +1254,8 @@ int backward_short(const Launch& l, cudaStream_t s) {
 template <typename T, int DP>
 int backward_tiles(const Launch& l, cudaStream_t s) {
   using F = Backward<DP>;
-  static const cudaError_t allowed =
-      cudaFuncSetAttribute(attention_backward_tiles<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-  if (allowed != cudaSuccess) return allowed;
+  static PerDevice allowed;
+  if (const int rc = allow_shared_memory(allowed, attention_backward_tiles<T, DP>, F::kSmem)) return rc;
   const HpAttention& a = l.p;
   const int64_t nq = (a.sq + kB - 1) / kB, nk = (a.sk + kB - 1) / kB, tiles = (nk * a.kv_heads + nq * a.heads) * a.batch;
   if (tiles > INT32_MAX) return HP_ERR_TOO_LARGE;

@@ -645,25 +645,34 @@ RingSize ring_size(int space, int64_t cols, int tensors, int weights, bool sums)
   return r;
 }
 
-// CTAs of the kernel that an SM holds, with the largest ring
+// CTAs of the kernel that an SM of the current device holds, with the largest ring; `known` is the kernel's own
 template <typename K>
-int prepared(K kernel, int threads, int smem) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 1;
-  int n = 1;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) n = 1;
-  return n;
+int resident(PerDevice& known, K kernel, int threads, int smem, int* ctas) {
+  int dev = 0;
+  if (const int rc = cudaGetDevice(&dev)) return rc;
+  return known.get(dev, [&](int* n) {
+    if (const int rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
+    const int rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kernel, threads, smem);
+    if (*n < 1) *n = 1;
+    return rc;
+  }, ctas);
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
 int forward_rows(const HpNormForward& a, uint32_t* status, cudaStream_t s) {
-  static const int per_sm = prepared(norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasOf<NW>));
+  static PerDevice known;
+  int per_sm;
+  if (const int rc = resident(known, norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasOf<NW>), &per_sm)) return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasOf<NW>), a.cols, a.residual ? 2 : 1, 2, false);
   return launch_behind(norm_forward_rows<T, NW, CH, RAGGED>, ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>,
                        r.bytes, s, a, r.depth, r.slot, r.ring, status);
 }
 template <typename T, int NW, int CH, bool RAGGED>
 int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
-  static const int per_sm = prepared(norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasBack<NW, RAGGED>));
+  static PerDevice known;
+  int per_sm;
+  if (const int rc = resident(known, norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasBack<NW, RAGGED>), &per_sm))
+    return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasBack<NW, RAGGED>), a.cols, a.dz ? 3 : 2, 1, true);
   const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
   const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, r.depth, r.slot,

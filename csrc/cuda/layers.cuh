@@ -7,6 +7,7 @@
 
 #include "hipress/capi.h"
 #include "hipress/layers.h"
+#include "hipress/per_device.h"
 
 namespace hipress {
 
@@ -120,6 +121,18 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+}
+
+// Lets the kernel have `smem` bytes of dynamic shared memory on the current device.  `done` is the
+// kernel's own.
+template <typename K>
+int allow_shared_memory(PerDevice& done, K kernel, int smem) {
+  int dev = 0, value;
+  if (const int rc = cudaGetDevice(&dev)) return rc;
+  return done.get(dev, [&](int* v) {
+    *v = 1;
+    return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  }, &value);
 }
 
 inline bool type_ok(int64_t t) { return t >= HP_F32 && t <= HP_F16; }

@@ -468,9 +468,8 @@ int run_product(Launch& l, int sms, cudaStream_t s) {
         (p.pre && !split && !tensor_map(&l.pre, p.pre, (int)p.type, 3, size, pitch, box)))
       return HP_ERR_BAD_ARG;
   }
-  static const cudaError_t allowed =
-      cudaFuncSetAttribute(product_kernel<T, CG, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (allowed != cudaSuccess) return allowed;
+  static PerDevice allowed;
+  if (const int rc = allow_shared_memory(allowed, product_kernel<T, CG, BN>, S::kSmem)) return rc;
   l.tiles_m = (int)((p.m + 128 * CG - 1) / (128 * CG));
   l.tiles_n = (int)((p.n + BN - 1) / BN);
   const int64_t units = (int64_t)l.tiles_m * l.tiles_n * l.splits;
