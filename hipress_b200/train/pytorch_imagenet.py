@@ -54,6 +54,10 @@ def main(argv=None):
                     help="fault injection on the host: this rank leaves the job before that step")
     add_hipress_args(ap)
     a = ap.parse_args(argv)
+    if a.fused_layers and not a.model.lower().startswith("bert"):
+        ap.error(f"--fused-layers is for the BERT models, not {a.model}")
+    if a.fused_layers and a.fp32 and torch.cuda.is_available():
+        ap.error("--fused-layers: the kernels take 16-bit activations, which --fp32 leaves out")
     hp.init()
     log = setup_logging()
     cfg = config_from_args(a)

@@ -75,3 +75,15 @@ def test_a_job_trains_on_fused_layers_on_the_gpu():
     losses = train(torch.device("cuda"), torch.bfloat16, fused=True)
     assert losses[-1] < losses[0]
     assert abs(losses[0] - train(torch.device("cuda"), torch.bfloat16)[0]) < 0.05 * losses[0]
+
+
+@pytest.mark.parametrize("args,what", [(["--model", "vgg19"], "BERT"), (["--model", "resnet50"], "BERT"), (["--model", "transformer"], "BERT"),
+                                       (["--model", "bert-base", "--fp32"], "fp32")])
+def test_the_launcher_refuses_fused_layers_that_cannot_be(args, what, monkeypatch, capsys):
+    from hipress_b200.train import pytorch_imagenet as T
+    monkeypatch.setattr(T.torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(T, "build_job", lambda *a, **kw: pytest.fail("a job was built"))
+    with pytest.raises(SystemExit) as stop:
+        T.main([*args, "--fused-layers"])
+    assert stop.value.code == 2
+    assert what in capsys.readouterr().err
