@@ -24,6 +24,23 @@ Encode encoder() {   // looked up in the driver, so that nothing links against i
 
 constexpr int kDevices = 64;
 
+// Two warps at a barrier that nobody arrives at: the first gives up after `limit`, the second, which
+// would wait for kWaitNs, because the first has.
+__global__ void wait_probe(uint64_t limit, uint64_t* took, uint32_t* status) {
+  __shared__ uint64_t bar;
+  __shared__ Guard guard;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    mbar_init_fence();
+    guard.gave_up = 0;
+    guard.status = status;
+  }
+  __syncthreads();
+  const uint64_t start = global_timer_ns();
+  const bool came = threadIdx.x < 32 ? guard_wait(&bar, 0, guard, 0x90000, limit) : guard_wait(&bar, 0, guard, 0x90001);
+  if (threadIdx.x % 32 == 0) took[threadIdx.x / 32] = came ? 0 : global_timer_ns() - start;
+}
+
 }  // namespace
 
 bool tensor_map(CUtensorMap* m, const void* base, int type, int rank, const uint64_t* sizes, const uint64_t* strides_bytes,
@@ -89,3 +106,13 @@ int layer_sms() {
 }
 
 }  // namespace hipress
+
+extern "C" int hp_cuda_layer_wait_probe(uint64_t limit_ns, uint64_t* took, void* stream) {
+  using namespace hipress;
+  if (!took || limit_ns > kWaitNs) return HP_ERR_BAD_ARG;
+  int rc;
+  uint32_t* status = layer_status(&rc);
+  if (rc) return rc;
+  wait_probe<<<1, 64, 0, (cudaStream_t)stream>>>(limit_ns, took, status);
+  return cudaGetLastError();
+}

@@ -22,7 +22,7 @@ struct Guard {
 };
 constexpr uint64_t kWaitNs = 2000000000ull;  // nothing remote is behind these waits
 
-__device__ __forceinline__ bool guard_wait(uint64_t* bar, uint32_t parity, Guard& g, uint32_t code) {
+__device__ __forceinline__ bool guard_wait(uint64_t* bar, uint32_t parity, Guard& g, uint32_t code, uint64_t limit = kWaitNs) {
   if (mbar_try_wait(bar, parity)) return true;
   uint64_t t0 = 0;
   for (uint32_t polls = 1;; ++polls) {
@@ -31,7 +31,7 @@ __device__ __forceinline__ bool guard_wait(uint64_t* bar, uint32_t parity, Guard
       if (g.gave_up) return false;
       const uint64_t now = global_timer_ns();
       if (t0 == 0) t0 = now;
-      else if (now - t0 > kWaitNs) {
+      else if (now - t0 > limit) {
         g.gave_up = 1;
         record_status(g.status, HP_STATUS_TIMEOUT | code);
         return false;

@@ -114,6 +114,10 @@ typedef struct {
 int hp_cuda_attention_forward(const HpAttention* a, void* stream);
 int hp_cuda_attention_backward(const HpAttention* a, void* stream);
 
+// A wait of the layer operators' kind that runs out after `limit_ns`, and one beside it, which then
+// ends too; the nanoseconds that each took to two words of device memory.  For tests.
+int hp_cuda_layer_wait_probe(uint64_t limit_ns, uint64_t* took, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

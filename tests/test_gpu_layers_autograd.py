@@ -139,3 +139,19 @@ def test_forward_mode_is_refused(name, leaf):
     op(x)
     with fwd.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
         op(fwd.make_dual(x.requires_grad_(leaf), t))
+
+
+def test_a_wait_that_ran_out_is_reported_by_the_next_call():
+    from hipress_b200._native import lib
+    from hipress_b200.ops import linear
+    x = rand(8, 16, dtype=BF16)
+    want = linear(x, x)
+    took = torch.zeros(2, dtype=torch.int64, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.cuda().hp_cuda_layer_wait_probe(50_000_000, took.data_ptr(), stream) == 0
+    torch.cuda.synchronize()
+    own, beside = took.tolist()
+    assert 50_000_000 <= own < 1_000_000_000 and 0 < beside < 1_000_000_000
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        linear(x, x)
+    assert torch.equal(linear(x, x), want)    # said once; the device is usable
