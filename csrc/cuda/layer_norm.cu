@@ -638,7 +638,7 @@ RingSize ring_size(int space, int64_t cols, int tensors, int weights, bool sums)
   const int w = Weights<T, RAGGED, NW>::kShared ? weights * (int)((cols + 2 * kPiece<T>) * 4) : 0;
   r.depth = (space - w) / set;
   if (r.depth > kMostSlots) r.depth = kMostSlots;
-  r.ring = (r.depth * set + 127) / 128 * 128;
+  r.ring = r.depth * set;   // whole pieces, as the weights behind it want
   r.bytes = r.ring + w;
   const int joint = sums && kGroupsOf<NW> > 1 ? kGroupsOf<NW> * 2 * kPiece<T> * 32 * NW * CH * 4 : 0;
   if (r.bytes < joint) r.bytes = joint;

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from _layers import U, act64, attention64
+from _layers import U, act64, attention64, norm64
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +154,28 @@ def test_attention_gradients_at_the_end_of_the_range():
         for name, g in zip(("dq", "dk", "dv"), got):
             assert torch.isfinite(g).all()
             assert (g.double() - want[name][0]).norm() <= (3 * U[FP16] + 2.0 ** -13) * want[name][1].norm(), name
+
+
+# lengths at which the ring and the weights together come within a few bytes of the shared memory that a CTA may have
+FULL = [(BF16, c) for c in (1954, 2490, 2497, 2613, 2617, 3944, 5009, 5528, 6482, 7896, 10034, 11041, 12280, 13816, 15777)] + \
+    [(FP32, c) for c in (460, 628, 677, 1228, 1245, 1305, 3948, 4252, 6140, 6908, 7889)]
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype,cols", FULL)
+def test_layer_norm_lengths_that_fill_shared_memory(dtype, cols, residual):
+    from hipress_b200.ops import layer_norm
+    torch.manual_seed(cols)
+    rows = 37
+    x, dy, dz = (rand(rows, cols, dtype=dtype) for _ in range(3))
+    r = rand(rows, cols, dtype=dtype) if residual else None
+    w, b = rand(cols, dtype=FP32, mean=1), rand(cols, dtype=FP32)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+    out = layer_norm(*leaves, residual=r)
+    z = (x.float() + r.float()).to(dtype) if residual else x
+    dx, dw, db = torch.autograd.grad(out, leaves, (dy, dz) if residual else dy)
+    want = norm64(z, w, b, dy, dz if residual else None, 1e-5)
+    steps = 64 + cols // 32
+    for name, got, kind in (("y", out[0] if residual else out, dtype), ("dx", dx, dtype), ("dw", dw, FP32), ("db", db, FP32)):
+        exact, scale = want[name]
+        assert ((got.double() - exact).abs() <= U[kind] * exact.abs() + steps * 2.0 ** -23 * scale.abs().amax(-1, keepdim=True)).all(), name
