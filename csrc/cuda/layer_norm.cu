@@ -649,10 +649,10 @@ RingSize ring_size(int space, int64_t cols, int tensors, int weights, bool sums)
 template <typename K>
 int resident(PerDevice& known, K kernel, int threads, int smem, int* ctas) {
   int dev = 0;
-  if (const int rc = cudaGetDevice(&dev)) return rc;
+  if (const int rc = told(cudaGetDevice(&dev))) return rc;
   return known.get(dev, [&](int* n) {
-    if (const int rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return rc;
-    const int rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kernel, threads, smem);
+    if (const int rc = told(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return rc;
+    const int rc = told(cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kernel, threads, smem));
     if (*n < 1) *n = 1;
     return rc;
   }, ctas);

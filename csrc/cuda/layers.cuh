@@ -108,6 +108,13 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
 __device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// The code that is returned for a call of the runtime.  The runtime keeps it as well, for whoever asks next
+// about a launch of their own: that is taken back.
+inline int told(cudaError_t rc) {
+  if (rc != cudaSuccess) cudaGetLastError();
+  return rc;
+}
+
 template <typename... Params, typename... Args>
 int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -120,7 +127,7 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  return told(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
 }
 
 // Lets the kernel have `smem` bytes of dynamic shared memory on the current device.  `done` is the
@@ -128,10 +135,10 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
 template <typename K>
 int allow_shared_memory(PerDevice& done, K kernel, int smem) {
   int dev = 0, value;
-  if (const int rc = cudaGetDevice(&dev)) return rc;
+  if (const int rc = told(cudaGetDevice(&dev))) return rc;
   return done.get(dev, [&](int* v) {
     *v = 1;
-    return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return told(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   }, &value);
 }
 

@@ -14,7 +14,7 @@ Encode encoder() {   // looked up in the driver, so that nothing links against i
   static const Encode f = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+    if (told(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q)) ||
         q != cudaDriverEntryPointSuccess)
       p = nullptr;
     return (Encode)p;
@@ -63,7 +63,7 @@ bool tensor_map(CUtensorMap* m, const void* base, int type, int rank, const uint
   if (encode() == CUDA_SUCCESS) return true;
   // a thread that has not used the device yet (autograd's, in its first backward pass) has no context
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+  if (told(cudaGetDevice(&dev)) || told(cudaSetDevice(dev))) return false;
   return encode() == CUDA_SUCCESS;
 }
 
@@ -71,7 +71,7 @@ uint32_t* layer_status(int* rc) {
   static uint32_t* words[kDevices] = {};
   static std::mutex lock;
   int dev = 0;
-  *rc = cudaGetDevice(&dev);
+  *rc = told(cudaGetDevice(&dev));
   if (*rc) return nullptr;
   if (dev >= kDevices) {
     *rc = HP_ERR_BAD_ARG;
@@ -80,7 +80,7 @@ uint32_t* layer_status(int* rc) {
   std::lock_guard<std::mutex> hold(lock);
   if (!words[dev]) {   // pinned for good, 64 bytes
     void* p = nullptr;
-    *rc = cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable);
+    *rc = told(cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable));
     if (*rc) return nullptr;
     *(volatile uint32_t*)p = 0;
     words[dev] = (uint32_t*)p;
@@ -97,9 +97,9 @@ uint32_t* layer_status(int* rc) {
 int layer_sms() {
   static int sms[kDevices] = {};
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kDevices) return 1;
+  if (told(cudaGetDevice(&dev)) || dev >= kDevices) return 1;
   if (!sms[dev]) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+    if (told(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev))) return 1;
     sms[dev] = n;
   }
   return sms[dev];

@@ -488,7 +488,7 @@ int run_product(Launch& l, int sms, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, product_kernel<T, CG, BN>, l);
+  return told(cudaLaunchKernelEx(&cfg, product_kernel<T, CG, BN>, l));
 }
 
 int alignment(const void* p, int64_t pitch_bytes) {

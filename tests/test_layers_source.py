@@ -47,3 +47,13 @@ def test_kernels_overlap_only_once_tensor_memory_is_allocated():
                 if body.index("tmem_alloc<") < body.index("dependents_may_start()") else ""
             assert "__syncthreads();" in between, name
     assert seen == 4
+
+
+def test_errors_that_are_returned_are_not_left_for_the_next_launch():
+    """The runtime keeps the last error for whoever asks: a refused call made the next kernel of
+    another library look as if it had failed."""
+    for name in ("layers.cuh", "layers_host.cu", "linear.cu", "attention.cu", "layer_norm.cu", "column_sums.cuh"):
+        text = re.sub(r"//[^\n]*", "", (CUDA / name).read_text())
+        for m in re.finditer(r"\bcuda[A-Z]\w+\(", text):
+            if m.group() not in ("cudaGetLastError(",):
+                assert text[:m.start()].endswith("told("), (name, m.group())
