@@ -38,6 +38,9 @@ struct Shape {
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
   static constexpr int kSmem = kStages * kStage + kEpiWarps * (kBuffers * kStaging + kCols * 4) + 512 + 1024;
   static constexpr int kTmem = 2 * BN;
+  // A pair allocates on two SMs.  Two pairs that shared both could each hold what the other waits for on
+  // its second SM, so that no SM may have room for two: half of its 228 KB.
+  static_assert(CG == 1 || kSmem > 114 * 1024, "two pairs of CTAs fit an SM");
 };
 
 struct Launch {

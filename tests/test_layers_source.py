@@ -57,3 +57,11 @@ def test_errors_that_are_returned_are_not_left_for_the_next_launch():
         for m in re.finditer(r"\bcuda[A-Z]\w+\(", text):
             if m.group() not in ("cudaGetLastError(",):
                 assert text[:m.start()].endswith("told("), (name, m.group())
+
+
+def test_two_pairs_of_ctas_never_share_an_sm():
+    """They allocate tensor memory on two SMs, and could wait for one another there."""
+    text = (CUDA / "linear.cu").read_text()
+    assert 'static_assert(CG == 1 || kSmem > 114 * 1024' in text
+    for name in ("attention.cu", "layer_norm.cu"):
+        assert "tmem_alloc<2>" not in (CUDA / name).read_text()
