@@ -309,21 +309,18 @@ void attention_backward(const Tensor& q0, const Tensor& k0, const Tensor& v0, co
   check(lib.attention_backward(&a, stream()), "attention backward");
 }
 
-void keep(AutogradContext* ctx, bool causal, double scale, const Tensor& lse, const Tensor& k, const Tensor& mask) {
+void keep(AutogradContext* ctx, bool causal, double scale, const Tensor& lse) {
   ctx->saved_data["causal"] = causal;
   ctx->saved_data["scale"] = scale;
-  ctx->saved_data["keys"] = k.sizes();
-  ctx->saved_data["masked"] = mask.defined();
   ctx->mark_non_differentiable({lse});
   ctx->set_materialize_grads(false);
 }
 
-// o, lse and the mask as they come back
-void kept_results(AutogradContext* ctx, const Tensor& o, const Tensor& lse, const Tensor& mask, const Tensor& d_o, const char* what) {
+// o, lse and the mask, if there is one, as they come back
+void kept_results(const Tensor& o, const Tensor& lse, const Tensor& mask, const Tensor& d_o, int64_t keys, const char* what) {
   kept(o, d_o, d_o.scalar_type(), d_o.sizes(), what);
   kept(lse, d_o, at::kFloat, {d_o.size(0), d_o.size(2), d_o.size(1)}, what);
-  const std::vector<int64_t> keys = ctx->saved_data["keys"].toIntVector();
-  if (ctx->saved_data["masked"].toBool()) kept(mask, d_o, at::kBool, {keys[0], keys[1]}, what);
+  if (mask.defined()) kept(mask, d_o, at::kBool, {d_o.size(0), keys}, what);
 }
 
 struct Attention : torch::autograd::Function<Attention> {
@@ -332,7 +329,7 @@ struct Attention : torch::autograd::Function<Attention> {
     const Tensor mask = get(m);
     auto [o, lse] = attention_forward(q, k, v, mask, causal, scale);
     ctx->save_for_backward({q, k, v, o, lse, mask});
-    keep(ctx, causal, scale, lse, k, mask);
+    keep(ctx, causal, scale, lse);
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -341,9 +338,12 @@ struct Attention : torch::autograd::Function<Attention> {
     if (!grads[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
     c10::cuda::CUDAGuard guard(grads[0].device());
-    const std::vector<int64_t> keys = ctx->saved_data["keys"].toIntVector();
-    for (int i = 0; i < 3; ++i) kept(s[i], grads[0], grads[0].scalar_type(), i ? at::IntArrayRef(keys) : grads[0].sizes(), "attention");
-    kept_results(ctx, s[3], s[4], s[5], grads[0], "attention");
+    const Tensor& d_o = grads[0];
+    const int64_t keys = s[1].dim() == 4 ? s[1].size(1) : 0, heads = s[1].dim() == 4 && s[1].size(2) ? s[1].size(2) : 1;
+    TORCH_CHECK(d_o.size(2) % heads == 0, "attention: a saved tensor came back as another");
+    kept(s[0], d_o, d_o.scalar_type(), d_o.sizes(), "attention");
+    for (int i = 1; i < 3; ++i) kept(s[i], d_o, d_o.scalar_type(), {d_o.size(0), keys, heads, d_o.size(3)}, "attention");
+    kept_results(s[3], s[4], s[5], d_o, keys, "attention");
     for (int i = 0; i < 3; ++i) out[i] = at::empty(s[i].sizes(), s[i].options());
     attention_backward(s[0], s[1], s[2], s[3], s[4], grads[0], s[5], ctx->saved_data["causal"].toBool(),
                        ctx->saved_data["scale"].toDouble(), out[0], out[1], out[2]);
@@ -358,7 +358,7 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
     const Tensor mask = get(m);
     auto [o, lse] = attention_forward(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2), mask, causal, scale);
     ctx->save_for_backward({qkv, o, lse, mask});
-    keep(ctx, causal, scale, lse, o, mask);
+    keep(ctx, causal, scale, lse);
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
@@ -369,7 +369,7 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
     c10::cuda::CUDAGuard guard(grads[0].device());
     const auto size = grads[0].sizes();
     const Tensor qkv = kept(s[0], grads[0], grads[0].scalar_type(), {size[0], size[1], 3, size[2], size[3]}, "self_attention");
-    kept_results(ctx, s[1], s[2], s[3], grads[0], "self_attention");
+    kept_results(s[1], s[2], s[3], grads[0], size[1], "self_attention");
     const Tensor d = at::empty(qkv.sizes(), qkv.options());
     attention_backward(qkv.select(2, 0), qkv.select(2, 1), qkv.select(2, 2), s[1], s[2], grads[0], s[3],
                        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(), d.select(2, 0), d.select(2, 1),
