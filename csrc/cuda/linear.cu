@@ -529,7 +529,8 @@ int product(const HpProduct& a, cudaStream_t s) {
 }
 
 // --------------------------------------------------- the gradient before the activation
-// g = dy act'(pre) and the sums of its columns, in one pass over dy and pre: traffic bound.  A
+// g = dy act'(pre) and the sums of its columns, in one pass over dy and pre: traffic bound.  pre is kept
+// in 16 bits, half the traffic of both passes, and g rounded to them, since products take no others.  A
 // thread has V columns (16 bytes where all rows lie on that boundary, else 4 or 2) and the rows
 // of its warp; the CTA's eight warps add up their sums, and leave one row of partial sums.
 constexpr int kSlopeWarps = 8;

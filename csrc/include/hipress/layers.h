@@ -2,8 +2,9 @@
 // attention.  Every function takes a structure of its arguments and the stream.
 //
 // Return values as in capi.h.  Kernels that wait (for copies or matrix products of their
-// own CTA) bound every wait; one that expired is reported by the next call on that device
-// with HP_ERR_TIMEOUT.
+// own CTA) bound every wait but that for room in tensor memory, which the CTAs that hold it end
+// (tcgen05.cuh says why); one that expired is reported by the next call on that device with
+// HP_ERR_TIMEOUT.
 #pragma once
 #include <stdint.h>
 
@@ -14,7 +15,7 @@
 #define HP_BF16 1
 #define HP_F16 2
 
-// activations of HpLinear
+// activations of HpProduct and HpSlope
 #define HP_ACT_NONE 0
 #define HP_ACT_RELU 1
 #define HP_ACT_GELU 2       // p Phi(p)
