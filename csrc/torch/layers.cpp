@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "hipress/capi.h"
@@ -74,9 +76,28 @@ bool wants(AutogradContext* ctx, int64_t present, int i) {
   for (int k = 0; k < i; ++k) edge += present >> k & 1;
   return (present >> i & 1) && ctx->needs_input_grad(edge);
 }
-void once(const variable_list& grads, const char* what) {
-  if (at::GradMode::is_enabled())
-    for (const Tensor& g : grads) TORCH_CHECK(!wanted(g), what, ": its gradient cannot be differentiated");
+// A backward pass whose results have no graph.  Where one is wanted (create_graph) they say so when they
+// are differentiated by what they were made from (the inputs, and the gradients that came in), whether
+// or not these gradients have a graph themselves.  What is handed on unchanged keeps the graph that it has.
+variable_list first_order(variable_list (*gradients)(AutogradContext*, const variable_list&), AutogradContext* ctx,
+                          const variable_list& grads) {
+  variable_list out;
+  {
+    at::NoGradGuard guard;
+    out = gradients(ctx, grads);
+  }
+  if (!at::GradMode::is_enabled()) return out;
+  torch::autograd::edge_list made_from = torch::autograd::get_current_node()->next_edges();
+  for (const Tensor& g : grads)
+    if (wanted(g)) made_from.push_back(torch::autograd::impl::gradient_edge(g));
+  const auto refused = std::make_shared<torch::autograd::Error>("a gradient of a layer operator cannot be differentiated",
+                                                                std::move(made_from));
+  for (Tensor& g : out) {
+    bool same = !g.defined();
+    for (const Tensor& x : grads) same = same || (x.defined() && g.is_same(x));
+    if (!same) torch::autograd::set_history(g = g.detach(), refused);
+  }
+  return out;
 }
 
 // A saved tensor as it comes back.  Hooks may have kept it elsewhere, and return it in strides of
@@ -132,7 +153,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return n.z.defined() ? variable_list{n.y, n.z} : variable_list{n.y};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once(grads, "layer_norm");
+    return first_order(gradients, ctx, grads);
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor dy = grads[0], dz = grads.size() > 1 ? grads[1] : Tensor(), any = dy.defined() ? dy : dz;
     if (!any.defined()) return variable_list(5);
@@ -227,7 +250,9 @@ struct Linear : torch::autograd::Function<Linear> {
     return f.y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once(grads, "linear");
+    return first_order(gradients, ctx, grads);
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     const auto saved = ctx->get_saved_variables();
     c10::cuda::CUDAGuard guard(grads[0].device());
     const Tensor dy = rows_of(grads[0]);
@@ -333,7 +358,9 @@ struct Attention : torch::autograd::Function<Attention> {
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once(grads, "attention");
+    return first_order(gradients, ctx, grads);
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(6);
     if (!grads[0].defined()) return out;
     const auto s = ctx->get_saved_variables();
@@ -362,7 +389,9 @@ struct SelfAttention : torch::autograd::Function<SelfAttention> {
     return {o, lse};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once(grads, "self_attention");
+    return first_order(gradients, ctx, grads);
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(4);
     if (!grads[0].defined()) return out;
     const auto s = ctx->get_saved_variables();

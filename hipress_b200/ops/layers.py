@@ -20,10 +20,10 @@ The reference (mark14wu/hipress) leaves the layers to its front ends.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .._native import lib as _lib
 
@@ -53,6 +53,34 @@ def _wide(x):
 
 def _rows(x):
     return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])   # also of no elements
+
+
+class _Refused(torch.autograd.Function):
+    """A value as it is, which cannot be differentiated by what it was made from."""
+
+    @staticmethod
+    def forward(ctx, x, *made_from):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("a gradient of a layer operator cannot be differentiated")
+
+
+def _first_order(backward):
+    """For a backward pass whose results have no graph; the node has saved all its inputs.  Where a graph is
+    wanted (``create_graph``) the results say so when they are differentiated, whether or not the
+    gradient that came in has a graph itself."""
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        made_from = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+        # what is handed on unchanged keeps the graph that it has
+        return tuple(g if g is None or any(g is x for x in grads) else _Refused.apply(g.detach(), *made_from) for g in out)
+    return run
 
 
 # ================================================================== layer norm
@@ -97,15 +125,15 @@ class _LayerNorm(torch.autograd.Function):
             y = y * _wide(weight)
         if bias is not None:
             y = y + _wide(bias)
-        ctx.save_for_backward(z, weight, mean, rstd)
+        ctx.save_for_backward(z, weight, mean, rstd, x, bias, residual)
         ctx.bias = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
         return y.to(x.dtype), None if residual is None else z
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, dz):
-        z, weight, mean, rstd = ctx.saved_tensors
+        z, weight, mean, rstd = ctx.saved_tensors[:4]
         if dy is None and dz is None:
             return None, None, None, None, None
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
@@ -183,14 +211,14 @@ class _Linear(torch.autograd.Function):
         y = _act(p, act)
         if residual is not None:
             y = y + _wide(residual)
-        ctx.save_for_backward(x, w, p.to(x.dtype) if act else None)
+        ctx.save_for_backward(x, w, p.to(x.dtype) if act else None, weight, bias, residual)
         ctx.act, ctx.types = act, (weight.dtype, None if bias is None else bias.dtype)
         return y.to(x.dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
-        x, w, pre = ctx.saved_tensors
+        x, w, pre = ctx.saved_tensors[:3]
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
         g = _wide(dy) if pre is None else _wide(dy) * _act_slope(_wide(pre), ctx.act)
         db = _rows(g).sum(0).to(ctx.types[1]) if need_b else None
@@ -296,7 +324,7 @@ class _Attention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, do, _):
         if do is None:
             return (None,) * 6

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from _layers import close, norm64
+from test_layers_cpu_edges import OPERATORS, check_second_derivatives
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,8 @@ def test_a_wait_that_ran_out_is_reported_by_the_next_call():
     with pytest.raises(RuntimeError, match="gave up waiting"):
         linear(x, x)
     assert torch.equal(linear(x, x), want)    # said once; the device is usable
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_second_derivatives_are_refused(name):
+    check_second_derivatives("cuda", BF16, name)

@@ -38,3 +38,37 @@ def test_slope_of_very_large_values(kind):
     y = linear(x, torch.ones(1, 1), activation=kind)
     dx, = torch.autograd.grad(y, x, torch.ones_like(y))
     assert dx.flatten().tolist() == [1.0, 1.0, 0.0, 0.0] and (y[2:] == 0).all()
+
+
+def operators(device, dtype):
+    """Each operator and the leaves of one call."""
+    from hipress_b200.ops import attention, layer_norm, self_attention
+    torch.manual_seed(7)
+    g = lambda *s: torch.randn(*s, device=device).to(dtype).requires_grad_(True)  # noqa: E731
+    x, r, nw, lw, q, k, qkv = g(6, 16), g(6, 16), g(16), g(8, 16), g(1, 5, 2, 8), g(1, 7, 2, 8), g(1, 5, 3, 2, 8)
+    return {"layer_norm": (lambda: layer_norm(x, nw), (x, nw)),
+            "layer_norm residual": (lambda: sum(layer_norm(x, nw, residual=r)), (x, nw, r)),
+            "linear": (lambda: linear(x, lw), (x, lw)), "linear gelu": (lambda: linear(x, lw, activation="gelu"), (x, lw)),
+            "attention": (lambda: attention(q, k, k), (q, k)), "self_attention": (lambda: self_attention(qkv), (qkv,))}
+
+
+def check_second_derivatives(device, dtype, name):
+    """They are refused, also where the gradient that comes in is a constant; the first ones are not."""
+    call, leaves = operators(device, dtype)[name]
+    want = torch.autograd.grad(call().sum(), leaves)
+    got = torch.autograd.grad(call().sum(), leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    penalty = sum(t.float().square().sum() for t in got)
+    with pytest.raises(RuntimeError, match="differentiate"):
+        torch.autograd.grad(call().float().square().sum() + penalty, leaves)
+    got = torch.autograd.grad(call().float().square().sum(), leaves, create_graph=True)   # a gradient that has one itself
+    with pytest.raises(RuntimeError, match="differentiate"):
+        torch.autograd.grad(got[0].float().square().sum(), leaves[0])
+
+
+OPERATORS = ["layer_norm", "layer_norm residual", "linear", "linear gelu", "attention", "self_attention"]
+
+
+@pytest.mark.parametrize("name", OPERATORS)
+def test_second_derivatives_are_refused(name):
+    check_second_derivatives("cpu", torch.float32, name)
