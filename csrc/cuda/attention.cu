@@ -506,22 +506,33 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
 // 64 rows, first -lse / c of each row in three parts that add up to it and have 11 bits each, then
 // -delta likewise.  The fourth word of such a row meets a zero in the product and is used otherwise:
 // in the first tile what dS of this row is multiplied by (2^..), in the second, for the first of the
-// rows that a CTA of attention_rows() has, the exponent of the largest of them.  Behind the last row, and where a row saw nothing, lse is so large that every
-// probability comes out as zero.
+// rows that a CTA of attention_rows() has, the exponent of the largest of them.  Behind the last row,
+// and where a row saw nothing, lse is so large that every probability comes out as zero.
 constexpr int kRowWords = 10, kPass = 64;
 constexpr float kNever = 1e35f;
 
 // In fp16 probabilities and dS = P (dP - delta) would leave the type's range downwards where rows are
 // long or d_o is small: P is 1 / keys on average, and below 2^-25 nothing is left.  Both are therefore
 // held times powers of two that the results' scale takes out again.  P, which is 1 at most, times
-// 2^kUpP.  dS times 2^(1 - m), with m the exponent of |d_o|: of the query's own row for dq, of the
+// 2^kUpP: all its bits down to 2^-24, and room for the 2^6 that scores near 2^26 may be off by, whose 32
+// bits no longer hold the digits behind the point; what is beyond stops at the largest number.  dS times 2^(1 - m), with m the exponent of |d_o|: of the query's own row for dq, of the
 // largest row for dk, whose sum runs over the queries.  It is less than 2 |v| then (P (1 - P) is 1/4
 // at most, and |dP - dP'| at most 2 |d_o| |v|), which fits for |v| up to 32752.  Bfloat16 has the
 // exponents of 32 bits and needs none of this.
 template <typename T>
 constexpr bool kNarrow = std::is_same<T, __half>::value;
 template <typename T>
-constexpr int kUpP = kNarrow<T> ? 14 : 0;
+constexpr int kUpP = kNarrow<T> ? 10 : 0;
+template <typename T>
+__device__ __forceinline__ uint32_t pack_p(float x, float y) {   // probabilities
+  if constexpr (kNarrow<T>) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+  } else {
+    return pack2<T>(x, y);
+  }
+}
 constexpr int kNoRow = -1000;   // exponent of a row of zeros, or of one that is not finite
 // m from the sum of a row's squares
 __device__ __forceinline__ int row_exponent(float squares) {
@@ -901,7 +912,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
             if (!(two & 1)) pr.x = ds.x = 0.f;
             if (!(two & 2)) pr.y = ds.y = 0.f;
           }
-          if (of_keys) x[i / 2] = pack2<T>(pr.x, pr.y);
+          if (of_keys) x[i / 2] = pack_p<T>(pr.x, pr.y);
           y[i / 2] = pack2<T>(ds.x, ds.y);
         }
       };
@@ -1114,7 +1125,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
                 if (!(two & 1)) pr.x = ds.x = 0.f;
                 if (!(two & 2)) pr.y = ds.y = 0.f;
               }
-              x[(i + k) / 2] = pack2<T>(pr.x, pr.y);
+              x[(i + k) / 2] = pack_p<T>(pr.x, pr.y);
               y[(i + k) / 2] = pack2<T>(ds.x, ds.y);
             }
           }

@@ -12,6 +12,9 @@ gradient in front of an activation are rounded to the inputs' type where they en
 product.  Results do not depend on the order in which thread blocks run: two calls with the
 same inputs give the same bits.
 
+First derivatives only: a gradient taken with ``create_graph`` refuses to be differentiated, and
+forward mode is refused.
+
 Under autocast ``linear`` and ``attention`` cast 32-bit activations to autocast's type;
 ``layer_norm`` keeps the type of ``x``.  Weights may be in 32 bits or in the activations'
 type, and get their gradient in their own type.

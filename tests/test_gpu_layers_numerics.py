@@ -179,3 +179,16 @@ def test_layer_norm_lengths_that_fill_shared_memory(dtype, cols, residual):
     for name, got, kind in (("y", out[0] if residual else out, dtype), ("dx", dx, dtype), ("dw", dw, FP32), ("db", db, FP32)):
         exact, scale = want[name]
         assert ((got.double() - exact).abs() <= U[kind] * exact.abs() + steps * 2.0 ** -23 * scale.abs().amax(-1, keepdim=True)).all(), name
+
+
+def test_attention_gradients_of_scores_that_32_bits_cannot_hold():
+    """Scores of 10^7: the probabilities are those of rounded scores, and every gradient a number."""
+    from hipress_b200.ops import attention
+    torch.manual_seed(8)
+    for sq, sk, dim in ((100, 128, 64), (300, 500, 64), (300, 260, 128)):
+        q, k = rand(1, sq, 1, dim, dtype=FP16, std=3000), rand(1, sk, 1, dim, dtype=FP16, std=3000)
+        v, do = rand(1, sk, 1, dim, dtype=FP16), rand(1, sq, 1, dim, dtype=FP16, std=2.0 ** -10)
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = attention(*leaves)
+        for t in (out, *torch.autograd.grad(out, leaves, do)):
+            assert torch.isfinite(t).all()
