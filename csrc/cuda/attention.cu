@@ -2,6 +2,7 @@
 #include <type_traits>
 
 #include "activation.cuh"
+#include "philox.cuh"
 #include "tcgen05.cuh"
 
 namespace hipress {
@@ -16,29 +17,6 @@ __device__ __forceinline__ uint32_t staged(int r, int b) { return (uint32_t)(r *
 // 2^x for the softmax is exp2_fast(); what a masked score becomes
 constexpr float kNone = -INFINITY;
 
-// Two values at a time: half the instructions for what is not 2^x.
-struct F2 {
-  float x, y;
-};
-__device__ __forceinline__ uint64_t bits(F2 v) {
-  return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
-}
-__device__ __forceinline__ F2 f2(uint64_t v) { return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))}; }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return f2(d);
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return f2(d);
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-  return f2(d);
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -116,10 +94,29 @@ struct Maps {
 struct Launch {
   Maps map;
   HpAttention p;
+  Drop drop;           // of the probabilities, in kernels with DROP
   float c;             // |scale| log2(e)
   int negative;        // scale < 0
   uint32_t* status;
 };
+
+// ---------------------------------------------------------------------- dropout
+// Rows of probabilities go by words of 32 keys.  The first word of a query's row:
+__device__ __forceinline__ uint64_t first_word(const HpAttention& p, int64_t b, int h, int row) {
+  return (uint64_t)((b * p.heads + h) * p.sq + row) * (uint64_t)((p.sk + 31) / 32);
+}
+// By a whole warp: lane i's bit j becomes lane j's bit i.  Where a thread has a key, each lane makes the word of
+// one query for the warp's 32 keys, and gets those of 32 queries for its own.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const uint32_t m = 0xffffffffu / ((1u << o) + 1);   // bits whose place has no o
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, o);
+    x = lane & o ? (x & ~m) | ((y & ~m) >> o) : (x & m) | ((y & m) << o);
+  }
+  return x;
+}
 
 // ---------------------------------------------------------------------- forward
 // A CTA has QT tiles of 128 queries of one head and walks over the keys, 128 at a time: scores
@@ -160,7 +157,7 @@ struct ForwardBars {
   Guard guard;
 };
 
-template <typename T, int DP, int QT, bool SHORT>
+template <typename T, int DP, int QT, bool SHORT, bool DROP>
 __global__ void __launch_bounds__((Forward<DP, QT, SHORT>::kThreads), (Forward<DP, QT, SHORT>::kPerSm))
 attention_forward_tiles(const __grid_constant__ Launch l) {
   using F = Forward<DP, QT, SHORT>;
@@ -316,7 +313,13 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     bool ok = true;
     int s = 0;
     uint32_t ph = 0;
+    Key key = {};
+    if (DROP) key = drop_key(l.drop);
     for (int j = 0; j < nt; ++j) {
+      Seen<kB> kept;
+      if (DROP)   // before the scores are there, and take the registers
+#pragma unroll
+        for (int i = 0; i < kB / 32; ++i) kept.w[i] = kept_word(l.drop, key, first_word(p, b, h, row) + j * (kB / 32) + i);
       Seen<kB> seen;
       bool whole = sees >= (j + 1) * kB;
       if (masked) {
@@ -434,6 +437,10 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
               e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
             }
             sums[i / 2 & 1] = add2(sums[i / 2 & 1], e);
+            if (DROP) {   // the sum is of all
+              const uint32_t two = kept.w[c / 32] >> (c % 32 + i);
+              e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
+            }
             to_y[i / 2] = pack2<T>(e.x, e.y);
           }
           if constexpr (SHORT) tmem_st8(tp + c / 2, *(const uint32_t(*)[8])y);
@@ -452,7 +459,7 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
       mbar_arrive(&bar.p_full[t]);
     }
     const bool some = sum != 0.f;   // NaN too
-    const float inv = some ? 1.f / sum : 0.f;
+    const float inv = some ? (DROP ? l.drop.up : 1.f) / sum : 0.f;
     if (row < p.sq) p.lse[(b * p.heads + h) * p.sq + row] = some ? (m + log2f(sum)) * 0.6931471805599453f : kNone;
     if (ok && nt) ok = guard_wait(&bar.o_full[t], (nt - 1) & 1, g, 0x30005);
     else if (ok && most) ok = guard_wait(&bar.q_full, 0, g, 0x30006);   // the copy into the space used below
@@ -552,8 +559,15 @@ __device__ __forceinline__ float4 three_parts(float v) {
 // delta is made from the result as the forward pass rounded it, o in 32 bits being kept by nobody: one
 // error for a whole row of dS.  With it fp16 dq and dk of short rows are off by up to 2.3 times what
 // a result is that is rounded once.
-template <typename T, int LANES>   // that share a row, 16 bytes each
-__global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ HpAttention a, float c) {
+//
+// With a dropout of probabilities, m / share times P in front of v, dP is zero where m is, and dS = P (m dP / share -
+// delta).  It is held times the share, P (m dP - share delta), and dq and dk are divided by it.  The product
+// cannot add delta to a dP that is dropped: in place of the second tile's parts lies share delta of each row,
+// 32 floats from the fifth on and 32 from the 69th, between the words that are used otherwise.
+__device__ __forceinline__ int delta_at(int row) { return 4 + row / 32 * 64 + row % 32; }
+
+template <typename T, int LANES, bool DROP>   // LANES share a row, 16 bytes each
+__global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ HpAttention a, float c, float share) {
   const int lane = threadIdx.x % LANES;
   const int64_t i = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES, h = blockIdx.y, b = blockIdx.z;
   const int64_t rows = padded(a.sq);
@@ -591,12 +605,19 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
     float* out = a.delta + (b * a.heads + h) * kRowWords * rows;
     float4* parts = (float4*)(out + 2 * rows) + i / kPass * 2 * kPass + i % kPass;
     const bool none = lse == -INFINITY;
+    if (DROP) s *= share;
     out[i] = none ? -kNever : (float)up - lse;
     out[rows + i] = -s;
     float4 first = none ? make_float4(-kNever, 0.f, 0.f, 0.f) : three_parts(((float)kUpP<T> - lse) / c), second = three_parts(-s);
     if (kNarrow<T>) first.w = power_of_two(up), second.w = (float)largest;
     parts[0] = first;
-    parts[kPass] = second;
+    if (!DROP) {
+      parts[kPass] = second;
+    } else {
+      float* tile = (float*)(parts - i % kPass + kPass);
+      tile[delta_at((int)(i % kPass))] = -s;
+      if (kNarrow<T> && i % (256 / LANES) == 0) tile[i % kPass * 4 + 3] = second.w;
+    }
   }
 }
 
@@ -651,7 +672,7 @@ __device__ __forceinline__ int largest_row(const float* delta, int heads, int64_
   return *shared;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool DROP>
 __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_constant__ Launch l) {
   using F = Backward<DP>;
   extern __shared__ uint8_t raw[];
@@ -802,7 +823,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
             tmem_fence_after();
             const uint32_t d = tmem + F::kBuffer * q + (of_dp ? kPass : 0);
             wide(d, a, in(s) + (of_dp ? F::kPassed : 0), id_w);
-            if (keys)
+            if (keys && !(DROP && of_dp))
               mma_tf32(leader, d, mma_desc_plain(smem_u32(ones) + (of_dp ? F::kOnes : 0), kB * 16, 128),
                        mma_desc_plain(smem_u32(parts + s * F::kParts), kPass * 16, 128), mma_idesc_tf32(128, kPass), true);
             mma_commit<1>(leader, &bar.s_full[turn]);
@@ -843,6 +864,8 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     }
     const int sees = p.causal ? min(sk, row + shift + 1) : sk;
     bool ok = true;
+    Key key = {};
+    if (DROP) key = drop_key(l.drop);
     // of tile j: stage, buffer, turn, and place among its head's tiles
     int s = half, q = half, turn = half, place = half;
     uint32_t ph = 0, round = 0;
@@ -855,6 +878,18 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     };
     if (n && place >= count) place -= count;   // a head of one tile
     for (int j = half; j < n; j += 2, advance()) {
+      Seen<kPass> kept;
+      if (DROP) {
+#pragma unroll
+        for (int i = 0; i < kPass / 32; ++i) {
+          if (keys) {
+            const int query = (first + place) * kPass + 32 * i + lane;
+            kept.w[i] = transposed(kept_word(l.drop, key, first_word(p, b, head * group + j / count, query) + (r0 / 32 + quad)));
+          } else {
+            kept.w[i] = kept_word(l.drop, key, first_word(p, b, head, row) + j * (kPass / 32) + i);
+          }
+        }
+      }
       Seen<kPass> seen;
       bool whole;
       if (keys) {
@@ -891,6 +926,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         }
       }
       if (!guard_wait(&bar.s_full[turn], round, g, 0x31003)) { ok = false; break; }
+      if (DROP && keys && !guard_wait(&bar.in_full[s], ph, g, 0x31004)) { ok = false; break; }   // delta, read below
       tmem_fence_after();
       const uint32_t at = tmem + lanes + F::kBuffer * q;
       uint32_t x[kPass], y[kPass];
@@ -900,13 +936,25 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         tmem_ld32(at + kPass + c, *(uint32_t(*)[32])(y + c));
       }
       tmem_wait_ld();
+      // with a dropout: of the passing queries
+      const float* deltas = (const float*)(parts + s * F::kParts) + 4 * kPass;
       auto gradients = [&](auto all, auto of_keys) {   // packed P into x, dS into y
 #pragma unroll
         for (int i = 0; i < kPass; i += 2) {
-          const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])}, u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
+          const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])};
+          F2 u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
           const F2 z = of_keys ? mul2(v, {l.c, l.c}) : fma2(v, {l.c, l.c}, {lse, lse});
           F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-          F2 ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys ? u : add2(u, {delta, delta}));
+          if (DROP) {
+            const uint32_t two = kept.w[i / 32] >> (i % 32);
+            u = {two & 1 ? u.x : 0.f, two & 2 ? u.y : 0.f};
+            u = add2(u, of_keys ? *(const F2*)(deltas + delta_at(i)) : F2{delta, delta});
+          }
+          F2 ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys || DROP ? u : add2(u, {delta, delta}));
+          if (DROP) {
+            const uint32_t two = kept.w[i / 32] >> (i % 32);
+            pr = {two & 1 ? pr.x : 0.f, two & 2 ? pr.y : 0.f};
+          }
           if (!all) {
             const uint32_t two = seen.w[i / 32] >> (i % 32);
             if (!(two & 1)) pr.x = ds.x = 0.f;
@@ -940,7 +988,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
         const bool is_v = keys && job < F::kPanels;   // dv first, then dk; or dq alone
         const int panel = job % F::kPanels;
         const uint32_t from = tmem + lanes + (is_v ? F::kAcc1 : F::kAcc2) + 64 * panel;
-        const float scale = is_v ? 1.f / (float)(1 << kUpP<T>) : (float)p.scale / ds_scale;
+        const float scale = (is_v ? 1.f / (float)(1 << kUpP<T>) : (float)p.scale / ds_scale) * (DROP ? l.drop.up : 1.f);
         uint8_t* to = stay + job * kPanel + 32 * quad * 128;
 #pragma unroll 1
         for (int c = 0; c < 64; c += 32) {
@@ -995,7 +1043,7 @@ struct ShortBars {
 };
 constexpr int kShortSmem = 6 * (int)kPanel + 2048 + 1024;
 
-template <typename T>
+template <typename T, bool DROP>
 __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_constant__ Launch l) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
@@ -1079,12 +1127,19 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
           for (int i = 0; i < 8; ++i) squares = fmaf(x[i], x[i], squares);
       }
       bar.lse[r] = lse == -INFINITY ? -INFINITY : (float)kUpP<T> - lse * kLog2e;
-      bar.delta[r] = -d;
+      bar.delta[r] = DROP ? -d * l.drop.share : -d;
       if (kNarrow<T>) {
         const int e = __reduce_max_sync(0xffffffffu, row_exponent(squares));
         if (lane == 0) atomicMax(&bar.largest, e);
       }
       mbar_arrive(&bar.rows_full);
+    }
+    uint32_t kept[2];   // of this thread's 64 queries
+    if (DROP) {
+      const Key key = drop_key(l.drop);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        kept[i] = transposed(kept_word(l.drop, key, first_word(p, b, h, 64 * half + 32 * i + lane) + quad));
     }
     const int from = p.causal ? r - shift : 0;   // the first query that sees this key
     bool whole = mine && from <= 0;
@@ -1119,7 +1174,11 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
             for (int k = 0; k < 4; k += 2) {
               const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {lv[k], lv[k + 1]});
               F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-              F2 ds = mul2(kNarrow<T> ? mul2(pr, {of_p, of_p}) : pr, add2({__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])}, {dv[k], dv[k + 1]}));
+              F2 u = {__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])};
+              const uint32_t stay = DROP ? (c & 32 ? kept[1] : kept[0]) >> (i + k) : 3;
+              if (DROP) u = {stay & 1 ? u.x : 0.f, stay & 2 ? u.y : 0.f};
+              F2 ds = mul2(kNarrow<T> ? mul2(pr, {of_p, of_p}) : pr, add2(u, {dv[k], dv[k + 1]}));
+              if (DROP) pr = {stay & 1 ? pr.x : 0.f, stay & 2 ? pr.y : 0.f};
               if (!all) {
                 const uint32_t two = bits_of >> (i + k);
                 if (!(two & 1)) pr.x = ds.x = 0.f;
@@ -1159,10 +1218,10 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
       }
     };
     if (ok) {
-      const float scale = (float)p.scale * power_of_two(-up);
+      const float of_all = DROP ? l.drop.up : 1.f, scale = (float)p.scale * power_of_two(-up) * of_all;
       uint8_t* to = half ? sq_ : sv_;
 #pragma unroll 1
-      for (int c = 0; c < 64; c += 32) emit(128 + 64 * half + c, half ? scale : 1.f / (float)(1 << kUpP<T>), to, c);
+      for (int c = 0; c < 64; c += 32) emit(128 + 64 * half + c, half ? scale : of_all / (float)(1 << kUpP<T>), to, c);
       emit(32 * half, scale, sg_, 32 * half);
       fence_async_shared();
       __syncwarp();
@@ -1221,13 +1280,14 @@ int prepare(Launch& l, const HpAttention& a) {
   l.c = (float)(a.scale < 0 ? -a.scale : a.scale) * kLog2e;
   if (l.c < 1e-20f) l.c = 1e-20f;
   l.negative = a.scale < 0;
+  if (a.drop.keep && !drop_of(&l.drop, a.drop)) return HP_ERR_BAD_ARG;
   return rc;
 }
 
-template <typename T, int DP, int QT, bool SHORT = false>
+template <typename T, int DP, int QT, bool SHORT, bool DROP>
 int forward_tiles(Launch& l, cudaStream_t s) {
   using F = Forward<DP, QT, SHORT>;
-  const auto kernel = attention_forward_tiles<T, DP, QT, SHORT>;
+  const auto kernel = attention_forward_tiles<T, DP, QT, SHORT, DROP>;
   static PerDevice allowed;
   if (const int rc = allow_shared_memory(allowed, kernel, F::kSmem)) return rc;
   const HpAttention& a = l.p;
@@ -1242,48 +1302,48 @@ int forward_tiles(Launch& l, cudaStream_t s) {
   return launch_behind(kernel, grid, F::kThreads, F::kSmem, s, l);
 }
 
-template <typename T>
+template <typename T, bool DROP>
 int forward(const HpAttention& a, cudaStream_t s) {
   Launch l;
   if (const int rc = prepare(l, a)) return rc;
   if (a.dim <= 64)
-    return a.sq <= kB && a.sk <= kB ? forward_tiles<T, 64, 1, true>(l, s) : forward_tiles<T, 64, 1>(l, s);
+    return a.sq <= kB && a.sk <= kB ? forward_tiles<T, 64, 1, true, DROP>(l, s) : forward_tiles<T, 64, 1, false, DROP>(l, s);
   // Two tiles of queries in a CTA pay once there are more tiles than SMs, and twice as many where the
   // mask makes them uneven.  One tile a CTA against two, in us, bfloat16, 148 SMs:
   //   1 x 1024, 8 heads: 20 to 26           1 x 2048, 16 heads, causal: 38 to 43
   //   1 x 2048, 12 heads: 66 to 46          1 x 2048, 24 heads, causal: 57 to 44
   const int64_t tiles = (a.sq + kB - 1) / kB * a.heads * a.batch;
   const bool two = a.sq > kB && tiles > (a.causal ? 2 : 1) * layer_sms();
-  return two ? forward_tiles<T, 128, 2>(l, s) : forward_tiles<T, 128, 1>(l, s);
+  return two ? forward_tiles<T, 128, 2, false, DROP>(l, s) : forward_tiles<T, 128, 1, false, DROP>(l, s);
 }
 
-template <typename T>
+template <typename T, bool DROP>
 int backward_short(const Launch& l, cudaStream_t s) {
-  const auto kernel = attention_backward_short<T>;
+  const auto kernel = attention_backward_short<T, DROP>;
   static PerDevice allowed;
   if (const int rc = allow_shared_memory(allowed, kernel, kShortSmem)) return rc;
   if (l.p.heads * l.p.batch > INT32_MAX) return HP_ERR_TOO_LARGE;
   return launch_behind(kernel, (unsigned)(l.p.heads * l.p.batch), 320, kShortSmem, s, l);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool DROP>
 int backward_tiles(const Launch& l, cudaStream_t s) {
   using F = Backward<DP>;
   static PerDevice allowed;
-  if (const int rc = allow_shared_memory(allowed, attention_backward_tiles<T, DP>, F::kSmem)) return rc;
+  if (const int rc = allow_shared_memory(allowed, attention_backward_tiles<T, DP, DROP>, F::kSmem)) return rc;
   const HpAttention& a = l.p;
   const int64_t nq = (a.sq + kB - 1) / kB, nk = (a.sk + kB - 1) / kB, tiles = (nk * a.kv_heads + nq * a.heads) * a.batch;
   if (tiles > INT32_MAX) return HP_ERR_TOO_LARGE;
   if (a.sq) {
     constexpr int kLanes = DP / 8;
-    if (const int rc = launch_behind(attention_rows<T, kLanes>, dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch),
-                                     256, 0, s, a, l.c))
+    if (const int rc = launch_behind(attention_rows<T, kLanes, DROP>, dim3((unsigned)(padded(a.sq) / (256 / kLanes)), (unsigned)a.heads, (unsigned)a.batch),
+                                     256, 0, s, a, l.c, DROP ? l.drop.share : 1.f))
       return rc;
   }
-  return launch_behind(attention_backward_tiles<T, DP>, (unsigned)tiles, F::kThreads, F::kSmem, s, l);
+  return launch_behind(attention_backward_tiles<T, DP, DROP>, (unsigned)tiles, F::kThreads, F::kSmem, s, l);
 }
 
-template <typename T>
+template <typename T, bool DROP>
 int backward(const HpAttention& a, cudaStream_t s) {
   if (!a.sq && !a.sk) return 0;
   Launch l;
@@ -1301,8 +1361,8 @@ int backward(const HpAttention& a, cudaStream_t s) {
       !map(&l.map.q64, a.q, false, a.q_b, a.q_s, a.q_h, kPass) || !map(&l.map.k64, a.k, true, a.k_b, a.k_s, a.k_h, kPass) ||
       !map(&l.map.v64, a.v, true, a.v_b, a.v_s, a.v_h, kPass) || !map(&l.map.do64, a.d_o, false, a.do_b, a.do_s, a.do_h, kPass))
     return HP_ERR_BAD_ARG;
-  if (a.dim <= 64 && a.sq <= kB && a.sk <= kB && a.heads == a.kv_heads && a.sq && a.sk) return backward_short<T>(l, s);
-  return a.dim <= 64 ? backward_tiles<T, 64>(l, s) : backward_tiles<T, 128>(l, s);
+  if (a.dim <= 64 && a.sq <= kB && a.sk <= kB && a.heads == a.kv_heads && a.sq && a.sk) return backward_short<T, DROP>(l, s);
+  return a.dim <= 64 ? backward_tiles<T, 64, DROP>(l, s) : backward_tiles<T, 128, DROP>(l, s);
 }
 
 }  // namespace
@@ -1314,12 +1374,14 @@ extern "C" int hp_cuda_attention_forward(const HpAttention* a, void* stream) {
   if (!args_ok(a)) return HP_ERR_BAD_ARG;
   if (!a->batch || !a->sq) return 0;
   cudaStream_t s = (cudaStream_t)stream;
-  return a->type == HP_BF16 ? forward<__nv_bfloat16>(*a, s) : forward<__half>(*a, s);
+  if (a->drop.keep) return a->type == HP_BF16 ? forward<__nv_bfloat16, true>(*a, s) : forward<__half, true>(*a, s);
+  return a->type == HP_BF16 ? forward<__nv_bfloat16, false>(*a, s) : forward<__half, false>(*a, s);
 }
 
 extern "C" int hp_cuda_attention_backward(const HpAttention* a, void* stream) {
   if (!args_ok(a)) return HP_ERR_BAD_ARG;
   if (!a->batch) return 0;
   cudaStream_t s = (cudaStream_t)stream;
-  return a->type == HP_BF16 ? backward<__nv_bfloat16>(*a, s) : backward<__half>(*a, s);
+  if (a->drop.keep) return a->type == HP_BF16 ? backward<__nv_bfloat16, true>(*a, s) : backward<__half, true>(*a, s);
+  return a->type == HP_BF16 ? backward<__nv_bfloat16, false>(*a, s) : backward<__half, false>(*a, s);
 }

@@ -3,11 +3,25 @@
 // No operand is used twice outside its row, so the bound is the traffic: x (residual) in, y (z)
 // out; z and dy (dz) in, dx out.  A row is read once and stays in registers, in 32 bits, for its
 // mean, the sum of its squared deviations and the result.
+//
+// Compiled twice, side by side: by itself, and by layer_norm_dropout.cu with HIPRESS_NORM_DROPOUT, which
+// makes the kernels of rows with a dropout of x in front of the residual sum.
 #include "column_sums.cuh"
+#include "philox.cuh"
 #include "tcgen05.cuh"
 
 namespace hipress {
 namespace {
+
+#ifdef HIPRESS_NORM_DROPOUT
+constexpr bool kDropout = true;
+using MaybeDrop = Drop;
+#else
+constexpr bool kDropout = false;
+struct MaybeDrop {
+  static constexpr float up = 1.f;
+};
+#endif
 
 template <typename T>
 __global__ void __launch_bounds__(256) norm_forward_kernel(const __grid_constant__ HpNormForward a) {
@@ -333,9 +347,54 @@ __device__ __forceinline__ void start_ring(Ring<T, N, RAGGED>& ring, uint8_t* sp
   for (int s = 0; s < ring.depth; ++s) ring.fetch(first + s * step, s);
 }
 
+// Which elements of a piece a dropout keeps, a bit each; by whole warps, whose lanes' pieces lie side by
+// side from element `at` of the tensor on (the lane's own).  Four lanes share a word of 32 elements or part
+// of one, and each makes one of its four calls; two words where their pieces lie across two.  A call's four
+// comparisons turn what the lower calls leave, m, into b | (a & m): a is what they make of ones, b of zeros.
+struct Bits {
+  const Drop* d;
+  Key key;
+  uint32_t mine[4];   // bits of t for this lane's call
+  template <typename D>
+  __device__ __forceinline__ void start(const D& drop) {
+    d = &drop, key = drop_key(drop);
+    const int call = threadIdx.x & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mine[i] = call == 0 ? drop.bit[i] : call == 1 ? drop.bit[4 + i] : call == 2 ? drop.bit[8 + i] : drop.bit[12 + i];
+  }
+  __device__ __forceinline__ uint32_t word(uint64_t w) const {
+    const uint32_t call = threadIdx.x & 3;
+    const uint4 r = philox(make_uint4((uint32_t)w, (uint32_t)(w >> 32), d->site, call), key);
+    uint32_t a = 0xffffffffu, b = 0;
+    a = majority(r.x, a, mine[0]), b = majority(r.x, b, mine[0]);
+    a = majority(r.y, a, mine[1]), b = majority(r.y, b, mine[1]);
+    a = majority(r.z, a, mine[2]), b = majority(r.z, b, mine[2]);
+    a = majority(r.w, a, mine[3]), b = majority(r.w, b, mine[3]);
+#pragma unroll
+    for (uint32_t o = 1; o < 4; o *= 2) {   // the upper calls' of the lower ones'
+      const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      const bool upper = call & o;
+      const uint32_t ua = upper ? a : oa, ub = upper ? b : ob, la = upper ? oa : a, lb = upper ? ob : b;
+      a = ub | (ua & la), b = ub | (ua & lb);
+    }
+    return b;
+  }
+  template <int V>
+  __device__ __forceinline__ uint32_t of_piece(int64_t at) const {
+    const int place = (threadIdx.x & 3) * V;
+    const int64_t first = at - place;     // the four lanes'
+    const int shift = (int)(first & 31);
+    uint64_t bits = word((uint64_t)(first >> 5));
+    if (first & (4 * V - 1)) bits |= (uint64_t)word((uint64_t)(first >> 5) + 1) << 32;   // the same for the whole warp
+    return (uint32_t)(bits >> (shift + place));
+  }
+};
+
 template <typename T, int NW, int CH, bool RAGGED>
 __global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 2 ? 3 : kCtasOf<NW>)
-norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
+norm_forward_rows(const __grid_constant__ HpNormForward a, const __grid_constant__ MaybeDrop drop, int depth, int slot_bytes, int ring_bytes,
+                  uint32_t* status) {
   constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
   extern __shared__ __align__(128) uint8_t space[];
   __shared__ float part[2][1][16];
@@ -363,9 +422,15 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
 #pragma unroll
   for (int i = 0; kHold && i < CH; ++i) weight.get(c[i], cols, phase, held[i][0]), bias.get(c[i], cols, phase, held[i][1]);
   const float inv = 1.f / (float)cols;
+  Bits random;
+  if constexpr (kDropout) random.start(drop);
   int s = 0;
   for (int64_t row = first; row < a.rows; row += step) {
     uint4 raw[CH];
+    uint32_t kept[CH];
+    if constexpr (kDropout)   // while the row is on its way
+#pragma unroll
+      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece<V>(row * cols + c[i].first);
     ring.wait(s, guard);
     if (ring.alone(row)) ring.template fill_ends<NW>(row, s, phase, t);
     auto piece = [&](int i, int k) { return c[i].take(ring.slot(s, k), cols, phase); };
@@ -379,6 +444,9 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
       if (sum_in_front) {
         float r[V];
         unpack<T>(piece(i, 1), r);
+        if constexpr (kDropout)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = kept[i] >> j & 1 ? v[j] * drop.up : 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] += r[j];
         raw[i] = pack<T>(v);   // the sum as it is stored is what is normalised
@@ -439,7 +507,8 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, int depth, int slot_b
 
 template <typename T, int NW, int CH, bool RAGGED>
 __global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 1 ? (CH == 4 ? 2 : 3) : kCtasBack<NW, RAGGED>)
-norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot_bytes, int ring_bytes, uint32_t* status) {
+norm_backward_rows(const __grid_constant__ HpNormBackward a, const __grid_constant__ MaybeDrop drop, int depth, int slot_bytes, int ring_bytes,
+                   uint32_t* status) {
   constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;
   extern __shared__ __align__(128) uint8_t space[];
   __shared__ float part[2][2][16];
@@ -481,10 +550,16 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
     }
   };
   const float inv = 1.f / (float)cols;
+  Bits random;
+  if constexpr (kDropout) random.start(drop);
   int s = 0, turn = 0;
   float mean_next = first < a.rows ? a.mean[first] : 0.f, rstd_next = first < a.rows ? a.rstd[first] : 0.f;
   for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
     uint4 zr[CH], gr[CH], ur[CH];
+    uint32_t kept[CH];
+    if constexpr (kDropout)
+#pragma unroll
+      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece<V>(row * cols + c[i].first);
     const float mean = mean_next, rstd = rstd_next;
     if (row + step < a.rows) mean_next = a.mean[row + step], rstd_next = a.rstd[row + step];
     ring.wait(s, guard);
@@ -512,7 +587,7 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
     slot_read<NW>();
     if (!guard.gave_up) ring.fetch(row + depth * step, s);
     if (++s == depth) s = 0;
-    if (!a.dx) continue;
+    if (!a.dx && !(kDropout && a.dropped)) continue;
     // rstd (g w - mean(g w) - h mean(g w h)), with h = (z - mean) rstd
     const float s1 = -sum[0] * inv * rstd, s2 = sum[1] * inv * rstd * rstd;
 #pragma unroll
@@ -529,7 +604,13 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, int depth, int slot
         d[j] = fmaf(mean - z[j], s2, fmaf(g[j], w[j] * rstd, s1));
         if (more) d[j] += up[j];
       }
-      c[i].store((T*)a.dx + row * a.cols, cols, pack<T>(d));
+      if (!kDropout || a.dx) c[i].store((T*)a.dx + row * a.cols, cols, pack<T>(d));
+      if constexpr (kDropout)
+        if (a.dropped) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[j] = kept[i] >> j & 1 ? d[j] * drop.up : 0.f;
+          c[i].store((T*)a.dropped + row * a.cols, cols, pack<T>(d));
+        }
     }
   }
   if (guard.gave_up) ring.drain(guard);
@@ -659,23 +740,23 @@ int resident(PerDevice& known, K kernel, int threads, int smem, int* ctas) {
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
-int forward_rows(const HpNormForward& a, uint32_t* status, cudaStream_t s) {
+int forward_rows(const HpNormForward& a, const MaybeDrop& d, uint32_t* status, cudaStream_t s) {
   static PerDevice known;
   int per_sm;
   if (const int rc = resident(known, norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasOf<NW>), &per_sm)) return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasOf<NW>), a.cols, a.residual ? 2 : 1, 2, false);
   return launch_behind(norm_forward_rows<T, NW, CH, RAGGED>, ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>,
-                       r.bytes, s, a, r.depth, r.slot, r.ring, status);
+                       r.bytes, s, a, d, r.depth, r.slot, r.ring, status);
 }
 template <typename T, int NW, int CH, bool RAGGED>
-int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
+int backward_rows(const HpNormBackward& a, const MaybeDrop& d, uint32_t* status, cudaStream_t s) {
   static PerDevice known;
   int per_sm;
   if (const int rc = resident(known, norm_backward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasBack<NW, RAGGED>), &per_sm))
     return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasBack<NW, RAGGED>), a.cols, a.dz ? 3 : 2, 1, true);
   const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
-  const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, r.depth, r.slot,
+  const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, d, r.depth, r.slot,
                                r.ring, status);
   if (rc || (!a.dweight && !a.dbias)) return rc;
   return column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);
@@ -700,8 +781,38 @@ int backward_rows(const HpNormBackward& a, uint32_t* status, cudaStream_t s) {
     default: break;                             \
   }
 
+// Tensors that no kernel of rows takes: a CTA a row, or (with a dropout) one operator after the other
 template <typename T>
-int forward(const HpNormForward& a, cudaStream_t s) {
+int forward_otherwise(const HpNormForward& a, cudaStream_t s) {
+#ifdef HIPRESS_NORM_DROPOUT
+  const HpDrop sum = {a.x, a.residual, a.z, a.rows * a.cols, a.type, a.drop};
+  if (const int rc = hp_cuda_dropout(&sum, s)) return rc;
+  HpNormForward n = a;
+  n.x = a.z, n.ldx = a.cols, n.residual = nullptr, n.z = nullptr, n.drop.keep = 0;
+  return hp_cuda_norm_forward(&n, s);
+#else
+  norm_forward_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
+  return cudaGetLastError();
+#endif
+}
+template <typename T>
+int backward_otherwise(const HpNormBackward& a, cudaStream_t s) {
+#ifdef HIPRESS_NORM_DROPOUT
+  HpNormBackward n = a;   // the gradient of x is made from the residual's as that is rounded
+  if (!n.dx) n.dx = a.dropped;
+  n.dropped = nullptr, n.drop.keep = 0;
+  if (const int rc = hp_cuda_norm_backward(&n, s)) return rc;
+  const HpDrop sum = {n.dx, nullptr, a.dropped, a.rows * a.cols, a.type, a.drop};
+  return a.dropped ? hp_cuda_dropout(&sum, s) : 0;
+#else
+  if (a.dx && a.rows) norm_dx_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
+  if (a.dweight || a.dbias) norm_dw_kernel<T><<<(unsigned)((a.cols + 31) / 32), dim3(32, 8), 0, s>>>(a);
+  return cudaGetLastError();
+#endif
+}
+
+template <typename T>
+int forward(const HpNormForward& a, const MaybeDrop& d, cudaStream_t s) {
   Rows r(sizeof(T), a.cols);
   r.add(a.x, a.ldx);
   r.add(a.residual, a.ldr);
@@ -712,32 +823,30 @@ int forward(const HpNormForward& a, cudaStream_t s) {
     int rc;
     uint32_t* status = layer_status(&rc);
     if (rc) return rc;
-#define CALL(nw, ch) r.ragged() ? forward_rows<T, nw, ch, true>(a, status, s) : forward_rows<T, nw, ch, false>(a, status, s)
+#define CALL(nw, ch) r.ragged() ? forward_rows<T, nw, ch, true>(a, d, status, s) : forward_rows<T, nw, ch, false>(a, d, status, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
-  norm_forward_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
-  return cudaGetLastError();
+  return forward_otherwise<T>(a, s);
 }
 template <typename T>
-int backward(const HpNormBackward& a, cudaStream_t s) {
+int backward(const HpNormBackward& a, const MaybeDrop& d, cudaStream_t s) {
   Rows r(sizeof(T), a.cols);
   r.add(a.z, a.ldz);
   r.add(a.dy, a.lddy);
   r.add(a.dz, a.lddz);
   r.add(a.dx, a.cols);
+  if (kDropout) r.add(a.dropped, a.cols);
   if (r.alike && a.rows) {
     const Split p = split_of<T>(a.cols, r.ragged());
     int rc;
     uint32_t* status = layer_status(&rc);
     if (rc) return rc;
-#define CALL(nw, ch) r.ragged() ? backward_rows<T, nw, ch, true>(a, status, s) : backward_rows<T, nw, ch, false>(a, status, s)
+#define CALL(nw, ch) r.ragged() ? backward_rows<T, nw, ch, true>(a, d, status, s) : backward_rows<T, nw, ch, false>(a, d, status, s)
     BY_SPLIT(CALL)
 #undef CALL
   }
-  if (a.dx && a.rows) norm_dx_kernel<T><<<(unsigned)a.rows, 256, 0, s>>>(a);
-  if (a.dweight || a.dbias) norm_dw_kernel<T><<<(unsigned)((a.cols + 31) / 32), dim3(32, 8), 0, s>>>(a);
-  return cudaGetLastError();
+  return backward_otherwise<T>(a, s);
 }
 
 template <typename A>
@@ -750,19 +859,45 @@ bool types_ok(const A& a) {
 
 using namespace hipress;
 
-#define BY_TYPE(fn) a->type == HP_F32 ? fn<float>(*a, s) : a->type == HP_BF16 ? fn<__nv_bfloat16>(*a, s) : fn<__half>(*a, s)
+#define BY_TYPE(fn) a->type == HP_F32 ? fn<float>(*a, d, s) : a->type == HP_BF16 ? fn<__nv_bfloat16>(*a, d, s) : fn<__half>(*a, d, s)
+
+#ifdef HIPRESS_NORM_DROPOUT
+namespace hipress {
+
+// Arguments as hp_cuda_norm_forward() and hp_cuda_norm_backward() have checked them; x and the residual are dense.
+int norm_forward_dropout(const HpNormForward* a, cudaStream_t s) {
+  Drop d;
+  if (!drop_of(&d, a->drop) || !a->residual || a->ldx != a->cols || a->ldr != a->cols) return HP_ERR_BAD_ARG;
+  return BY_TYPE(forward);
+}
+int norm_backward_dropout(const HpNormBackward* a, cudaStream_t s) {
+  Drop d;
+  if (!drop_of(&d, a->drop)) return HP_ERR_BAD_ARG;
+  return BY_TYPE(backward);
+}
+
+}  // namespace hipress
+#else
+namespace hipress {
+int norm_forward_dropout(const HpNormForward* a, cudaStream_t s);
+int norm_backward_dropout(const HpNormBackward* a, cudaStream_t s);
+}  // namespace hipress
 
 extern "C" int hp_cuda_norm_forward(const HpNormForward* a, void* stream) {
   if (!a || a->rows < 0 || a->cols < 1 || a->rows > INT32_MAX || !types_ok(*a) || (a->residual && !a->z))
     return HP_ERR_BAD_ARG;
   if (!a->rows) return 0;
   cudaStream_t s = (cudaStream_t)stream;
+  if (a->drop.keep) return norm_forward_dropout(a, s);
+  const MaybeDrop d = {};
   return BY_TYPE(forward);
 }
 
 extern "C" int hp_cuda_norm_backward(const HpNormBackward* a, void* stream) {
   if (!a || a->rows < 0 || a->cols < 1 || a->rows > INT32_MAX || !types_ok(*a)) return HP_ERR_BAD_ARG;
   cudaStream_t s = (cudaStream_t)stream;
+  if (a->drop.keep) return norm_backward_dropout(a, s);
+  const MaybeDrop d = {};
   return BY_TYPE(backward);
 }
 
@@ -770,3 +905,4 @@ extern "C" uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols) {
   const int64_t ctas = rows + 8 < kMostCtas ? rows + 8 : kMostCtas;
   return (uint64_t)ctas * 2 * cols * 4;
 }
+#endif

@@ -48,6 +48,30 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*(const __half2*)&v);
 }
 
+// Two values at a time: half the instructions.
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ uint64_t bits(F2 v) {
+  return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x);
+}
+__device__ __forceinline__ F2 f2(uint64_t v) { return {__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))}; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return f2(d);
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return f2(d);
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+  return f2(d);
+}
+
 // 16 bytes of elements, in 32 bits
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);

@@ -1,0 +1,502 @@
+// Log probabilities of one token in each row of logits, the entropy of the row and its likeliest tokens,
+// in one pass over the logits; the gradient in a second one.
+//
+// A thread keeps a running maximum m, the sum s of exp(x - m) and the sum e of (x - m) exp(x - m): then
+// log p = (x - m) - log s, and the entropy is log s - e / s, in which a large m has cancelled already.
+// Bound: the traffic; exp takes 16 a cycle and SM, two thirds of the time that 16-bit logits take to arrive.
+//
+// The likeliest tokens need no second pass.  The k-th largest of the maxima of 64 (32) groups of threads
+// is no larger than the k-th largest value, so what is smaller than it is none of the k.  It is taken
+// from the first few batches of pieces, and what is not smaller, a few dozen values as a rule, goes to a list that
+// is put in order in the end.  Values are compared together with their place, so that of equals the first counts
+// and a row of equal values does not flood the list; should it overflow, or a value be no number, the row is read
+// again once for each of the k.
+#include "activation.cuh"
+#include "tcgen05.cuh"
+
+namespace hipress {
+namespace {
+
+constexpr int kThreads = 256, kBatch = 4, kMostTop = 32;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Values and their places in one order: larger values first, then lower places.  Zero: nothing.
+__device__ __forceinline__ uint64_t key_of(float v, int col) {
+  const uint32_t u = v != v ? 0x7fc00000u : __float_as_uint(v + 0.f);   // -0 is 0, a NaN the largest of all
+  return (uint64_t)(u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u)) << 32 | ~(uint32_t)col;
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u ^ ((int)u < 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int place_of(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// The sums of exp over some of a row's values.
+struct Sums {
+  float m, s, e;
+};
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return {m, a.s + b.s, a.e + b.e};   // nothing but zeros, or NaN
+  const float da = a.m == -INFINITY ? 0.f : a.m - m, db = b.m == -INFINITY ? 0.f : b.m - m;
+  const float fa = exp2_fast(da * kLog2e), fb = exp2_fast(db * kLog2e);
+  return {m, fmaf(a.s, fa, b.s * fb), fa * fmaf(da, a.s, a.e) + fb * fmaf(db, b.s, b.e)};
+}
+__device__ __forceinline__ Sums of_warp(Sums v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    v = joined(v, {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.e, o)});
+  return v;
+}
+
+// One row (or part of it) in pieces of 16 bytes, cut at their boundaries; what is outside reads as -inf.
+template <typename T>
+struct Row {
+  static constexpr int V = kPiece<T>;
+  const T* x;
+  int vocab, phase, pieces;
+  __device__ __forceinline__ Row(const void* logits, int64_t row, int64_t inner, int64_t ld_outer, int64_t ld, int64_t cols) {
+    x = (const T*)logits + row / inner * ld_outer + row % inner * ld;
+    vocab = (int)cols;
+    phase = (int)((uintptr_t)x / sizeof(T) % V);
+    pieces = (vocab + phase + V - 1) / V;
+  }
+  __device__ __forceinline__ uint4 piece(int p, int end) const {
+    const int col = p * V - phase;
+    if (p < end && col >= 0 && col + V <= vocab) return *(const uint4*)(x + col);
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = p < end && col + j >= 0 && col + j < vocab ? to_f(x[col + j]) : -INFINITY;
+    return pack<T>(v);
+  }
+};
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// the address of the first CTA's `p`
+__device__ __forceinline__ uint32_t first_cta(const void* p) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(smem_u32(p)));
+  return at;
+}
+__device__ __forceinline__ void store_there(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ void store_there(uint32_t at, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+
+constexpr int kMostSplit = 8;   // CTAs that share a row
+
+// What G threads that share a row keep of its largest values.
+template <int G>
+struct Largest {
+  static constexpr int kGroups = G == 32 ? 32 : 64, kList = G == 32 ? 256 : 2048;
+  uint64_t group[kGroups], least, best[kMostTop], found[G / 32], list[kList];
+  int n;
+};
+
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if (G == 32) __syncwarp();
+  else __syncthreads();
+}
+
+// The k-th largest of the groups' maxima; `t` in the row's threads
+template <int G>
+__device__ __forceinline__ uint64_t least_of(Largest<G>& l, uint64_t best, int k, int t) {
+  constexpr int kShare = G / Largest<G>::kGroups, kEach = Largest<G>::kGroups / kShare;   // threads to a group, keys to each
+#pragma unroll
+  for (int o = 1; o < kShare; o *= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, o));
+  const int g = t / kShare, part = t % kShare;
+  if (part == 0) l.group[g] = best;
+  group_sync<G>();
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < kEach; ++i) above += l.group[part * kEach + i] > best;
+#pragma unroll
+  for (int o = 1; o < kShare; o *= 2) above += __shfl_xor_sync(0xffffffffu, above, o);
+  if (above == k - 1 && part == 0) l.least = best;   // one group's, or all those that have none
+  group_sync<G>();
+  return l.least;
+}
+
+// `n` keys into the k largest of them, in order; zeros where there are fewer
+template <int G>
+__device__ __forceinline__ void in_order(const uint64_t* keys, int n, uint64_t* best, int k, int t) {
+  if (t < k) best[t] = 0;
+  group_sync<G>();
+  for (int i = t; i < n; i += G) {
+    const uint64_t mine = keys[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
+    if (mine && above < k) best[above] = mine;
+  }
+  group_sync<G>();
+}
+
+template <typename T, int G, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_constant__ HpLogProbs a) {
+  constexpr int V = kPiece<T>, kRows = kThreads / G;
+  __shared__ Sums part[G == 32 ? 1 : kThreads / 32], parts[kMostSplit];
+  __shared__ uint64_t others[TOP && G != 32 ? kMostSplit * kMostTop : 1];
+  __shared__ Largest<G> largest[TOP ? kRows : 1];
+  __shared__ float losses[kRows][2];
+  const int t = threadIdx.x % G, lane = threadIdx.x & 31, k = (int)a.top;
+  const int split = G == 32 ? 1 : (int)cluster_size(), rank = split > 1 ? (int)cluster_rank() : 0;
+  const int64_t row = (int64_t)(blockIdx.x / split) * kRows + threadIdx.x / G;
+  const bool there = row < a.rows;
+  Largest<G>& l = largest[TOP ? threadIdx.x / G : 0];
+  dependents_may_start();
+  if (split > 1) cluster_arrive();   // whose shared memory is written has started
+  if (TOP && t == 0) l.n = 0, l.least = 0;
+  wait_for_kernel_before();
+  const int64_t token = there ? a.tokens[row] : a.ignored;
+  const bool read = there && (ENTROPY || TOP || token != a.ignored);
+  const Row<T> r(a.logits, there ? row : 0, a.inner, a.ld_outer, a.ld, a.vocab);
+  const int each = (r.pieces + split - 1) / split, first = rank * each, end = read ? min(first + each, r.pieces) : 0;
+  if (TOP) group_sync<G>();
+
+  Sums sum = {-INFINITY, 0.f, 0.f};
+  uint64_t best = 0, least = 0;
+  float bar = -INFINITY;   // the value of `least`
+  for (int p = first, batch = 0; p < end; p += G * kBatch, ++batch) {   // the same for all threads of a row
+    uint4 raw[kBatch];
+    float top[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) raw[i] = r.piece(p + t + i * G, end);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      float v[V];
+      unpack<T>(raw[i], v);
+      top[i] = v[0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) top[i] = fmaxf(top[i], v[j]);
+    }
+    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (high > sum.m) {
+      if (sum.m != -INFINITY) {
+        const float d = sum.m - high, f = exp2_fast(d * kLog2e);
+        sum.e = f * fmaf(d, sum.s, sum.e), sum.s *= f;
+      }
+      sum.m = high;
+      if (TOP) {   // the first of the places that hold it
+        int at = -1;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          if (at < 0 && top[i] == high) {
+            float v[V];
+            unpack<T>(raw[i], v);
+#pragma unroll
+            for (int j = V - 1; j >= 0; --j)
+              if (v[j] == high) at = (p + t + i * G) * V - r.phase + j;
+          }
+        best = larger(best, key_of(high, at));
+      }
+    }
+    const float minus = sum.m == -INFINITY ? 0.f : -sum.m;
+    F2 s = {0.f, 0.f}, e = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      float v[V];
+      unpack<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        F2 d = add2({v[j], v[j + 1]}, {minus, minus});
+        const F2 z = mul2(d, {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
+        s = add2(s, x);
+        if (ENTROPY) {
+          d = {fmaxf(d.x, -200.f), fmaxf(d.y, -200.f)};   // no infinity times zero
+          e = fma2(x, d, e);
+        }
+      }
+    }
+    sum.s += s.x + s.y, sum.e += e.x + e.y;
+    if (TOP) {
+      if ((batch & (batch - 1)) == 0) {   // batches 0, 1, 2, 4, 8 ..
+        least = least_of<G>(l, best, k, t);
+        bar = least ? value_of(least) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (top[i] >= bar) {
+          float v[V];
+          unpack<T>(raw[i], v);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int col = (p + t + i * G) * V - r.phase + j;
+            if (v[j] >= bar && p + t + i * G < end && col >= 0 && col < r.vocab) {
+              const uint64_t key = key_of(v[j], col);
+              if (key >= least) {
+                const int at = atomicAdd(&l.n, 1);
+                if (at < Largest<G>::kList) l.list[at] = key;
+              }
+            }
+          }
+        }
+    }
+  }
+  // a NaN is no maximum and in no list, but in the sum
+  sum = of_warp(sum);
+  if (G != 32) {
+    if (lane == 0) part[threadIdx.x / 32] = sum;
+    __syncthreads();
+    sum = part[0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 32; ++i) sum = joined(sum, part[i]);
+  }
+  if (TOP) {
+    group_sync<G>();
+    const int n = l.n;
+    if (n <= Largest<G>::kList && sum.s == sum.s) {
+      in_order<G>(l.list, n, l.best, k, t);
+    } else {
+      uint64_t last = ~0ull;
+      for (int i = 0; i < k; ++i) {
+        uint64_t next = 0;
+        for (int p = first + t; p < end; p += G) {
+          float v[V];
+          unpack<T>(r.piece(p, end), v);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int col = p * V - r.phase + j;
+            const uint64_t key = key_of(v[j], col);
+            if (col >= 0 && col < r.vocab && key < last) next = larger(next, key);
+          }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) next = larger(next, __shfl_xor_sync(0xffffffffu, next, o));
+        group_sync<G>();
+        if (lane == 0) l.found[t / 32] = next;
+        group_sync<G>();
+        for (int w = 0; w < G / 32; ++w) next = larger(next, l.found[w]);
+        if (t == 0) l.best[i] = next;
+        last = next;
+      }
+      group_sync<G>();
+    }
+  }
+  if (split > 1) {
+    cluster_wait();
+    if (threadIdx.x == 0) {
+      const uint32_t to = first_cta(&parts[rank]);
+      store_there(to, sum.m), store_there(to + 4, sum.s), store_there(to + 8, sum.e);
+    }
+    if (TOP && G != 32 && t < k) store_there(first_cta(&others[rank * k + t]), l.best[t]);
+    cluster_arrive();
+    cluster_wait();
+    if (rank) return;
+    sum = parts[0];
+    for (int i = 1; i < split; ++i) sum = joined(sum, parts[i]);
+    if (TOP && G != 32) in_order<G>(others, split * k, l.best, k, t);
+  }
+  const bool none = sum.s == 0.f;   // nothing above -inf
+  const float lns = none ? 0.f : logf(sum.s);
+  auto log_p = [&](float v) { return none ? -INFINITY : (v - sum.m) - lns; };
+  float lp = 0.f;
+  if (t == 0 && there) {
+    if (token != a.ignored) lp = token >= 0 && token < r.vocab ? log_p(to_f(r.x[token])) : NAN;
+    if (a.log_probs) a.log_probs[row] = lp;
+    a.stats[2 * row] = sum.m, a.stats[2 * row + 1] = lns;
+    if (ENTROPY) a.entropy[row] = none ? 0.f : lns - sum.e / sum.s;
+  }
+  if (TOP && there && t < k) {
+    a.top_log_probs[row * k + t] = log_p(value_of(l.best[t]));
+    a.top_tokens[row * k + t] = place_of(l.best[t]);
+  }
+  if (a.loss) {
+    const float one = there && token != a.ignored ? 1.f : 0.f;
+    float* out = (float*)a.workspace;
+    if (G != 32) {
+      if (t == 0) out[2 * row] = -lp, out[2 * row + 1] = one;
+    } else {
+      if (t == 0) losses[threadIdx.x / G][0] = -lp, losses[threadIdx.x / G][1] = one;
+      __syncthreads();
+      if (threadIdx.x < 2) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) s += losses[i][threadIdx.x];
+        out[2 * (int64_t)blockIdx.x + threadIdx.x] = s;
+      }
+    }
+  }
+}
+
+// The parts' losses and rows, added in their order by one CTA, in 64 bits; their mean or sum.
+__global__ void __launch_bounds__(1024) loss_kernel(const float2* parts, int64_t n, float* loss, float* count, int summed) {
+  __shared__ double sums[2][32];
+  dependents_may_start();
+  wait_for_kernel_before();
+  double s = 0., c = 0.;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const float2 v = parts[i];
+    s += v.x, c += v.y;
+  }
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (pass) break;
+    if ((threadIdx.x & 31) == 0) sums[0][threadIdx.x / 32] = s, sums[1][threadIdx.x / 32] = c;
+    __syncthreads();
+    s = sums[0][threadIdx.x & 31], c = sums[1][threadIdx.x & 31];
+  }
+  if (threadIdx.x == 0) {
+    *loss = (float)(summed ? s : s / c);   // of no rows the mean is no number
+    *count = (float)c;
+  }
+}
+
+// dx = g (1 at the token - p) - h p (log p + entropy).  Pieces go by the boundaries of the result; logits that
+// lie otherwise are read element by element.
+template <typename T, int G, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __grid_constant__ HpLogProbsBackward a, int chunks) {
+  constexpr int V = kPiece<T>, kRows = kThreads / G;
+  const int t = threadIdx.x % G;
+  const int64_t row = (int64_t)(blockIdx.x / chunks) * kRows + threadIdx.x / G;
+  const int chunk = blockIdx.x % chunks;
+  dependents_may_start();
+  wait_for_kernel_before();
+  if (row >= a.rows) return;
+  const Row<T> in(a.logits, row, a.inner, a.ld_outer, a.ld, a.vocab), out(a.dlogits, row, a.rows, 0, a.vocab, a.vocab);
+  const int64_t token = a.tokens[row];
+  float g = token == a.ignored || !a.dlog_probs ? 0.f : a.dlog_probs[a.one ? 0 : row];
+  if (g != 0.f && a.count) g /= *a.count;
+  if (a.negative) g = -g;
+  const float h = ENTROPY ? a.dentropy[row] : 0.f, m = a.stats[2 * row], lns = a.stats[2 * row + 1];
+  if (token != a.ignored && (token < 0 || token >= in.vocab)) g = NAN;
+  const float own = ENTROPY ? a.entropy[row] - lns : 0.f;
+  const bool some = (g != 0.f || h != 0.f) && m != -INFINITY, alike = in.phase == out.phase;
+  T* to = (T*)a.dlogits + row * a.vocab;
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int p = (chunk * kBatch + i) * G + t, col = p * V - out.phase;
+    if (p >= out.pieces) break;
+    const bool whole = col >= 0 && col + V <= out.vocab;
+    float v[V];
+    if (!some) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+    } else {
+      if (alike && whole) {
+        unpack<T>(*(const uint4*)(in.x + col), v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = col + j >= 0 && col + j < out.vocab ? to_f(in.x[col + j]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float d = v[j] - m;
+        const float pr = exp2_fast((d - lns) * kLog2e);
+        float by = g;
+        if (ENTROPY) by = fmaf(h, fmaxf(d, -200.f) + own, g);   // no infinity times zero
+        v[j] = -(pr * by);
+      }
+      const int at = (int)token - col;
+      if (token == col + at && at >= 0 && at < V && g != 0.f) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j == at) v[j] += g;
+      }
+    }
+    if (whole) {
+      *(uint4*)(to + col) = pack<T>(v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (col + j >= 0 && col + j < out.vocab) to[col + j] = from_f<T>(v[j]);
+    }
+  }
+}
+
+// Rows of up to this many pieces have a warp each; longer ones a CTA
+constexpr int kWarpPieces = 128;
+
+template <typename T, int G, bool ENTROPY, bool TOP>
+int forward_of(const HpLogProbs& a, int split, cudaStream_t s) {
+  const int64_t ctas = G == 32 ? (a.rows + 7) / 8 : a.rows * split;
+  if (ctas > INT32_MAX) return HP_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = (unsigned)ctas, cfg.blockDim = kThreads, cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)split, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = split > 1 ? 2 : 1;
+  if (const int rc = told(cudaLaunchKernelEx(&cfg, log_probs_kernel<T, G, ENTROPY, TOP>, a))) return rc;
+  if (!a.loss) return 0;
+  return launch_behind(loss_kernel, 1, 1024, 0, s, (const float2*)a.workspace, G == 32 ? ctas : a.rows, a.loss, a.count, (int)a.summed);
+}
+
+template <typename T>
+int64_t most_pieces(int64_t vocab) {
+  return (vocab + 2 * kPiece<T> - 2) / kPiece<T>;
+}
+
+template <typename T>
+int forward(const HpLogProbs& a, cudaStream_t s) {
+  const int64_t pieces = most_pieces<T>(a.vocab);
+#define BY_USE(G, split)                                                                                           a.entropy ? (a.top ? forward_of<T, G, true, true>(a, split, s) : forward_of<T, G, true, false>(a, split, s))               : (a.top ? forward_of<T, G, false, true>(a, split, s) : forward_of<T, G, false, false>(a, split, s))
+  if (pieces <= kWarpPieces) return BY_USE(32, 1);
+  int split = 1;   // few rows are shared by up to eight CTAs, as long as each has a batch
+  while (split < kMostSplit && a.rows * split < 2 * layer_sms() && pieces > 2 * split * kThreads) split *= 2;
+  return BY_USE(256, split);
+#undef BY_USE
+}
+
+template <typename T, int G, bool ENTROPY>
+int backward_of(const HpLogProbsBackward& a, cudaStream_t s) {
+  const int64_t chunks = G == 32 ? 1 : (most_pieces<T>(a.vocab) + G * kBatch - 1) / (G * kBatch);
+  const int64_t ctas = G == 32 ? (a.rows + 7) / 8 : a.rows * chunks;
+  if (ctas > INT32_MAX) return HP_ERR_TOO_LARGE;
+  return launch_behind(log_probs_backward_kernel<T, G, ENTROPY>, (unsigned)ctas, kThreads, 0, s, a, (int)chunks);
+}
+template <typename T>
+int backward(const HpLogProbsBackward& a, cudaStream_t s) {
+  if (most_pieces<T>(a.vocab) <= kWarpPieces)
+    return a.dentropy ? backward_of<T, 32, true>(a, s) : backward_of<T, 32, false>(a, s);
+  return a.dentropy ? backward_of<T, 256, true>(a, s) : backward_of<T, 256, false>(a, s);
+}
+
+bool sizes_ok(int64_t rows, int64_t inner, int64_t vocab, int64_t type) {
+  return rows >= 0 && rows <= INT32_MAX && inner >= 1 && vocab >= 1 && vocab <= 1 << 30 && type_ok(type);
+}
+
+}  // namespace
+}  // namespace hipress
+
+using namespace hipress;
+
+#define BY_TYPE(fn) a->type == HP_F32 ? fn<float>(*a, s) : a->type == HP_BF16 ? fn<__nv_bfloat16>(*a, s) : fn<__half>(*a, s)
+
+extern "C" int hp_cuda_log_probs(const HpLogProbs* a, void* stream) {
+  if (!a || !sizes_ok(a->rows, a->inner, a->vocab, a->type) || a->top < 0 || a->top > kMostTop || a->top > a->vocab ||
+      (a->loss && (!a->count || (a->rows && !a->workspace))))
+    return HP_ERR_BAD_ARG;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (!a->rows)
+    return a->loss ? launch_behind(loss_kernel, 1, 1024, 0, s, (const float2*)nullptr, (int64_t)0, a->loss, a->count, (int)a->summed) : 0;
+  return BY_TYPE(forward);
+}
+
+extern "C" uint64_t hp_cuda_log_probs_workspace(int64_t rows) { return (uint64_t)rows * 8; }
+
+extern "C" int hp_cuda_log_probs_backward(const HpLogProbsBackward* a, void* stream) {
+  if (!a || !sizes_ok(a->rows, a->inner, a->vocab, a->type) || (a->dentropy && !a->entropy) || (uintptr_t)a->dlogits % 16)
+    return HP_ERR_BAD_ARG;
+  if (!a->rows) return 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  return BY_TYPE(backward);
+}

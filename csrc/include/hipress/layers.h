@@ -1,5 +1,5 @@
-// C ABI of the layer operators: layer norm, the matrix product with an epilogue and
-// attention.  Every function takes a structure of its arguments and the stream.
+// C ABI of the layer operators: dropout, layer norm, the matrix product with an epilogue, attention
+// and log probabilities.  Every function takes a structure of its arguments and the stream.
 //
 // Return values as in capi.h.  Kernels that wait (for copies or matrix products of their
 // own CTA) bound every wait but that for room in tensor memory, which the CTAs that hold it end
@@ -25,6 +25,24 @@
 extern "C" {
 #endif
 
+// Which elements a dropout keeps follows from these numbers alone (csrc/cuda/philox.cuh).
+typedef struct {
+  const int64_t* seed_at;  // on the device, read when the kernel runs; or NULL:
+  int64_t seed;
+  int64_t site;            // tells calls under one seed apart, 0 .. 2^32 - 1
+  int64_t keep;            // an element is kept with the probability keep / 2^16, 1 .. 65535; 0: no dropout
+} HpDropout;
+
+// y = dropout(x) + residual over n elements; the backward pass is the same call with the gradient for x.
+typedef struct {
+  const void* x;
+  const void* residual;  // or NULL
+  void* y;
+  int64_t n, type;
+  HpDropout drop;
+} HpDrop;
+int hp_cuda_dropout(const HpDrop* a, void* stream);
+
 // z = x (+ residual, rounded to the type); y = (z - mean) rstd weight + bias, by rows of
 // `cols` elements.  Outputs are dense; inputs have a pitch in elements.
 typedef struct {
@@ -39,6 +57,7 @@ typedef struct {
   int64_t rows, cols, ldx, ldr;
   int64_t type, wtype;   // of x, residual, y, z; of weight and bias
   double eps;
+  HpDropout drop;        // of x, only with a residual; elements counted through rows of `cols`
 } HpNormForward;
 int hp_cuda_norm_forward(const HpNormForward* a, void* stream);
 
@@ -56,6 +75,8 @@ typedef struct {
   void* workspace;       // hp_cuda_norm_workspace(rows, cols) bytes
   int64_t rows, cols, ldz, lddy, lddz;
   int64_t type, wtype;
+  void* dropped;         // with a dropout: the gradient of x (dx is the residual's)
+  HpDropout drop;
 } HpNormBackward;
 int hp_cuda_norm_backward(const HpNormBackward* a, void* stream);
 uint64_t hp_cuda_norm_workspace(int64_t rows, int64_t cols);
@@ -111,9 +132,44 @@ typedef struct {
   int64_t mask_b;
   int64_t type, causal;
   double scale;
+  HpDropout drop;           // of the probabilities, [batch, heads, sq, sk rounded up to 32]
 } HpAttention;
 int hp_cuda_attention_forward(const HpAttention* a, void* stream);
 int hp_cuda_attention_backward(const HpAttention* a, void* stream);
+
+// Log probabilities of one token in each row of logits, with the entropy and the likeliest tokens.
+// Row r of `rows` starts at (r / inner) ld_outer + (r % inner) ld elements.
+typedef struct {
+  const void* logits;
+  const int64_t* tokens;     // [rows]; `ignored`: no token, log probability zero
+  float* log_probs;          // [rows]
+  float* entropy;            // [rows] or NULL
+  float* top_log_probs;      // [rows, top]
+  int64_t* top_tokens;       // [rows, top]
+  float* stats;              // [rows, 2]: the largest logit, the logarithm of the sum of exp(logit - largest)
+  float* loss;               // the mean (or sum, `summed`) of -log_probs over rows that have a token; or NULL
+  float* count;              // with it: those rows
+  void* workspace;           // hp_cuda_log_probs_workspace(rows) bytes, with it
+  int64_t rows, inner, vocab, ld_outer, ld;
+  int64_t type, top, ignored, summed;
+} HpLogProbs;
+int hp_cuda_log_probs(const HpLogProbs* a, void* stream);
+uint64_t hp_cuda_log_probs_workspace(int64_t rows);
+
+// dlogits = dlog_probs (1 at the token - p) - dentropy p (log p + entropy), dense rows.
+typedef struct {
+  const void* logits;
+  const int64_t* tokens;
+  const float* stats;
+  const float* entropy;      // or NULL
+  const float* dlog_probs;   // [rows], or one number for all rows (`one`); or NULL
+  const float* dentropy;     // [rows] or NULL
+  const float* count;        // dlog_probs are divided by it; or NULL
+  void* dlogits;             // [rows, vocab]
+  int64_t rows, inner, vocab, ld_outer, ld;
+  int64_t type, ignored, one, negative;   // negative: dlog_probs count with the other sign
+} HpLogProbsBackward;
+int hp_cuda_log_probs_backward(const HpLogProbsBackward* a, void* stream);
 
 // A wait of the layer operators' kind that runs out after `limit_ns`, and one beside it, which then
 // ends too; the nanoseconds that each took to two words of device memory.  For tests.

@@ -5,6 +5,9 @@ activation and residual in its epilogue, and attention, each with its gradient.
     y = linear(x, weight, bias, activation="gelu")  y = linear(x, weight, bias, residual=r)
     o = attention(q, k, v, causal=True)             o = self_attention(qkv, key_mask=mask)
 
+The layer norm's first term and the attention's probabilities can be dropped out (``dropout``, ``seed``, ``site``: see
+:func:`hipress_b200.ops.dropout`).
+
 CUDA tensors run the sm_100a kernels (csrc/cuda/layer_norm.cu, linear.cu, attention.cu) on
 the current stream of their device; CPU tensors the same formulas in torch.  Statistics,
 softmax sums and products are kept in 32 bits; probabilities, their gradient and the
@@ -23,24 +26,16 @@ The reference (mark14wu/hipress) leaves the layers to its front ends.
 """
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
 
 from .._native import lib as _lib
+from . import random_drop as _d
+from ._common import TYPES, first_order as _first_order, same_device as _same_device, wide as _wide
 
-TYPES = (torch.float32, torch.bfloat16, torch.float16)
 HALF = (torch.bfloat16, torch.float16)
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}
-
-
-def _same_device(what, *ts):
-    dev = ts[0].device
-    for t in ts[1:]:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    return dev
 
 
 def _autocast(x):
@@ -50,48 +45,19 @@ def _autocast(x):
     return x
 
 
-def _wide(x):
-    return x if x.dtype == torch.float64 else x.float()   # CPU: float64 is taken as it is
-
-
 def _rows(x):
     return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])   # also of no elements
 
 
-class _Refused(torch.autograd.Function):
-    """A value as it is, which cannot be differentiated by what it was made from."""
-
-    @staticmethod
-    def forward(ctx, x, *made_from):
-        return x.view_as(x)
-
-    @staticmethod
-    def backward(ctx, _):
-        raise RuntimeError("a gradient of a layer operator cannot be differentiated")
-
-
-def _first_order(backward):
-    """For a backward pass whose results have no graph; the node has saved all its inputs.  Where a graph is
-    wanted (``create_graph``) the results say so when they are differentiated, whether or not the
-    gradient that came in has a graph itself."""
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        with torch.no_grad():
-            out = backward(ctx, *grads)
-        if not torch.is_grad_enabled():
-            return out
-        made_from = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
-        # what is handed on unchanged keeps the graph that it has
-        return tuple(g if g is None or any(g is x for x in grads) else _Refused.apply(g.detach(), *made_from) for g in out)
-    return run
-
-
 # ================================================================== layer norm
-def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
+def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5, dropout: float = 0.0, seed=None,
+               site: int = 0):
     """Normalises the last axis of ``x``: ``(z - mean) / sqrt(var + eps) * weight + bias``.
 
     With ``residual`` (of ``x``'s shape and type) ``z = x + residual``, rounded to that type,
-    is normalised and returned too: ``(y, z)``; both have gradients.  ``x``: float32, bfloat16
+    is normalised and returned too: ``(y, z)``; both have gradients.  With ``dropout`` as well, ``z`` is
+    the residual plus :func:`~hipress_b200.ops.dropout` of ``x`` under ``seed`` and ``site``, with the same elements
+    kept and one rounding.  ``x``: float32, bfloat16
     or float16; ``weight``, ``bias``: one value per column, float32 or ``x``'s type, the same
     for both."""
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -111,7 +77,10 @@ def layer_norm(x, weight=None, bias=None, *, residual=None, eps: float = 1e-5):
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"layer_norm: a residual of {tuple(residual.shape)} {residual.dtype} for x of "
                          f"{tuple(x.shape)} {x.dtype}")
-    y, z = (_lib.layers().layer_norm if x.is_cuda else _LayerNorm.apply)(x, weight, bias, residual, eps)
+    if dropout and residual is None:
+        raise ValueError("layer_norm: a dropout goes in front of a residual sum; there is no residual")
+    random = _d.random_args("layer_norm", x, dropout, seed, site)
+    y, z = (_lib.layers().layer_norm if x.is_cuda else _LayerNorm.apply)(x, weight, bias, residual, eps, *random)
     return y if residual is None else (y, z)
 
 
@@ -119,8 +88,9 @@ class _LayerNorm(torch.autograd.Function):
     """On CPU tensors."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, eps):
-        z = x if residual is None else (_wide(x) + _wide(residual)).to(x.dtype)
+    def forward(ctx, x, weight, bias, residual, eps, *random):
+        w = _d.dropped(_wide(x), _d.kept_elements(x.shape, random), random[3]) if random[3] else _wide(x)
+        z = x if residual is None else (w + _wide(residual)).to(x.dtype)
         var, mean = torch.var_mean(_wide(z), -1, unbiased=False, keepdim=True)
         rstd = (var + eps).rsqrt()
         y = (_wide(z) - mean) * rstd
@@ -128,7 +98,8 @@ class _LayerNorm(torch.autograd.Function):
             y = y * _wide(weight)
         if bias is not None:
             y = y + _wide(bias)
-        ctx.save_for_backward(z, weight, mean, rstd, x, bias, residual)
+        ctx.save_for_backward(z, weight, mean, rstd, random[0], x, bias, residual)
+        ctx.random = random[1:]
         ctx.bias = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
         return y.to(x.dtype), None if residual is None else z
@@ -136,10 +107,10 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, dy, dz):
-        z, weight, mean, rstd = ctx.saved_tensors[:4]
+        z, weight, mean, rstd, seed_at = ctx.saved_tensors[:5]
         if dy is None and dz is None:
-            return None, None, None, None, None
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+            return (None,) * 9
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         g = torch.zeros_like(mean).expand_as(z) if dy is None else _wide(dy)   # only the sum was used further on
         h = (_wide(z) - mean) * rstd
         dw = _rows(g * h).sum(0).to(weight.dtype) if need_w else None
@@ -149,8 +120,11 @@ class _LayerNorm(torch.autograd.Function):
         dx = rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
         if dz is not None:
             dx = dx + _wide(dz)
-        dx = dx.to(z.dtype)
-        return dx if need_x else None, dw, db, dx if need_r else None, None
+        dr = dx.to(z.dtype)
+        if need_x and ctx.random[2]:
+            random = (seed_at, *ctx.random)
+            dx = _d.dropped(dx, _d.kept_elements(dx.shape, random), random[3])
+        return dx.to(z.dtype) if need_x else None, dw, db, dr if need_r else None, None, *(None,) * 4
 
 
 # ====================================================================== linear
@@ -232,7 +206,8 @@ class _Linear(torch.autograd.Function):
 
 
 # =================================================================== attention
-def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: float | None = None, return_lse: bool = False):
+def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: float | None = None, return_lse: bool = False,
+              dropout: float = 0.0, seed=None, site: int = 0):
     """``softmax(scale q k^T) v`` for ``q`` [batch, queries, heads, dim] and ``k``, ``v``
     [batch, keys, key heads, dim], as [batch, queries, heads, dim].
 
@@ -241,17 +216,21 @@ def attention(q, k, v, *, causal: bool = False, key_mask=None, scale: float | No
     ``key_mask`` [batch, keys], bool: the keys that may be seen; what the others hold, NaN
     among it, has no effect.  A query that sees no key gets zeros and no gradient.  ``scale``: 1 /
     sqrt(dim) unless given.  ``return_lse``: also the logarithm of each row's softmax sum
-    [batch, heads, queries], float32, without a gradient (-inf where no key is seen).
+    [batch, heads, queries], float32, without a gradient (-inf where no key is seen).  ``dropout``:
+    probabilities are dropped before they meet ``v`` (see :func:`~hipress_b200.ops.dropout` for ``seed`` and
+    ``site``); the logarithm is that of all of them.
 
     On a GPU: bfloat16 or float16, ``dim`` a multiple of 8 up to 128.  The backward pass
-    computes the probabilities again, from that logarithm; there is no dropout."""
+    computes the probabilities again, from that logarithm, and which were dropped from the seed."""
     q, k, v = _autocast(q), _autocast(k), _autocast(v)
     scale = _check_attention(q, k, v, key_mask, scale)
-    o, lse = (_lib.layers().attention if q.is_cuda else _Attention.apply)(q, k, v, key_mask, causal, scale)
+    random = _d.random_args("attention", q, dropout, seed, site)
+    o, lse = (_lib.layers().attention if q.is_cuda else _Attention.apply)(q, k, v, key_mask, causal, scale, *random)
     return (o, lse) if return_lse else o
 
 
-def self_attention(qkv, *, causal: bool = False, key_mask=None, scale: float | None = None, return_lse: bool = False):
+def self_attention(qkv, *, causal: bool = False, key_mask=None, scale: float | None = None, return_lse: bool = False,
+                   dropout: float = 0.0, seed=None, site: int = 0):
     """:func:`attention` of ``q, k, v = qkv.unbind(2)``, [batch, length, 3, heads, dim] as one
     projection leaves them; the gradient has the same form, so that nothing is copied."""
     qkv = _autocast(qkv)
@@ -259,10 +238,11 @@ def self_attention(qkv, *, causal: bool = False, key_mask=None, scale: float | N
         raise ValueError(f"self_attention: [batch, length, 3, heads, dim] is wanted, not {tuple(qkv.shape)}")
     q, k, v = qkv.unbind(2)
     scale = _check_attention(q, k, v, key_mask, scale)
+    random = _d.random_args("self_attention", qkv, dropout, seed, site)
     if qkv.is_cuda:
-        o, lse = _lib.layers().self_attention(qkv, key_mask, causal, scale)
+        o, lse = _lib.layers().self_attention(qkv, key_mask, causal, scale, *random)
     else:
-        o, lse = _Attention.apply(q, k, v, key_mask, causal, scale)
+        o, lse = _Attention.apply(q, k, v, key_mask, causal, scale, *random)
     return (o, lse) if return_lse else o
 
 
@@ -313,15 +293,17 @@ class _Attention(torch.autograd.Function):
     """On CPU tensors."""
 
     @staticmethod
-    def forward(ctx, q, k, v, mask, causal, scale):
+    def forward(ctx, q, k, v, mask, causal, scale, *random):
         (b, sq, h, _), sk = q.shape, k.shape[1]
         qh, kh, vh = _cpu_heads(q, k, v, mask)
         s = (qh @ kh.transpose(2, 3) * scale).masked_fill(~_hidden(q, k, mask, causal), -math.inf)
         lse = torch.logsumexp(s, -1) if sk else s.new_full((b, h, sq), -math.inf)
         p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
+        if random[3]:
+            p = _d.dropped(p, _d.kept_probabilities(b, h, sq, sk, random), random[3])
         o = (p @ vh).transpose(1, 2).to(q.dtype).contiguous()
-        ctx.save_for_backward(q, k, v, o, lse, mask)
-        ctx.causal, ctx.scale = causal, scale
+        ctx.save_for_backward(q, k, v, o, lse, mask, random[0])
+        ctx.causal, ctx.scale, ctx.random = causal, scale, random[1:]
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return o, lse
@@ -330,15 +312,20 @@ class _Attention(torch.autograd.Function):
     @_first_order
     def backward(ctx, do, _):
         if do is None:
-            return (None,) * 6
-        q, k, v, o, lse, mask = ctx.saved_tensors
-        (b, _, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
+            return (None,) * 10
+        q, k, v, o, lse, mask, seed_at = ctx.saved_tensors
+        (b, sq, h, d), sk, hk = q.shape, k.shape[1], k.shape[2]
         qh, kh, vh = _cpu_heads(q, k, v, mask)
         g, oh = _wide(do).transpose(1, 2), _wide(o).transpose(1, 2)
         s = (qh @ kh.transpose(2, 3) * ctx.scale).masked_fill(~_hidden(q, k, mask, ctx.causal), -math.inf)
         p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
-        ds = p * (g @ vh.transpose(2, 3) - (g * oh).sum(-1, keepdim=True)) * ctx.scale
+        dp, pv = g @ vh.transpose(2, 3), p
+        if ctx.random[2]:
+            random = (seed_at, *ctx.random)
+            kept = _d.kept_probabilities(b, h, sq, sk, random)
+            dp, pv = _d.dropped(dp, kept, random[3]), _d.dropped(p, kept, random[3])
+        ds = p * (dp - (g * oh).sum(-1, keepdim=True)) * ctx.scale
         group = lambda x: x.view(b, hk, h // hk, sk, d).sum(2)  # noqa: E731
-        out = ds @ kh, group(ds.transpose(2, 3) @ qh), group(p.transpose(2, 3) @ g)
+        out = ds @ kh, group(ds.transpose(2, 3) @ qh), group(pv.transpose(2, 3) @ g)
         need = ctx.needs_input_grad
-        return (*(x.transpose(1, 2).to(q.dtype) if n else None for x, n in zip(out, need)), None, None, None)
+        return (*(x.transpose(1, 2).to(q.dtype) if n else None for x, n in zip(out, need)), *(None,) * 7)
