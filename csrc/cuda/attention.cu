@@ -315,11 +315,13 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
     uint32_t ph = 0;
     Key key = {};
     if (DROP) key = drop_key(l.drop);
+    const uint64_t words = first_word(p, b, h, row);
     for (int j = 0; j < nt; ++j) {
       Seen<kB> kept;
-      if (DROP)   // before the scores are there, and take the registers
-#pragma unroll
-        for (int i = 0; i < kB / 32; ++i) kept.w[i] = kept_word(l.drop, key, first_word(p, b, h, row) + j * (kB / 32) + i);
+      if (DROP) {   // before the scores are there, and take the registers
+        const uint64_t w = words + j * (kB / 32), ws[4] = {w, w + 1, w + 2, w + 3};
+        kept_words(l.drop, key, ws, kept.w);
+      }
       Seen<kB> seen;
       bool whole = sees >= (j + 1) * kB;
       if (masked) {
@@ -866,6 +868,7 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     bool ok = true;
     Key key = {};
     if (DROP) key = drop_key(l.drop);
+    const uint64_t of_row = (uint64_t)(p.sk + 31) / 32, words = keys ? 0 : first_word(p, b, head, row);
     // of tile j: stage, buffer, turn, and place among its head's tiles
     int s = half, q = half, turn = half, place = half;
     uint32_t ph = 0, round = 0;
@@ -880,15 +883,12 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     for (int j = half; j < n; j += 2, advance()) {
       Seen<kPass> kept;
       if (DROP) {
-#pragma unroll
-        for (int i = 0; i < kPass / 32; ++i) {
-          if (keys) {
-            const int query = (first + place) * kPass + 32 * i + lane;
-            kept.w[i] = transposed(kept_word(l.drop, key, first_word(p, b, head * group + j / count, query) + (r0 / 32 + quad)));
-          } else {
-            kept.w[i] = kept_word(l.drop, key, first_word(p, b, head, row) + j * (kPass / 32) + i);
-          }
-        }
+        uint64_t w = words + (uint64_t)j * (kPass / 32), more = 1;
+        if (keys)   // of the query that this lane makes them for
+          w = first_word(p, b, head * group + j / count, (first + place) * kPass + lane) + (r0 / 32 + quad), more = 32 * of_row;
+        const uint64_t ws[2] = {w, w + more};
+        kept_words(l.drop, key, ws, kept.w);
+        if (keys) kept.w[0] = transposed(kept.w[0]), kept.w[1] = transposed(kept.w[1]);
       }
       Seen<kPass> seen;
       bool whole;
@@ -1137,9 +1137,9 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
     uint32_t kept[2];   // of this thread's 64 queries
     if (DROP) {
       const Key key = drop_key(l.drop);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        kept[i] = transposed(kept_word(l.drop, key, first_word(p, b, h, 64 * half + 32 * i + lane) + quad));
+      const uint64_t w = first_word(p, b, h, 64 * half + lane) + quad, ws[2] = {w, w + 32 * ((uint64_t)(p.sk + 31) / 32)};
+      kept_words(l.drop, key, ws, kept);
+      kept[0] = transposed(kept[0]), kept[1] = transposed(kept[1]);
     }
     const int from = p.causal ? r - shift : 0;   // the first query that sees this key
     bool whole = mine && from <= 0;

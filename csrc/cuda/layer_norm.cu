@@ -347,47 +347,65 @@ __device__ __forceinline__ void start_ring(Ring<T, N, RAGGED>& ring, uint8_t* sp
   for (int s = 0; s < ring.depth; ++s) ring.fetch(first + s * step, s);
 }
 
-// Which elements of a piece a dropout keeps, a bit each; by whole warps, whose lanes' pieces lie side by
-// side from element `at` of the tensor on (the lane's own).  Four lanes share a word of 32 elements or part
-// of one, and each makes one of its four calls; two words where their pieces lie across two.  A call's four
-// comparisons turn what the lower calls leave, m, into b | (a & m): a is what they make of ones, b of zeros.
+// Which elements of a row a dropout keeps: the words of 32 that the row lies in, in shared memory, made by the
+// row's warps one row ahead, while that row is on its way.  One, two or four lanes make a word, so that every
+// lane has one to four of the calls to make.  The comparisons of some calls turn what the lower calls
+// leave, m, into b | (a & m): a is what they make of ones, b of zeros.  Each lane making the calls for its own pieces
+// took twice the instructions, and four times where rows lie across words.
+template <typename T, int NW, int CH, bool RAGGED>
 struct Bits {
+  static constexpr int V = kPiece<T>, kLanes = CH * V >= 24 ? 1 : CH * V >= 12 ? 2 : 4;
+  static constexpr int kWords = NW * CH * V + 4;   // one in front of the row's first, for pieces that begin there
+  using Space = uint32_t[2][kWords];
   const Drop* d;
   Key key;
-  uint32_t mine[4];   // bits of t for this lane's call
+  uint32_t (*space)[kWords];
+  uint32_t bit[kLanes > 1 ? 16 / kLanes : 1];      // of t, for this lane's calls
   template <typename D>
-  __device__ __forceinline__ void start(const D& drop) {
-    d = &drop, key = drop_key(drop);
-    const int call = threadIdx.x & 3;
+  __device__ __forceinline__ void start(const D& drop, Space& to) {
+    d = &drop, key = drop_key(drop), space = to;
+    if (kLanes > 1)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      mine[i] = call == 0 ? drop.bit[i] : call == 1 ? drop.bit[4 + i] : call == 2 ? drop.bit[8 + i] : drop.bit[12 + i];
+      for (int i = 0; i < 16 / kLanes; ++i) {
+        bit[i] = 0;
+#pragma unroll
+        for (int c = 0; c < kLanes; ++c) bit[i] = (threadIdx.x & (kLanes - 1)) == c ? drop.bit[16 / kLanes * c + i] : bit[i];
+      }
   }
-  __device__ __forceinline__ uint32_t word(uint64_t w) const {
-    const uint32_t call = threadIdx.x & 3;
-    const uint4 r = philox(make_uint4((uint32_t)w, (uint32_t)(w >> 32), d->site, call), key);
+  __device__ __forceinline__ uint32_t shared_word(uint64_t w) const {
+    const uint32_t lane = threadIdx.x & (kLanes - 1);
     uint32_t a = 0xffffffffu, b = 0;
-    a = majority(r.x, a, mine[0]), b = majority(r.x, b, mine[0]);
-    a = majority(r.y, a, mine[1]), b = majority(r.y, b, mine[1]);
-    a = majority(r.z, a, mine[2]), b = majority(r.z, b, mine[2]);
-    a = majority(r.w, a, mine[3]), b = majority(r.w, b, mine[3]);
 #pragma unroll
-    for (uint32_t o = 1; o < 4; o *= 2) {   // the upper calls' of the lower ones'
-      const uint32_t oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-      const bool upper = call & o;
-      const uint32_t ua = upper ? a : oa, ub = upper ? b : ob, la = upper ? oa : a, lb = upper ? ob : b;
-      a = ub | (ua & la), b = ub | (ua & lb);
+    for (int i = 0; i < 4 / kLanes; ++i) {
+      const uint4 r = philox(make_uint4((uint32_t)w, (uint32_t)(w >> 32), d->site, 4 / kLanes * lane + i), key);
+      a = majority4(r, a, bit + 4 * i), b = majority4(r, b, bit + 4 * i);
+    }
+#pragma unroll
+    for (uint32_t o = 1; o < kLanes; o *= 2) {   // the upper calls' of the lower ones'; the last lane has it all
+      const uint32_t la = __shfl_xor_sync(0xffffffffu, a, o), lb = __shfl_xor_sync(0xffffffffu, b, o);
+      a = b | (a & la), b = b | (a & lb);
     }
     return b;
   }
-  template <int V>
-  __device__ __forceinline__ uint32_t of_piece(int64_t at) const {
-    const int place = (threadIdx.x & 3) * V;
-    const int64_t first = at - place;     // the four lanes'
-    const int shift = (int)(first & 31);
-    uint64_t bits = word((uint64_t)(first >> 5));
-    if (first & (4 * V - 1)) bits |= (uint64_t)word((uint64_t)(first >> 5) + 1) << 32;   // the same for the whole warp
-    return (uint32_t)(bits >> (shift + place));
+  // by the threads of the row, `t` in them
+  __device__ __forceinline__ void make(int64_t row, int cols, int t, int which) const {
+    const int64_t first = row * cols >> 5;
+    const int n = (int)((row * cols + cols - 1 >> 5) - first) + 1;
+    uint32_t* to = space[which] + 1;
+    if (kLanes == 1 || d->first == 3) {
+      for (int i = t; i < n; i += 32 * NW) to[i] = kept_word(*d, key, (uint64_t)(first + i));
+    } else {
+      for (int i = t; i - (t & 31) < n * kLanes; i += 32 * NW) {   // whole warps
+        const uint32_t m = shared_word((uint64_t)(first + i / kLanes));
+        if (i % kLanes == kLanes - 1 && i < n * kLanes) to[i / kLanes] = m;
+      }
+    }
+  }
+  // of the piece that begins `col` elements from the row's first on
+  __device__ __forceinline__ uint32_t of_piece(int64_t row, int cols, int col, int which) const {
+    const int from = (int)(row * cols & 31) + col;
+    const uint32_t* w = space[which] + 1 + (from >> 5);
+    return RAGGED ? __funnelshift_r(w[0], w[1], from) : w[0] >> (from & 31);
   }
 };
 
@@ -416,21 +434,27 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, const __grid_constant
   Weights<T, RAGGED, NW> weight, bias;
   weight.place(a.weight, (int)a.wtype, 1.f, cols, phase, (float4*)(space + ring_bytes));
   bias.place(a.bias, (int)a.wtype, 0.f, cols, phase, (float4*)(space + ring_bytes) + weight.half * (V / 4));
+  Bits<T, NW, CH, RAGGED> random;
+  if constexpr (kDropout) {
+    __shared__ typename Bits<T, NW, CH, RAGGED>::Space words[kGroups];
+    random.start(drop, words[threadIdx.x / (32 * NW)]);
+    if (first < a.rows) random.make(first, cols, t, 0);
+  }
   __syncthreads();
   constexpr bool kHold = NW == 1 || CH <= 2;   // in registers
   float held[kHold ? CH : 1][2][V];
 #pragma unroll
   for (int i = 0; kHold && i < CH; ++i) weight.get(c[i], cols, phase, held[i][0]), bias.get(c[i], cols, phase, held[i][1]);
   const float inv = 1.f / (float)cols;
-  Bits random;
-  if constexpr (kDropout) random.start(drop);
-  int s = 0;
-  for (int64_t row = first; row < a.rows; row += step) {
+  int s = 0, which = 0;
+  for (int64_t row = first; row < a.rows; row += step, which ^= 1) {
     uint4 raw[CH];
     uint32_t kept[CH];
-    if constexpr (kDropout)   // while the row is on its way
+    if constexpr (kDropout) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece<V>(row * cols + c[i].first);
+      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece(row, cols, c[i].first, which);
+      if (row + step < a.rows) random.make(row + step, cols, t, which ^ 1);   // row_sums() is between this and its use
+    }
     ring.wait(s, guard);
     if (ring.alone(row)) ring.template fill_ends<NW>(row, s, phase, t);
     auto piece = [&](int i, int k) { return c[i].take(ring.slot(s, k), cols, phase); };
@@ -534,6 +558,12 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, const __grid_consta
   }
   Weights<T, RAGGED, NW> weight;
   weight.place(a.weight, (int)a.wtype, 1.f, cols, phase, (float4*)(space + ring_bytes));
+  Bits<T, NW, CH, RAGGED> random;
+  if constexpr (kDropout) {
+    __shared__ typename Bits<T, NW, CH, RAGGED>::Space words[kGroups];
+    random.start(drop, words[group]);
+    if (first < a.rows) random.make(first, cols, t, 0);
+  }
   __syncthreads();
   // the sums take the registers; what is left holds the weights of short rows
   constexpr bool kHold = NW <= 4;
@@ -550,16 +580,16 @@ norm_backward_rows(const __grid_constant__ HpNormBackward a, const __grid_consta
     }
   };
   const float inv = 1.f / (float)cols;
-  Bits random;
-  if constexpr (kDropout) random.start(drop);
   int s = 0, turn = 0;
   float mean_next = first < a.rows ? a.mean[first] : 0.f, rstd_next = first < a.rows ? a.rstd[first] : 0.f;
   for (int64_t row = first; row < a.rows; row += step, turn ^= 1) {
     uint4 zr[CH], gr[CH], ur[CH];
     uint32_t kept[CH];
-    if constexpr (kDropout)
+    if constexpr (kDropout) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece<V>(row * cols + c[i].first);
+      for (int i = 0; i < CH; ++i) kept[i] = random.of_piece(row, cols, c[i].first, turn);
+      if (row + step < a.rows) random.make(row + step, cols, t, turn ^ 1);
+    }
     const float mean = mean_next, rstd = rstd_next;
     if (row + step < a.rows) mean_next = a.mean[row + step], rstd_next = a.rstd[row + step];
     ring.wait(s, guard);
@@ -739,14 +769,22 @@ int resident(PerDevice& known, K kernel, int threads, int smem, int* ctas) {
   }, ctas);
 }
 
+// Whether a kernel may start while the one in front of it still runs.  Not where its CTAs fill the SMs: the
+// first ones settle between those of the kernel in front, and what is left once these are gone does not lie
+// together, so that the last one that an SM should hold finds no room and goes through its rows when the others
+// are done.  32767 x 1021 fp16, forward and backward: 317 us that way, 221 this way.
+bool may_start_early(unsigned grid, int per_sm, int bytes) {
+  return 2 * (int64_t)grid <= (int64_t)per_sm * layer_sms() || per_sm * (bytes + 2048) <= 160 * 1024;
+}
+
 template <typename T, int NW, int CH, bool RAGGED>
 int forward_rows(const HpNormForward& a, const MaybeDrop& d, uint32_t* status, cudaStream_t s) {
   static PerDevice known;
   int per_sm;
   if (const int rc = resident(known, norm_forward_rows<T, NW, CH, RAGGED>, kThreadsOf<NW>, space_of(kCtasOf<NW>), &per_sm)) return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasOf<NW>), a.cols, a.residual ? 2 : 1, 2, false);
-  return launch_behind(norm_forward_rows<T, NW, CH, RAGGED>, ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED), kThreadsOf<NW>,
-                       r.bytes, s, a, d, r.depth, r.slot, r.ring, status);
+  const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
+  return launch(may_start_early(grid, per_sm, r.bytes), norm_forward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, d, r.depth, r.slot, r.ring, status);
 }
 template <typename T, int NW, int CH, bool RAGGED>
 int backward_rows(const HpNormBackward& a, const MaybeDrop& d, uint32_t* status, cudaStream_t s) {
@@ -756,7 +794,7 @@ int backward_rows(const HpNormBackward& a, const MaybeDrop& d, uint32_t* status,
     return rc;
   const RingSize r = ring_size<T, NW, CH, RAGGED>(space_of(kCtasBack<NW, RAGGED>), a.cols, a.dz ? 3 : 2, 1, true);
   const unsigned grid = ctas_for(a.rows, kGroupsOf<NW>, per_sm, RAGGED);
-  const int rc = launch_behind(norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, d, r.depth, r.slot,
+  const int rc = launch(may_start_early(grid, per_sm, r.bytes), norm_backward_rows<T, NW, CH, RAGGED>, grid, kThreadsOf<NW>, r.bytes, s, a, d, r.depth, r.slot,
                                r.ring, status);
   if (rc || (!a.dweight && !a.dbias)) return rc;
   return column_sums((const float*)a.workspace, (int)grid, 2 * a.cols, a.cols, a.dweight, a.dbias, (int)a.wtype, s);

@@ -140,7 +140,7 @@ inline int told(cudaError_t rc) {
 }
 
 template <typename... Params, typename... Args>
-int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
+int launch(bool early, void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -150,8 +150,12 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem,
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 1 : 0;
   return told(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
+}
+template <typename... Params, typename... Args>
+int launch_behind(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
+  return launch(true, kernel, grid, block, smem, s, args...);
 }
 
 // Lets the kernel have `smem` bytes of dynamic shared memory on the current device.  `done` is the

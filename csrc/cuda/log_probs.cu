@@ -1,9 +1,11 @@
 // Log probabilities of one token in each row of logits, the entropy of the row and its likeliest tokens,
 // in one pass over the logits; the gradient in a second one.
 //
-// A thread keeps a running maximum m, the sum s of exp(x - m) and the sum e of (x - m) exp(x - m): then
-// log p = (x - m) - log s, and the entropy is log s - e / s, in which a large m has cancelled already.
-// Bound: the traffic; exp takes 16 a cycle and SM, two thirds of the time that 16-bit logits take to arrive.
+// A thread keeps the largest logit so far m, the sum s of exp(x - m) and the sum e of z 2^z, with z = (x - m)
+// log2(e): then log p = x - m - log s, and the entropy is log s - ln 2 e / s; a large m has cancelled in both
+// already, and logits at the type's lowest value stay apart from -inf.  Bound: the traffic; 2^z takes 16 a
+// cycle and SM, which is as long as 16-bit logits take to arrive.  A thread fetches its own pieces ahead into
+// shared memory (cp.async), so that what is in flight costs no registers and no barrier.
 //
 // The likeliest tokens need no second pass.  The k-th largest of the maxima of 64 (32) groups of threads
 // is no larger than the k-th largest value, so what is smaller than it is none of the k.  It is taken
@@ -17,8 +19,14 @@
 namespace hipress {
 namespace {
 
-constexpr int kThreads = 256, kBatch = 4, kMostTop = 32;
+constexpr int kBatch = 4, kMostTop = 32;   // pieces of 16 bytes that a thread takes at a time
+constexpr int kLong = 128;                 // threads of a long row
 constexpr float kLn2 = 0.6931471805599453f;
+// Rows of G = 32 threads lie in CTAs of eight
+template <int G>
+constexpr int kCta = G == 32 ? 256 : G;
+template <int G>
+constexpr int kAhead = G == 32 ? 1 : 3;    // batches of a thread in shared memory
 
 // Values and their places in one order: larger values first, then lower places.  Zero: nothing.
 __device__ __forceinline__ uint64_t key_of(float v, int col) {
@@ -32,16 +40,18 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 __device__ __forceinline__ int place_of(uint64_t key) { return (int)~(uint32_t)key; }
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// The sums of exp over some of a row's values.
+// The sums over some of a row's values.
 struct Sums {
   float m, s, e;
+  __device__ __forceinline__ void raise(float to) {   // the largest value
+    const float d = fmaxf(m - to, -1e4f) * kLog2e, f = exp2_fast(d);   // of -inf the sums are zero, or NaN
+    e = f * fmaf(d, s, e), s *= f, m = to;
+  }
 };
-__device__ __forceinline__ Sums joined(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.e + b.e};   // nothing but zeros, or NaN
-  const float da = a.m == -INFINITY ? 0.f : a.m - m, db = b.m == -INFINITY ? 0.f : b.m - m;
-  const float fa = exp2_fast(da * kLog2e), fb = exp2_fast(db * kLog2e);
-  return {m, fmaf(a.s, fa, b.s * fb), fa * fmaf(da, a.s, a.e) + fb * fmaf(db, b.s, b.e)};
+__device__ __forceinline__ Sums joined(Sums x, Sums y) {
+  const float m = fmaxf(x.m, y.m);
+  x.raise(m), y.raise(m);
+  return {m, x.s + y.s, x.e + y.e};
 }
 __device__ __forceinline__ Sums of_warp(Sums v) {
 #pragma unroll
@@ -62,15 +72,88 @@ struct Row {
     phase = (int)((uintptr_t)x / sizeof(T) % V);
     pieces = (vocab + phase + V - 1) / V;
   }
+  __device__ __forceinline__ bool whole(int p, int end) const {
+    const int col = p * V - phase;
+    return p < end && col >= 0 && col + V <= vocab;
+  }
   __device__ __forceinline__ uint4 piece(int p, int end) const {
     const int col = p * V - phase;
-    if (p < end && col >= 0 && col + V <= vocab) return *(const uint4*)(x + col);
+    if (whole(p, end)) return *(const uint4*)(x + col);
     float v[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = p < end && col + j >= 0 && col + j < vocab ? to_f(x[col + j]) : -INFINITY;
     return pack<T>(v);
   }
+  // the same into shared memory, some time
+  __device__ __forceinline__ void fetch(uint4* to, int p, int end) const {
+    if (whole(p, end))
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(x + p * V - phase) : "memory");
+    else
+      *to = piece(p, end);
+  }
 };
+
+// The largest of a piece; a NaN is none
+template <typename T>
+__device__ __forceinline__ float highest(uint4 v);
+template <>
+__device__ __forceinline__ float highest<float>(uint4 v) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+template <typename T2>
+__device__ __forceinline__ T2 highest2(uint4 v) {
+  return __hmax2(__hmax2(*(T2*)&v.x, *(T2*)&v.y), __hmax2(*(T2*)&v.z, *(T2*)&v.w));
+}
+template <>
+__device__ __forceinline__ float highest<__nv_bfloat16>(uint4 v) {
+  const float2 f = __bfloat1622float2(highest2<__nv_bfloat162>(v));
+  return fmaxf(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ float highest<__half>(uint4 v) {
+  const float2 f = __half22float2(highest2<__half2>(v));
+  return fmaxf(f.x, f.y);
+}
+// Where z 2^z is wanted, no z is infinite: values that lie far below the largest count as one for which 2^z is
+// zero as well.  NaN stays.
+__device__ __forceinline__ float far_below(float m, float lowest) {
+  return m == -INFINITY ? -1e4f : fmaxf(m - fmaxf(300.f, fabsf(m) * 0.015625f), lowest);   // after rounding to 8 bits too
+}
+template <typename T>
+struct AtLeast;
+template <>
+struct AtLeast<float> {
+  float low;
+  __device__ __forceinline__ void set(float m) { low = far_below(m, -3e38f); }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(__uint_as_float(x)), "f"(low));
+    return __float_as_uint(y);
+  }
+};
+template <>
+struct AtLeast<__nv_bfloat16> {
+  uint32_t low;
+  __device__ __forceinline__ void set(float m) { low = pack2<__nv_bfloat16>(far_below(m, -3e38f), far_below(m, -3e38f)); }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    const __nv_bfloat162 y = __hmax2_nan(*(const __nv_bfloat162*)&x, *(const __nv_bfloat162*)&low);
+    return *(const uint32_t*)&y;
+  }
+};
+template <>
+struct AtLeast<__half> {
+  uint32_t low;
+  __device__ __forceinline__ void set(float m) { low = pack2<__half>(far_below(m, -65504.f), far_below(m, -65504.f)); }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    const __half2 y = __hmax2_nan(*(const __half2*)&x, *(const __half2*)&low);
+    return *(const uint32_t*)&y;
+  }
+};
+template <bool ENTROPY, typename T>
+__device__ __forceinline__ uint4 finite(uint4 v, const AtLeast<T>& at_least) {
+  if (ENTROPY) v = make_uint4(at_least.of(v.x), at_least.of(v.y), at_least.of(v.z), at_least.of(v.w));
+  return v;
+}
 
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
@@ -102,7 +185,7 @@ constexpr int kMostSplit = 8;   // CTAs that share a row
 // What G threads that share a row keep of its largest values.
 template <int G>
 struct Largest {
-  static constexpr int kGroups = G == 32 ? 32 : 64, kList = G == 32 ? 256 : 2048;
+  static constexpr int kGroups = G == 32 ? 32 : 64, kList = G == 32 ? 256 : 1024;
   uint64_t group[kGroups], least, best[kMostTop], found[G / 32], list[kList];
   int n;
 };
@@ -147,9 +230,10 @@ __device__ __forceinline__ void in_order(const uint64_t* keys, int n, uint64_t* 
 }
 
 template <typename T, int G, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_constant__ HpLogProbs a) {
-  constexpr int V = kPiece<T>, kRows = kThreads / G;
-  __shared__ Sums part[G == 32 ? 1 : kThreads / 32], parts[kMostSplit];
+__global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(const __grid_constant__ HpLogProbs a) {
+  constexpr int V = kPiece<T>, kThreads = kCta<G>, kRows = kThreads / G;
+  extern __shared__ uint4 fetched[];   // [kAhead][kBatch][threads]
+  __shared__ Sums part[G / 32], parts[kMostSplit];
   __shared__ uint64_t others[TOP && G != 32 ? kMostSplit * kMostTop : 1];
   __shared__ Largest<G> largest[TOP ? kRows : 1];
   __shared__ float losses[kRows][2];
@@ -168,58 +252,60 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
   const int each = (r.pieces + split - 1) / split, first = rank * each, end = read ? min(first + each, r.pieces) : 0;
   if (TOP) group_sync<G>();
 
+  uint4* slot = fetched + threadIdx.x;   // of the next batch
+  auto fetch = [&](int p) {
+    if (p < end)
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) r.fetch(slot + i * kThreads, p + t + i * G, end);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot += kBatch * kThreads;
+    if (slot >= fetched + kAhead<G> * kBatch * kThreads) slot -= kAhead<G> * kBatch * kThreads;
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead<G>; ++i) fetch(first + i * G * kBatch);
   Sums sum = {-INFINITY, 0.f, 0.f};
+  AtLeast<T> at_least;
+  at_least.set(-INFINITY);
   uint64_t best = 0, least = 0;
   float bar = -INFINITY;   // the value of `least`
   for (int p = first, batch = 0; p < end; p += G * kBatch, ++batch) {   // the same for all threads of a row
     uint4 raw[kBatch];
     float top[kBatch];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead<G> - 1) : "memory");
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) raw[i] = r.piece(p + t + i * G, end);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      float v[V];
-      unpack<T>(raw[i], v);
-      top[i] = v[0];
-#pragma unroll
-      for (int j = 1; j < V; ++j) top[i] = fmaxf(top[i], v[j]);
-    }
-    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    if (high > sum.m) {
-      if (sum.m != -INFINITY) {
-        const float d = sum.m - high, f = exp2_fast(d * kLog2e);
-        sum.e = f * fmaf(d, sum.s, sum.e), sum.s *= f;
-      }
-      sum.m = high;
+    for (int i = 0; i < kBatch; ++i) raw[i] = slot[i * kThreads], top[i] = highest<T>(raw[i]);
+    const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    if (now > sum.m) {
+      sum.raise(now);
+      if (ENTROPY) at_least.set(now);
       if (TOP) {   // the first of the places that hold it
         int at = -1;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
-          if (at < 0 && top[i] == high) {
+          if (at < 0 && top[i] == now) {
             float v[V];
             unpack<T>(raw[i], v);
 #pragma unroll
             for (int j = V - 1; j >= 0; --j)
-              if (v[j] == high) at = (p + t + i * G) * V - r.phase + j;
+              if (v[j] == now) at = (p + t + i * G) * V - r.phase + j;
           }
-        best = larger(best, key_of(high, at));
+        best = larger(best, key_of(now, at));
       }
+    } else if (TOP && batch == 0 && p + t < end) {   // nothing but -inf so far
+      best = key_of(-INFINITY, max((p + t) * V - r.phase, 0));
     }
+    fetch(p + kAhead<G> * G * kBatch);   // where this thread alone has read, and has what it read
     const float minus = sum.m == -INFINITY ? 0.f : -sum.m;
     F2 s = {0.f, 0.f}, e = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       float v[V];
-      unpack<T>(raw[i], v);
+      unpack<T>(finite<ENTROPY>(raw[i], at_least), v);
 #pragma unroll
       for (int j = 0; j < V; j += 2) {
-        F2 d = add2({v[j], v[j + 1]}, {minus, minus});
-        const F2 z = mul2(d, {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
+        const F2 z = mul2(add2({v[j], v[j + 1]}, {minus, minus}), {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
         s = add2(s, x);
-        if (ENTROPY) {
-          d = {fmaxf(d.x, -200.f), fmaxf(d.y, -200.f)};   // no infinity times zero
-          e = fma2(x, d, e);
-        }
+        if (ENTROPY) e = fma2(x, z, e);
       }
     }
     sum.s += s.x + s.y, sum.e += e.x + e.y;
@@ -254,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
     __syncthreads();
     sum = part[0];
 #pragma unroll
-    for (int i = 1; i < kThreads / 32; ++i) sum = joined(sum, part[i]);
+    for (int i = 1; i < G / 32; ++i) sum = joined(sum, part[i]);
   }
   if (TOP) {
     group_sync<G>();
@@ -309,7 +395,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_kernel(const __grid_consta
     if (token != a.ignored) lp = token >= 0 && token < r.vocab ? log_p(to_f(r.x[token])) : NAN;
     if (a.log_probs) a.log_probs[row] = lp;
     a.stats[2 * row] = sum.m, a.stats[2 * row + 1] = lns;
-    if (ENTROPY) a.entropy[row] = none ? 0.f : lns - sum.e / sum.s;
+    if (ENTROPY) a.entropy[row] = none ? 0.f : fmaf(-kLn2, sum.e / sum.s, lns);
   }
   if (TOP && there && t < k) {
     a.top_log_probs[row * k + t] = log_p(value_of(l.best[t]));
@@ -359,10 +445,10 @@ __global__ void __launch_bounds__(1024) loss_kernel(const float2* parts, int64_t
 }
 
 // dx = g (1 at the token - p) - h p (log p + entropy).  Pieces go by the boundaries of the result; logits that
-// lie otherwise are read element by element.
+// lie otherwise are read element by element.  A row's batches are shared by `chunks` CTAs, which fetch one ahead.
 template <typename T, int G, bool ENTROPY>
-__global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __grid_constant__ HpLogProbsBackward a, int chunks) {
-  constexpr int V = kPiece<T>, kRows = kThreads / G;
+__global__ void __launch_bounds__(256) log_probs_backward_kernel(const __grid_constant__ HpLogProbsBackward a, int chunks) {
+  constexpr int V = kPiece<T>, kRows = 256 / G;
   const int t = threadIdx.x % G;
   const int64_t row = (int64_t)(blockIdx.x / chunks) * kRows + threadIdx.x / G;
   const int chunk = blockIdx.x % chunks;
@@ -374,48 +460,64 @@ __global__ void __launch_bounds__(kThreads) log_probs_backward_kernel(const __gr
   float g = token == a.ignored || !a.dlog_probs ? 0.f : a.dlog_probs[a.one ? 0 : row];
   if (g != 0.f && a.count) g /= *a.count;
   if (a.negative) g = -g;
-  const float h = ENTROPY ? a.dentropy[row] : 0.f, m = a.stats[2 * row], lns = a.stats[2 * row + 1];
+  const float h = ENTROPY ? a.dentropy[row] : 0.f, m = a.stats[2 * row], log2s = a.stats[2 * row + 1] * kLog2e;
   if (token != a.ignored && (token < 0 || token >= in.vocab)) g = NAN;
-  const float own = ENTROPY ? a.entropy[row] - lns : 0.f;
   const bool some = (g != 0.f || h != 0.f) && m != -INFINITY, alike = in.phase == out.phase;
+  // p times by + hz z, z = log2 p
+  const float hz = h * -kLn2, by = ENTROPY ? fmaf(-h, a.entropy[row], -g) : -g;
+  const int mine = g != 0.f && token >= 0 && token < in.vocab ? (int)token : -V;
   T* to = (T*)a.dlogits + row * a.vocab;
+  AtLeast<T> at_least;
+  at_least.set(m);
+  auto take = [&](uint4 (&raw)[kBatch], int p) {
 #pragma unroll
-  for (int i = 0; i < kBatch; ++i) {
-    const int p = (chunk * kBatch + i) * G + t, col = p * V - out.phase;
-    if (p >= out.pieces) break;
-    const bool whole = col >= 0 && col + V <= out.vocab;
-    float v[V];
-    if (!some) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = 0.f;
-    } else {
-      if (alike && whole) {
-        unpack<T>(*(const uint4*)(in.x + col), v);
+    for (int i = 0; i < kBatch; ++i) {
+      const int col = (p + i * G + t) * V - out.phase;
+      if (!some || col >= out.vocab) {
+        raw[i] = make_uint4(0, 0, 0, 0);
+      } else if (alike && col >= 0 && col + V <= out.vocab) {
+        raw[i] = *(const uint4*)(in.x + col);
       } else {
+        float v[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = col + j >= 0 && col + j < out.vocab ? to_f(in.x[col + j]) : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float d = v[j] - m;
-        const float pr = exp2_fast((d - lns) * kLog2e);
-        float by = g;
-        if (ENTROPY) by = fmaf(h, fmaxf(d, -200.f) + own, g);   // no infinity times zero
-        v[j] = -(pr * by);
-      }
-      const int at = (int)token - col;
-      if (token == col + at && at >= 0 && at < V && g != 0.f) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j == at) v[j] += g;
+        raw[i] = pack<T>(v);
       }
     }
-    if (whole) {
-      *(uint4*)(to + col) = pack<T>(v);
-    } else {
+  };
+  uint4 next[kBatch];
+  take(next, chunk * G * kBatch);
+  for (int p = chunk * G * kBatch; p < out.pieces; p += chunks * G * kBatch) {
+    uint4 raw[kBatch];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (col + j >= 0 && col + j < out.vocab) to[col + j] = from_f<T>(v[j]);
+    for (int i = 0; i < kBatch; ++i) raw[i] = next[i];
+    if (p + chunks * G * kBatch < out.pieces) take(next, p + chunks * G * kBatch);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int col = (p + i * G + t) * V - out.phase;
+      if (col >= out.vocab) break;
+      float v[V];
+      unpack<T>(finite<ENTROPY>(raw[i], at_least), v);
+      if (some) {
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const F2 z = fma2(add2({v[j], v[j + 1]}, {-m, -m}), {kLog2e, kLog2e}, {-log2s, -log2s});
+          const F2 x = mul2({exp2_fast(z.x), exp2_fast(z.y)}, ENTROPY ? fma2(z, {hz, hz}, {by, by}) : F2{by, by});
+          v[j] = x.x, v[j + 1] = x.y;
+        }
+        const int at = mine - col;
+        if (at >= 0 && at < V)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j == at) v[j] += g;
+      }
+      if (col >= 0 && col + V <= out.vocab) {
+        *(uint4*)(to + col) = pack<T>(v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (col + j >= 0 && col + j < out.vocab) to[col + j] = from_f<T>(v[j]);
+      }
     }
   }
 }
@@ -427,8 +529,9 @@ template <typename T, int G, bool ENTROPY, bool TOP>
 int forward_of(const HpLogProbs& a, int split, cudaStream_t s) {
   const int64_t ctas = G == 32 ? (a.rows + 7) / 8 : a.rows * split;
   if (ctas > INT32_MAX) return HP_ERR_TOO_LARGE;
+  const int space = kAhead<G> * kBatch * kCta<G> * 16;   // at most 24 KB
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = (unsigned)ctas, cfg.blockDim = kThreads, cfg.stream = s;
+  cfg.gridDim = (unsigned)ctas, cfg.blockDim = kCta<G>, cfg.dynamicSmemBytes = space, cfg.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -451,17 +554,22 @@ int forward(const HpLogProbs& a, cudaStream_t s) {
 #define BY_USE(G, split)                                                                                           a.entropy ? (a.top ? forward_of<T, G, true, true>(a, split, s) : forward_of<T, G, true, false>(a, split, s))               : (a.top ? forward_of<T, G, false, true>(a, split, s) : forward_of<T, G, false, false>(a, split, s))
   if (pieces <= kWarpPieces) return BY_USE(32, 1);
   int split = 1;   // few rows are shared by up to eight CTAs, as long as each has a batch
-  while (split < kMostSplit && a.rows * split < 2 * layer_sms() && pieces > 2 * split * kThreads) split *= 2;
-  return BY_USE(256, split);
+  while (split < kMostSplit && a.rows * split < 4 * layer_sms() && pieces > split * kLong * kBatch) split *= 2;
+  return BY_USE(kLong, split);
 #undef BY_USE
 }
 
 template <typename T, int G, bool ENTROPY>
 int backward_of(const HpLogProbsBackward& a, cudaStream_t s) {
-  const int64_t chunks = G == 32 ? 1 : (most_pieces<T>(a.vocab) + G * kBatch - 1) / (G * kBatch);
+  // CTAs that a row takes: enough for four to an SM, a batch each at least
+  int64_t chunks = 1;
+  if (G != 32) {
+    const int64_t most = (most_pieces<T>(a.vocab) + G * kBatch - 1) / (G * kBatch), want = (4 * layer_sms() + a.rows - 1) / a.rows;
+    chunks = want < most ? want : most;
+  }
   const int64_t ctas = G == 32 ? (a.rows + 7) / 8 : a.rows * chunks;
   if (ctas > INT32_MAX) return HP_ERR_TOO_LARGE;
-  return launch_behind(log_probs_backward_kernel<T, G, ENTROPY>, (unsigned)ctas, kThreads, 0, s, a, (int)chunks);
+  return launch_behind(log_probs_backward_kernel<T, G, ENTROPY>, (unsigned)ctas, 256, 0, s, a, (int)chunks);
 }
 template <typename T>
 int backward(const HpLogProbsBackward& a, cudaStream_t s) {

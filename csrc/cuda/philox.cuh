@@ -9,8 +9,8 @@
 //
 // The 32 comparisons of a word are made at once, a bit of t at a time from the lowest on: where it is set the
 // upper bits decide for 1 or leave it as it is, r | m, else for 0, r & m.  Both are the majority of r, m
-// and the bit of t, one instruction for 32 elements.  Calls that hold only zeros of t below its lowest
-// one decide nothing and are not made: p = 1/2 takes one of the four.
+// and the bit of t, one instruction for 32 elements.  Zeros of t below its lowest one decide nothing: where the
+// upper four bits are all there is (p = 1/2, 1/4 ..), only the last call is made.
 #pragma once
 #include "layers.cuh"
 
@@ -19,7 +19,7 @@ namespace hipress {
 struct Drop {
   const int64_t* seed_at;
   int64_t seed;
-  uint32_t site, first;    // the first call that counts
+  uint32_t site, first;    // the first call whose bits of t are not all zero
   uint32_t bit[16];        // bits of t, all ones or zeros
   float up, share;         // 2^16 / t, t / 2^16
 };
@@ -39,9 +39,11 @@ inline bool drop_of(Drop* d, const HpDropout& a) {
 struct Key {
   uint32_t lo, hi;
 };
+// By a whole warp.  The compiler knows that it is the same in all threads, and keeps the rounds' keys in
+// uniform registers: added up in each thread they were an eighth of the instructions of a dropped attention.
 __device__ __forceinline__ Key drop_key(const Drop& d) {
   const int64_t s = d.seed_at ? *d.seed_at : d.seed;
-  return {(uint32_t)s, (uint32_t)(s >> 32)};
+  return {__shfl_sync(0xffffffffu, (uint32_t)s, 0), __shfl_sync(0xffffffffu, (uint32_t)(s >> 32), 0)};
 }
 
 __device__ __forceinline__ uint4 philox(uint4 c, Key k) {
@@ -56,19 +58,32 @@ __device__ __forceinline__ uint4 philox(uint4 c, Key k) {
 
 __device__ __forceinline__ uint32_t majority(uint32_t a, uint32_t b, uint32_t c) { return (a & b) | (c & (a | b)); }
 
-// The bits of word w: set where an element is kept.
-__device__ __forceinline__ uint32_t kept_word(const Drop& d, Key k, uint64_t w) {
-  uint32_t m = 0;
+__device__ __forceinline__ uint32_t majority4(uint4 r, uint32_t m, const uint32_t* bit) {
+  return majority(r.w, majority(r.z, majority(r.y, majority(r.x, m, bit[0]), bit[1]), bit[2]), bit[3]);
+}
+
+// The bits of words w: set where an element is kept.  Several at once, since a call is one chain of seven
+// rounds, and without a branch between them.
+template <int N>
+__device__ __forceinline__ void kept_words(const Drop& d, Key k, const uint64_t (&w)[N], uint32_t (&m)[N]) {
+  auto call = [&](int n, uint32_t c) { return philox(make_uint4((uint32_t)w[n], (uint32_t)(w[n] >> 32), d.site, c), k); };
+  if (d.first == 3) {
 #pragma unroll
-  for (uint32_t call = 0; call < 4; ++call) {
-    if (call < d.first) continue;
-    const uint4 r = philox(make_uint4((uint32_t)w, (uint32_t)(w >> 32), d.site, call), k);
-    m = majority(r.x, m, d.bit[4 * call]);
-    m = majority(r.y, m, d.bit[4 * call + 1]);
-    m = majority(r.z, m, d.bit[4 * call + 2]);
-    m = majority(r.w, m, d.bit[4 * call + 3]);
+    for (int n = 0; n < N; ++n) m[n] = majority4(call(n, 3), 0, d.bit + 12);
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      m[n] = 0;
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) m[n] = majority4(call(n, c), m[n], d.bit + 4 * c);
+    }
   }
-  return m;
+}
+__device__ __forceinline__ uint32_t kept_word(const Drop& d, Key k, uint64_t w) {
+  const uint64_t ws[1] = {w};
+  uint32_t m[1];
+  kept_words<1>(d, k, ws, m);
+  return m[0];
 }
 
 }  // namespace hipress
