@@ -440,8 +440,8 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
             }
             sums[i / 2 & 1] = add2(sums[i / 2 & 1], e);
             if (DROP) {   // the sum is of all
-              const uint32_t two = kept.w[c / 32] >> (c % 32 + i);
-              e.x = two & 1 ? e.x : 0.f, e.y = two & 2 ? e.y : 0.f;
+              e.x = kept.w[c / 32] & 1u << (c % 32 + i) ? e.x : 0.f;
+              e.y = kept.w[c / 32] & 2u << (c % 32 + i) ? e.y : 0.f;
             }
             to_y[i / 2] = pack2<T>(e.x, e.y);
           }
@@ -941,19 +941,18 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
       auto gradients = [&](auto all, auto of_keys) {   // packed P into x, dS into y
 #pragma unroll
         for (int i = 0; i < kPass; i += 2) {
-          const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])};
-          F2 u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
+          const F2 v = {__uint_as_float(x[i]), __uint_as_float(x[i + 1])}, u = {__uint_as_float(y[i]), __uint_as_float(y[i + 1])};
           const F2 z = of_keys ? mul2(v, {l.c, l.c}) : fma2(v, {l.c, l.c}, {lse, lse});
           F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-          if (DROP) {
-            const uint32_t two = kept.w[i / 32] >> (i % 32);
-            u = {two & 1 ? u.x : 0.f, two & 2 ? u.y : 0.f};
-            u = add2(u, of_keys ? *(const F2*)(deltas + delta_at(i)) : F2{delta, delta});
-          }
-          F2 ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys || DROP ? u : add2(u, {delta, delta}));
-          if (DROP) {
-            const uint32_t two = kept.w[i / 32] >> (i % 32);
-            pr = {two & 1 ? pr.x : 0.f, two & 2 ? pr.y : 0.f};
+          F2 ds;
+          if (DROP) {   // what is kept of P times dP, and all of it times delta
+            const F2 all_p = pr;
+            pr.x = kept.w[i / 32] & 1u << (i % 32) ? pr.x : 0.f;
+            pr.y = kept.w[i / 32] & 2u << (i % 32) ? pr.y : 0.f;
+            ds = fma2(pr, u, mul2(all_p, of_keys ? *(const F2*)(deltas + delta_at(i)) : F2{delta, delta}));
+            if (kNarrow<T> && of_keys) ds = mul2(ds, {of_p, of_p});
+          } else {
+            ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys ? u : add2(u, {delta, delta}));
           }
           if (!all) {
             const uint32_t two = seen.w[i / 32] >> (i % 32);
@@ -1174,11 +1173,17 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
             for (int k = 0; k < 4; k += 2) {
               const F2 z = fma2({__uint_as_float(x[i + k]), __uint_as_float(x[i + k + 1])}, {l.c, l.c}, {lv[k], lv[k + 1]});
               F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
-              F2 u = {__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])};
-              const uint32_t stay = DROP ? (c & 32 ? kept[1] : kept[0]) >> (i + k) : 3;
-              if (DROP) u = {stay & 1 ? u.x : 0.f, stay & 2 ? u.y : 0.f};
-              F2 ds = mul2(kNarrow<T> ? mul2(pr, {of_p, of_p}) : pr, add2(u, {dv[k], dv[k + 1]}));
-              if (DROP) pr = {stay & 1 ? pr.x : 0.f, stay & 2 ? pr.y : 0.f};
+              const F2 u = {__uint_as_float(y[i + k]), __uint_as_float(y[i + k + 1])};
+              F2 ds;
+              if (DROP) {
+                const uint32_t stay = c & 32 ? kept[1] : kept[0];
+                const F2 all_p = pr;
+                pr.x = stay & 1u << (i + k) ? pr.x : 0.f, pr.y = stay & 2u << (i + k) ? pr.y : 0.f;
+                ds = fma2(pr, u, mul2(all_p, {dv[k], dv[k + 1]}));
+                if (kNarrow<T>) ds = mul2(ds, {of_p, of_p});
+              } else {
+                ds = mul2(kNarrow<T> ? mul2(pr, {of_p, of_p}) : pr, add2(u, {dv[k], dv[k + 1]}));
+              }
               if (!all) {
                 const uint32_t two = bits_of >> (i + k);
                 if (!(two & 1)) pr.x = ds.x = 0.f;

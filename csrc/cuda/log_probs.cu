@@ -13,6 +13,10 @@
 // is put in order in the end.  Values are compared together with their place, so that of equals the first counts
 // and a row of equal values does not flood the list; should it overflow, or a value be no number, the row is read
 // again once for each of the k.
+#include <limits.h>
+
+#include <type_traits>
+
 #include "activation.cuh"
 #include "tcgen05.cuh"
 
@@ -54,10 +58,19 @@ __device__ __forceinline__ Sums joined(Sums x, Sums y) {
   return {m, x.s + y.s, x.e + y.e};
 }
 __device__ __forceinline__ Sums of_warp(Sums v) {
+  float m = v.m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
-    v = joined(v, {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o), __shfl_xor_sync(0xffffffffu, v.e, o)});
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  v.raise(m);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v.s += __shfl_xor_sync(0xffffffffu, v.s, o), v.e += __shfl_xor_sync(0xffffffffu, v.e, o);
   return v;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t none16() {
+  if constexpr (sizeof(T) == 2) return pack2<T>(-INFINITY, -INFINITY);
+  else return 0;
 }
 
 // One row (or part of it) in pieces of 16 bytes, cut at their boundaries; what is outside reads as -inf.
@@ -66,8 +79,14 @@ struct Row {
   static constexpr int V = kPiece<T>;
   const T* x;
   int vocab, phase, pieces;
-  __device__ __forceinline__ Row(const void* logits, int64_t row, int64_t inner, int64_t ld_outer, int64_t ld, int64_t cols) {
-    x = (const T*)logits + row / inner * ld_outer + row % inner * ld;
+  __device__ __forceinline__ Row(const void* logits, int row, int64_t inner, int64_t ld_outer, int64_t ld, int64_t cols) {
+    x = (const T*)logits;
+    if (row < inner) {
+      x += row * ld;
+    } else {
+      const uint32_t o = (uint32_t)row / (uint32_t)inner;
+      x += o * ld_outer + (row - o * inner) * ld;
+    }
     vocab = (int)cols;
     phase = (int)((uintptr_t)x / sizeof(T) % V);
     pieces = (vocab + phase + V - 1) / V;
@@ -76,20 +95,43 @@ struct Row {
     const int col = p * V - phase;
     return p < end && col >= 0 && col + V <= vocab;
   }
-  __device__ __forceinline__ uint4 piece(int p, int end) const {
-    const int col = p * V - phase;
-    if (whole(p, end)) return *(const uint4*)(x + col);
+  static __device__ __forceinline__ uint4 nothing() {
+    const uint32_t none = sizeof(T) == 4 ? 0xff800000u : none16<T>();
+    return make_uint4(none, none, none, none);
+  }
+  // the first or the last piece, one element at a time
+  static __device__ __noinline__ uint4 end_piece(const T* x, int col, int vocab) {
     float v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = p < end && col + j >= 0 && col + j < vocab ? to_f(x[col + j]) : -INFINITY;
+    for (int j = 0; j < V; ++j) v[j] = col + j >= 0 && col + j < vocab ? to_f(x[col + j]) : -INFINITY;
     return pack<T>(v);
   }
-  // the same into shared memory, some time
-  __device__ __forceinline__ void fetch(uint4* to, int p, int end) const {
-    if (whole(p, end))
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(x + p * V - phase) : "memory");
-    else
-      *to = piece(p, end);
+  __device__ __forceinline__ uint4 piece(int p, int end) const {
+    const int col = p * V - phase;
+    return p >= end ? nothing() : whole(p, end) ? *(const uint4*)(x + col) : end_piece(x, col, vocab);
+  }
+  // N pieces, `step` apart, into shared memory some time, `stride` apart; -inf from `end` on
+  template <int N>
+  __device__ __forceinline__ void fetch(uint4* to, int stride, int p, int step, int end) const {
+    const int col = p * V - phase;
+    if (col >= 0 && col + ((N - 1) * step + 1) * V <= vocab && p + (N - 1) * step < end) {
+      const uint4* from = (const uint4*)(x + col);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to + i * stride)), "l"(from + i * step) : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = col + i * step * V;
+        uint4* at = to + i * stride;
+        if (p + i * step >= end || c >= vocab)
+          *at = nothing();
+        else if (c >= 0 && c + V <= vocab)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at)), "l"(x + c) : "memory");
+        else
+          *at = end_piece(x, c, vocab);
+      }
+    }
   }
 };
 
@@ -185,9 +227,10 @@ constexpr int kMostSplit = 8;   // CTAs that share a row
 // What G threads that share a row keep of its largest values.
 template <int G>
 struct Largest {
-  static constexpr int kGroups = G == 32 ? 32 : 64, kList = G == 32 ? 256 : 1024;
-  uint64_t group[kGroups], least, best[kMostTop], found[G / 32], list[kList];
-  int n;
+  static constexpr int kGroups = G == 32 ? 32 : 64, kList = G == 32 ? 256 : 1024, kKeys = G == 32 ? 256 : 512;
+  alignas(16) uint64_t group[kGroups];
+  uint64_t least, best[kMostTop], found[G / 32], keys[kKeys];
+  int list[kList], n, left;   // pieces; of what they hold
 };
 
 template <int G>
@@ -207,7 +250,10 @@ __device__ __forceinline__ uint64_t least_of(Largest<G>& l, uint64_t best, int k
   group_sync<G>();
   int above = 0;
 #pragma unroll 8
-  for (int i = 0; i < kEach; ++i) above += l.group[part * kEach + i] > best;
+  for (int i = 0; i < kEach; i += 2) {
+    const ulonglong2 g2 = *(const ulonglong2*)(l.group + part * kEach + i);
+    above += (int)(g2.x > best) + (int)(g2.y > best);
+  }
 #pragma unroll
   for (int o = 1; o < kShare; o *= 2) above += __shfl_xor_sync(0xffffffffu, above, o);
   if (above == k - 1 && part == 0) l.least = best;   // one group's, or all those that have none
@@ -244,19 +290,17 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
   Largest<G>& l = largest[TOP ? threadIdx.x / G : 0];
   dependents_may_start();
   if (split > 1) cluster_arrive();   // whose shared memory is written has started
-  if (TOP && t == 0) l.n = 0, l.least = 0;
+  if (TOP && t == 0) l.n = l.left = 0, l.least = 0;
   wait_for_kernel_before();
   const int64_t token = there ? a.tokens[row] : a.ignored;
   const bool read = there && (ENTROPY || TOP || token != a.ignored);
-  const Row<T> r(a.logits, there ? row : 0, a.inner, a.ld_outer, a.ld, a.vocab);
+  const Row<T> r(a.logits, there ? (int)row : 0, a.inner, a.ld_outer, a.ld, a.vocab);
   const int each = (r.pieces + split - 1) / split, first = rank * each, end = read ? min(first + each, r.pieces) : 0;
   if (TOP) group_sync<G>();
 
   uint4* slot = fetched + threadIdx.x;   // of the next batch
   auto fetch = [&](int p) {
-    if (p < end)
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) r.fetch(slot + i * kThreads, p + t + i * G, end);
+    if (p < end) r.template fetch<kBatch>(slot, kThreads, p + t, G, end);
     asm volatile("cp.async.commit_group;" ::: "memory");
     slot += kBatch * kThreads;
     if (slot >= fetched + kAhead<G> * kBatch * kThreads) slot -= kAhead<G> * kBatch * kThreads;
@@ -267,7 +311,8 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
   AtLeast<T> at_least;
   at_least.set(-INFINITY);
   uint64_t best = 0, least = 0;
-  float bar = -INFINITY;   // the value of `least`
+  float high = -INFINITY, bar = -INFINITY;   // the thread's largest value; that of `least`
+  int turn = 0;
   for (int p = first, batch = 0; p < end; p += G * kBatch, ++batch) {   // the same for all threads of a row
     uint4 raw[kBatch];
     float top[kBatch];
@@ -275,62 +320,66 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) raw[i] = slot[i * kThreads], top[i] = highest<T>(raw[i]);
     const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    if (now > sum.m) {
-      sum.raise(now);
-      if (ENTROPY) at_least.set(now);
-      if (TOP) {   // the first of the places that hold it
-        int at = -1;
+    // the sums bear values that are larger by a few powers of two: raised is seldom more than once
+    if (now > sum.m + 8.f || sum.m == -INFINITY) {
+      sum.raise(fmaxf(now, sum.m));
+      if (ENTROPY) at_least.set(sum.m);
+    }
+    if (TOP) {
+      if (batch == 0 && p + t < end) {   // the first of the places that hold the largest value
+        int at = max((p + t) * V - r.phase, 0);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-          if (at < 0 && top[i] == now) {
+        for (int i = kBatch - 1; i >= 0; --i)
+          if (top[i] == now && now != -INFINITY) {
             float v[V];
             unpack<T>(raw[i], v);
 #pragma unroll
             for (int j = V - 1; j >= 0; --j)
               if (v[j] == now) at = (p + t + i * G) * V - r.phase + j;
           }
-        best = larger(best, key_of(now, at));
+        best = key_of(now, at);
+        high = now;
       }
-    } else if (TOP && batch == 0 && p + t < end) {   // nothing but -inf so far
-      best = key_of(-INFINITY, max((p + t) * V - r.phase, 0));
+      high = fmaxf(high, now);
     }
     fetch(p + kAhead<G> * G * kBatch);   // where this thread alone has read, and has what it read
     const float minus = sum.m == -INFINITY ? 0.f : -sum.m;
-    F2 s = {0.f, 0.f}, e = {0.f, 0.f};
+    F2 s, e;
+    auto add_up = [&](auto infinite) {
+      s = e = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      float v[V];
-      unpack<T>(finite<ENTROPY>(raw[i], at_least), v);
+      for (int i = 0; i < kBatch; ++i) {
+        float v[V];
+        unpack<T>(finite<infinite>(raw[i], at_least), v);
 #pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        const F2 z = mul2(add2({v[j], v[j + 1]}, {minus, minus}), {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
-        s = add2(s, x);
-        if (ENTROPY) e = fma2(x, z, e);
+        for (int j = 0; j < V; j += 2) {
+          const F2 z = mul2(add2({v[j], v[j + 1]}, {minus, minus}), {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
+          s = add2(s, x);
+          if (ENTROPY) e = fma2(x, z, e);
+        }
       }
-    }
+    };
+    add_up(std::false_type());
+    if (ENTROPY && !(e.x + e.y > -INFINITY)) add_up(std::true_type());   // zero times an infinity, or a NaN of the logits'
     sum.s += s.x + s.y, sum.e += e.x + e.y;
     if (TOP) {
-      if ((batch & (batch - 1)) == 0) {   // batches 0, 1, 2, 4, 8 ..
+      if (batch == turn) {   // batches 0, 2, 8, 32 ..
+        turn = turn ? 4 * turn : 2;
+        if (high > value_of(best) || !best) best = high == -INFINITY ? best : key_of(high, -1);   // wherever it is
         least = least_of<G>(l, best, k, t);
         bar = least ? value_of(least) : -INFINITY;
       }
+      if (now >= bar) {
+        const int place = least ? place_of(least) : INT_MAX;   // of equal values the first count
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (top[i] >= bar) {
-          float v[V];
-          unpack<T>(raw[i], v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int col = (p + t + i * G) * V - r.phase + j;
-            if (v[j] >= bar && p + t + i * G < end && col >= 0 && col < r.vocab) {
-              const uint64_t key = key_of(v[j], col);
-              if (key >= least) {
-                const int at = atomicAdd(&l.n, 1);
-                if (at < Largest<G>::kList) l.list[at] = key;
-              }
-            }
+        for (int i = 0; i < kBatch; ++i) {
+          const int q = p + t + i * G;
+          if (q < end && (top[i] > bar || (top[i] == bar && q * V - r.phase <= place))) {
+            const int at = atomicAdd(&l.n, 1);
+            if (at < Largest<G>::kList) l.list[at] = q;
           }
         }
+      }
     }
   }
   // a NaN is no maximum and in no list, but in the sum
@@ -338,15 +387,45 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
   if (G != 32) {
     if (lane == 0) part[threadIdx.x / 32] = sum;
     __syncthreads();
-    sum = part[0];
+    if (TOP || threadIdx.x < 32) {
+      sum = part[lane % (G / 32)];
+      float m = sum.m;
 #pragma unroll
-    for (int i = 1; i < G / 32; ++i) sum = joined(sum, part[i]);
+      for (int o = G / 64; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      sum.raise(m);
+#pragma unroll
+      for (int o = G / 64; o; o >>= 1)
+        sum.s += __shfl_xor_sync(0xffffffffu, sum.s, o), sum.e += __shfl_xor_sync(0xffffffffu, sum.e, o);
+    }
   }
   if (TOP) {
     group_sync<G>();
     const int n = l.n;
-    if (n <= Largest<G>::kList && sum.s == sum.s) {
-      in_order<G>(l.list, n, l.best, k, t);
+    bool listed = n <= Largest<G>::kList && sum.s == sum.s;
+    if (listed) {
+      if (n > 16) {   // the first ones were let in by lower bars
+        if (high > value_of(best)) best = key_of(high, -1);
+        least = least_of<G>(l, best, k, t);
+      }
+      for (int i = t; i < n; i += G) {
+        const int q = l.list[i];
+        float v[V];
+        unpack<T>(r.piece(q, end), v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int col = q * V - r.phase + j;
+          const uint64_t key = key_of(v[j], col);
+          if (key >= least && col >= 0 && col < r.vocab) {
+            const int at = atomicAdd(&l.left, 1);
+            if (at < Largest<G>::kKeys) l.keys[at] = key;
+          }
+        }
+      }
+      group_sync<G>();
+      listed = l.left <= Largest<G>::kKeys;
+    }
+    if (listed) {
+      in_order<G>(l.keys, l.left, l.best, k, t);
     } else {
       uint64_t last = ~0ull;
       for (int i = 0; i < k; ++i) {
@@ -447,7 +526,7 @@ __global__ void __launch_bounds__(1024) loss_kernel(const float2* parts, int64_t
 // dx = g (1 at the token - p) - h p (log p + entropy).  Pieces go by the boundaries of the result; logits that
 // lie otherwise are read element by element.  A row's batches are shared by `chunks` CTAs, which fetch one ahead.
 template <typename T, int G, bool ENTROPY>
-__global__ void __launch_bounds__(256) log_probs_backward_kernel(const __grid_constant__ HpLogProbsBackward a, int chunks) {
+__global__ void __launch_bounds__(256, 4) log_probs_backward_kernel(const __grid_constant__ HpLogProbsBackward a, int chunks) {
   constexpr int V = kPiece<T>, kRows = 256 / G;
   const int t = threadIdx.x % G;
   const int64_t row = (int64_t)(blockIdx.x / chunks) * kRows + threadIdx.x / G;
@@ -455,7 +534,7 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(const __grid_co
   dependents_may_start();
   wait_for_kernel_before();
   if (row >= a.rows) return;
-  const Row<T> in(a.logits, row, a.inner, a.ld_outer, a.ld, a.vocab), out(a.dlogits, row, a.rows, 0, a.vocab, a.vocab);
+  const Row<T> in(a.logits, (int)row, a.inner, a.ld_outer, a.ld, a.vocab), out(a.dlogits, (int)row, a.rows, 0, a.vocab, a.vocab);
   const int64_t token = a.tokens[row];
   float g = token == a.ignored || !a.dlog_probs ? 0.f : a.dlog_probs[a.one ? 0 : row];
   if (g != 0.f && a.count) g /= *a.count;
