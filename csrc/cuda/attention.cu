@@ -100,22 +100,41 @@ struct Launch {
   uint32_t* status;
 };
 
+__device__ __forceinline__ float4 shared_float4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
+
 // ---------------------------------------------------------------------- dropout
 // Rows of probabilities go by words of 32 keys.  The first word of a query's row:
 __device__ __forceinline__ uint64_t first_word(const HpAttention& p, int64_t b, int h, int row) {
   return (uint64_t)((b * p.heads + h) * p.sq + row) * (uint64_t)((p.sk + 31) / 32);
 }
+// x where the bit of `w` is set, else zero.  As a choice of the language it became shifts and logic on the bits of
+// x, two more instructions.
+__device__ __forceinline__ float where_kept(uint32_t w, uint32_t bit, float x) {
+  float y;
+  asm("{\n.reg .pred p;\n.reg .b32 t;\nand.b32 t, %2, %3;\nsetp.ne.u32 p, t, 0;\nselp.f32 %0, %1, 0f00000000, p;\n}"
+      : "=f"(y) : "f"(x), "r"(w), "r"(bit));
+  return y;
+}
 // By a whole warp: lane i's bit j becomes lane j's bit i.  Where a thread has a key, each lane makes the word of
 // one query for the warp's 32 keys, and gets those of 32 queries for its own.
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+template <int N>
+__device__ __forceinline__ void transpose(uint32_t (&x)[N]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const uint32_t m = 0xffffffffu / ((1u << o) + 1);   // bits whose place has no o
-    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, o);
-    x = lane & o ? (x & ~m) | ((y & ~m) >> o) : (x & m) | ((y & m) << o);
+    const bool upper = lane & o;
+    const uint32_t m = 0xffffffffu / ((1u << o) + 1), stay = upper ? ~m : m;   // bits whose place has no o
+#pragma unroll
+    for (int i = 0; i < N; ++i) {   // half of the bits stay, half come from the other lane, o further on
+      const uint32_t y = __shfl_xor_sync(0xffffffffu, x[i], o);
+      if (o >= 8) x[i] = __byte_perm(x[i], y, o == 16 ? (upper ? 0x3276 : 0x5410) : (upper ? 0x3715 : 0x6240));
+      else x[i] = (x[i] & stay) | (__funnelshift_l(y, y, upper ? 32 - o : o) & ~stay);
+    }
   }
-  return x;
 }
 
 // ---------------------------------------------------------------------- forward
@@ -440,8 +459,8 @@ attention_forward_tiles(const __grid_constant__ Launch l) {
             }
             sums[i / 2 & 1] = add2(sums[i / 2 & 1], e);
             if (DROP) {   // the sum is of all
-              e.x = kept.w[c / 32] & 1u << (c % 32 + i) ? e.x : 0.f;
-              e.y = kept.w[c / 32] & 2u << (c % 32 + i) ? e.y : 0.f;
+              e.x = where_kept(kept.w[c / 32], 1u << (c % 32 + i), e.x);
+              e.y = where_kept(kept.w[c / 32], 2u << (c % 32 + i), e.y);
             }
             to_y[i / 2] = pack2<T>(e.x, e.y);
           }
@@ -868,27 +887,35 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
     bool ok = true;
     Key key = {};
     if (DROP) key = drop_key(l.drop);
-    const uint64_t of_row = (uint64_t)(p.sk + 31) / 32, words = keys ? 0 : first_word(p, b, head, row);
+    // this thread's first word of tile j, and how far the second and the next tile's lie: of its query that stays, or
+    // of the queries that pass, which it makes for the warp's keys
+    const uint64_t of_row = (uint64_t)(p.sk + 31) / 32, word_apart = keys ? 32 * of_row : 1, tile_apart = keys ? kPass * of_row : kPass / 32;
+    auto word_of = [&](int j) {
+      return keys ? first_word(p, b, head * group + j / count, (first + j % count) * kPass + lane) + (r0 / 32 + quad)
+                  : first_word(p, b, head, row) + (uint64_t)j * tile_apart;
+    };
+    uint64_t word = DROP && n > half ? word_of(half) : 0;
     // of tile j: stage, buffer, turn, and place among its head's tiles
     int s = half, q = half, turn = half, place = half;
     uint32_t ph = 0, round = 0;
-    auto advance = [&] {
+    auto advance = [&](int j) {
       s += 2, q += 2, turn += 2, place += 2;
       if (s >= F::kStages) s -= F::kStages, ph ^= 1;
       if (q >= buffers) q -= buffers;
       if (turn >= turns) turn -= turns, round ^= 1;
-      while (place >= count) place -= count;
+      word += 2 * tile_apart;
+      if (place >= count) {   // the next head
+        while (place >= count) place -= count;
+        if (DROP && keys && j + 2 < n) word = word_of(j + 2);
+      }
     };
     if (n && place >= count) place -= count;   // a head of one tile
-    for (int j = half; j < n; j += 2, advance()) {
+    for (int j = half; j < n; advance(j), j += 2) {
       Seen<kPass> kept;
       if (DROP) {
-        uint64_t w = words + (uint64_t)j * (kPass / 32), more = 1;
-        if (keys)   // of the query that this lane makes them for
-          w = first_word(p, b, head * group + j / count, (first + place) * kPass + lane) + (r0 / 32 + quad), more = 32 * of_row;
-        const uint64_t ws[2] = {w, w + more};
+        const uint64_t ws[2] = {word, word + word_apart};
         kept_words(l.drop, key, ws, kept.w);
-        if (keys) kept.w[0] = transposed(kept.w[0]), kept.w[1] = transposed(kept.w[1]);
+        if (keys) transpose(kept.w);
       }
       Seen<kPass> seen;
       bool whole;
@@ -937,7 +964,8 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
       }
       tmem_wait_ld();
       // with a dropout: of the passing queries
-      const float* deltas = (const float*)(parts + s * F::kParts) + 4 * kPass;
+      const uint32_t deltas = smem_u32(parts + s * F::kParts) + 16 * kPass;
+      float4 four;
       auto gradients = [&](auto all, auto of_keys) {   // packed P into x, dS into y
 #pragma unroll
         for (int i = 0; i < kPass; i += 2) {
@@ -946,10 +974,11 @@ __global__ void __launch_bounds__(384, 1) attention_backward_tiles(const __grid_
           F2 pr = {exp2_fast(z.x), exp2_fast(z.y)};
           F2 ds;
           if (DROP) {   // what is kept of P times dP, and all of it times delta
-            const F2 all_p = pr;
-            pr.x = kept.w[i / 32] & 1u << (i % 32) ? pr.x : 0.f;
-            pr.y = kept.w[i / 32] & 2u << (i % 32) ? pr.y : 0.f;
-            ds = fma2(pr, u, mul2(all_p, of_keys ? *(const F2*)(deltas + delta_at(i)) : F2{delta, delta}));
+            if (of_keys && i % 4 == 0) four = shared_float4(deltas + 4 * delta_at(i));
+            const F2 t = mul2(pr, !of_keys ? F2{delta, delta} : i % 4 ? F2{four.z, four.w} : F2{four.x, four.y});
+            pr.x = where_kept(kept.w[i / 32], 1u << (i % 32), pr.x);
+            pr.y = where_kept(kept.w[i / 32], 2u << (i % 32), pr.y);
+            ds = {fmaf(pr.x, u.x, t.x), fmaf(pr.y, u.y, t.y)};   // in pairs they would have to be moved together
             if (kNarrow<T> && of_keys) ds = mul2(ds, {of_p, of_p});
           } else {
             ds = mul2(kNarrow<T> && of_keys ? mul2(pr, {of_p, of_p}) : pr, of_keys ? u : add2(u, {delta, delta}));
@@ -1138,7 +1167,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
       const Key key = drop_key(l.drop);
       const uint64_t w = first_word(p, b, h, 64 * half + lane) + quad, ws[2] = {w, w + 32 * ((uint64_t)(p.sk + 31) / 32)};
       kept_words(l.drop, key, ws, kept);
-      kept[0] = transposed(kept[0]), kept[1] = transposed(kept[1]);
+      transpose(kept);
     }
     const int from = p.causal ? r - shift : 0;   // the first query that sees this key
     bool whole = mine && from <= 0;
@@ -1178,7 +1207,7 @@ __global__ void __launch_bounds__(320, 2) attention_backward_short(const __grid_
               if (DROP) {
                 const uint32_t stay = c & 32 ? kept[1] : kept[0];
                 const F2 all_p = pr;
-                pr.x = stay & 1u << (i + k) ? pr.x : 0.f, pr.y = stay & 2u << (i + k) ? pr.y : 0.f;
+                pr.x = where_kept(stay, 1u << (i + k), pr.x), pr.y = where_kept(stay, 2u << (i + k), pr.y);
                 ds = fma2(pr, u, mul2(all_p, {dv[k], dv[k + 1]}));
                 if (kNarrow<T>) ds = mul2(ds, {of_p, of_p});
               } else {

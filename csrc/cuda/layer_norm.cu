@@ -374,12 +374,13 @@ struct Bits {
   }
   __device__ __forceinline__ uint32_t shared_word(uint64_t w) const {
     const uint32_t lane = threadIdx.x & (kLanes - 1);
+    uint4 c[4 / kLanes];
+#pragma unroll
+    for (int i = 0; i < 4 / kLanes; ++i) c[i] = make_uint4((uint32_t)w, (uint32_t)(w >> 32), d->site, 4 / kLanes * lane + i);
+    philox(c, key);
     uint32_t a = 0xffffffffu, b = 0;
 #pragma unroll
-    for (int i = 0; i < 4 / kLanes; ++i) {
-      const uint4 r = philox(make_uint4((uint32_t)w, (uint32_t)(w >> 32), d->site, 4 / kLanes * lane + i), key);
-      a = majority4(r, a, bit + 4 * i), b = majority4(r, b, bit + 4 * i);
-    }
+    for (int i = 0; i < 4 / kLanes; ++i) a = majority4(c[i], a, bit + 4 * i), b = majority4(c[i], b, bit + 4 * i);
 #pragma unroll
     for (uint32_t o = 1; o < kLanes; o *= 2) {   // the upper calls' of the lower ones'; the last lane has it all
       const uint32_t la = __shfl_xor_sync(0xffffffffu, a, o), lb = __shfl_xor_sync(0xffffffffu, b, o);

@@ -46,14 +46,20 @@ __device__ __forceinline__ Key drop_key(const Drop& d) {
   return {__shfl_sync(0xffffffffu, (uint32_t)s, 0), __shfl_sync(0xffffffffu, (uint32_t)(s >> 32), 0)};
 }
 
-__device__ __forceinline__ uint4 philox(uint4 c, Key k) {
+__device__ __forceinline__ uint4 philox_round(uint4 c, Key k) {
+  const uint64_t a = (uint64_t)c.x * 0xD2511F53u, b = (uint64_t)c.z * 0xCD9E8D57u;
+  return make_uint4((uint32_t)(b >> 32) ^ c.y ^ k.lo, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k.hi, (uint32_t)a);
+}
+// N counters round by round, side by side: one alone is a chain of fourteen instructions, each of which waits
+// for the last.
+template <int N>
+__device__ __forceinline__ void philox(uint4 (&c)[N], Key k) {
 #pragma unroll
   for (int i = 0; i < 7; ++i) {
-    const uint64_t a = (uint64_t)c.x * 0xD2511F53u, b = (uint64_t)c.z * 0xCD9E8D57u;
-    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k.lo, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k.hi, (uint32_t)a);
+#pragma unroll
+    for (int n = 0; n < N; ++n) c[n] = philox_round(c[n], k);
     k.lo += 0x9E3779B9u, k.hi += 0xBB67AE85u;
   }
-  return c;
 }
 
 __device__ __forceinline__ uint32_t majority(uint32_t a, uint32_t b, uint32_t c) { return (a & b) | (c & (a | b)); }
@@ -62,21 +68,26 @@ __device__ __forceinline__ uint32_t majority4(uint4 r, uint32_t m, const uint32_
   return majority(r.w, majority(r.z, majority(r.y, majority(r.x, m, bit[0]), bit[1]), bit[2]), bit[3]);
 }
 
-// The bits of words w: set where an element is kept.  Several at once, since a call is one chain of seven
-// rounds, and without a branch between them.
+// The bits of words w: set where an element is kept.
 template <int N>
 __device__ __forceinline__ void kept_words(const Drop& d, Key k, const uint64_t (&w)[N], uint32_t (&m)[N]) {
-  auto call = [&](int n, uint32_t c) { return philox(make_uint4((uint32_t)w[n], (uint32_t)(w[n] >> 32), d.site, c), k); };
+  auto counter = [&](int n, uint32_t call) { return make_uint4((uint32_t)w[n], (uint32_t)(w[n] >> 32), d.site, call); };
   if (d.first == 3) {
+    uint4 c[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) m[n] = majority4(call(n, 3), 0, d.bit + 12);
+    for (int n = 0; n < N; ++n) c[n] = counter(n, 3);
+    philox(c, k);
+#pragma unroll
+    for (int n = 0; n < N; ++n) m[n] = majority4(c[n], 0, d.bit + 12);
   } else {
+    uint4 c[4 * N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      m[n] = 0;
+    for (int n = 0; n < 4 * N; ++n) c[n] = counter(n / 4, n % 4);
+    philox(c, k);
 #pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) m[n] = majority4(call(n, c), m[n], d.bit + 4 * c);
-    }
+    for (int n = 0; n < N; ++n) m[n] = 0;
+#pragma unroll
+    for (int n = 0; n < 4 * N; ++n) m[n / 4] = majority4(c[n], m[n / 4], d.bit + 4 * (n % 4));
   }
 }
 __device__ __forceinline__ uint32_t kept_word(const Drop& d, Key k, uint64_t w) {
