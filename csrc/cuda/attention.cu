@@ -23,13 +23,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-struct Yes {
-  __device__ constexpr operator bool() const { return true; }
-};
-struct No {
-  __device__ constexpr operator bool() const { return false; }
-};
-
 // Which of a tile's columns a row may see, a bit each.
 template <int COLS>
 struct Seen {
@@ -636,8 +629,15 @@ __global__ void __launch_bounds__(256) attention_rows(const __grid_constant__ Hp
       parts[kPass] = second;
     } else {
       float* tile = (float*)(parts - i % kPass + kPass);
-      tile[delta_at((int)(i % kPass))] = -s;
-      if (kNarrow<T> && i % (256 / LANES) == 0) tile[i % kPass * 4 + 3] = second.w;
+      const int r = (int)(i % kPass);
+      tile[delta_at(r)] = -s;
+      // the product of S multiplies all of the tile by zeros, so that every word has to hold a number: three more a row
+#pragma unroll
+      for (int k = 3 * r; k < 3 * r + 3; ++k) {
+        const int at = k < 4 ? k : k < 36 ? k + 32 : k + 64;
+        if (at % 64 != 3) tile[at] = 0.f;
+      }
+      if (r % 16 == 0) tile[4 * r + 3] = second.w;
     }
   }
 }

@@ -48,6 +48,14 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*(const __half2*)&v);
 }
 
+// A choice that is made when a generic function is compiled
+struct Yes {
+  __device__ constexpr operator bool() const { return true; }
+};
+struct No {
+  __device__ constexpr operator bool() const { return false; }
+};
+
 // Two values at a time: half the instructions.
 struct F2 {
   float x, y;

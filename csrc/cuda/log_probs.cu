@@ -13,10 +13,6 @@
 // is put in order in the end.  Values are compared together with their place, so that of equals the first counts
 // and a row of equal values does not flood the list; should it overflow, or a value be no number, the row is read
 // again once for each of the k.
-#include <limits.h>
-
-#include <type_traits>
-
 #include "activation.cuh"
 #include "tcgen05.cuh"
 
@@ -156,45 +152,11 @@ __device__ __forceinline__ float highest<__half>(uint4 v) {
   const float2 f = __half22float2(highest2<__half2>(v));
   return fmaxf(f.x, f.y);
 }
-// Where z 2^z is wanted, no z is infinite: values that lie far below the largest count as one for which 2^z is
-// zero as well.  NaN stays.
-__device__ __forceinline__ float far_below(float m, float lowest) {
-  return m == -INFINITY ? -1e4f : fmaxf(m - fmaxf(300.f, fabsf(m) * 0.015625f), lowest);   // after rounding to 8 bits too
-}
-template <typename T>
-struct AtLeast;
-template <>
-struct AtLeast<float> {
-  float low;
-  __device__ __forceinline__ void set(float m) { low = far_below(m, -3e38f); }
-  __device__ __forceinline__ uint32_t of(uint32_t x) const {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(__uint_as_float(x)), "f"(low));
-    return __float_as_uint(y);
-  }
-};
-template <>
-struct AtLeast<__nv_bfloat16> {
-  uint32_t low;
-  __device__ __forceinline__ void set(float m) { low = pack2<__nv_bfloat16>(far_below(m, -3e38f), far_below(m, -3e38f)); }
-  __device__ __forceinline__ uint32_t of(uint32_t x) const {
-    const __nv_bfloat162 y = __hmax2_nan(*(const __nv_bfloat162*)&x, *(const __nv_bfloat162*)&low);
-    return *(const uint32_t*)&y;
-  }
-};
-template <>
-struct AtLeast<__half> {
-  uint32_t low;
-  __device__ __forceinline__ void set(float m) { low = pack2<__half>(far_below(m, -65504.f), far_below(m, -65504.f)); }
-  __device__ __forceinline__ uint32_t of(uint32_t x) const {
-    const __half2 y = __hmax2_nan(*(const __half2*)&x, *(const __half2*)&low);
-    return *(const uint32_t*)&y;
-  }
-};
-template <bool ENTROPY, typename T>
-__device__ __forceinline__ uint4 finite(uint4 v, const AtLeast<T>& at_least) {
-  if (ENTROPY) v = make_uint4(at_least.of(v.x), at_least.of(v.y), at_least.of(v.z), at_least.of(v.w));
-  return v;
+// Where z 2^z is wanted: no z is infinite, and one whose 2^z is zero may be any other such.  NaN stays.
+__device__ __forceinline__ float finite(float z) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(z), "f"(-1e4f));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -308,8 +270,6 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
 #pragma unroll
   for (int i = 0; i < kAhead<G>; ++i) fetch(first + i * G * kBatch);
   Sums sum = {-INFINITY, 0.f, 0.f};
-  AtLeast<T> at_least;
-  at_least.set(-INFINITY);
   uint64_t best = 0, least = 0;
   float high = -INFINITY, bar = -INFINITY;   // the thread's largest value; that of `least`
   int turn = 0;
@@ -323,7 +283,6 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
     // the sums bear values that are larger by a few powers of two: raised is seldom more than once
     if (now > sum.m + 8.f || sum.m == -INFINITY) {
       sum.raise(fmaxf(now, sum.m));
-      if (ENTROPY) at_least.set(sum.m);
     }
     if (TOP) {
       if (batch == 0 && p + t < end) {   // the first of the places that hold the largest value
@@ -350,17 +309,19 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         float v[V];
-        unpack<T>(finite<infinite>(raw[i], at_least), v);
+        unpack<T>(raw[i], v);
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
-          const F2 z = mul2(add2({v[j], v[j + 1]}, {minus, minus}), {kLog2e, kLog2e}), x = {exp2_fast(z.x), exp2_fast(z.y)};
+          F2 z = mul2(add2({v[j], v[j + 1]}, {minus, minus}), {kLog2e, kLog2e});
+          if (infinite) z = {finite(z.x), finite(z.y)};
+          const F2 x = {exp2_fast(z.x), exp2_fast(z.y)};
           s = add2(s, x);
           if (ENTROPY) e = fma2(x, z, e);
         }
       }
     };
-    add_up(std::false_type());
-    if (ENTROPY && !(e.x + e.y > -INFINITY)) add_up(std::true_type());   // zero times an infinity, or a NaN of the logits'
+    add_up(No());
+    if (ENTROPY && !(e.x + e.y > -INFINITY)) add_up(Yes());   // zero times an infinity, or a NaN of the logits'
     sum.s += s.x + s.y, sum.e += e.x + e.y;
     if (TOP) {
       if (batch == turn) {   // batches 0, 2, 8, 32 ..
@@ -370,11 +331,11 @@ __global__ void __launch_bounds__(kCta<G>, 1024 / kCta<G>) log_probs_kernel(cons
         bar = least ? value_of(least) : -INFINITY;
       }
       if (now >= bar) {
-        const int place = least ? place_of(least) : INT_MAX;   // of equal values the first count
+        const uint32_t place = ~(uint32_t)least;   // of equal values the first count; all, where no place is known
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           const int q = p + t + i * G;
-          if (q < end && (top[i] > bar || (top[i] == bar && q * V - r.phase <= place))) {
+          if (q < end && (top[i] > bar || (top[i] == bar && (uint32_t)max(q * V - r.phase, 0) <= place))) {
             const int at = atomicAdd(&l.n, 1);
             if (at < Largest<G>::kList) l.list[at] = q;
           }
@@ -546,8 +507,6 @@ __global__ void __launch_bounds__(256, 4) log_probs_backward_kernel(const __grid
   const float hz = h * -kLn2, by = ENTROPY ? fmaf(-h, a.entropy[row], -g) : -g;
   const int mine = g != 0.f && token >= 0 && token < in.vocab ? (int)token : -V;
   T* to = (T*)a.dlogits + row * a.vocab;
-  AtLeast<T> at_least;
-  at_least.set(m);
   auto take = [&](uint4 (&raw)[kBatch], int p) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -576,11 +535,12 @@ __global__ void __launch_bounds__(256, 4) log_probs_backward_kernel(const __grid
       const int col = (p + i * G + t) * V - out.phase;
       if (col >= out.vocab) break;
       float v[V];
-      unpack<T>(finite<ENTROPY>(raw[i], at_least), v);
+      unpack<T>(raw[i], v);
       if (some) {
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
-          const F2 z = fma2(add2({v[j], v[j + 1]}, {-m, -m}), {kLog2e, kLog2e}, {-log2s, -log2s});
+          F2 z = fma2(add2({v[j], v[j + 1]}, {-m, -m}), {kLog2e, kLog2e}, {-log2s, -log2s});
+          if (ENTROPY) z = {finite(z.x), finite(z.y)};
           const F2 x = mul2({exp2_fast(z.x), exp2_fast(z.y)}, ENTROPY ? fma2(z, {hz, hz}, {by, by}) : F2{by, by});
           v[j] = x.x, v[j + 1] = x.y;
         }
