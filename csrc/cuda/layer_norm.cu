@@ -182,7 +182,8 @@ constexpr int kCtasOf = NW == 1 ? 4 : NW == 3 ? 6 : NW <= 5 ? 4 : NW == 6 ? 3 : 
 
 // Backward, where three tensors fill the ring: one CTA of ten warps instead of two took 89 us
 // instead of 97 for 8192 x 5000 fp16, but 134 instead of 110 for the ragged rows of 8191 x 4999
-// (their ends cost latency); of eight warps 74 instead of 64 for 8192 x 4096.
+// (their ends cost latency); of eight warps 74 instead of 64 for 8192 x 4096.  With a dropout three pieces in
+// one warp spill at three CTAs to an SM: two take 112 us instead of 135 for 65536 x 768 bf16.
 template <int NW, bool RAGGED>
 constexpr int kCtasBack = NW == 3 ? 4 + RAGGED : NW == 4 ? 3 : NW == 5 || NW == 6 || NW == 10 ? kCtasOf<NW> - !RAGGED : kCtasOf<NW>;
 
@@ -531,7 +532,7 @@ norm_forward_rows(const __grid_constant__ HpNormForward a, const __grid_constant
 }
 
 template <typename T, int NW, int CH, bool RAGGED>
-__global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 1 ? (CH == 4 ? 2 : 3) : kCtasBack<NW, RAGGED>)
+__global__ void __launch_bounds__(kThreadsOf<NW>, NW == 1 && CH > 1 ? (CH == 4 || (kDropout && CH == 3) ? 2 : 3) : kCtasBack<NW, RAGGED>)
 norm_backward_rows(const __grid_constant__ HpNormBackward a, const __grid_constant__ MaybeDrop drop, int depth, int slot_bytes, int ring_bytes,
                    uint32_t* status) {
   constexpr int V = kPiece<T>, kGroups = kGroupsOf<NW>;

@@ -321,6 +321,46 @@ def test_expected_output_is_that_without_a_dropout(dtype):
     assert ((outs.mean(0) - want).abs() <= 6 * sigma + 4 * U[dtype] * want.abs() + 4 * U[dtype]).all()
 
 
+def test_attention_without_keys_or_queries():
+    for sq, sk in ((5, 0), (0, 5), (200, 0)):
+        q = rand(2, sq, 4, 64, dtype=BF16).requires_grad_(True)
+        k, v = (rand(2, sk, 2, 64, dtype=BF16).requires_grad_(True) for _ in range(2))
+        o = attention(q, k, v, dropout=0.5, seed=1)
+        assert o.shape == q.shape and not o.any()
+        for g in torch.autograd.grad(o, (q, k, v), torch.ones_like(o)):
+            assert not g.any()
+
+
+# ------------------------------------------------------------------ kept tensors
+def test_tensors_kept_elsewhere_and_recomputed_passes():
+    from torch.utils.checkpoint import checkpoint
+    from hipress_b200.ops import cross_entropy
+    torch.manual_seed(0)
+    x, r, w = rand(40, 3 * 128, dtype=BF16), rand(40, 3 * 128, dtype=BF16), rand(3 * 128, dtype=FP32)
+    seed, labels = torch.tensor([12], device="cuda"), torch.randint(0, 128, (40,), device="cuda")
+
+    def step(x, r, w):
+        y, z = layer_norm(dropout(x, 0.1, seed=seed, site=1), w, residual=r, dropout=0.2, seed=seed, site=2)
+        o = self_attention(y.view(2, 20, 3, 2, 64), dropout=0.3, seed=seed, site=3)
+        return cross_entropy(o.reshape(40, 128), labels) + z.float().mean()
+
+    def run(how):
+        leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+        loss = how(leaves)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    want = run(lambda l: step(*l))
+    with torch.autograd.graph.save_on_cpu():
+        leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+        loss = step(*leaves)
+    got = [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    again = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    loss = checkpoint(step, *again, use_reentrant=False)   # the same masks when the forward pass is run again
+    loss.backward()
+    assert all(torch.equal(a, b.grad) for a, b in zip(want[1:], again))
+
+
 # ------------------------------------------------------------------------ BERT
 def test_bert_trains_with_all_of_its_dropouts():
     from hipress_b200.models import bert_tiny
